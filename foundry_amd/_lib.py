@@ -91,6 +91,15 @@ class LlamaModel(ctypes.Structure):
     ]
 
 
+class LogitRules(ctypes.Structure):
+    """fh_logit_rules: what fh_logits_process applies (device pointers; a rule
+    whose pointer is None is left out)."""
+    _fields_ = [("history", ctypes.c_void_p), ("history_ld", ctypes.c_int64), ("history_len", ctypes.c_void_p),
+                ("prompt_len", ctypes.c_void_p), ("repetition", ctypes.c_void_p), ("frequency", ctypes.c_void_p),
+                ("presence", ctypes.c_void_p), ("bias_ids", ctypes.c_void_p), ("bias_values", ctypes.c_void_p),
+                ("bias_ld", ctypes.c_int64), ("bias_len", ctypes.c_void_p), ("mask", ctypes.c_void_p)]
+
+
 _I64x4 = ctypes.c_int64 * 4
 
 
@@ -169,6 +178,15 @@ SIGNATURES = {
     "fh_advance_positions": [_vp, _vp, _i64, _i64],
     "fh_append_token": [_vp, _vp, _i64, _vp, _vp, _i64, _i64],
     "fh_append_token_advance": [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64],
+    "fh_paged_rope_kv": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64,
+                         _i64, _vp],
+    "fh_paged_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(ctypes.c_uint64)],
+    "fh_paged_attention": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, ctypes.c_float,
+                           _vp, ctypes.c_uint64, _vp],
+    "fh_lora_workspace": [_i64, _i64, _i64, ctypes.POINTER(ctypes.c_uint64)],
+    "fh_lora_add": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _int, _vp,
+                    ctypes.c_uint64],
+    "fh_logits_process": [_vp, _vp, _int, _i64, _i64, ctypes.POINTER(LogitRules), _vp],
     "fh_llama_forward": [_vp, _vp, _i64, _vp, _vp, _vp],
     "fh_copy_strided": [_vp, _int, _vp, ctypes.POINTER(View), _vp],
     "fh_to_dtype": [_vp, _int, _vp, ctypes.POINTER(View), _int, _vp],
@@ -224,6 +242,19 @@ def attention_workspace_bytes(tokens: int, n_heads: int, n_kv: int, head_dim: in
 def decode_attention_workspace_bytes(batch: int, n_heads: int, n_kv: int, head_dim: int, max_len: int) -> int:
     out = ctypes.c_uint64()
     call("fh_decode_attention_workspace", batch, n_heads, n_kv, head_dim, max_len, ctypes.byref(out))
+    return out.value
+
+
+def paged_attention_workspace_bytes(batch: int, n_heads: int, n_kv: int, head_dim: int, page_size: int,
+                                    max_pages: int) -> int:
+    out = ctypes.c_uint64()
+    call("fh_paged_attention_workspace", batch, n_heads, n_kv, head_dim, page_size, max_pages, ctypes.byref(out))
+    return out.value
+
+
+def lora_workspace_bytes(m: int, k: int, rank: int) -> int:
+    out = ctypes.c_uint64()
+    call("fh_lora_workspace", m, k, rank, ctypes.byref(out))
     return out.value
 
 

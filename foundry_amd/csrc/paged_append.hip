@@ -1,0 +1,122 @@
+// Appending to a paged cache with the rotation on the way (fh_paged_rope_kv).
+#include "paged_cache.hpp"
+
+namespace fh {
+
+// x' = RNE(x * cos + rot * sin) of 8 dims: fp32 throughout, one rounding.
+__device__ __forceinline__ uint4 rotate8(const uint4 x4, const uint4 r4, const uint4 c4, const uint4 s4,
+                                         bool first_half) {
+    const float sign = first_half ? -1.0f : 1.0f;
+    float xv[8], rv[8], cv[8], sv[8];
+    unpack8(x4, xv);
+    unpack8(r4, rv);
+    unpack8(c4, cv);
+    unpack8(s4, sv);
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        o[e] = f32x2_to_bf16x2_rne(fmaf(xv[2 * e], cv[2 * e], sign * rv[2 * e] * sv[2 * e]),
+                                   fmaf(xv[2 * e + 1], cv[2 * e + 1], sign * rv[2 * e + 1] * sv[2 * e + 1]));
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// One block per token; a thread takes pieces of 8 dims.
+__global__ __launch_bounds__(256) void paged_rope_kv_kernel(
+    const uint16_t *__restrict__ qkv, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim,
+    const uint16_t *__restrict__ cos_tab, const uint16_t *__restrict__ sin_tab, uint32_t table_len,
+    const uint32_t *__restrict__ sequences, const uint32_t *__restrict__ positions,
+    const uint32_t *__restrict__ page_table, uint32_t n_seqs, uint32_t max_pages, uint16_t *__restrict__ k_pages,
+    uint16_t *__restrict__ v_pages, uint32_t n_pages, uint32_t page_size, uint16_t *__restrict__ q_out) {
+    const uint32_t t = blockIdx.x;
+    const uint32_t pos = positions[t], seq = sequences ? sequences[t] : t;
+    // device data the host cannot check: such a token writes nothing
+    if (pos >= max_pages * page_size || pos >= table_len || seq >= n_seqs) return;
+    const uint32_t page = page_table[static_cast<uint64_t>(seq) * max_pages + pos / page_size];
+    if (page >= n_pages) return;
+    const uint32_t slot = pos % page_size, heads = n_heads + 2 * n_kv, ppw = head_dim / 8, hp = ppw / 2;
+    const uint16_t *row = qkv + static_cast<uint64_t>(t) * heads * head_dim;
+    const uint16_t *c = cos_tab + static_cast<uint64_t>(pos) * head_dim;
+    const uint16_t *s = sin_tab + static_cast<uint64_t>(pos) * head_dim;
+    const uint64_t region = static_cast<uint64_t>(page_size) * head_dim;
+    const uint64_t base = static_cast<uint64_t>(page) * n_kv * region;
+    for (uint32_t i = threadIdx.x; i < heads * ppw; i += blockDim.x) {
+        const uint32_t h = i / ppw, p = i % ppw;
+        const uint16_t *head = row + h * head_dim;
+        uint4 x = *reinterpret_cast<const uint4 *>(head + p * 8);
+        if (h < n_heads + n_kv) {
+            const uint32_t partner = p < hp ? p + hp : p - hp;
+            x = rotate8(x, *reinterpret_cast<const uint4 *>(head + partner * 8),
+                        *reinterpret_cast<const uint4 *>(c + p * 8), *reinterpret_cast<const uint4 *>(s + p * 8),
+                        p < hp);
+        }
+        uint16_t *to;
+        if (h < n_heads)
+            to = q_out + (static_cast<uint64_t>(t) * n_heads + h) * head_dim + p * 8;
+        else if (h < n_heads + n_kv)
+            to = k_pages + base + (h - n_heads) * region + k_offset(slot, p * 8, page_size, head_dim);
+        else
+            to = v_pages + base + (h - n_heads - n_kv) * region + slot * head_dim + p * 8;
+        *reinterpret_cast<uint4 *>(to) = x;
+    }
+}
+
+}  // namespace fh
+
+using namespace fh;
+
+extern "C" int fh_paged_rope_kv(fh_device *dev, const uint16_t *qkv, int64_t tokens, int64_t n_heads, int64_t n_kv,
+                                int64_t head_dim, const uint16_t *cos_tab, const uint16_t *sin_tab, int64_t table_len,
+                                const uint32_t *sequences, const uint32_t *positions, const uint32_t *page_table,
+                                int64_t n_seqs, int64_t max_pages, uint16_t *k_pages, uint16_t *v_pages,
+                                int64_t n_pages, int64_t page_size, uint16_t *q_out) {
+    const char *fn = "fh_paged_rope_kv";
+    if (int rc = check_usable(dev, fn)) return rc;
+    if (int rc = fh_check_dims(fn, {tokens, n_heads, n_kv, head_dim, table_len, n_seqs, max_pages, n_pages, page_size}))
+        return rc;
+    if (tokens == 0) return FH_OK;
+    if (int rc = check_pages(fn, n_pages, page_size, max_pages)) return rc;
+    if (head_dim < 32 || head_dim > 256 || head_dim % 32 != 0)
+        return fail(FH_ERR_UNSUPPORTED, "%s: head_dim %lld must be a multiple of 32, at most 256", fn,
+                    (long long)head_dim);
+    if (n_heads < 1 || n_kv < 1 || (n_heads + 2 * n_kv) * head_dim > 0x7FFFFFFFll)
+        return fail(FH_ERR_INVALID_ARGUMENT, "%s: %lld heads and %lld KV heads", fn, (long long)n_heads,
+                    (long long)n_kv);
+    if (n_seqs < 1 || table_len < 1)
+        return fail(FH_ERR_INVALID_ARGUMENT, "%s: n_seqs and table_len must be at least 1", fn);
+    if (sequences == nullptr && tokens > n_seqs)
+        return fail(FH_ERR_INVALID_ARGUMENT, "%s: %lld tokens of %lld sequences need their sequences named", fn,
+                    (long long)tokens, (long long)n_seqs);
+    for (const void *p : {static_cast<const void *>(qkv), static_cast<const void *>(cos_tab),
+                          static_cast<const void *>(sin_tab), static_cast<const void *>(q_out)})
+        if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
+            return fail(FH_ERR_INVALID_ARGUMENT, "%s: operands must be 16-byte aligned", fn);
+    const uint64_t width = static_cast<uint64_t>(n_heads + 2 * n_kv) * head_dim, t = static_cast<uint64_t>(tokens);
+    const uint64_t table = static_cast<uint64_t>(table_len) * head_dim * 2;
+    uint64_t pool;
+    if (int rc = check_pools(dev, fn, k_pages, v_pages, n_pages, n_kv, page_size, head_dim, page_table, n_seqs,
+                             max_pages, &pool))
+        return rc;
+    if (int rc = check_range(dev, qkv, t * width * 2, fn, "qkv")) return rc;
+    if (int rc = check_range(dev, cos_tab, table, fn, "cos_tab")) return rc;
+    if (int rc = check_range(dev, sin_tab, table, fn, "sin_tab")) return rc;
+    if (sequences)
+        if (int rc = check_range(dev, sequences, t * 4, fn, "sequences")) return rc;
+    if (int rc = check_range(dev, positions, t * 4, fn, "positions")) return rc;
+    if (int rc = check_range(dev, q_out, t * n_heads * head_dim * 2, fn, "q_out")) return rc;
+    const uint64_t q_bytes = t * n_heads * head_dim * 2;
+    if (int rc = refuse_overlap(fn, "v_pages", v_pages, pool, "k_pages", k_pages, pool)) return rc;
+    if (int rc = refuse_overlap(fn, "q_out", q_out, q_bytes, "qkv", qkv, t * width * 2)) return rc;
+    if (int rc = refuse_overlap(fn, "q_out", q_out, q_bytes, "k_pages", k_pages, pool)) return rc;
+    if (int rc = refuse_overlap(fn, "q_out", q_out, q_bytes, "v_pages", v_pages, pool)) return rc;
+    if (int rc = refuse_overlap(fn, "k_pages", k_pages, pool, "qkv", qkv, t * width * 2)) return rc;
+    if (int rc = refuse_overlap(fn, "v_pages", v_pages, pool, "qkv", qkv, t * width * 2)) return rc;
+    if (int rc = set_current(dev, fn)) return rc;
+    return dispatch(dev, fn, [&] {
+        hipLaunchKernelGGL(paged_rope_kv_kernel, dim3(static_cast<uint32_t>(tokens)), dim3(256), 0, dev->stream, qkv,
+                           static_cast<uint32_t>(n_heads), static_cast<uint32_t>(n_kv),
+                           static_cast<uint32_t>(head_dim), cos_tab, sin_tab, static_cast<uint32_t>(table_len),
+                           sequences, positions, page_table, static_cast<uint32_t>(n_seqs),
+                           static_cast<uint32_t>(max_pages), k_pages, v_pages, static_cast<uint32_t>(n_pages),
+                           static_cast<uint32_t>(page_size), q_out);
+    });
+}

@@ -492,6 +492,127 @@ int fh_append_token_advance(fh_device *dev, const uint32_t *token, int64_t rows,
                             uint32_t *position, int64_t base, int64_t capacity, int64_t by);
 
 /* ======================================================================
+ * Serving many requests at once: a paged KV cache, low-rank adapters and
+ * logit rules. No counterpart in the reference, which decodes equal-length
+ * sequences over one static cache each (src/nn/kv_cache.rs:13-39), with one
+ * set of weights, greedily. Unlike the decoder-step ops above, which round
+ * where the reference's op sequence rounds, these keep fp32 inside and round
+ * each output once.
+ *
+ * A paged cache is a pool of n_pages pages of page_size tokens (a multiple of
+ * 16). Page p of the K pool and of the V pool holds n_kv regions of page_size
+ * * head_dim elements, each laid out as a cache of max_len = page_size (K
+ * grouped by 16 keys, V [page_size][head_dim]); the pools are
+ * [n_pages][n_kv][page_size * head_dim]. page_table (device u32 [n_seqs,
+ * max_pages]) names sequence s's pages in order: position j of s is slot j %
+ * page_size of page page_table[s * max_pages + j / page_size]. Entries behind
+ * a sequence's last page are not read. Positions, sequences and page ids are
+ * device data that the host cannot check: an entry that names no page
+ * (>= n_pages) is left alone, as described for each call. max_pages *
+ * page_size is at most 2^31 - 1; pools may pass 4 GiB. Pools and 2-byte
+ * operands are 16-byte aligned.
+ * ====================================================================== */
+
+/* apply_rotary_pos_emb on q and k of each token, then k and v written to the
+ * token's place in the paged cache (fh_rope_kv for requests of any lengths, as
+ * a packed batch of prompts or one new token each):
+ *   q' = RNE(q * cos + rot(q) * sin), k' the same, v as it is.
+ * qkv: [tokens, (n_heads + 2 n_kv) * head_dim]; cos_tab / sin_tab:
+ * [table_len, head_dim]; sequences: u32 [tokens], or null where token t is of
+ * sequence t (tokens <= n_seqs); positions: u32 [tokens]; q_out: [tokens,
+ * n_heads, head_dim], not overlapping qkv. A token whose position is >=
+ * max_pages * page_size or >= table_len, whose sequence is >= n_seqs or whose
+ * page is >= n_pages writes nothing, neither to the pools nor to q_out (a
+ * padded row takes a position past the pages, far enough below 2^32 where
+ * fh_advance_positions moves it on). Two tokens of one sequence and position
+ * leave the values of either in each 16-byte piece. head_dim is a multiple of
+ * 32, at most 256. */
+int fh_paged_rope_kv(fh_device *dev, const uint16_t *qkv, int64_t tokens, int64_t n_heads,
+                     int64_t n_kv, int64_t head_dim, const uint16_t *cos_tab,
+                     const uint16_t *sin_tab, int64_t table_len, const uint32_t *sequences,
+                     const uint32_t *positions, const uint32_t *page_table, int64_t n_seqs,
+                     int64_t max_pages, uint16_t *k_pages, uint16_t *v_pages, int64_t n_pages,
+                     int64_t page_size, uint16_t *q_out);
+
+/* Bytes of device workspace fh_paged_attention needs for these sizes. */
+int fh_paged_attention_workspace(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
+                                 int64_t page_size, int64_t max_pages, uint64_t *bytes);
+
+/* Attention of one new token of each sequence over the paged cache, whose
+ * keys and values (the new token's among them) fh_paged_rope_kv has written:
+ *   s_j = scale * (q . k_j), j = 0..positions[b],
+ *   out[b] = RNE(sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s))
+ * with fp32 sums. q, out: [batch, n_heads * head_dim]; row b of page_table
+ * and positions[b] belong to sequence b; query head h uses KV head h /
+ * (n_heads / n_kv). A sequence whose position is >= max_pages * page_size is
+ * idle: zeros to its rows of out. Keys of a table entry that names no page
+ * are left out; a sequence left with no key gets zeros. What lies in a page
+ * behind the position is not used, whatever its bits. A row whose every score
+ * is -inf is NaN. head_dim is 64, 128 or 256; any n_heads / n_kv; batch at
+ * most 65535; out does not overlap the inputs. workspace: at least
+ * fh_paged_attention_workspace() bytes, 16-byte aligned, no initial contents;
+ * calls that share a workspace must not run concurrently. */
+int fh_paged_attention(fh_device *dev, const uint16_t *q, int64_t batch, int64_t n_heads,
+                       int64_t n_kv, int64_t head_dim, const uint16_t *k_pages,
+                       const uint16_t *v_pages, int64_t n_pages, int64_t page_size,
+                       const uint32_t *page_table, int64_t max_pages, const uint32_t *positions,
+                       float scale, void *workspace, uint64_t workspace_bytes, uint16_t *out);
+
+/* Bytes of device workspace fh_lora_add needs for these sizes. */
+int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *bytes);
+
+/* The low-rank adapters of many requests beside a shared projection (base,
+ * what fh_q4_matmul gave for the same x):
+ *   y[i, :] = RNE(base[i, :] + scales[a] * (x[i, :] . A_a^T) . B_a^T),
+ *   a = adapters[i],
+ * with fp32 sums. x: bf16 [m, k] with row stride x_ld (a multiple of 8, >= k);
+ * a: bf16 [n_adapters, rank, k]; b: bf16 [n_adapters, n, rank]; scales: f32
+ * [n_adapters]; adapters: u32 [m], in any order, a row of a value >=
+ * n_adapters taking no adapter (y = base there). An adapter of a lower rank
+ * is filled up with zeros. base, y: [m, n] of `dtype` (FH_BF16 or FH_F32)
+ * with row strides base_ld, y_ld >= n; y is base itself (the same pointer and
+ * stride) or does not overlap the operands. rank and k are multiples of 8,
+ * rank at most 128; n is any; x, a, b 16-byte aligned. workspace: at least
+ * fh_lora_workspace() bytes, 16-byte aligned, no initial contents; calls that
+ * share a workspace must not run concurrently. */
+int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t k, int64_t x_ld,
+                const uint16_t *a, const uint16_t *b, const float *scales, int64_t n_adapters,
+                int64_t rank, int64_t n, const uint32_t *adapters, const void *base,
+                int64_t base_ld, void *y, int64_t y_ld, int dtype, void *workspace,
+                uint64_t workspace_bytes);
+
+/* What fh_logits_process applies; every pointer is device memory, and each
+ * rule whose pointer is null is left out. */
+typedef struct fh_logit_rules {
+    const uint32_t *history;     /* [rows, history_ld] token ids: the prompt, then what was generated */
+    int64_t history_ld;
+    const uint32_t *history_len; /* [rows] ids in use (at most history_ld are) */
+    const uint32_t *prompt_len;  /* [rows] leading ids that are the prompt's; null: 0 */
+    const float *repetition;     /* [rows] */
+    const float *frequency;      /* [rows] */
+    const float *presence;       /* [rows] */
+    const uint32_t *bias_ids;    /* [rows, bias_ld] */
+    const float *bias_values;    /* [rows, bias_ld] */
+    int64_t bias_ld;
+    const uint32_t *bias_len;    /* [rows] entries in use (at most bias_ld are); null: bias_ld */
+    const uint32_t *mask;        /* [rows, ceil(n / 32)]: bit j % 32 of word j / 32 allows token j */
+} fh_logit_rules;
+
+/* Penalties for repeated tokens, biases and a grammar's mask on logits, before
+ * fh_argmax. For token j of a row, c = its count among the generated ids:
+ *   1. repetition, where j is among the history's ids: z = z > 0 ? z / r : z * r
+ *   2. frequency and presence: z = (z - f * c) - (c > 0 ? p : 0)
+ *   3. bias: z = z + value (an id listed twice: the last entry counts)
+ *   4. mask: z = -inf where j's bit is 0, whatever z was
+ * each step rounded to fp32, then z once to dtype. logits, out: [rows, n] of
+ * `dtype` (FH_BF16 or FH_F32); out may be logits itself, else does not
+ * overlap the inputs. An id >= n is passed over. history and history_len go
+ * together (the three penalties need them), as do bias_ids and bias_values.
+ * rows is at most 65535. */
+int fh_logits_process(fh_device *dev, const void *logits, int dtype, int64_t rows, int64_t n,
+                      const fh_logit_rules *rules, void *out);
+
+/* ======================================================================
  * The decoder forward issued from native code: the layer loop that a
  * caller would otherwise drive op by op, so an eager prefill is not bound
  * by per-call host overhead.
