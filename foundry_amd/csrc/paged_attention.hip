@@ -1,64 +1,388 @@
 // Attention of one new token per sequence over a paged cache
 // (fh_paged_attention).
+#include <algorithm>
 #include <tuple>
 
 #include "paged_cache.hpp"
 
 namespace fh {
 
+// The mathematics: one pass over a sequence's keys with the running maximum m,
+// sum l and weighted values o of each query head,
+//   m' = max(m, s), l' = l e^(m - m') + e^(s - m'), o' = o e^(m - m') + e^(s - m') v,
+// joined over disjoint key ranges by the same rule. Exponentials are taken as
+// powers of two of scores scaled by log2 e.
+//
+// The split: a block of four wavefronts takes one part of a sequence (whole
+// steps of kStepKeys keys) for one KV head and up to 8 of the query heads that
+// share it; each wavefront streams its quarter of the part's keys, 32 at a
+// time, and the four join in LDS. The parts of all sequences are laid out from
+// the positions on the device (see find_part), so the same launch serves one
+// long context and a ragged batch, and may be captured.
+//
+// Per 32 keys the scores are S^T = K Q^T on the matrix cores
+// (v_mfma_f32_16x16x32_bf16, 16 keys x 16 columns): a lane ends up with its
+// column's scores of keys 4 q .. 4 q + 3 (q = lane / 16) of both 16-key groups.
+// Those eight probabilities are the fragment that O^T = V^T P^T needs of that
+// lane if its keys are numbered so, so P never leaves its lane; V's rows, read
+// as they lie, become V^T fragments by byte permutes within a lane. The 16
+// columns are 8 heads twice: columns 0..7 hold the probabilities rounded to
+// bf16, columns 8..15 what that rounding lost, so that P V has 16 bits of P at
+// the cost of none (the columns would idle).
 constexpr uint32_t kPagedThreads = 256;
+constexpr uint32_t kPagedWaves = kPagedThreads / 64;
+constexpr uint32_t kStepKeys = 32 * kPagedWaves;
+constexpr uint32_t kHeadTile = 8;
+// Blocks that the parts of a batch aim for (the parts of one KV head and head
+// tile: that divided by their number).
+constexpr uint32_t kPartBlocks = 1024;
+// Larger batches take one part per sequence, laid out without a search.
+constexpr uint32_t kPlanBatch = 1024;
 
-// One block per (query head, sequence). A pass takes 256 keys: each thread
-// scores one key, then (the running maximum and sum updated) each thread of a
-// dim adds the pass's 256 weighted values.
-__global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(
-    const uint16_t *__restrict__ q, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim,
-    const uint16_t *__restrict__ k_pages, const uint16_t *__restrict__ v_pages, uint32_t n_pages, uint32_t page_size,
-    const uint32_t *__restrict__ page_table, uint32_t max_pages, const uint32_t *__restrict__ positions, float scale,
-    uint16_t *__restrict__ out) {
-    __shared__ float qs[256], ps[kPagedThreads], red[4];
-    __shared__ uint64_t where[kPagedThreads];
-    const uint32_t h = blockIdx.x, b = blockIdx.y, kv = h / (n_heads / n_kv), t = threadIdx.x;
-    const uint32_t pos = positions[b], keys = pos < max_pages * page_size ? pos + 1 : 0;
-    const uint64_t row = (static_cast<uint64_t>(b) * n_heads + h) * head_dim;
-    if (t < head_dim) qs[t] = bf(q[row + t]);
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    bool any = false;
-    for (uint32_t k0 = 0; k0 < keys; k0 += kPagedThreads) {
-        const uint32_t j = k0 + t;
-        const uint32_t page = j < keys ? page_table[static_cast<uint64_t>(b) * max_pages + j / page_size] : n_pages;
-        const bool live = page < n_pages;
-        const uint64_t at = (static_cast<uint64_t>(live ? page : 0) * n_kv + kv) * page_size * head_dim;
-        __syncthreads();
-        float s = -INFINITY;
-        if (live) {
-            s = 0.0f;
-            for (uint32_t d = 0; d < head_dim; ++d)
-                s = fmaf(qs[d], bf(k_pages[at + k_offset(j % page_size, d, page_size, head_dim)]), s);
-            s *= scale;
-        }
-        float top = s;
+typedef __attribute__((ext_vector_type(8))) __bf16 pa_bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) float pa_f32x4_t;
+
+__device__ __forceinline__ pa_f32x4_t pa_mfma(uint4 a, uint4 b, pa_f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8_t, a),
+                                                   __builtin_bit_cast(pa_bf16x8_t, b), c, 0, 0, 0);
+}
+
+struct PagedArgs {
+    const uint16_t *q, *k_pages, *v_pages;
+    const uint32_t *page_table, *positions;
+    uint32_t batch, n_heads, n_kv, n_pages, page_size, max_pages;
+    uint32_t want_parts;  // parts that one (KV head, head tile) aims for; 0: one per sequence
+    float scale;
+    float *records;
+    uint16_t *out;
+};
+
+__device__ __forceinline__ uint32_t steps_of(const PagedArgs &a, uint32_t b) {
+    const uint32_t pos = a.positions[b];
+    return pos < a.max_pages * a.page_size ? pos / kStepKeys + 1 : 0;
+}
+
+__device__ __forceinline__ uint32_t scan_wave(uint32_t v, uint32_t lane) {
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-        if (t % 64 == 0) red[t / 64] = top;
-        where[t] = live ? at + static_cast<uint64_t>(j % page_size) * head_dim : ~0ull;
-        __syncthreads();
-        const float next = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-        const float ref = next == -INFINITY ? 0.0f : next;
-        const float keep = expf(m - ref);
-        ps[t] = live ? expf(s - ref) : 0.0f;
-        m = next;
-        __syncthreads();
-        acc *= keep;
-        l *= keep;
-        for (uint32_t i = 0; i < kPagedThreads && k0 + i < keys; ++i)
-            if (where[i] != ~0ull) {
-                any = true;
-                l += ps[i];
-                if (t < head_dim) acc = fmaf(ps[i], bf(v_pages[where[i] + t]), acc);
-            }
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t o = __shfl_up(v, off, 64);
+        if (lane >= static_cast<uint32_t>(off)) v += o;
     }
-    if (t < head_dim) out[row + t] = any ? rne(acc / l) : 0;
+    return v;
+}
+
+// Where a part lies: steps first .. first + count - 1 of a sequence cut into
+// `parts` parts, whose records start at `base`.
+struct Part {
+    uint32_t seq, first, count, parts, base;
+    bool found;
+};
+
+// With P = ceil(all steps / want_parts), sequence b has ceil(steps_b / P)
+// parts, numbered through the batch: at most want_parts + batch in all. Every
+// wavefront works the numbering out for itself, 64 sequences at a time.
+// BY_SEQ: the parts of sequence `at` (count is then 0); else part number `at`.
+template <bool BY_SEQ>
+__device__ __forceinline__ Part find_part(const PagedArgs &a, uint32_t at, uint32_t lane) {
+    if (a.want_parts == 0) {
+        const uint32_t n = steps_of(a, at);
+        return {at, 0, n, n ? 1u : 0u, at, true};
+    }
+    uint32_t total = 0, mine = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+        mine = b0 + lane < a.batch ? steps_of(a, b0 + lane) : 0;
+        total += __builtin_amdgcn_readlane(scan_wave(mine, lane), 63);
+    }
+    const uint32_t size = max(1u, (total + a.want_parts - 1) / a.want_parts);
+    uint32_t base = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+        if (a.batch > 64) mine = b0 + lane < a.batch ? steps_of(a, b0 + lane) : 0;
+        const uint32_t parts = (mine + size - 1) / size, upto = scan_wave(parts, lane);
+        const uint64_t hit = BY_SEQ ? (at - b0 < 64 ? 1ull << (at - b0) : 0) : __ballot(at < base + upto);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            const uint32_t n = __builtin_amdgcn_readlane(mine, l), k = __builtin_amdgcn_readlane(parts, l);
+            const uint32_t start = base + __builtin_amdgcn_readlane(upto, l) - k;
+            const uint32_t first = BY_SEQ ? 0 : (at - start) * size;
+            return {b0 + l, first, BY_SEQ ? 0 : min(size, n - first), k, start, true};
+        }
+        base += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return {0, 0, 0, 0, 0, false};
+}
+
+// A record: what a part leaves to be joined, [8 heads][HD] weighted values,
+// then m, l and (in the third row) whether any key was there, of each head.
+template <int HD>
+constexpr uint32_t record_floats() { return kHeadTile * HD + 3 * kHeadTile; }
+
+template <int HD>
+__global__ __launch_bounds__(kPagedThreads, HD == 256 ? 1 : 2) void paged_part_kernel(const PagedArgs a) {
+    constexpr int KC = HD / 32;                    // score products per 16 keys
+    constexpr int VP = HD == 64 ? 1 : HD / 128;    // pieces of a lane's V row
+    constexpr int PD = HD == 64 ? 4 : 8;           // dims of a piece
+    constexpr int VT = VP * PD;                    // products per 32 keys
+    __shared__ float part_o[kPagedWaves][kHeadTile][HD + 4];
+    __shared__ float part_ml[kPagedWaves][3][kHeadTile];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
+    const Part p = find_part<false>(a, blockIdx.x, lane);
+    if (!p.found) return;
+    const uint32_t group = a.n_heads / a.n_kv, tiles = (group + kHeadTile - 1) / kHeadTile;
+    const uint32_t kv = blockIdx.y / tiles, head0 = (blockIdx.y % tiles) * kHeadTile;
+    const uint32_t heads = min(kHeadTile, group - head0);  // this block's, from kv * group + head0
+    const uint64_t row0 = (static_cast<uint64_t>(p.seq) * a.n_heads + kv * group + head0) * HD;
+    const uint32_t keys = p.count ? a.positions[p.seq] + 1 : 0;
+    // this wavefront's keys: from .. to, in tiles of 32
+    const uint32_t from = (p.first * kPagedWaves + wave * p.count) * 32, to = min(from + p.count * 32, keys);
+    const uint32_t n_tiles = from < to ? (to - from + 31) / 32 : 0;
+
+    uint4 qf[KC];
+    const uint16_t *qrow = a.q + row0 + min(c & 7u, heads - 1) * HD + q * 8;
+#pragma unroll
+    for (int s = 0; s < KC; ++s) qf[s] = *reinterpret_cast<const uint4 *>(qrow + s * 32);
+
+    pa_f32x4_t acc[VT];
+#pragma unroll
+    for (int t = 0; t < VT; ++t) acc[t] = pa_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    bool any = false;
+    const float scale2 = a.scale * 1.4426950408889634f;
+    const uint32_t groups_pp = a.page_size / 16;
+
+    for (uint32_t t0 = 0; t0 < n_tiles; t0 += 32) {
+        // lane i: where the i-th 16-key group of the next 32 tiles lies, in
+        // groups from the pools' start; ~0 for none (past the keys, no page)
+        const uint32_t g = from / 16 + t0 * 2 + lane;
+        uint32_t where = ~0u;
+        if (g * 16 < to) {
+            const uint32_t pi = g / groups_pp;
+            const uint32_t page = a.page_table[static_cast<uint64_t>(p.seq) * a.max_pages + pi];
+            if (page < a.n_pages) where = (page * a.n_kv + kv) * groups_pp + (g - pi * groups_pp);
+        }
+        const uint32_t batch_tiles = min(32u, n_tiles - t0);
+        uint4 kf[2][KC];
+        uint4 vf[8][VP];
+        // a missing group reads the pool's first group, whose scores are left out
+        auto group_at = [&](uint32_t t, int half) {
+            const uint32_t w = __builtin_amdgcn_readlane(where, t * 2 + half);
+            return static_cast<uint64_t>(w == ~0u ? 0u : w) * (16 * HD);
+        };
+        auto load_k = [&](uint32_t t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint16_t *src = a.k_pages + group_at(t, h) + c * 32 + q * 8;
+#pragma unroll
+                for (int s = 0; s < KC; ++s) kf[h][s] = *reinterpret_cast<const uint4 *>(src + s * 512);
+            }
+        };
+        auto load_v = [&](uint32_t t) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint16_t *src = a.v_pages + group_at(t, i / 4) + (q * 4 + i % 4) * HD + c * PD;
+#pragma unroll
+                for (int u = 0; u < VP; ++u) {
+                    if constexpr (HD == 64) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(src);
+                        vf[i][u] = make_uint4(v.x, v.y, 0, 0);
+                    } else {
+                        vf[i][u] = *reinterpret_cast<const uint4 *>(src + u * 128);
+                    }
+                }
+            }
+        };
+        pa_f32x4_t s0, s1;
+        auto scores = [&] {
+            s0 = s1 = pa_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < KC; ++s) {
+                s0 = pa_mfma(kf[0][s], qf[s], s0);
+                s1 = pa_mfma(kf[1][s], qf[s], s1);
+            }
+        };
+        uint4 pf;
+        auto weigh = [&](uint32_t t) {
+            float s[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = s0[i] * scale2, s[4 + i] = s1[i] * scale2;
+            const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2), w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
+            const uint32_t key0 = from + (t0 + t) * 32;
+            if (w0 == ~0u || w1 == ~0u || key0 + 32 > to) {
+                // keys past the position or of no page: no score, and no value, whatever lies there
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t key = key0 + (i / 4) * 16 + q * 4 + i % 4;
+                    if (key >= to || (i < 4 ? w0 : w1) == ~0u) {
+                        s[i] = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < VP; ++u) vf[i][u] = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                any = any || w0 != ~0u || w1 != ~0u;
+            } else {
+                any = true;
+            }
+            float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float next = fmaxf(m, top);
+            const float ref = next == -INFINITY ? 0.0f : next;
+            if (__any(next != m)) {
+                const float keep = __builtin_amdgcn_exp2f(m - ref);
+                l *= keep;
+#pragma unroll
+                for (int t = 0; t < VT; ++t) acc[t] *= keep;
+            }
+            m = next;
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p0 = __builtin_amdgcn_exp2f(s[2 * i] - ref), p1 = __builtin_amdgcn_exp2f(s[2 * i + 1] - ref);
+                l += p0 + p1;
+                const uint32_t hi = f32x2_to_bf16x2_rne(p0, p1);
+                // what the rounding lost; nothing of an inf or NaN
+                const uint32_t lo = f32x2_to_bf16x2_rne(p0 - bf(hi & 0xFFFFu), p1 - bf(hi >> 16));
+                w[i] = c < 8 ? hi : lo;
+            }
+            pf = make_uint4(w[0], w[1], w[2], w[3]);
+        };
+        auto values = [&] {
+#pragma unroll
+            for (int t = 0; t < VT; ++t) {
+                const int u = t / PD, d = t % PD;
+                auto word = [&](int i) {
+                    const uint4 v = vf[i][u];
+                    return d / 2 == 0 ? v.x : d / 2 == 1 ? v.y : d / 2 == 2 ? v.z : v.w;
+                };
+                const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
+                const uint4 f = make_uint4(__builtin_amdgcn_perm(word(1), word(0), sel), __builtin_amdgcn_perm(word(3), word(2), sel),
+                                           __builtin_amdgcn_perm(word(5), word(4), sel), __builtin_amdgcn_perm(word(7), word(6), sel));
+                acc[t] = pa_mfma(f, pf, acc[t]);
+            }
+        };
+        // each tile's keys are in flight behind the values before them
+        load_k(0);
+        load_v(0);
+        for (uint32_t t = 0; t + 1 < batch_tiles; ++t) {
+            scores();
+            load_k(t + 1);
+            weigh(t);
+            values();
+            load_v(t + 1);
+        }
+        scores();
+        weigh(batch_tiles - 1);
+        values();
+    }
+
+    // the wavefront's result: l over its four key quarters, the two parts of P
+    // together (a sum that is inf or NaN already stays as it is)
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float lo = __shfl_xor(acc[t][r], 8, 64), hi = acc[t][r];
+            const int d = (t / PD) * 128 + (q * 4 + r) * PD + t % PD;
+            if (c < 8) part_o[wave][c][d] = fabsf(hi) < INFINITY ? hi + lo : hi;
+        }
+    if (lane < 8) {
+        part_ml[wave][0][c] = m;
+        part_ml[wave][1][c] = l;
+        part_ml[wave][2][c] = any ? 1.0f : 0.0f;
+    }
+    __syncthreads();
+
+    // the four joined: thread (head, dims)
+    constexpr int DT = kHeadTile * HD / kPagedThreads;  // dims of a thread
+    const uint32_t h = threadIdx.x / (HD / DT), d0 = threadIdx.x % (HD / DT) * DT;
+    float top = -INFINITY;
+    bool some = false;
+#pragma unroll
+    for (uint32_t w = 0; w < kPagedWaves; ++w) {
+        top = fmaxf(top, part_ml[w][0][h]);
+        some = some || part_ml[w][2][h] != 0.0f;
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < kPagedWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(part_ml[w][0][h] - ref);
+        sum = fmaf(f, part_ml[w][1][h], sum);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part_o[w][h][d0 + d], o[d]);
+    }
+    if (p.parts <= 1) {
+        if (h >= heads) return;
+        uint16_t *to = a.out + row0 + h * HD + d0;
+#pragma unroll
+        for (int d = 0; d < DT; d += 2)
+            *reinterpret_cast<uint32_t *>(to + d) = some ? f32x2_to_bf16x2_rne(o[d] / sum, o[d + 1] / sum) : 0u;
+        return;
+    }
+    float *rec = a.records + (static_cast<uint64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * record_floats<HD>();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) rec[h * HD + d0 + d] = o[d];
+    if (d0 == 0) {
+        rec[kHeadTile * HD + h] = top;
+        rec[kHeadTile * HD + kHeadTile + h] = sum;
+        rec[kHeadTile * HD + 2 * kHeadTile + h] = some ? 1.0f : 0.0f;
+    }
+}
+
+// Joins the parts of one sequence's query head: block (sequence, head). Rows of
+// HD / 4 threads take every (256 / that)-th part, then join in LDS in order.
+template <int HD>
+__global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedArgs a) {
+    constexpr uint32_t kRow = HD / 4, kRows = kPagedThreads / kRow;
+    __shared__ float rows_o[kRows][HD + 4];
+    __shared__ float rows_ml[kRows][3];
+    const uint32_t h = blockIdx.y, row = threadIdx.x / kRow, d = threadIdx.x % kRow * 4;
+    const Part p = find_part<true>(a, blockIdx.x, threadIdx.x & 63u);
+    if (p.parts == 1) return;  // written by its part
+    uint16_t *to = a.out + (static_cast<uint64_t>(blockIdx.x) * a.n_heads + h) * HD;
+    if (p.parts == 0) {
+        if (row == 0) *reinterpret_cast<uint2 *>(to + d) = make_uint2(0, 0);
+        return;
+    }
+    const uint32_t group = a.n_heads / a.n_kv, tiles = (group + kHeadTile - 1) / kHeadTile;
+    const uint32_t y = h / group * tiles + h % group / kHeadTile, slot = h % group % kHeadTile;
+    const uint64_t stride = static_cast<uint64_t>(a.n_kv) * tiles * record_floats<HD>();
+    const float *rec = a.records + p.base * stride + static_cast<uint64_t>(y) * record_floats<HD>();
+    float m = -INFINITY, l = 0.0f, some = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (uint32_t i = row; i < p.parts; i += kRows) {
+        const float *x = rec + i * stride;
+        const float pm = x[kHeadTile * HD + slot], pl = x[kHeadTile * HD + kHeadTile + slot];
+        some = fmaxf(some, x[kHeadTile * HD + 2 * kHeadTile + slot]);
+        const float4 v = *reinterpret_cast<const float4 *>(x + slot * HD + d);
+        const float next = fmaxf(m, pm), ref = next == -INFINITY ? 0.0f : next;
+        const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(pm - ref);
+        m = next;
+        l = l * f + pl * g;
+        o.x = o.x * f + v.x * g, o.y = o.y * f + v.y * g, o.z = o.z * f + v.z * g, o.w = o.w * f + v.w * g;
+    }
+    *reinterpret_cast<float4 *>(&rows_o[row][d]) = o;
+    if (d == 0) rows_ml[row][0] = m, rows_ml[row][1] = l, rows_ml[row][2] = some;
+    __syncthreads();
+    if (row != 0) return;
+    for (uint32_t r = 0; r < kRows; ++r) m = fmaxf(m, rows_ml[r][0]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    l = 0.0f, some = 0.0f;
+    o = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (uint32_t r = 0; r < kRows; ++r) {
+        const float f = __builtin_amdgcn_exp2f(rows_ml[r][0] - ref);
+        const float4 v = *reinterpret_cast<const float4 *>(&rows_o[r][d]);
+        l = fmaf(f, rows_ml[r][1], l);
+        some = fmaxf(some, rows_ml[r][2]);
+        o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+    }
+    *reinterpret_cast<uint2 *>(to + d) = some != 0.0f ? make_uint2(f32x2_to_bf16x2_rne(o.x / l, o.y / l),
+                                                                  f32x2_to_bf16x2_rne(o.z / l, o.w / l))
+                                                      : make_uint2(0, 0);
 }
 
 }  // namespace fh
@@ -80,6 +404,24 @@ int check_shape(const char *fn, int64_t batch, int64_t n_heads, int64_t n_kv, in
     return FH_OK;
 }
 
+// The launch for these sizes: parts wanted per (KV head, head tile), parts at
+// most, and the bytes of their records.
+struct Plan {
+    uint32_t want_parts, grid_parts, grid_heads;
+    uint64_t bytes;
+};
+
+Plan plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t page_size, int64_t max_pages) {
+    const uint64_t tiles = n_kv * ((n_heads / n_kv + kHeadTile - 1) / kHeadTile);
+    if (batch > kPlanBatch) return {0, static_cast<uint32_t>(batch), static_cast<uint32_t>(tiles), 16};
+    const uint64_t want = std::max<uint64_t>(1, kPartBlocks / tiles);
+    const uint64_t steps = (static_cast<uint64_t>(max_pages) * page_size + kStepKeys - 1) / kStepKeys;
+    const uint64_t parts = std::min<uint64_t>(want + batch, batch * steps);
+    const uint64_t record = (kHeadTile * head_dim + 3 * kHeadTile) * 4;
+    return {static_cast<uint32_t>(want), static_cast<uint32_t>(parts), static_cast<uint32_t>(tiles),
+            parts * tiles * record + 16};
+}
+
 }  // namespace
 
 extern "C" int fh_paged_attention_workspace(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
@@ -87,7 +429,7 @@ extern "C" int fh_paged_attention_workspace(int64_t batch, int64_t n_heads, int6
     const char *fn = "fh_paged_attention_workspace";
     if (bytes == nullptr) return fail(FH_ERR_INVALID_ARGUMENT, "%s: bytes is null", fn);
     if (int rc = check_shape(fn, batch, n_heads, n_kv, head_dim, page_size, max_pages)) return rc;
-    *bytes = 16;
+    *bytes = plan(batch, n_heads, n_kv, head_dim, page_size, max_pages).bytes;
     return FH_OK;
 }
 
@@ -127,11 +469,40 @@ extern "C" int fh_paged_attention(fh_device *dev, const uint16_t *q, int64_t bat
     }
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "out", out, rows)) return rc;
     if (int rc = set_current(dev, fn)) return rc;
+    const Plan w = plan(batch, n_heads, n_kv, head_dim, page_size, max_pages);
+    const PagedArgs a{q,
+                      k_pages,
+                      v_pages,
+                      page_table,
+                      positions,
+                      static_cast<uint32_t>(batch),
+                      static_cast<uint32_t>(n_heads),
+                      static_cast<uint32_t>(n_kv),
+                      static_cast<uint32_t>(n_pages),
+                      static_cast<uint32_t>(page_size),
+                      static_cast<uint32_t>(max_pages),
+                      w.want_parts,
+                      scale,
+                      static_cast<float *>(workspace),
+                      out};
+    const dim3 grid(w.grid_parts, w.grid_heads), threads(kPagedThreads);
+    if (int rc = dispatch(dev, fn, [&] {
+            if (head_dim == 64)
+                hipLaunchKernelGGL(paged_part_kernel<64>, grid, threads, 0, dev->stream, a);
+            else if (head_dim == 128)
+                hipLaunchKernelGGL(paged_part_kernel<128>, grid, threads, 0, dev->stream, a);
+            else
+                hipLaunchKernelGGL(paged_part_kernel<256>, grid, threads, 0, dev->stream, a);
+        }))
+        return rc;
+    if (w.want_parts == 0) return FH_OK;
+    const dim3 join(static_cast<uint32_t>(batch), static_cast<uint32_t>(n_heads));
     return dispatch(dev, fn, [&] {
-        hipLaunchKernelGGL(paged_attention_kernel, dim3(static_cast<uint32_t>(n_heads), static_cast<uint32_t>(batch)),
-                           dim3(kPagedThreads), 0, dev->stream, q, static_cast<uint32_t>(n_heads),
-                           static_cast<uint32_t>(n_kv), static_cast<uint32_t>(head_dim), k_pages, v_pages,
-                           static_cast<uint32_t>(n_pages), static_cast<uint32_t>(page_size), page_table,
-                           static_cast<uint32_t>(max_pages), positions, scale, out);
+        if (head_dim == 64)
+            hipLaunchKernelGGL(paged_join_kernel<64>, join, threads, 0, dev->stream, a);
+        else if (head_dim == 128)
+            hipLaunchKernelGGL(paged_join_kernel<128>, join, threads, 0, dev->stream, a);
+        else
+            hipLaunchKernelGGL(paged_join_kernel<256>, join, threads, 0, dev->stream, a);
     });
 }
