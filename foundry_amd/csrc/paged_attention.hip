@@ -33,9 +33,8 @@ constexpr uint32_t kPagedThreads = 256;
 constexpr uint32_t kPagedWaves = kPagedThreads / 64;
 constexpr uint32_t kStepKeys = 32 * kPagedWaves;
 constexpr uint32_t kHeadTile = 8;
-// Blocks that the parts of a batch aim for (the parts of one KV head and head
-// tile: that divided by their number).
-constexpr uint32_t kPartBlocks = 1024;
+// Blocks of a launch: what the GPU holds at once.
+constexpr uint32_t kPartBlocks = 512;
 // Larger batches take one part per sequence, laid out without a search.
 constexpr uint32_t kPlanBatch = 1024;
 
@@ -51,7 +50,7 @@ struct PagedArgs {
     const uint16_t *q, *k_pages, *v_pages;
     const uint32_t *page_table, *positions;
     uint32_t batch, n_heads, n_kv, n_pages, page_size, max_pages;
-    uint32_t want_parts;  // parts that one (KV head, head tile) aims for; 0: one per sequence
+    uint32_t want_parts;  // parts of one (KV head, head tile); 0: a block per sequence
     float scale;
     float *records;
     uint16_t *out;
@@ -71,44 +70,53 @@ __device__ __forceinline__ uint32_t scan_wave(uint32_t v, uint32_t lane) {
     return v;
 }
 
-// Where a part lies: steps first .. first + count - 1 of a sequence cut into
-// `parts` parts, whose records start at `base`.
-struct Part {
-    uint32_t seq, first, count, parts, base;
-    bool found;
+// The steps of all sequences, in order, are cut into equal parts, one per
+// block of a (KV head, head tile): part x takes steps x * size .. of them,
+// which may be the end of one sequence, whole ones, and the start of another.
+// Such a piece of sequence b in part x leaves record x + b: no two pieces
+// share one (a later piece has a larger x or b), and those of one sequence
+// follow each other. Every wavefront works the layout out for itself from the
+// positions, 64 sequences at a time.
+struct Layout {
+    uint32_t size;   // steps of a part
+    uint32_t b0;     // first sequence of the 64 at hand
+    uint32_t mine;   // lane's sequence's steps
+    uint32_t upto;   // and the batch's steps up to its end
 };
 
-// With P = ceil(all steps / want_parts), sequence b has ceil(steps_b / P)
-// parts, numbered through the batch: at most want_parts + batch in all. Every
-// wavefront works the numbering out for itself, 64 sequences at a time.
-// BY_SEQ: the parts of sequence `at` (count is then 0); else part number `at`.
-template <bool BY_SEQ>
-__device__ __forceinline__ Part find_part(const PagedArgs &a, uint32_t at, uint32_t lane) {
-    if (a.want_parts == 0) {
-        const uint32_t n = steps_of(a, at);
-        return {at, 0, n, n ? 1u : 0u, at, true};
-    }
-    uint32_t total = 0, mine = 0;
+__device__ __forceinline__ void layout_at(const PagedArgs &a, Layout &y, uint32_t b0, uint32_t before, uint32_t lane) {
+    y.b0 = b0;
+    y.mine = b0 + lane < a.batch ? steps_of(a, b0 + lane) : 0;
+    y.upto = before + scan_wave(y.mine, lane);
+}
+
+__device__ __forceinline__ Layout layout_of(const PagedArgs &a, uint32_t lane) {
+    Layout y;
+    uint32_t total = 0;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-        mine = b0 + lane < a.batch ? steps_of(a, b0 + lane) : 0;
-        total += __builtin_amdgcn_readlane(scan_wave(mine, lane), 63);
+        layout_at(a, y, b0, total, lane);
+        total = __builtin_amdgcn_readlane(y.upto, 63);
     }
-    const uint32_t size = max(1u, (total + a.want_parts - 1) / a.want_parts);
-    uint32_t base = 0;
-    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-        if (a.batch > 64) mine = b0 + lane < a.batch ? steps_of(a, b0 + lane) : 0;
-        const uint32_t parts = (mine + size - 1) / size, upto = scan_wave(parts, lane);
-        const uint64_t hit = BY_SEQ ? (at - b0 < 64 ? 1ull << (at - b0) : 0) : __ballot(at < base + upto);
+    y.size = max(1u, (total + a.want_parts - 1) / a.want_parts);
+    if (a.batch > 64) layout_at(a, y, 0, 0, lane);
+    return y;
+}
+
+// Moves to the sequence that holds step `at` of the batch and returns it, its
+// steps in n and the steps before it in `start`; ~0 behind the last one.
+__device__ __forceinline__ uint32_t sequence_of(const PagedArgs &a, Layout &y, uint32_t at, uint32_t lane, uint32_t &n,
+                                                uint32_t &start) {
+    for (;;) {
+        const uint64_t hit = __ballot(at < y.upto);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            const uint32_t n = __builtin_amdgcn_readlane(mine, l), k = __builtin_amdgcn_readlane(parts, l);
-            const uint32_t start = base + __builtin_amdgcn_readlane(upto, l) - k;
-            const uint32_t first = BY_SEQ ? 0 : (at - start) * size;
-            return {b0 + l, first, BY_SEQ ? 0 : min(size, n - first), k, start, true};
+            n = __builtin_amdgcn_readlane(y.mine, l);
+            start = __builtin_amdgcn_readlane(y.upto, l) - n;
+            return y.b0 + l;
         }
-        base += __builtin_amdgcn_readlane(upto, 63);
+        if (y.b0 + 64 >= a.batch) return ~0u;
+        layout_at(a, y, y.b0 + 64, __builtin_amdgcn_readlane(y.upto, 63), lane);
     }
-    return {0, 0, 0, 0, 0, false};
 }
 
 // A record: what a part leaves to be joined, [8 heads][HD] weighted values,
@@ -125,244 +133,296 @@ __global__ __launch_bounds__(kPagedThreads, HD == 256 ? 1 : 2) void paged_part_k
     __shared__ float part_o[kPagedWaves][kHeadTile][HD + 4];
     __shared__ float part_ml[kPagedWaves][3][kHeadTile];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
-    const Part p = find_part<false>(a, blockIdx.x, lane);
-    if (!p.found) return;
     const uint32_t group = a.n_heads / a.n_kv, tiles = (group + kHeadTile - 1) / kHeadTile;
     const uint32_t kv = blockIdx.y / tiles, head0 = (blockIdx.y % tiles) * kHeadTile;
     const uint32_t heads = min(kHeadTile, group - head0);  // this block's, from kv * group + head0
-    const uint64_t row0 = (static_cast<uint64_t>(p.seq) * a.n_heads + kv * group + head0) * HD;
-    const uint32_t keys = p.count ? a.positions[p.seq] + 1 : 0;
-    // this wavefront's keys: from .. to, in tiles of 32
-    const uint32_t from = (p.first * kPagedWaves + wave * p.count) * 32, to = min(from + p.count * 32, keys);
-    const uint32_t n_tiles = from < to ? (to - from + 31) / 32 : 0;
-
-    uint4 qf[KC];
-    const uint16_t *qrow = a.q + row0 + min(c & 7u, heads - 1) * HD + q * 8;
-#pragma unroll
-    for (int s = 0; s < KC; ++s) qf[s] = *reinterpret_cast<const uint4 *>(qrow + s * 32);
-
-    pa_f32x4_t acc[VT];
-#pragma unroll
-    for (int t = 0; t < VT; ++t) acc[t] = pa_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
-    bool any = false;
     const float scale2 = a.scale * 1.4426950408889634f;
     const uint32_t groups_pp = a.page_size / 16;
-
-    for (uint32_t t0 = 0; t0 < n_tiles; t0 += 32) {
-        // lane i: where the i-th 16-key group of the next 32 tiles lies, in
-        // groups from the pools' start; ~0 for none (past the keys, no page)
-        const uint32_t g = from / 16 + t0 * 2 + lane;
-        uint32_t where = ~0u;
-        if (g * 16 < to) {
-            const uint32_t pi = g / groups_pp;
-            const uint32_t page = a.page_table[static_cast<uint64_t>(p.seq) * a.max_pages + pi];
-            if (page < a.n_pages) where = (page * a.n_kv + kv) * groups_pp + (g - pi * groups_pp);
+    Layout y;
+    uint32_t at = 0, end = 1;
+    if (a.want_parts) {
+        y = layout_of(a, lane);
+        at = blockIdx.x * y.size;
+        end = at + y.size;
+    }
+    while (at < end) {
+        // the next piece: `count` steps from `first` of sequence seq
+        uint32_t seq = blockIdx.x, first = 0, count, whole = 1;
+        if (a.want_parts) {
+            uint32_t n, start;
+            seq = sequence_of(a, y, at, lane, n, start);
+            if (seq == ~0u) break;
+            first = at - start;
+            count = min(n - first, end - at);
+            whole = count == n;
+            at += count;
+        } else {
+            count = steps_of(a, seq);
+            at = end;
         }
-        const uint32_t batch_tiles = min(32u, n_tiles - t0);
-        uint4 kf[2][KC];
-        uint4 vf[8][VP];
-        // a missing group reads the pool's first group, whose scores are left out
-        auto group_at = [&](uint32_t t, int half) {
-            const uint32_t w = __builtin_amdgcn_readlane(where, t * 2 + half);
-            return static_cast<uint64_t>(w == ~0u ? 0u : w) * (16 * HD);
-        };
-        auto load_k = [&](uint32_t t) {
+        const uint64_t row0 = (static_cast<uint64_t>(seq) * a.n_heads + kv * group + head0) * HD;
+        const uint32_t keys = count ? a.positions[seq] + 1 : 0;
+        // this wavefront's keys: from .. to, in tiles of 32
+        const uint32_t from = (first * kPagedWaves + wave * count) * 32, to = min(from + count * 32, keys);
+        const uint32_t n_tiles = from < to ? (to - from + 31) / 32 : 0;
+
+        uint4 qf[KC];
+        const uint16_t *qrow = a.q + row0 + min(c & 7u, heads - 1) * HD + q * 8;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint16_t *src = a.k_pages + group_at(t, h) + c * 32 + q * 8;
+        for (int s = 0; s < KC; ++s) qf[s] = *reinterpret_cast<const uint4 *>(qrow + s * 32);
+
+        pa_f32x4_t acc[VT];
 #pragma unroll
-                for (int s = 0; s < KC; ++s) kf[h][s] = *reinterpret_cast<const uint4 *>(src + s * 512);
+        for (int t = 0; t < VT; ++t) acc[t] = pa_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        bool any = false;
+
+        for (uint32_t t0 = 0; t0 < n_tiles; t0 += 32) {
+            // lane i: where the i-th 16-key group of the next 32 tiles lies, in
+            // groups from the pools' start; ~0 for none (past the keys, no page)
+            const uint32_t g = from / 16 + t0 * 2 + lane;
+            uint32_t where = ~0u;
+            if (g * 16 < to) {
+                const uint32_t pi = g / groups_pp;
+                const uint32_t page = a.page_table[static_cast<uint64_t>(seq) * a.max_pages + pi];
+                if (page < a.n_pages) where = (page * a.n_kv + kv) * groups_pp + (g - pi * groups_pp);
             }
-        };
-        auto load_v = [&](uint32_t t) {
+            const uint32_t batch_tiles = min(32u, n_tiles - t0);
+            uint4 kf[2][KC];
+            uint4 vf[8][VP];
+            // a missing group reads the pool's first group, whose scores are left out
+            auto group_at = [&](uint32_t t, int half) {
+                const uint32_t w = __builtin_amdgcn_readlane(where, t * 2 + half);
+                return static_cast<uint64_t>(w == ~0u ? 0u : w) * (16 * HD);
+            };
+            auto load_k = [&](uint32_t t) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint16_t *src = a.v_pages + group_at(t, i / 4) + (q * 4 + i % 4) * HD + c * PD;
+                for (int h = 0; h < 2; ++h) {
+                    const uint16_t *src = a.k_pages + group_at(t, h) + c * 32 + q * 8;
 #pragma unroll
-                for (int u = 0; u < VP; ++u) {
-                    if constexpr (HD == 64) {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(src);
-                        vf[i][u] = make_uint4(v.x, v.y, 0, 0);
-                    } else {
-                        vf[i][u] = *reinterpret_cast<const uint4 *>(src + u * 128);
-                    }
+                    for (int s = 0; s < KC; ++s) kf[h][s] = load_stream16(reinterpret_cast<const uint4 *>(src + s * 512));
                 }
-            }
-        };
-        pa_f32x4_t s0, s1;
-        auto scores = [&] {
-            s0 = s1 = pa_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = 0; s < KC; ++s) {
-                s0 = pa_mfma(kf[0][s], qf[s], s0);
-                s1 = pa_mfma(kf[1][s], qf[s], s1);
-            }
-        };
-        uint4 pf;
-        auto weigh = [&](uint32_t t) {
-            float s[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = s0[i] * scale2, s[4 + i] = s1[i] * scale2;
-            const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2), w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
-            const uint32_t key0 = from + (t0 + t) * 32;
-            if (w0 == ~0u || w1 == ~0u || key0 + 32 > to) {
-                // keys past the position or of no page: no score, and no value, whatever lies there
+            };
+            auto load_v = [&](uint32_t t) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t key = key0 + (i / 4) * 16 + q * 4 + i % 4;
-                    if (key >= to || (i < 4 ? w0 : w1) == ~0u) {
-                        s[i] = -INFINITY;
+                    const uint16_t *src = a.v_pages + group_at(t, i / 4) + (q * 4 + i % 4) * HD + c * PD;
 #pragma unroll
-                        for (int u = 0; u < VP; ++u) vf[i][u] = make_uint4(0, 0, 0, 0);
+                    for (int u = 0; u < VP; ++u) {
+                        if constexpr (HD == 64) {
+                            const uint2 v = load_stream8(reinterpret_cast<const uint2 *>(src));
+                            vf[i][u] = make_uint4(v.x, v.y, 0, 0);
+                        } else {
+                            vf[i][u] = load_stream16(reinterpret_cast<const uint4 *>(src + u * 128));
+                        }
                     }
                 }
-                any = any || w0 != ~0u || w1 != ~0u;
-            } else {
-                any = true;
-            }
-            float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float next = fmaxf(m, top);
-            const float ref = next == -INFINITY ? 0.0f : next;
-            if (__any(next != m)) {
-                const float keep = __builtin_amdgcn_exp2f(m - ref);
-                l *= keep;
+            };
+            pa_f32x4_t s0, s1;
+            auto scores = [&] {
+                s0 = s1 = pa_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int t = 0; t < VT; ++t) acc[t] *= keep;
-            }
-            m = next;
-            uint32_t w[4];
+                for (int s = 0; s < KC; ++s) {
+                    s0 = pa_mfma(kf[0][s], qf[s], s0);
+                    s1 = pa_mfma(kf[1][s], qf[s], s1);
+                }
+            };
+            uint4 pf;
+            auto weigh = [&](uint32_t t) {
+                float s[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p0 = __builtin_amdgcn_exp2f(s[2 * i] - ref), p1 = __builtin_amdgcn_exp2f(s[2 * i + 1] - ref);
-                l += p0 + p1;
-                const uint32_t hi = f32x2_to_bf16x2_rne(p0, p1);
-                // what the rounding lost; nothing of an inf or NaN
-                const uint32_t lo = f32x2_to_bf16x2_rne(p0 - bf(hi & 0xFFFFu), p1 - bf(hi >> 16));
-                w[i] = c < 8 ? hi : lo;
-            }
-            pf = make_uint4(w[0], w[1], w[2], w[3]);
-        };
-        auto values = [&] {
+                for (int i = 0; i < 4; ++i) s[i] = s0[i] * scale2, s[4 + i] = s1[i] * scale2;
+                const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2), w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
+                const uint32_t key0 = from + (t0 + t) * 32;
+                if (w0 == ~0u || w1 == ~0u || key0 + 32 > to) {
+                    // keys past the position or of no page: no score, and no value, whatever lies there
 #pragma unroll
-            for (int t = 0; t < VT; ++t) {
-                const int u = t / PD, d = t % PD;
-                auto word = [&](int i) {
-                    const uint4 v = vf[i][u];
-                    return d / 2 == 0 ? v.x : d / 2 == 1 ? v.y : d / 2 == 2 ? v.z : v.w;
-                };
-                const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
-                const uint4 f = make_uint4(__builtin_amdgcn_perm(word(1), word(0), sel), __builtin_amdgcn_perm(word(3), word(2), sel),
-                                           __builtin_amdgcn_perm(word(5), word(4), sel), __builtin_amdgcn_perm(word(7), word(6), sel));
-                acc[t] = pa_mfma(f, pf, acc[t]);
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t key = key0 + (i / 4) * 16 + q * 4 + i % 4;
+                        if (key >= to || (i < 4 ? w0 : w1) == ~0u) {
+                            s[i] = -INFINITY;
+#pragma unroll
+                            for (int u = 0; u < VP; ++u) vf[i][u] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    any = any || w0 != ~0u || w1 != ~0u;
+                } else {
+                    any = true;
+                }
+                float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float next = fmaxf(m, top);
+                const float ref = next == -INFINITY ? 0.0f : next;
+                if (__any(next != m)) {
+                    const float keep = __builtin_amdgcn_exp2f(m - ref);
+                    l *= keep;
+#pragma unroll
+                    for (int t = 0; t < VT; ++t) acc[t] *= keep;
+                }
+                m = next;
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p0 = __builtin_amdgcn_exp2f(s[2 * i] - ref), p1 = __builtin_amdgcn_exp2f(s[2 * i + 1] - ref);
+                    l += p0 + p1;
+                    const uint32_t hi = f32x2_to_bf16x2_rne(p0, p1);
+                    // what the rounding lost; nothing of an inf or NaN
+                    const uint32_t lo = f32x2_to_bf16x2_rne(p0 - bf(hi & 0xFFFFu), p1 - bf(hi >> 16));
+                    w[i] = c < 8 ? hi : lo;
+                }
+                pf = make_uint4(w[0], w[1], w[2], w[3]);
+            };
+            auto values = [&] {
+#pragma unroll
+                for (int t = 0; t < VT; ++t) {
+                    const int u = t / PD, d = t % PD;
+                    auto word = [&](int i) {
+                        const uint4 v = vf[i][u];
+                        return d / 2 == 0 ? v.x : d / 2 == 1 ? v.y : d / 2 == 2 ? v.z : v.w;
+                    };
+                    const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
+                    const uint4 f = make_uint4(__builtin_amdgcn_perm(word(1), word(0), sel), __builtin_amdgcn_perm(word(3), word(2), sel),
+                                               __builtin_amdgcn_perm(word(5), word(4), sel), __builtin_amdgcn_perm(word(7), word(6), sel));
+                    acc[t] = pa_mfma(f, pf, acc[t]);
+                }
+            };
+            // each tile's keys are in flight behind the values before them
+            load_k(0);
+            load_v(0);
+            for (uint32_t t = 0; t + 1 < batch_tiles; ++t) {
+                scores();
+                load_k(t + 1);
+                weigh(t);
+                values();
+                load_v(t + 1);
             }
-        };
-        // each tile's keys are in flight behind the values before them
-        load_k(0);
-        load_v(0);
-        for (uint32_t t = 0; t + 1 < batch_tiles; ++t) {
             scores();
-            load_k(t + 1);
-            weigh(t);
+            weigh(batch_tiles - 1);
             values();
-            load_v(t + 1);
         }
-        scores();
-        weigh(batch_tiles - 1);
-        values();
-    }
 
-    // the wavefront's result: l over its four key quarters, the two parts of P
-    // together (a sum that is inf or NaN already stays as it is)
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+        // the wavefront's result: l over its four key quarters, the two parts of P
+        // together (a sum that is inf or NaN already stays as it is)
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
 #pragma unroll
-    for (int t = 0; t < VT; ++t)
+        for (int t = 0; t < VT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float lo = __shfl_xor(acc[t][r], 8, 64), hi = acc[t][r];
-            const int d = (t / PD) * 128 + (q * 4 + r) * PD + t % PD;
-            if (c < 8) part_o[wave][c][d] = fabsf(hi) < INFINITY ? hi + lo : hi;
+            for (int r = 0; r < 4; ++r) {
+                const float lo = __shfl_xor(acc[t][r], 8, 64), hi = acc[t][r];
+                const int d = (t / PD) * 128 + (q * 4 + r) * PD + t % PD;
+                if (c < 8) part_o[wave][c][d] = fabsf(hi) < INFINITY ? hi + lo : hi;
+            }
+        if (lane < 8) {
+            part_ml[wave][0][c] = m;
+            part_ml[wave][1][c] = l;
+            part_ml[wave][2][c] = any ? 1.0f : 0.0f;
         }
-    if (lane < 8) {
-        part_ml[wave][0][c] = m;
-        part_ml[wave][1][c] = l;
-        part_ml[wave][2][c] = any ? 1.0f : 0.0f;
-    }
-    __syncthreads();
+        __syncthreads();
 
-    // the four joined: thread (head, dims)
-    constexpr int DT = kHeadTile * HD / kPagedThreads;  // dims of a thread
-    const uint32_t h = threadIdx.x / (HD / DT), d0 = threadIdx.x % (HD / DT) * DT;
-    float top = -INFINITY;
-    bool some = false;
+        // the four joined: thread (head, dims)
+        constexpr int DT = kHeadTile * HD / kPagedThreads;  // dims of a thread
+        const uint32_t h = threadIdx.x / (HD / DT), d0 = threadIdx.x % (HD / DT) * DT;
+        float top = -INFINITY;
+        bool some = false;
 #pragma unroll
-    for (uint32_t w = 0; w < kPagedWaves; ++w) {
-        top = fmaxf(top, part_ml[w][0][h]);
-        some = some || part_ml[w][2][h] != 0.0f;
-    }
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, o[DT];
+        for (uint32_t w = 0; w < kPagedWaves; ++w) {
+            top = fmaxf(top, part_ml[w][0][h]);
+            some = some || part_ml[w][2][h] != 0.0f;
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, o[DT];
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = 0.0f;
+        for (int d = 0; d < DT; ++d) o[d] = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < kPagedWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(part_ml[w][0][h] - ref);
-        sum = fmaf(f, part_ml[w][1][h], sum);
+        for (uint32_t w = 0; w < kPagedWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(part_ml[w][0][h] - ref);
+            sum = fmaf(f, part_ml[w][1][h], sum);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part_o[w][h][d0 + d], o[d]);
-    }
-    if (p.parts <= 1) {
-        if (h >= heads) return;
-        uint16_t *to = a.out + row0 + h * HD + d0;
+            for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part_o[w][h][d0 + d], o[d]);
+        }
+        if (whole) {
+            if (h < heads) {
+                uint16_t *to = a.out + row0 + h * HD + d0;
 #pragma unroll
-        for (int d = 0; d < DT; d += 2)
-            *reinterpret_cast<uint32_t *>(to + d) = some ? f32x2_to_bf16x2_rne(o[d] / sum, o[d + 1] / sum) : 0u;
-        return;
-    }
-    float *rec = a.records + (static_cast<uint64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * record_floats<HD>();
+                for (int d = 0; d < DT; d += 2)
+                    *reinterpret_cast<uint32_t *>(to + d) = some ? f32x2_to_bf16x2_rne(o[d] / sum, o[d + 1] / sum) : 0u;
+            }
+        } else {
+            float *rec = a.records + (static_cast<uint64_t>(blockIdx.x + seq) * gridDim.y + blockIdx.y) * record_floats<HD>();
 #pragma unroll
-    for (int d = 0; d < DT; ++d) rec[h * HD + d0 + d] = o[d];
-    if (d0 == 0) {
-        rec[kHeadTile * HD + h] = top;
-        rec[kHeadTile * HD + kHeadTile + h] = sum;
-        rec[kHeadTile * HD + 2 * kHeadTile + h] = some ? 1.0f : 0.0f;
+            for (int d = 0; d < DT; ++d) rec[h * HD + d0 + d] = o[d];
+            if (d0 == 0) {
+                rec[kHeadTile * HD + h] = top;
+                rec[kHeadTile * HD + kHeadTile + h] = sum;
+                rec[kHeadTile * HD + 2 * kHeadTile + h] = some ? 1.0f : 0.0f;
+            }
+        }
+        __syncthreads();  // the LDS is read: the next piece may write it
     }
 }
 
-// Joins the parts of one sequence's query head: block (sequence, head). Rows of
-// HD / 4 threads take every (256 / that)-th part, then join in LDS in order.
+// Joins the pieces of one sequence's query head: block (sequence, head). Rows
+// of HD / 4 threads each take every (256 / that)-th piece, kJoinLoads of them
+// requested together, then join in LDS in order.
+constexpr int kJoinLoads = 8;
+
 template <int HD>
 __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedArgs a) {
     constexpr uint32_t kRow = HD / 4, kRows = kPagedThreads / kRow;
     __shared__ float rows_o[kRows][HD + 4];
     __shared__ float rows_ml[kRows][3];
-    const uint32_t h = blockIdx.y, row = threadIdx.x / kRow, d = threadIdx.x % kRow * 4;
-    const Part p = find_part<true>(a, blockIdx.x, threadIdx.x & 63u);
-    if (p.parts == 1) return;  // written by its part
-    uint16_t *to = a.out + (static_cast<uint64_t>(blockIdx.x) * a.n_heads + h) * HD;
-    if (p.parts == 0) {
+    const uint32_t h = blockIdx.y, row = threadIdx.x / kRow, d = threadIdx.x % kRow * 4, lane = threadIdx.x & 63u;
+    Layout y = layout_of(a, lane);
+    // this sequence among the 64 at hand, and the pieces that it was cut into
+    const uint32_t seq = blockIdx.x;
+    while (y.b0 + 64 <= seq) layout_at(a, y, y.b0 + 64, __builtin_amdgcn_readlane(y.upto, 63), lane);
+    const uint32_t n = __builtin_amdgcn_readlane(y.mine, seq - y.b0);
+    uint16_t *to = a.out + (static_cast<uint64_t>(seq) * a.n_heads + h) * HD;
+    if (n == 0) {  // idle
         if (row == 0) *reinterpret_cast<uint2 *>(to + d) = make_uint2(0, 0);
         return;
     }
+    const uint32_t start = __builtin_amdgcn_readlane(y.upto, seq - y.b0) - n;
+    const uint32_t first = start / y.size, pieces = (start + n - 1) / y.size - first + 1;
+    if (pieces == 1) return;  // written by its block
     const uint32_t group = a.n_heads / a.n_kv, tiles = (group + kHeadTile - 1) / kHeadTile;
-    const uint32_t y = h / group * tiles + h % group / kHeadTile, slot = h % group % kHeadTile;
+    const uint32_t slot = h % group % kHeadTile;
     const uint64_t stride = static_cast<uint64_t>(a.n_kv) * tiles * record_floats<HD>();
-    const float *rec = a.records + p.base * stride + static_cast<uint64_t>(y) * record_floats<HD>();
+    const float *rec = a.records + (first + seq) * stride +
+                       static_cast<uint64_t>(h / group * tiles + h % group / kHeadTile) * record_floats<HD>();
     float m = -INFINITY, l = 0.0f, some = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
-    for (uint32_t i = row; i < p.parts; i += kRows) {
-        const float *x = rec + i * stride;
-        const float pm = x[kHeadTile * HD + slot], pl = x[kHeadTile * HD + kHeadTile + slot];
-        some = fmaxf(some, x[kHeadTile * HD + 2 * kHeadTile + slot]);
-        const float4 v = *reinterpret_cast<const float4 *>(x + slot * HD + d);
-        const float next = fmaxf(m, pm), ref = next == -INFINITY ? 0.0f : next;
-        const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(pm - ref);
+    for (uint32_t i0 = row; i0 < pieces; i0 += kRows * kJoinLoads) {
+        float pm[kJoinLoads], pl[kJoinLoads], ps[kJoinLoads];
+        float4 v[kJoinLoads];
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u) {
+            const float *x = rec + min(i0 + u * kRows, pieces - 1) * stride;
+            pm[u] = x[kHeadTile * HD + slot];
+            pl[u] = x[kHeadTile * HD + kHeadTile + slot];
+            ps[u] = x[kHeadTile * HD + 2 * kHeadTile + slot];
+            v[u] = *reinterpret_cast<const float4 *>(x + slot * HD + d);
+        }
+        float next = m;
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u) {
+            if (i0 + u * kRows >= pieces) pm[u] = -INFINITY;
+            next = fmaxf(next, pm[u]);
+        }
+        const float ref = next == -INFINITY ? 0.0f : next, f = __builtin_amdgcn_exp2f(m - ref);
         m = next;
-        l = l * f + pl * g;
-        o.x = o.x * f + v.x * g, o.y = o.y * f + v.y * g, o.z = o.z * f + v.z * g, o.w = o.w * f + v.w * g;
+        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u)
+            if (i0 + u * kRows < pieces) {
+                const float g = __builtin_amdgcn_exp2f(pm[u] - ref);
+                some = fmaxf(some, ps[u]);
+                l = fmaf(pl[u], g, l);
+                o.x = fmaf(v[u].x, g, o.x), o.y = fmaf(v[u].y, g, o.y);
+                o.z = fmaf(v[u].z, g, o.z), o.w = fmaf(v[u].w, g, o.w);
+            }
     }
     *reinterpret_cast<float4 *>(&rows_o[row][d]) = o;
     if (d == 0) rows_ml[row][0] = m, rows_ml[row][1] = l, rows_ml[row][2] = some;
@@ -404,8 +464,8 @@ int check_shape(const char *fn, int64_t batch, int64_t n_heads, int64_t n_kv, in
     return FH_OK;
 }
 
-// The launch for these sizes: parts wanted per (KV head, head tile), parts at
-// most, and the bytes of their records.
+// The launch for these sizes: parts per (KV head, head tile), or 0 for a block
+// per sequence, the grid, and the bytes of the pieces' records.
 struct Plan {
     uint32_t want_parts, grid_parts, grid_heads;
     uint64_t bytes;
@@ -414,12 +474,12 @@ struct Plan {
 Plan plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t page_size, int64_t max_pages) {
     const uint64_t tiles = n_kv * ((n_heads / n_kv + kHeadTile - 1) / kHeadTile);
     if (batch > kPlanBatch) return {0, static_cast<uint32_t>(batch), static_cast<uint32_t>(tiles), 16};
-    const uint64_t want = std::max<uint64_t>(1, kPartBlocks / tiles);
+    // a table of few steps has no use for more parts than steps
     const uint64_t steps = (static_cast<uint64_t>(max_pages) * page_size + kStepKeys - 1) / kStepKeys;
-    const uint64_t parts = std::min<uint64_t>(want + batch, batch * steps);
+    const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>(kPartBlocks / tiles, batch * steps));
     const uint64_t record = (kHeadTile * head_dim + 3 * kHeadTile) * 4;
-    return {static_cast<uint32_t>(want), static_cast<uint32_t>(parts), static_cast<uint32_t>(tiles),
-            parts * tiles * record + 16};
+    return {static_cast<uint32_t>(parts), static_cast<uint32_t>(parts), static_cast<uint32_t>(tiles),
+            (parts + batch) * tiles * record + 16};
 }
 
 }  // namespace
