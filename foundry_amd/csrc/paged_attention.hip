@@ -30,11 +30,16 @@ namespace fh {
 // bf16, columns 8..15 what that rounding lost, so that P V has 16 bits of P at
 // the cost of none (the columns would idle).
 constexpr uint32_t kPagedThreads = 256;
-constexpr uint32_t kPagedWaves = kPagedThreads / 64;
-constexpr uint32_t kStepKeys = 32 * kPagedWaves;
+constexpr uint32_t kStepKeys = 128;
 constexpr uint32_t kHeadTile = 8;
 // Blocks of a launch: what the GPU holds at once.
 constexpr uint32_t kPartBlocks = 512;
+// Tables of so few positions (times head_dim) take one block per sequence, of 8
+// wavefronts (4 at head_dim 256), and no join: one launch. One sequence of 500
+// keys of 128: 8.5 us against 10.1 split, of 1000: 14.2 against 10.7; of 1000
+// keys of 64: 9.1 against 9.2, of 1500: 11.3 against 9.2; of 300 of 256: 11.2
+// against 12.3, of 500: 13.3 against 12.6. 48 sequences: even up to 4000 keys.
+constexpr uint32_t kWholeElements = 65536;
 // Larger batches take one part per sequence, laid out without a search.
 constexpr uint32_t kPlanBatch = 1024;
 
@@ -124,14 +129,14 @@ __device__ __forceinline__ uint32_t sequence_of(const PagedArgs &a, Layout &y, u
 template <int HD>
 constexpr uint32_t record_floats() { return kHeadTile * HD + 3 * kHeadTile; }
 
-template <int HD>
-__global__ __launch_bounds__(kPagedThreads, HD == 256 ? 1 : 2) void paged_part_kernel(const PagedArgs a) {
+template <int HD, int W>
+__global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(const PagedArgs a) {
     constexpr int KC = HD / 32;                    // score products per 16 keys
     constexpr int VP = HD == 64 ? 1 : HD / 128;    // pieces of a lane's V row
     constexpr int PD = HD == 64 ? 4 : 8;           // dims of a piece
     constexpr int VT = VP * PD;                    // products per 32 keys
-    __shared__ float part_o[kPagedWaves][kHeadTile][HD + 4];
-    __shared__ float part_ml[kPagedWaves][3][kHeadTile];
+    __shared__ float part_o[W][kHeadTile][HD + 4];
+    __shared__ float part_ml[W][3][kHeadTile];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
     const uint32_t group = a.n_heads / a.n_kv, tiles = (group + kHeadTile - 1) / kHeadTile;
     const uint32_t kv = blockIdx.y / tiles, head0 = (blockIdx.y % tiles) * kHeadTile;
@@ -163,7 +168,8 @@ __global__ __launch_bounds__(kPagedThreads, HD == 256 ? 1 : 2) void paged_part_k
         const uint64_t row0 = (static_cast<uint64_t>(seq) * a.n_heads + kv * group + head0) * HD;
         const uint32_t keys = count ? a.positions[seq] + 1 : 0;
         // this wavefront's keys: from .. to, in tiles of 32
-        const uint32_t from = (first * kPagedWaves + wave * count) * 32, to = min(from + count * 32, keys);
+        const uint32_t share = (count * (kStepKeys / 32) + W - 1) / W * 32;
+        const uint32_t from = first * kStepKeys + wave * share, to = min(from + share, min(keys, (first + count) * kStepKeys));
         const uint32_t n_tiles = from < to ? (to - from + 31) / 32 : 0;
 
         uint4 qf[KC];
@@ -322,12 +328,13 @@ __global__ __launch_bounds__(kPagedThreads, HD == 256 ? 1 : 2) void paged_part_k
         __syncthreads();
 
         // the four joined: thread (head, dims)
-        constexpr int DT = kHeadTile * HD / kPagedThreads;  // dims of a thread
-        const uint32_t h = threadIdx.x / (HD / DT), d0 = threadIdx.x % (HD / DT) * DT;
+        constexpr int DT = std::max<int>(2, kHeadTile * HD / (64 * W));  // dims of a thread
+        const uint32_t own = threadIdx.x / (HD / DT), h = min(own, kHeadTile - 1);
+        const uint32_t d0 = threadIdx.x % (HD / DT) * DT;
         float top = -INFINITY;
         bool some = false;
 #pragma unroll
-        for (uint32_t w = 0; w < kPagedWaves; ++w) {
+        for (uint32_t w = 0; w < W; ++w) {
             top = fmaxf(top, part_ml[w][0][h]);
             some = some || part_ml[w][2][h] != 0.0f;
         }
@@ -336,21 +343,22 @@ __global__ __launch_bounds__(kPagedThreads, HD == 256 ? 1 : 2) void paged_part_k
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < kPagedWaves; ++w) {
+        for (uint32_t w = 0; w < W; ++w) {
             const float f = __builtin_amdgcn_exp2f(part_ml[w][0][h] - ref);
             sum = fmaf(f, part_ml[w][1][h], sum);
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part_o[w][h][d0 + d], o[d]);
         }
         if (whole) {
-            if (h < heads) {
+            if (own < heads) {
                 uint16_t *to = a.out + row0 + h * HD + d0;
 #pragma unroll
                 for (int d = 0; d < DT; d += 2)
                     *reinterpret_cast<uint32_t *>(to + d) = some ? f32x2_to_bf16x2_rne(o[d] / sum, o[d + 1] / sum) : 0u;
             }
-        } else {
-            float *rec = a.records + (static_cast<uint64_t>(blockIdx.x + seq) * gridDim.y + blockIdx.y) * record_floats<HD>();
+        } else if (own < kHeadTile) {
+            float *rec =
+                a.records + (static_cast<uint64_t>(blockIdx.x + seq) * gridDim.y + blockIdx.y) * record_floats<HD>();
 #pragma unroll
             for (int d = 0; d < DT; ++d) rec[h * HD + d0 + d] = o[d];
             if (d0 == 0) {
@@ -469,17 +477,21 @@ int check_shape(const char *fn, int64_t batch, int64_t n_heads, int64_t n_kv, in
 struct Plan {
     uint32_t want_parts, grid_parts, grid_heads;
     uint64_t bytes;
+    bool wide;  // 8 wavefronts to a block, where each takes a whole sequence
 };
 
 Plan plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t page_size, int64_t max_pages) {
     const uint64_t tiles = n_kv * ((n_heads / n_kv + kHeadTile - 1) / kHeadTile);
-    if (batch > kPlanBatch) return {0, static_cast<uint32_t>(batch), static_cast<uint32_t>(tiles), 16};
+    const uint64_t capacity = static_cast<uint64_t>(max_pages) * page_size;
+    const bool whole = capacity * head_dim <= kWholeElements;
+    if (batch > kPlanBatch || whole)
+        return {0, static_cast<uint32_t>(batch), static_cast<uint32_t>(tiles), 16, whole};
     // a table of few steps has no use for more parts than steps
-    const uint64_t steps = (static_cast<uint64_t>(max_pages) * page_size + kStepKeys - 1) / kStepKeys;
+    const uint64_t steps = (capacity + kStepKeys - 1) / kStepKeys;
     const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>(kPartBlocks / tiles, batch * steps));
     const uint64_t record = (kHeadTile * head_dim + 3 * kHeadTile) * 4;
     return {static_cast<uint32_t>(parts), static_cast<uint32_t>(parts), static_cast<uint32_t>(tiles),
-            (parts + batch) * tiles * record + 16};
+            (parts + batch) * tiles * record + 16, false};
 }
 
 }  // namespace
@@ -545,14 +557,18 @@ extern "C" int fh_paged_attention(fh_device *dev, const uint16_t *q, int64_t bat
                       scale,
                       static_cast<float *>(workspace),
                       out};
-    const dim3 grid(w.grid_parts, w.grid_heads), threads(kPagedThreads);
+    const dim3 grid(w.grid_parts, w.grid_heads), threads(kPagedThreads), wide(2 * kPagedThreads);
     if (int rc = dispatch(dev, fn, [&] {
-            if (head_dim == 64)
-                hipLaunchKernelGGL(paged_part_kernel<64>, grid, threads, 0, dev->stream, a);
+            if (head_dim == 256)
+                hipLaunchKernelGGL((paged_part_kernel<256, 4>), grid, threads, 0, dev->stream, a);
+            else if (head_dim == 128 && w.wide)
+                hipLaunchKernelGGL((paged_part_kernel<128, 8>), grid, wide, 0, dev->stream, a);
             else if (head_dim == 128)
-                hipLaunchKernelGGL(paged_part_kernel<128>, grid, threads, 0, dev->stream, a);
+                hipLaunchKernelGGL((paged_part_kernel<128, 4>), grid, threads, 0, dev->stream, a);
+            else if (w.wide)
+                hipLaunchKernelGGL((paged_part_kernel<64, 8>), grid, wide, 0, dev->stream, a);
             else
-                hipLaunchKernelGGL(paged_part_kernel<256>, grid, threads, 0, dev->stream, a);
+                hipLaunchKernelGGL((paged_part_kernel<64, 4>), grid, threads, 0, dev->stream, a);
         }))
         return rc;
     if (w.want_parts == 0) return FH_OK;

@@ -205,10 +205,11 @@ def test_attention_many_ragged_sequences(device):
     check_attention(device, *cache(77, lens, 4, 1, 64, 16), 64 ** -0.5)
 
 
-def test_attention_more_sequences_than_one_layout_holds(device):
+@pytest.mark.parametrize("width", [8, 80])
+def test_attention_more_sequences_than_one_layout_holds(device, width):
     """Past 1024 sequences each is a part of its own."""
     lens = [(i * 31) % 70 if i % 13 else 0 for i in range(1100)]
-    check_attention(device, *cache(79, lens, 2, 1, 64, 16), 64 ** -0.5)
+    check_attention(device, *cache(79, lens, 2, 1, 64, 16, width=width), 64 ** -0.5)
 
 
 def test_attention_a_wide_table_of_short_sequences(device):
