@@ -1,53 +1,382 @@
 // Low-rank adapters of many requests beside a shared projection (fh_lora_add).
+#include <algorithm>
 #include <tuple>
+#include <type_traits>
 
 #include "serving_checks.hpp"
 
 namespace fh {
 
-// v[i, r] = scales[a] * sum_j x[i, j] A_a[r, j]: one block per row, a
-// wavefront per rank at a time.
-__global__ __launch_bounds__(256) void lora_down_kernel(const uint16_t *__restrict__ x, uint32_t k, uint64_t x_ld,
-                                                        const uint16_t *__restrict__ a,
-                                                        const float *__restrict__ scales, uint32_t n_adapters,
-                                                        uint32_t rank, const uint32_t *__restrict__ adapters,
-                                                        float *__restrict__ v) {
-    const uint32_t i = blockIdx.x, id = adapters[i], lane = threadIdx.x & 63u;
-    if (id >= n_adapters) return;
-    for (uint32_t r = threadIdx.x >> 6; r < rank; r += 4) {
-        const uint16_t *ar = a + (static_cast<uint64_t>(id) * rank + r) * k;
-        float sum = 0.0f;
-        for (uint32_t j = lane; j < k; j += 64) sum = fmaf(bf(x[i * x_ld + j]), bf(ar[j]), sum);
-        sum = wave_sum(sum);
-        if (lane == 0) v[static_cast<uint64_t>(i) * rank + r] = sum * scales[id];
+// The mathematics: y = base + (scale x A^T) B^T per row, with A, B and scale of
+// the row's adapter. Two launches, since every column of y needs all of v =
+// scale x A^T: lora_down_kernel leaves v's sums over ranges of k in the
+// workspace, lora_up_kernel adds them in order and goes on to y. Both are bound
+// by memory: x, base and y go through once, an adapter's A and B once per
+// window of rows that uses it.
+//
+// Grouping: rows come with their adapters in any order, so a block takes a
+// window of rows (64, or 256) and finds in it the groups of rows that share an
+// adapter, by ballots over the adapter ids; each group is cut into chunks of
+// up to 64 rows, and a block takes every (number of slots)-th chunk. Whatever
+// the order, the products run on the matrix cores with the adapter's rows read
+// once for up to 64 rows (four tiles of 16).
+typedef __attribute__((ext_vector_type(8))) __bf16 lo_bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) float lo_f32x4_t;
+
+__device__ __forceinline__ lo_f32x4_t lo_mfma(uint4 a, uint4 b, lo_f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lo_bf16x8_t, a),
+                                                   __builtin_bit_cast(lo_bf16x8_t, b), c, 0, 0, 0);
+}
+
+// Blocks of 64 rows and a range of k that the down product aims for, the ranges
+// at most, and the least steps of 32 k that a wavefront takes.
+constexpr uint32_t kDownBlocks = 512, kMaxSplits = 16, kDownSteps = 2;
+// Rows up to which a window is 256 rows (and an adapter that they share is
+// read once for all of them).
+constexpr uint32_t kWideRows = 1024;
+// Blocks that the chunks of the windows are spread over, down and up.
+constexpr uint32_t kDownSlots = 1024, kUpSlots = 2048;
+constexpr uint32_t kLoraThreads = 256;
+constexpr uint32_t kLoraWaves = kLoraThreads / 64;
+constexpr uint32_t kLoraCols = 64 * kLoraWaves;  // columns of an up block
+
+// Calls take(adapter, rows, list) for each chunk that falls to `slot`: the
+// chunk's rows are list[0..rows) (in the window). list: this wavefront's
+// 64 * Q entries of LDS. Every wavefront of a block goes through the same
+// chunks.
+template <int Q, typename Take>
+__device__ __forceinline__ void for_chunks(const uint32_t *adapters, uint32_t row0, uint32_t m, uint32_t n_adapters,
+                                           uint32_t slot, uint32_t slots, uint32_t lane, uint8_t *list, Take take) {
+    uint32_t id[Q];
+    uint64_t left[Q];
+#pragma unroll
+    for (int w = 0; w < Q; ++w) {
+        const uint32_t row = row0 + w * 64 + lane;
+        id[w] = row < m ? adapters[row] : ~0u;
+        left[w] = __ballot(id[w] < n_adapters);
+    }
+    for (uint32_t item = 0;;) {
+        uint32_t group = ~0u;
+#pragma unroll
+        for (int w = Q - 1; w >= 0; --w)
+            if (left[w]) group = __builtin_amdgcn_readlane(id[w], __builtin_ctzll(left[w]));
+        if (group == ~0u) return;
+        uint64_t mask[Q];
+        uint32_t rows = 0;
+#pragma unroll
+        for (int w = 0; w < Q; ++w) {
+            mask[w] = __ballot(id[w] == group);
+            left[w] &= ~mask[w];
+            rows += __builtin_popcountll(mask[w]);
+        }
+        bool listed = false;
+        for (uint32_t r = 0; r < rows; r += 64, ++item) {
+            if (item % slots != slot) continue;
+            if (!listed) {
+                uint32_t before = 0;
+#pragma unroll
+                for (int w = 0; w < Q; ++w) {
+                    if (mask[w] >> lane & 1)
+                        list[before + __builtin_popcountll(mask[w] & ((1ull << lane) - 1))] =
+                            static_cast<uint8_t>(w * 64 + lane);
+                    before += __builtin_popcountll(mask[w]);
+                }
+                __builtin_amdgcn_wave_barrier();
+                listed = true;
+            }
+            take(group, min(rows - r, 64u), list + r);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
-// y[i, c] = base[i, c] + sum_r v[i, r] B_a[c, r]: a thread per column.
-template <typename T>
-__global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ v, const uint16_t *__restrict__ b,
-                                                      uint32_t n_adapters, uint32_t rank, uint32_t n,
-                                                      const uint32_t *__restrict__ adapters, const T *base,
-                                                      uint64_t base_ld, T *y, uint64_t y_ld) {
-    const uint32_t i = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x, id = adapters[i];
-    if (c >= n) return;
-    constexpr bool kBf16 = sizeof(T) == 2;
-    if (id >= n_adapters) {
-        y[i * y_ld + c] = base[i * base_ld + c];
-        return;
+// v[split][row][r] = sum over the split's k of x[row, k] A[r, k]. Block (slot,
+// split, window); its wavefronts take a quarter of the split's k each and add
+// up in LDS in their order. RT row tiles of 16, NR rank tiles of 16; a product
+// has the rank along its rows, so that a lane ends up with 4 ranks of a row.
+template <int RT, int NR>
+__device__ __forceinline__ void lora_down_chunk(const uint16_t *x, uint32_t k, uint64_t x_ld, const uint16_t *a,
+                                                uint32_t rank, uint32_t k0, uint32_t k1, uint32_t row0, uint32_t rows,
+                                                const uint8_t *list, float4 *sums, float *v, uint32_t lane,
+                                                uint32_t wave) {
+    constexpr int U = RT * NR >= 16 ? 2 : 4;  // steps of 32 requested together
+    const uint32_t c = lane & 15u, q = lane >> 4;
+    const uint16_t *xr[RT], *ar[NR];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) xr[t] = x + (row0 + list[min(t * 16 + c, rows - 1)]) * x_ld;
+#pragma unroll
+    for (int t = 0; t < NR; ++t) ar[t] = a + static_cast<uint64_t>(min(t * 16 + c, rank - 1)) * k;
+    lo_f32x4_t acc[RT][NR];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) acc[t][r] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t s = k0; s < k1; s += 32 * U) {
+        uint4 xf[U][RT], af[U][NR];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t at = min(s + u * 32 + q * 8, k - 8);  // clamped: the pieces past k1 are zeroed below
+#pragma unroll
+            for (int t = 0; t < RT; ++t) xf[u][t] = *reinterpret_cast<const uint4 *>(xr[t] + at);
+#pragma unroll
+            for (int t = 0; t < NR; ++t) af[u][t] = *reinterpret_cast<const uint4 *>(ar[t] + at);
+        }
+        if (s + 32 * U > k1) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s + u * 32 + q * 8 >= k1) {
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) xf[u][t] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < NR; ++t) af[u][t] = make_uint4(0, 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) acc[t][r] = lo_mfma(af[u][r], xf[u][t], acc[t][r]);
     }
-    float sum = 0.0f;
-    for (uint32_t r = 0; r < rank; ++r)
-        sum = fmaf(v[static_cast<uint64_t>(i) * rank + r], bf(b[(static_cast<uint64_t>(id) * n + c) * rank + r]), sum);
-    if constexpr (kBf16)
-        y[i * y_ld + c] = rne(bf(base[i * base_ld + c]) + sum);
-    else
-        y[i * y_ld + c] = base[i * base_ld + c] + sum;
+    // wavefront w adds to what those before it left; the last one's sums go out
+    for (uint32_t w = 0; w < kLoraWaves; ++w) {
+        if (w == wave) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const lo_f32x4_t p = acc[t][r];
+                    float4 f = make_float4(p[0], p[1], p[2], p[3]);
+                    if (w) {
+                        const float4 o = sums[(t * NR + r) * 64 + lane];
+                        f = make_float4(o.x + f.x, o.y + f.y, o.z + f.z, o.w + f.w);
+                    }
+                    if (w + 1 < kLoraWaves) {
+                        sums[(t * NR + r) * 64 + lane] = f;
+                    } else if (t * 16 + c < rows && r * 16 + q * 4 < rank) {
+                        const uint64_t row = row0 + list[t * 16 + c];
+                        *reinterpret_cast<float4 *>(v + row * rank + r * 16 + q * 4) = f;
+                    }
+                }
+        }
+        __syncthreads();
+    }
+}
+
+template <int Q, int NR>
+__global__ __launch_bounds__(kLoraThreads) void lora_down_kernel(const uint16_t *__restrict__ x, uint32_t m, uint32_t k,
+                                                                 uint64_t x_ld, const uint16_t *__restrict__ a,
+                                                                 uint32_t n_adapters, uint32_t rank,
+                                                                 const uint32_t *__restrict__ adapters, uint32_t steps,
+                                                                 float *__restrict__ v) {
+    __shared__ uint8_t lists[kLoraWaves][64 * Q];
+    __shared__ float4 sums[4 * NR * 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.z * 64 * Q;
+    // steps: of 32 k, of each wavefront
+    const uint32_t k0 = min((blockIdx.y * kLoraWaves + wave) * steps * 32, k), k1 = min(k0 + steps * 32, k);
+    v += static_cast<uint64_t>(blockIdx.y) * m * rank;
+    for_chunks<Q>(adapters, row0, m, n_adapters, blockIdx.x, gridDim.x, lane, lists[wave],
+                  [&](uint32_t id, uint32_t rows, const uint8_t *list) {
+                      const uint16_t *au = a + static_cast<uint64_t>(id) * rank * k;
+                      if (rows <= 16)
+                          lora_down_chunk<1, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, list, sums, v, lane, wave);
+                      else
+                          lora_down_chunk<4, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, list, sums, v, lane, wave);
+                  });
+}
+
+// 16 neighbouring values of a row of base or y, `count` of them in the matrix;
+// vec: rows and columns keep 16-byte alignment.
+template <typename T>
+__device__ __forceinline__ void load16(const T *p, uint32_t count, bool vec, float (&f)[16]) {
+    if (vec && count >= 16) {
+        if constexpr (sizeof(T) == 2) {
+            float h[8];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                unpack8(*reinterpret_cast<const uint4 *>(p + i * 8), h);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[i * 8 + e] = h[e];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 h = *reinterpret_cast<const float4 *>(p + i * 4);
+                f[i * 4] = h.x, f[i * 4 + 1] = h.y, f[i * 4 + 2] = h.z, f[i * 4 + 3] = h.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 16; ++e) {
+            f[e] = 0.0f;
+            if (e < count) {
+                if constexpr (sizeof(T) == 2)
+                    f[e] = bf(p[e]);
+                else
+                    f[e] = p[e];
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store16(T *p, uint32_t count, bool vec, const float (&f)[16]) {
+    if (vec && count >= 16) {
+        if constexpr (sizeof(T) == 2) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = f32x2_to_bf16x2_rne(f[2 * e], f[2 * e + 1]);
+            reinterpret_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                reinterpret_cast<float4 *>(p)[i] = make_float4(f[i * 4], f[i * 4 + 1], f[i * 4 + 2], f[i * 4 + 3]);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 16; ++e)
+            if (e < count) {
+                if constexpr (sizeof(T) == 2)
+                    p[e] = rne(f[e]);
+                else
+                    p[e] = f[e];
+            }
+    }
+}
+
+// y = base + v B^T of one chunk and this wavefront's 64 columns. A product has
+// 16 of the columns along its rows, taken so that a lane ends up with 16
+// neighbouring columns of a row over the four products. vs holds each row's v
+// in two bf16 parts, [row][2][rank]: along a product's 32 terms lie 16 ranks,
+// 8 at a time as (first part, second part), so that 16 bits of v take part.
+template <typename T, int RT, int NJ>
+__device__ __forceinline__ void lora_up_chunk(const uint16_t *b, uint32_t rank, uint32_t n, const T *base,
+                                              uint64_t base_ld, T *y, uint64_t y_ld, bool vec, uint32_t row0,
+                                              uint32_t rows, const uint8_t *list, const uint16_t *vs, uint32_t vs_ld,
+                                              uint32_t col0, uint32_t lane) {
+    const uint32_t c = lane & 15u, q = lane >> 4;
+    uint4 bfr[4][NJ];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const uint16_t *br = b + static_cast<uint64_t>(min(col0 + c / 4 * 16 + t * 4 + c % 4, n - 1)) * rank;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const uint32_t r = (2 * j + q / 2) * 8;
+            bfr[t][j] = *reinterpret_cast<const uint4 *>(br + min(r, rank - 8));
+            if (r >= rank) bfr[t][j] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    const uint32_t col = col0 + q * 16, count = col < n ? n - col : 0;
+    float f[RT][16];
+    uint64_t row[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        row[t] = row0 + list[min(t * 16 + c, rows - 1)];
+        load16(base + row[t] * base_ld + (count ? col : 0), count, vec, f[t]);
+    }
+    __syncthreads();  // vs is written
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        lo_f32x4_t acc[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[u] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const uint32_t r = (2 * j + q / 2) * 8;
+            uint4 vf = *reinterpret_cast<const uint4 *>(vs + min(t * 16 + c, rows - 1) * vs_ld + (q & 1) * rank +
+                                                        min(r, rank - 8));
+            if (r >= rank) vf = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[u] = lo_mfma(bfr[u][j], vf, acc[u]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[t][e] += acc[e / 4][e % 4];
+        if (t * 16 + c < rows && count) store16(y + row[t] * y_ld + col, count, vec, f[t]);
+    }
+}
+
+// Block (columns, slot, window).
+template <typename T, int Q, int NJ>
+__global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__restrict__ v, uint32_t splits, uint32_t m,
+                                                               const uint16_t *__restrict__ b,
+                                                               const float *__restrict__ scales, uint32_t n_adapters,
+                                                               uint32_t rank, uint32_t n,
+                                                               const uint32_t *__restrict__ adapters, const T *base,
+                                                               uint64_t base_ld, T *y, uint64_t y_ld, bool vec) {
+    __shared__ uint8_t lists[kLoraWaves][64 * Q];
+    __shared__ __attribute__((aligned(16))) uint16_t vs[64 * (2 * 16 * NJ + 8)];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.z * 64 * Q;
+    const uint32_t col0 = blockIdx.x * kLoraCols + wave * 64, vs_ld = 2 * rank + 8, quads = rank / 4;
+    for_chunks<Q>(adapters, row0, m, n_adapters, blockIdx.y, gridDim.y, lane, lists[wave],
+                  [&](uint32_t id, uint32_t rows, const uint8_t *list) {
+                      const float scale = scales[id];
+                      for (uint32_t i = threadIdx.x; i < rows * quads; i += kLoraThreads) {
+                          const uint32_t member = i / quads, r = i % quads * 4;
+                          const float *p = v + static_cast<uint64_t>(row0 + list[member]) * rank + r;
+                          float4 s = *reinterpret_cast<const float4 *>(p);
+                          for (uint32_t u = 1; u < splits; ++u) {
+                              const float4 o = *reinterpret_cast<const float4 *>(p + static_cast<uint64_t>(u) * m * rank);
+                              s = make_float4(s.x + o.x, s.y + o.y, s.z + o.z, s.w + o.w);
+                          }
+                          const float f[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
+                          uint32_t hi[2], lo[2];
+#pragma unroll
+                          for (int e = 0; e < 2; ++e) {
+                              hi[e] = f32x2_to_bf16x2_rne(f[2 * e], f[2 * e + 1]);
+                              // what the rounding lost; nothing where it is inf or NaN
+                              const float h0 = bf(hi[e] & 0xFFFFu), h1 = bf(hi[e] >> 16);
+                              lo[e] = f32x2_to_bf16x2_rne(fabsf(h0) < INFINITY ? f[2 * e] - h0 : 0.0f,
+                                                          fabsf(h1) < INFINITY ? f[2 * e + 1] - h1 : 0.0f);
+                          }
+                          *reinterpret_cast<uint2 *>(vs + member * vs_ld + r) = make_uint2(hi[0], hi[1]);
+                          *reinterpret_cast<uint2 *>(vs + member * vs_ld + rank + r) = make_uint2(lo[0], lo[1]);
+                      }
+                      const uint16_t *bu = b + static_cast<uint64_t>(id) * n * rank;
+                      if (rows <= 16)
+                          lora_up_chunk<T, 1, NJ>(bu, rank, n, base, base_ld, y, y_ld, vec, row0, rows, list, vs, vs_ld,
+                                                  col0, lane);
+                      else
+                          lora_up_chunk<T, 4, NJ>(bu, rank, n, base, base_ld, y, y_ld, vec, row0, rows, list, vs, vs_ld,
+                                                  col0, lane);
+                      __syncthreads();  // vs is read
+                  });
+    // rows without an adapter are base, where y is not
+    if (y == base) return;
+    for (uint32_t i = blockIdx.y; i < min(64u * Q, m - row0); i += gridDim.y) {
+        if (adapters[row0 + i] < n_adapters) continue;
+        const T *from = base + (row0 + i) * base_ld;
+        T *to = y + (row0 + i) * y_ld;
+        for (uint32_t c = blockIdx.x * kLoraCols + threadIdx.x; c < min(n, (blockIdx.x + 1) * kLoraCols); c += kLoraThreads)
+            to[c] = from[c];
+    }
 }
 
 }  // namespace fh
 
 using namespace fh;
+
+namespace {
+
+// Windows of 64 * quads rows, and k cut into `splits` ranges of 4 wavefronts x
+// `steps` x 32.
+struct Split {
+    uint32_t quads, windows, splits, steps;
+};
+
+Split split_of(int64_t m, int64_t k) {
+    Split s;
+    s.quads = m > 64 && m <= kWideRows ? 4 : 1;
+    s.windows = static_cast<uint32_t>((m + 64 * s.quads - 1) / (64 * s.quads));
+    const uint64_t steps = (k + 31) / 32, least = kLoraWaves * kDownSteps;
+    const uint64_t want = std::max<uint64_t>(1, kDownBlocks / std::max<uint64_t>(1, (m + 63) / 64));
+    const uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>({want, (steps + least - 1) / least, kMaxSplits}));
+    s.steps = static_cast<uint32_t>((steps + splits * kLoraWaves - 1) / (splits * kLoraWaves));
+    s.splits = static_cast<uint32_t>((steps + s.steps * kLoraWaves - 1) / (s.steps * kLoraWaves));
+    return s;
+}
+
+}  // namespace
 
 extern "C" int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *bytes) {
     const char *fn = "fh_lora_workspace";
@@ -57,7 +386,7 @@ extern "C" int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *b
         return fail(FH_ERR_UNSUPPORTED, "%s: rank %lld must be a multiple of 8, at most 128", fn, (long long)rank);
     if (k < 8 || k % 8 != 0)
         return fail(FH_ERR_UNSUPPORTED, "%s: k %lld must be a multiple of 8", fn, (long long)k);
-    *bytes = static_cast<uint64_t>(m) * rank * 4 + 16;
+    *bytes = static_cast<uint64_t>(split_of(m, k).splits) * m * rank * 4 + 16;
     return FH_OK;
 }
 
@@ -118,27 +447,47 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     }
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "y", y, y_bytes)) return rc;
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "base", base, base_bytes)) return rc;
-    if ((n + 255) / 256 > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: n %lld", fn, (long long)n);
+    const Split w = split_of(m, k);
+    if (w.windows > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: m %lld", fn, (long long)m);
     if (int rc = set_current(dev, fn)) return rc;
+    const uint32_t cols = static_cast<uint32_t>((n + kLoraCols - 1) / kLoraCols);
+    // a window has at most as many chunks as rows
+    const uint32_t most = static_cast<uint32_t>(std::min<int64_t>(m, 64 * w.quads));
+    const uint32_t down_slots = std::clamp(kDownSlots / (w.windows * w.splits), 1u, most);
+    const uint32_t up_slots = std::clamp(static_cast<uint32_t>(kUpSlots / (static_cast<uint64_t>(w.windows) * cols)), 1u,
+                                         most);
+    const dim3 down(down_slots, w.splits, w.windows), up(cols, up_slots, w.windows), threads(kLoraThreads);
     float *v = static_cast<float *>(workspace);
-    if (int rc = dispatch(dev, fn, [&] {
-            hipLaunchKernelGGL(lora_down_kernel, dim3(static_cast<uint32_t>(m)), dim3(256), 0, dev->stream, x,
-                               static_cast<uint32_t>(k), static_cast<uint64_t>(x_ld), a, scales,
-                               static_cast<uint32_t>(n_adapters), static_cast<uint32_t>(rank), adapters, v);
-        }))
-        return rc;
-    const dim3 grid(static_cast<uint32_t>(m), static_cast<uint32_t>((n + 255) / 256));
-    return dispatch(dev, fn, [&] {
-        if (dtype == FH_F32)
-            hipLaunchKernelGGL(lora_up_kernel<float>, grid, dim3(256), 0, dev->stream, v, b,
-                               static_cast<uint32_t>(n_adapters), static_cast<uint32_t>(rank),
-                               static_cast<uint32_t>(n), adapters, static_cast<const float *>(base),
-                               static_cast<uint64_t>(base_ld), static_cast<float *>(y), static_cast<uint64_t>(y_ld));
-        else
-            hipLaunchKernelGGL(lora_up_kernel<uint16_t>, grid, dim3(256), 0, dev->stream, v, b,
-                               static_cast<uint32_t>(n_adapters), static_cast<uint32_t>(rank),
-                               static_cast<uint32_t>(n), adapters, static_cast<const uint16_t *>(base),
-                               static_cast<uint64_t>(base_ld), static_cast<uint16_t *>(y),
-                               static_cast<uint64_t>(y_ld));
-    });
+    const uint32_t m32 = static_cast<uint32_t>(m), k32 = static_cast<uint32_t>(k), n32 = static_cast<uint32_t>(n);
+    const uint32_t rank32 = static_cast<uint32_t>(rank), u32 = static_cast<uint32_t>(n_adapters);
+    const bool vec = ((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0 &&
+                     base_ld * elem % 16 == 0 && y_ld * elem % 16 == 0;
+    auto run_down = [&](auto kernel) {
+        return dispatch(dev, fn, [&] {
+            hipLaunchKernelGGL(kernel, down, threads, 0, dev->stream, x, m32, k32, static_cast<uint64_t>(x_ld), a, u32,
+                               rank32, adapters, w.steps, v);
+        });
+    };
+    auto run_up = [&](auto kernel, auto *of) {
+        using T = std::remove_pointer_t<decltype(of)>;
+        return dispatch(dev, fn, [&] {
+            hipLaunchKernelGGL(kernel, up, threads, 0, dev->stream, v, w.splits, m32, b, scales, u32, rank32, n32,
+                               adapters, static_cast<const T *>(base), static_cast<uint64_t>(base_ld),
+                               static_cast<T *>(y), static_cast<uint64_t>(y_ld), vec);
+        });
+    };
+    // rank tiles of 16: 1, 2, 4 or 8
+    auto run = [&](auto q, auto tiles) {
+        constexpr int Q = decltype(q)::value, N = decltype(tiles)::value;
+        if (int rc = run_down(lora_down_kernel<Q, N>)) return rc;
+        return dtype == FH_F32 ? run_up(lora_up_kernel<float, Q, N>, static_cast<float *>(nullptr))
+                               : run_up(lora_up_kernel<uint16_t, Q, N>, static_cast<uint16_t *>(nullptr));
+    };
+    auto by_rank = [&](auto q) {
+        if (rank <= 16) return run(q, std::integral_constant<int, 1>{});
+        if (rank <= 32) return run(q, std::integral_constant<int, 2>{});
+        if (rank <= 64) return run(q, std::integral_constant<int, 4>{});
+        return run(q, std::integral_constant<int, 8>{});
+    };
+    return w.quads == 4 ? by_rank(std::integral_constant<int, 4>{}) : by_rank(std::integral_constant<int, 1>{});
 }

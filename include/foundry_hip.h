@@ -572,7 +572,7 @@ int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *bytes);
  * is filled up with zeros. base, y: [m, n] of `dtype` (FH_BF16 or FH_F32)
  * with row strides base_ld, y_ld >= n; y is base itself (the same pointer and
  * stride) or does not overlap the operands. rank and k are multiples of 8,
- * rank at most 128; n is any; x, a, b 16-byte aligned. workspace: at least
+ * rank at most 128; n is any, m at most 4194240; x, a, b 16-byte aligned. workspace: at least
  * fh_lora_workspace() bytes, 16-byte aligned, no initial contents; calls that
  * share a workspace must not run concurrently. */
 int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t k, int64_t x_ld,
