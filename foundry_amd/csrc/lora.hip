@@ -34,90 +34,137 @@ constexpr uint32_t kDownBlocks = 512, kMaxSplits = 16, kDownSteps = 2;
 // Rows up to which a window is 256 rows (and an adapter that they share is
 // read once for all of them).
 constexpr uint32_t kWideRows = 1024;
-// Blocks that the chunks of the windows are spread over, down and up.
+// Blocks that the chunks of the windows are spread over, down and up. Slots are
+// a grid's slowest dimension: a window has often fewer chunks than slots, and
+// neighbouring blocks run on different XCDs (with slots fastest, 4096 packed
+// rows ran on every second one: 62 us against 44).
 constexpr uint32_t kDownSlots = 1024, kUpSlots = 2048;
 constexpr uint32_t kLoraThreads = 256;
 constexpr uint32_t kLoraWaves = kLoraThreads / 64;
 constexpr uint32_t kLoraCols = 64 * kLoraWaves;  // columns of an up block
 
-// Calls take(adapter, rows, list) for each chunk that falls to `slot`: the
-// chunk's rows are list[0..rows) (in the window). list: this wavefront's
-// 64 * Q entries of LDS. Every wavefront of a block goes through the same
-// chunks.
-template <int Q, typename Take>
-__device__ __forceinline__ void for_chunks(const uint32_t *adapters, uint32_t row0, uint32_t m, uint32_t n_adapters,
-                                           uint32_t slot, uint32_t slots, uint32_t lane, uint8_t *list, Take take) {
-    uint32_t id[Q];
-    uint64_t left[Q];
+// The rows of a window and its chunks. A row's rank is the number of rows
+// before it with its adapter; rows of rank 0, 64, .. lead a chunk, and the
+// chunks are numbered by their leaders' order. Ranks come from match masks,
+// formed bit by bit of the ids: a ballot per bit and 64 rows, instead of a
+// round per adapter (48 adapters in 256 rows: 6 us a block).
+template <int Q>
+struct Window {
+    uint32_t id[Q];     // lane's rows' adapters
+    uint64_t live[Q];   // rows that have one
+    uint64_t leads[Q];  // chunk leaders
+    uint32_t chunks;
+};
+
+// shared: Q words that the block's wavefronts exchange leaders through (Q > 1,
+// when wavefront w works out those of rows 64 w .. 64 w + 63).
+template <int Q>
+__device__ __forceinline__ Window<Q> window_of(const uint32_t *adapters, uint32_t row0, uint32_t m, uint32_t n_adapters,
+                                               uint32_t lane, uint32_t wave, uint64_t *shared) {
+    Window<Q> o;
+    uint64_t match[Q];
+    uint32_t own = 0;
+    bool alive = false;
 #pragma unroll
     for (int w = 0; w < Q; ++w) {
         const uint32_t row = row0 + w * 64 + lane;
-        id[w] = row < m ? adapters[row] : ~0u;
-        left[w] = __ballot(id[w] < n_adapters);
+        o.id[w] = row < m ? adapters[row] : ~0u;
+        match[w] = o.live[w] = __ballot(o.id[w] < n_adapters);
+        if (Q == 1 || w == static_cast<int>(wave)) own = o.id[w], alive = o.id[w] < n_adapters;
     }
-    for (uint32_t item = 0;;) {
-        uint32_t group = ~0u;
-#pragma unroll
-        for (int w = Q - 1; w >= 0; --w)
-            if (left[w]) group = __builtin_amdgcn_readlane(id[w], __builtin_ctzll(left[w]));
-        if (group == ~0u) return;
-        uint64_t mask[Q];
-        uint32_t rows = 0;
+    for (uint32_t bit = 0; (n_adapters - 1) >> bit; ++bit) {
+        const bool set = own >> bit & 1;
 #pragma unroll
         for (int w = 0; w < Q; ++w) {
-            mask[w] = __ballot(id[w] == group);
-            left[w] &= ~mask[w];
-            rows += __builtin_popcountll(mask[w]);
+            const uint64_t have = __ballot(o.id[w] >> bit & 1);
+            match[w] &= set ? have : ~have;
         }
-        bool listed = false;
-        for (uint32_t r = 0; r < rows; r += 64, ++item) {
-            if (item % slots != slot) continue;
-            if (!listed) {
-                uint32_t before = 0;
-#pragma unroll
-                for (int w = 0; w < Q; ++w) {
-                    if (mask[w] >> lane & 1)
-                        list[before + __builtin_popcountll(mask[w] & ((1ull << lane) - 1))] =
-                            static_cast<uint8_t>(w * 64 + lane);
-                    before += __builtin_popcountll(mask[w]);
-                }
-                __builtin_amdgcn_wave_barrier();
-                listed = true;
-            }
-            take(group, min(rows - r, 64u), list + r);
-        }
-        __builtin_amdgcn_wave_barrier();
     }
+    uint32_t rank = 0;
+#pragma unroll
+    for (int w = 0; w < Q; ++w) {
+        const uint64_t before = Q == 1 || w == static_cast<int>(wave) ? (1ull << lane) - 1
+                                : w < static_cast<int>(wave)          ? ~0ull
+                                                                      : 0ull;
+        rank += __builtin_popcountll(match[w] & before);
+    }
+    const uint64_t lead = __ballot(alive && rank % 64 == 0);
+    o.chunks = 0;
+    if constexpr (Q == 1) {
+        o.leads[0] = lead;
+        o.chunks = __builtin_popcountll(lead);
+    } else {
+        if (lane == 0) shared[wave] = lead;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < Q; ++w) {
+            const uint64_t v = shared[w];
+            o.leads[w] = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32))) << 32 |
+                         static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)));
+            o.chunks += __builtin_popcountll(o.leads[w]);
+        }
+    }
+    return o;
 }
 
-// v[split][row][r] = sum over the split's k of x[row, k] A[r, k]. Block (slot,
-// split, window); its wavefronts take a quarter of the split's k each and add
-// up in LDS in their order. RT row tiles of 16, NR rank tiles of 16; a product
-// has the rank along its rows, so that a lane ends up with 4 ranks of a row.
-template <int RT, int NR>
-__device__ __forceinline__ void lora_down_chunk(const uint16_t *x, uint32_t k, uint64_t x_ld, const uint16_t *a,
-                                                uint32_t rank, uint32_t k0, uint32_t k1, uint32_t row0, uint32_t rows,
-                                                const uint8_t *list, float4 *sums, float *v, uint32_t lane,
-                                                uint32_t wave) {
-    constexpr int U = RT * NR >= 16 ? 2 : 4;  // steps of 32 requested together
-    const uint32_t c = lane & 15u, q = lane >> 4;
-    const uint16_t *xr[RT], *ar[NR];
+// Chunk `item` of the window: its adapter, its rows (in the window) in list[0
+// .. rows), this wavefront's 64 bytes of LDS.
+template <int Q>
+__device__ __forceinline__ uint32_t chunk_of(const Window<Q> &o, uint32_t item, uint32_t lane, uint8_t *list,
+                                             uint32_t &rows) {
+    uint32_t id = 0, lead = 0, skip = item;
+    bool found = false;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) xr[t] = x + (row0 + list[min(t * 16 + c, rows - 1)]) * x_ld;
+    for (int w = 0; w < Q; ++w) {
+        const uint32_t here = __builtin_popcountll(o.leads[w]);
+        if (!found && skip < here) {
+            uint64_t bits = o.leads[w];
+            for (uint32_t i = 0; i < skip; ++i) bits &= bits - 1;
+            lead = __builtin_ctzll(bits);
+            id = __builtin_amdgcn_readlane(o.id[w], lead);
+            lead += w * 64;
+            found = true;
+        }
+        if (!found) skip -= here;
+    }
+    // the leader's rank, then the rows of ranks from there on
+    uint64_t mask[Q];
+    uint32_t all = 0, first = 0;
 #pragma unroll
-    for (int t = 0; t < NR; ++t) ar[t] = a + static_cast<uint64_t>(min(t * 16 + c, rank - 1)) * k;
-    lo_f32x4_t acc[RT][NR];
+    for (int w = 0; w < Q; ++w) {
+        mask[w] = __ballot(o.id[w] == id);
+        all += __builtin_popcountll(mask[w]);
+        const uint64_t before = lead >= w * 64u + 64u ? ~0ull : lead > w * 64u ? (1ull << (lead - w * 64u)) - 1 : 0ull;
+        first += __builtin_popcountll(mask[w] & before);
+    }
+    uint32_t before = 0;
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+    for (int w = 0; w < Q; ++w) {
+        const uint32_t at = before + __builtin_popcountll(mask[w] & ((1ull << lane) - 1)) - first;
+        if ((mask[w] >> lane & 1) && at < 64) list[at] = static_cast<uint8_t>(w * 64 + lane);
+        before += __builtin_popcountll(mask[w]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    rows = min(all - first, 64u);
+    return id;
+}
+
+// Sums over k0 .. k1 - 1 of 16 rows (xr: lane's) by NR tiles of 16 ranks (ar:
+// lane's). A product has the ranks along its rows, so that a lane ends up with
+// 4 ranks of a row.
+template <int NR>
+__device__ __forceinline__ void lora_down_tile(const uint16_t *xr, const uint16_t *const (&ar)[NR], uint32_t k, uint32_t k0,
+                                               uint32_t k1, uint32_t q, lo_f32x4_t (&acc)[NR]) {
+    constexpr int U = NR >= 8 ? 2 : NR >= 4 ? 4 : 8;  // steps of 32 requested together
 #pragma unroll
-        for (int r = 0; r < NR; ++r) acc[t][r] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r = 0; r < NR; ++r) acc[r] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t s = k0; s < k1; s += 32 * U) {
-        uint4 xf[U][RT], af[U][NR];
+        uint4 xf[U], af[U][NR];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t at = min(s + u * 32 + q * 8, k - 8);  // clamped: the pieces past k1 are zeroed below
-#pragma unroll
-            for (int t = 0; t < RT; ++t) xf[u][t] = *reinterpret_cast<const uint4 *>(xr[t] + at);
+            xf[u] = *reinterpret_cast<const uint4 *>(xr + at);
 #pragma unroll
             for (int t = 0; t < NR; ++t) af[u][t] = *reinterpret_cast<const uint4 *>(ar[t] + at);
         }
@@ -125,8 +172,7 @@ __device__ __forceinline__ void lora_down_chunk(const uint16_t *x, uint32_t k, u
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (s + u * 32 + q * 8 >= k1) {
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) xf[u][t] = make_uint4(0, 0, 0, 0);
+                    xf[u] = make_uint4(0, 0, 0, 0);
 #pragma unroll
                     for (int t = 0; t < NR; ++t) af[u][t] = make_uint4(0, 0, 0, 0);
                 }
@@ -134,55 +180,72 @@ __device__ __forceinline__ void lora_down_chunk(const uint16_t *x, uint32_t k, u
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int r = 0; r < NR; ++r) acc[t][r] = lo_mfma(af[u][r], xf[u][t], acc[t][r]);
-    }
-    // wavefront w adds to what those before it left; the last one's sums go out
-    for (uint32_t w = 0; w < kLoraWaves; ++w) {
-        if (w == wave) {
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const lo_f32x4_t p = acc[t][r];
-                    float4 f = make_float4(p[0], p[1], p[2], p[3]);
-                    if (w) {
-                        const float4 o = sums[(t * NR + r) * 64 + lane];
-                        f = make_float4(o.x + f.x, o.y + f.y, o.z + f.z, o.w + f.w);
-                    }
-                    if (w + 1 < kLoraWaves) {
-                        sums[(t * NR + r) * 64 + lane] = f;
-                    } else if (t * 16 + c < rows && r * 16 + q * 4 < rank) {
-                        const uint64_t row = row0 + list[t * 16 + c];
-                        *reinterpret_cast<float4 *>(v + row * rank + r * 16 + q * 4) = f;
-                    }
-                }
-        }
-        __syncthreads();
+            for (int r = 0; r < NR; ++r) acc[r] = lo_mfma(af[u][r], xf[u], acc[r]);
     }
 }
 
+// v[split][row][r] = sum over the split's k of x[row, k] A[r, k]. Block (split,
+// window, slot). Up to 16 rows of a chunk: each wavefront takes a quarter of
+// the split's k, and they add up in LDS in their order. More: each takes 16 of
+// the rows over all of the split's k.
 template <int Q, int NR>
 __global__ __launch_bounds__(kLoraThreads) void lora_down_kernel(const uint16_t *__restrict__ x, uint32_t m, uint32_t k,
                                                                  uint64_t x_ld, const uint16_t *__restrict__ a,
                                                                  uint32_t n_adapters, uint32_t rank,
                                                                  const uint32_t *__restrict__ adapters, uint32_t steps,
                                                                  float *__restrict__ v) {
-    __shared__ uint8_t lists[kLoraWaves][64 * Q];
-    __shared__ float4 sums[4 * NR * 64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.z * 64 * Q;
-    // steps: of 32 k, of each wavefront
-    const uint32_t k0 = min((blockIdx.y * kLoraWaves + wave) * steps * 32, k), k1 = min(k0 + steps * 32, k);
-    v += static_cast<uint64_t>(blockIdx.y) * m * rank;
-    for_chunks<Q>(adapters, row0, m, n_adapters, blockIdx.x, gridDim.x, lane, lists[wave],
-                  [&](uint32_t id, uint32_t rows, const uint8_t *list) {
-                      const uint16_t *au = a + static_cast<uint64_t>(id) * rank * k;
-                      if (rows <= 16)
-                          lora_down_chunk<1, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, list, sums, v, lane, wave);
-                      else
-                          lora_down_chunk<4, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, list, sums, v, lane, wave);
-                  });
+    __shared__ uint8_t lists[kLoraWaves][64];
+    __shared__ uint64_t leads[Q];
+    __shared__ float4 sums[NR * 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.y * 64 * Q;
+    const uint32_t c = lane & 15u, q = lane >> 4;
+    // steps: of 32 k, of a quarter of the split
+    const uint32_t k0 = min(blockIdx.x * kLoraWaves * steps * 32, k), k1 = min(k0 + kLoraWaves * steps * 32, k);
+    v += static_cast<uint64_t>(blockIdx.x) * m * rank;
+    const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
+    for (uint32_t item = blockIdx.z; item < o.chunks; item += gridDim.z) {
+        uint32_t rows;
+        const uint32_t id = chunk_of<Q>(o, item, lane, lists[wave], rows);
+        const uint8_t *list = lists[wave];
+        const bool few = rows <= 16;
+        const uint32_t member = (few ? 0 : wave * 16) + c;
+        const uint16_t *ar[NR];
+#pragma unroll
+        for (int t = 0; t < NR; ++t) ar[t] = a + (static_cast<uint64_t>(id) * rank + min(t * 16 + c, rank - 1)) * k;
+        const uint16_t *xr = x + (row0 + list[min(member, rows - 1)]) * x_ld;
+        const uint32_t from = few ? min(k0 + wave * steps * 32, k1) : k0;
+        lo_f32x4_t acc[NR];
+        lora_down_tile<NR>(xr, ar, k, from, few ? min(from + steps * 32, k1) : wave * 16 < rows ? k1 : from, q, acc);
+        float *to = v + static_cast<uint64_t>(row0 + list[min(member, rows - 1)]) * rank;
+        if (!few) {
+            if (member < rows) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+                    if (r * 16 + q * 4 < rank)
+                        *reinterpret_cast<float4 *>(to + r * 16 + q * 4) =
+                            make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+            }
+            continue;
+        }
+        // wavefront w adds to what those before it left; the last one's sums go out
+        for (uint32_t w = 0; w < kLoraWaves; ++w) {
+            if (w == wave) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float4 f = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+                    if (w) {
+                        const float4 p = sums[r * 64 + lane];
+                        f = make_float4(p.x + f.x, p.y + f.y, p.z + f.z, p.w + f.w);
+                    }
+                    if (w + 1 < kLoraWaves)
+                        sums[r * 64 + lane] = f;
+                    else if (member < rows && r * 16 + q * 4 < rank)
+                        *reinterpret_cast<float4 *>(to + r * 16 + q * 4) = f;
+                }
+            }
+            __syncthreads();
+        }
+    }
 }
 
 // 16 neighbouring values of a row of base or y, `count` of them in the matrix;
@@ -268,16 +331,19 @@ __device__ __forceinline__ void lora_up_chunk(const uint16_t *b, uint32_t rank, 
         }
     }
     const uint32_t col = col0 + q * 16, count = col < n ? n - col : 0;
-    float f[RT][16];
-    uint64_t row[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        row[t] = row0 + list[min(t * 16 + c, rows - 1)];
-        load16(base + row[t] * base_ld + (count ? col : 0), count, vec, f[t]);
-    }
+    // the next row tile's base is requested before a tile's products
+    float f[2][16];
+    uint64_t row[2];
+    row[0] = row0 + list[min(c, rows - 1)];
+    load16(base + row[0] * base_ld + (count ? col : 0), count, vec, f[0]);
     __syncthreads();  // vs is written
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
+        if (t * 16 >= rows) break;
+        if (t + 1 < RT) {
+            row[(t + 1) & 1] = row0 + list[min((t + 1) * 16 + c, rows - 1)];
+            load16(base + row[(t + 1) & 1] * base_ld + (count ? col : 0), count, vec, f[(t + 1) & 1]);
+        }
         lo_f32x4_t acc[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) acc[u] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -291,12 +357,12 @@ __device__ __forceinline__ void lora_up_chunk(const uint16_t *b, uint32_t rank, 
             for (int u = 0; u < 4; ++u) acc[u] = lo_mfma(bfr[u][j], vf, acc[u]);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) f[t][e] += acc[e / 4][e % 4];
-        if (t * 16 + c < rows && count) store16(y + row[t] * y_ld + col, count, vec, f[t]);
+        for (int e = 0; e < 16; ++e) f[t & 1][e] += acc[e / 4][e % 4];
+        if (t * 16 + c < rows && count) store16(y + row[t & 1] * y_ld + col, count, vec, f[t & 1]);
     }
 }
 
-// Block (columns, slot, window).
+// Block (columns, window, slot).
 template <typename T, int Q, int NJ>
 __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__restrict__ v, uint32_t splits, uint32_t m,
                                                                const uint16_t *__restrict__ b,
@@ -304,51 +370,65 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
                                                                uint32_t rank, uint32_t n,
                                                                const uint32_t *__restrict__ adapters, const T *base,
                                                                uint64_t base_ld, T *y, uint64_t y_ld, bool vec) {
-    __shared__ uint8_t lists[kLoraWaves][64 * Q];
+    constexpr int kLoads = 8;  // splits' sums requested together
+    __shared__ uint8_t lists[kLoraWaves][64];
+    __shared__ uint64_t leads[Q];
     __shared__ __attribute__((aligned(16))) uint16_t vs[64 * (2 * 16 * NJ + 8)];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.z * 64 * Q;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.y * 64 * Q;
     const uint32_t col0 = blockIdx.x * kLoraCols + wave * 64, vs_ld = 2 * rank + 8, quads = rank / 4;
-    for_chunks<Q>(adapters, row0, m, n_adapters, blockIdx.y, gridDim.y, lane, lists[wave],
-                  [&](uint32_t id, uint32_t rows, const uint8_t *list) {
-                      const float scale = scales[id];
-                      for (uint32_t i = threadIdx.x; i < rows * quads; i += kLoraThreads) {
-                          const uint32_t member = i / quads, r = i % quads * 4;
-                          const float *p = v + static_cast<uint64_t>(row0 + list[member]) * rank + r;
-                          float4 s = *reinterpret_cast<const float4 *>(p);
-                          for (uint32_t u = 1; u < splits; ++u) {
-                              const float4 o = *reinterpret_cast<const float4 *>(p + static_cast<uint64_t>(u) * m * rank);
-                              s = make_float4(s.x + o.x, s.y + o.y, s.z + o.z, s.w + o.w);
-                          }
-                          const float f[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
-                          uint32_t hi[2], lo[2];
+    const uint64_t split = static_cast<uint64_t>(m) * rank;
+    const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
+    for (uint32_t item = blockIdx.z; item < o.chunks; item += gridDim.z) {
+        uint32_t rows;
+        const uint8_t *list = lists[wave];
+        const uint32_t id = chunk_of<Q>(o, item, lane, lists[wave], rows);
+        const float scale = scales[id];
+        for (uint32_t i = threadIdx.x; i < rows * quads; i += kLoraThreads) {
+            const uint32_t member = i / quads, r = i % quads * 4;
+            const float *p = v + static_cast<uint64_t>(row0 + list[member]) * rank + r;
+            float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t u0 = 0; u0 < splits; u0 += kLoads) {
+                float4 part[kLoads];
 #pragma unroll
-                          for (int e = 0; e < 2; ++e) {
-                              hi[e] = f32x2_to_bf16x2_rne(f[2 * e], f[2 * e + 1]);
-                              // what the rounding lost; nothing where it is inf or NaN
-                              const float h0 = bf(hi[e] & 0xFFFFu), h1 = bf(hi[e] >> 16);
-                              lo[e] = f32x2_to_bf16x2_rne(fabsf(h0) < INFINITY ? f[2 * e] - h0 : 0.0f,
-                                                          fabsf(h1) < INFINITY ? f[2 * e + 1] - h1 : 0.0f);
-                          }
-                          *reinterpret_cast<uint2 *>(vs + member * vs_ld + r) = make_uint2(hi[0], hi[1]);
-                          *reinterpret_cast<uint2 *>(vs + member * vs_ld + rank + r) = make_uint2(lo[0], lo[1]);
-                      }
-                      const uint16_t *bu = b + static_cast<uint64_t>(id) * n * rank;
-                      if (rows <= 16)
-                          lora_up_chunk<T, 1, NJ>(bu, rank, n, base, base_ld, y, y_ld, vec, row0, rows, list, vs, vs_ld,
-                                                  col0, lane);
-                      else
-                          lora_up_chunk<T, 4, NJ>(bu, rank, n, base, base_ld, y, y_ld, vec, row0, rows, list, vs, vs_ld,
-                                                  col0, lane);
-                      __syncthreads();  // vs is read
-                  });
+                for (uint32_t u = 0; u < kLoads; ++u)
+                    part[u] = *reinterpret_cast<const float4 *>(p + min(u0 + u, splits - 1) * split);
+#pragma unroll
+                for (uint32_t u = 0; u < kLoads; ++u)
+                    if (u0 + u < splits) f[0] += part[u].x, f[1] += part[u].y, f[2] += part[u].z, f[3] += part[u].w;
+            }
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float f0 = f[2 * e] * scale, f1 = f[2 * e + 1] * scale;
+                hi[e] = f32x2_to_bf16x2_rne(f0, f1);
+                // what the rounding lost; nothing where it is inf or NaN
+                const float h0 = bf(hi[e] & 0xFFFFu), h1 = bf(hi[e] >> 16);
+                lo[e] = f32x2_to_bf16x2_rne(fabsf(h0) < INFINITY ? f0 - h0 : 0.0f, fabsf(h1) < INFINITY ? f1 - h1 : 0.0f);
+            }
+            *reinterpret_cast<uint2 *>(vs + member * vs_ld + r) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2 *>(vs + member * vs_ld + rank + r) = make_uint2(lo[0], lo[1]);
+        }
+        const uint16_t *bu = b + static_cast<uint64_t>(id) * n * rank;
+        if (rows <= 16)
+            lora_up_chunk<T, 1, NJ>(bu, rank, n, base, base_ld, y, y_ld, vec, row0, rows, list, vs, vs_ld, col0, lane);
+        else
+            lora_up_chunk<T, 4, NJ>(bu, rank, n, base, base_ld, y, y_ld, vec, row0, rows, list, vs, vs_ld, col0, lane);
+        __syncthreads();  // vs is read
+    }
     // rows without an adapter are base, where y is not
     if (y == base) return;
-    for (uint32_t i = blockIdx.y; i < min(64u * Q, m - row0); i += gridDim.y) {
-        if (adapters[row0 + i] < n_adapters) continue;
-        const T *from = base + (row0 + i) * base_ld;
-        T *to = y + (row0 + i) * y_ld;
-        for (uint32_t c = blockIdx.x * kLoraCols + threadIdx.x; c < min(n, (blockIdx.x + 1) * kLoraCols); c += kLoraThreads)
-            to[c] = from[c];
+    uint32_t turn = 0;
+#pragma unroll
+    for (int w = 0; w < Q; ++w) {
+        const uint32_t here = m - row0 > w * 64u ? min(m - row0 - w * 64u, 64u) : 0;
+        uint64_t bare = ~o.live[w] & (here < 64 ? (1ull << here) - 1 : ~0ull);
+        for (; bare; bare &= bare - 1, ++turn) {
+            if (turn % gridDim.z != blockIdx.z) continue;
+            const uint64_t row = row0 + w * 64 + __builtin_ctzll(bare);
+            for (uint32_t e = blockIdx.x * kLoraCols + threadIdx.x; e < min(n, (blockIdx.x + 1) * kLoraCols);
+                 e += kLoraThreads)
+                y[row * y_ld + e] = base[row * base_ld + e];
+        }
     }
 }
 
@@ -456,7 +536,7 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     const uint32_t down_slots = std::clamp(kDownSlots / (w.windows * w.splits), 1u, most);
     const uint32_t up_slots = std::clamp(static_cast<uint32_t>(kUpSlots / (static_cast<uint64_t>(w.windows) * cols)), 1u,
                                          most);
-    const dim3 down(down_slots, w.splits, w.windows), up(cols, up_slots, w.windows), threads(kLoraThreads);
+    const dim3 down(w.splits, w.windows, down_slots), up(cols, w.windows, up_slots), threads(kLoraThreads);
     float *v = static_cast<float *>(workspace);
     const uint32_t m32 = static_cast<uint32_t>(m), k32 = static_cast<uint32_t>(k), n32 = static_cast<uint32_t>(n);
     const uint32_t rank32 = static_cast<uint32_t>(rank), u32 = static_cast<uint32_t>(n_adapters);
