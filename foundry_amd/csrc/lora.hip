@@ -30,18 +30,19 @@ __device__ __forceinline__ lo_f32x4_t lo_mfma(uint4 a, uint4 b, lo_f32x4_t c) {
 
 // Blocks of 64 rows and a range of k that the down product aims for, the ranges
 // at most, and the least steps of 32 k that a wavefront takes.
-constexpr uint32_t kDownBlocks = 512, kMaxSplits = 16, kDownSteps = 2;
+constexpr uint32_t kDownBlocks = 512, kMaxSplits = 4, kDownSteps = 2;
 // Rows up to which a window is 256 rows (and an adapter that they share is
 // read once for all of them).
 constexpr uint32_t kWideRows = 1024;
 // Blocks that the chunks of the windows are spread over, down and up. Slots are
 // a grid's slowest dimension: a window has often fewer chunks than slots, and
 // neighbouring blocks run on different XCDs (with slots fastest, 4096 packed
-// rows ran on every second one: 62 us against 44).
-constexpr uint32_t kDownSlots = 1024, kUpSlots = 2048;
+// rows ran on every second one: 62 us against 48).
+constexpr uint32_t kDownSlots = 512, kUpSlots = 2048;
 constexpr uint32_t kLoraThreads = 256;
 constexpr uint32_t kLoraWaves = kLoraThreads / 64;
-constexpr uint32_t kLoraCols = 64 * kLoraWaves;  // columns of an up block
+// Wavefronts that the up product aims for, and 64-column tiles of one at most.
+constexpr uint32_t kUpWaves = 1024, kMaxTiles = 8;
 
 // The rows of a window and its chunks. A row's rank is the number of rows
 // before it with its adapter; rows of rank 0, 64, .. lead a chunk, and the
@@ -65,12 +66,13 @@ __device__ __forceinline__ Window<Q> window_of(const uint32_t *adapters, uint32_
     uint64_t match[Q];
     uint32_t own = 0;
     bool alive = false;
+    const int word = wave % Q;
 #pragma unroll
     for (int w = 0; w < Q; ++w) {
         const uint32_t row = row0 + w * 64 + lane;
         o.id[w] = row < m ? adapters[row] : ~0u;
         match[w] = o.live[w] = __ballot(o.id[w] < n_adapters);
-        if (Q == 1 || w == static_cast<int>(wave)) own = o.id[w], alive = o.id[w] < n_adapters;
+        if (Q == 1 || w == word) own = o.id[w], alive = o.id[w] < n_adapters;
     }
     for (uint32_t bit = 0; (n_adapters - 1) >> bit; ++bit) {
         const bool set = own >> bit & 1;
@@ -83,9 +85,7 @@ __device__ __forceinline__ Window<Q> window_of(const uint32_t *adapters, uint32_
     uint32_t rank = 0;
 #pragma unroll
     for (int w = 0; w < Q; ++w) {
-        const uint64_t before = Q == 1 || w == static_cast<int>(wave) ? (1ull << lane) - 1
-                                : w < static_cast<int>(wave)          ? ~0ull
-                                                                      : 0ull;
+        const uint64_t before = Q == 1 || w == word ? (1ull << lane) - 1 : w < word ? ~0ull : 0ull;
         rank += __builtin_popcountll(match[w] & before);
     }
     const uint64_t lead = __ballot(alive && rank % 64 == 0);
@@ -94,7 +94,7 @@ __device__ __forceinline__ Window<Q> window_of(const uint32_t *adapters, uint32_
         o.leads[0] = lead;
         o.chunks = __builtin_popcountll(lead);
     } else {
-        if (lane == 0) shared[wave] = lead;
+        if (lane == 0 && wave < Q) shared[wave] = lead;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < Q; ++w) {
@@ -248,171 +248,265 @@ __global__ __launch_bounds__(kLoraThreads) void lora_down_kernel(const uint16_t 
     }
 }
 
-// 16 neighbouring values of a row of base or y, `count` of them in the matrix;
-// vec: rows and columns keep 16-byte alignment.
+// 16 neighbouring values of a row of base, as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load16(const T *p, uint32_t count, bool vec, float (&f)[16]) {
-    if (vec && count >= 16) {
+struct Raw16 {
+    uint4 w[sizeof(T)];
+};
+
+// Requests them from an aligned row.
+template <typename T>
+__device__ __forceinline__ Raw16<T> request16(const T *p) {
+    Raw16<T> r;
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(T); ++i) r.w[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void floats16(const Raw16<T> &raw, float (&f)[16]) {
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(T); ++i) {
         if constexpr (sizeof(T) == 2) {
             float h[8];
+            unpack8(raw.w[i], h);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                unpack8(*reinterpret_cast<const uint4 *>(p + i * 8), h);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[i * 8 + e] = h[e];
-            }
+            for (int e = 0; e < 8; ++e) f[i * 8 + e] = h[e];
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 h = *reinterpret_cast<const float4 *>(p + i * 4);
-                f[i * 4] = h.x, f[i * 4 + 1] = h.y, f[i * 4 + 2] = h.z, f[i * 4 + 3] = h.w;
-            }
-        }
-    } else {
-#pragma unroll
-        for (uint32_t e = 0; e < 16; ++e) {
-            f[e] = 0.0f;
-            if (e < count) {
-                if constexpr (sizeof(T) == 2)
-                    f[e] = bf(p[e]);
-                else
-                    f[e] = p[e];
-            }
+            f[i * 4] = __uint_as_float(raw.w[i].x), f[i * 4 + 1] = __uint_as_float(raw.w[i].y);
+            f[i * 4 + 2] = __uint_as_float(raw.w[i].z), f[i * 4 + 3] = __uint_as_float(raw.w[i].w);
         }
     }
 }
 
 template <typename T>
-__device__ __forceinline__ void store16(T *p, uint32_t count, bool vec, const float (&f)[16]) {
-    if (vec && count >= 16) {
-        if constexpr (sizeof(T) == 2) {
-            uint32_t w[8];
+__device__ __forceinline__ void store16(T *p, const float (&f)[16]) {
+    if constexpr (sizeof(T) == 2) {
+        uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = f32x2_to_bf16x2_rne(f[2 * e], f[2 * e + 1]);
-            reinterpret_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            reinterpret_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                reinterpret_cast<float4 *>(p)[i] = make_float4(f[i * 4], f[i * 4 + 1], f[i * 4 + 2], f[i * 4 + 3]);
-        }
+        for (int e = 0; e < 8; ++e) w[e] = f32x2_to_bf16x2_rne(f[2 * e], f[2 * e + 1]);
+        reinterpret_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
     } else {
 #pragma unroll
-        for (uint32_t e = 0; e < 16; ++e)
-            if (e < count) {
-                if constexpr (sizeof(T) == 2)
-                    p[e] = rne(f[e]);
-                else
-                    p[e] = f[e];
-            }
+        for (int i = 0; i < 4; ++i)
+            reinterpret_cast<float4 *>(p)[i] = make_float4(f[i * 4], f[i * 4 + 1], f[i * 4 + 2], f[i * 4 + 3]);
     }
 }
 
-// y = base + v B^T of one chunk and this wavefront's 64 columns. A product has
-// 16 of the columns along its rows, taken so that a lane ends up with 16
-// neighbouring columns of a row over the four products. vs holds each row's v
-// in two bf16 parts, [row][2][rank]: along a product's 32 terms lie 16 ranks,
-// 8 at a time as (first part, second part), so that 16 bits of v take part.
-template <typename T, int RT, int NJ>
-__device__ __forceinline__ void lora_up_chunk(const uint16_t *b, uint32_t rank, uint32_t n, const T *base,
-                                              uint64_t base_ld, T *y, uint64_t y_ld, bool vec, uint32_t row0,
-                                              uint32_t rows, const uint8_t *list, const uint16_t *vs, uint32_t vs_ld,
-                                              uint32_t col0, uint32_t lane) {
-    const uint32_t c = lane & 15u, q = lane >> 4;
-    uint4 bfr[4][NJ];
+// Two parts of a value in bf16: rounded, and what the rounding lost (nothing of
+// an inf or NaN). part: 0 the first, 1 the second, of two values.
+__device__ __forceinline__ uint32_t parts_of(float x, float y, uint32_t part) {
+    const uint32_t hi = f32x2_to_bf16x2_rne(x, y);
+    const float h0 = bf(hi & 0xFFFFu), h1 = bf(hi >> 16);
+    const uint32_t lo = f32x2_to_bf16x2_rne(fabsf(h0) < INFINITY ? x - h0 : 0.0f, fabsf(h1) < INFINITY ? y - h1 : 0.0f);
+    return part ? lo : hi;
+}
+
+// v B^T of 16 rows and 64 columns. A product has 16 of the columns along its
+// rows and the rows along its columns, so that a lane holds 4 columns of row c
+// per product; along its 32 terms lie 16 ranks, 8 at a time as (first part,
+// second part) of v, so that 16 bits of v take part. WIDE: the columns of the
+// four products are taken so that a lane's 16 are neighbours (from q * 16 on),
+// else product t has columns 16 t .. 16 t + 15 and a lane 4 from t * 16 + q * 4.
+template <int NJ, bool WIDE>
+__device__ __forceinline__ void request_b(const uint16_t *b, uint32_t rank, uint32_t n, uint32_t col0, uint32_t c,
+                                          uint32_t q, uint4 (&f)[4][NJ]) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const uint16_t *br = b + static_cast<uint64_t>(min(col0 + c / 4 * 16 + t * 4 + c % 4, n - 1)) * rank;
+        const uint32_t col = min(col0 + (WIDE ? c / 4 * 16 + t * 4 + c % 4 : t * 16 + c), n - 1);
+        const uint16_t *br = b + static_cast<uint64_t>(col) * rank;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const uint32_t r = (2 * j + q / 2) * 8;
-            bfr[t][j] = *reinterpret_cast<const uint4 *>(br + min(r, rank - 8));
-            if (r >= rank) bfr[t][j] = make_uint4(0, 0, 0, 0);
-        }
-    }
-    const uint32_t col = col0 + q * 16, count = col < n ? n - col : 0;
-    // the next row tile's base is requested before a tile's products
-    float f[2][16];
-    uint64_t row[2];
-    row[0] = row0 + list[min(c, rows - 1)];
-    load16(base + row[0] * base_ld + (count ? col : 0), count, vec, f[0]);
-    __syncthreads();  // vs is written
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        if (t * 16 >= rows) break;
-        if (t + 1 < RT) {
-            row[(t + 1) & 1] = row0 + list[min((t + 1) * 16 + c, rows - 1)];
-            load16(base + row[(t + 1) & 1] * base_ld + (count ? col : 0), count, vec, f[(t + 1) & 1]);
-        }
-        lo_f32x4_t acc[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) acc[u] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const uint32_t r = (2 * j + q / 2) * 8;
-            uint4 vf = *reinterpret_cast<const uint4 *>(vs + min(t * 16 + c, rows - 1) * vs_ld + (q & 1) * rank +
-                                                        min(r, rank - 8));
-            if (r >= rank) vf = make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) acc[u] = lo_mfma(bfr[u][j], vf, acc[u]);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) f[t & 1][e] += acc[e / 4][e % 4];
-        if (t * 16 + c < rows && count) store16(y + row[t & 1] * y_ld + col, count, vec, f[t & 1]);
+        for (int j = 0; j < NJ; ++j) f[t][j] = *reinterpret_cast<const uint4 *>(br + min((2 * j + q / 2) * 8, rank - 8));
     }
 }
 
-// Block (columns, window, slot).
+// vf: lane's terms of v, zero past the rank.
+template <int NJ>
+__device__ __forceinline__ void products(const uint4 (&bfr)[4][NJ], const uint4 (&vf)[NJ], uint32_t rank, uint32_t q,
+                                         lo_f32x4_t (&acc)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc[u] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            acc[u] = lo_mfma((2 * j + q / 2) * 8 < rank ? bfr[u][j] : make_uint4(0, 0, 0, 0), vf[j], acc[u]);
+}
+
+template <typename T>
+__device__ __forceinline__ T plus(T base, float d) {
+    if constexpr (sizeof(T) == 2)
+        return rne(bf(base) + d);
+    else
+        return base + d;
+}
+
+// Up to R rows of a chunk through LDS (tile: this wavefront's), `tiles` times 64
+// columns: a lane has one column of each row, so that rows are read and written
+// in whole lines whatever their alignment and however few they are. The next 64
+// columns are requested before a tile's products.
+template <typename T, int NJ, int R>
+struct RowsTile {
+    uint4 b[4][NJ];
+    T base[R];
+};
+
+template <typename T, int NJ, int R>
+__device__ __forceinline__ void lora_up_rows(const uint16_t *b, const uint4 (&vf)[NJ], uint32_t rank, uint32_t n,
+                                             const T *base, uint64_t base_ld, T *y, uint64_t y_ld, uint32_t mine,
+                                             uint32_t rows, uint32_t col0, uint32_t tiles, float (*tile)[68],
+                                             uint32_t lane) {
+    const uint32_t c = lane & 15u, q = lane >> 4;
+    auto row = [&](int i) { return static_cast<uint64_t>(__builtin_amdgcn_readlane(mine, min(i, static_cast<int>(rows) - 1))); };
+    auto request = [&](RowsTile<T, NJ, R> &x, uint32_t u) {
+        const uint32_t at = col0 + min(u, tiles - 1) * 64;
+        request_b<NJ, false>(b, rank, n, at, c, q, x.b);
+#pragma unroll
+        for (int i = 0; i < R; ++i) x.base[i] = (base + row(i) * base_ld)[min(at + lane, n - 1)];
+    };
+    auto finish = [&](const RowsTile<T, NJ, R> &x, uint32_t u) {
+        const uint32_t col = col0 + u * 64 + lane;
+        lo_f32x4_t acc[4];
+        products<NJ>(x.b, vf, rank, q, acc);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            *reinterpret_cast<lo_f32x4_t *>(&tile[c][t * 16 + q * 4]) = acc[t];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (i < static_cast<int>(rows) && col < n) (y + row(i) * y_ld)[col] = plus(x.base[i], tile[i][lane]);
+        __builtin_amdgcn_wave_barrier();
+    };
+    RowsTile<T, NJ, R> one, two;
+    request(one, 0);
+    for (uint32_t u = 0; u < tiles; u += 2) {
+        request(two, u + 1);
+        finish(one, u);
+        if (u + 1 >= tiles) break;
+        request(one, u + 2);
+        finish(two, u + 1);
+    }
+}
+
+// Block (columns, window, slot); a wavefront takes `tiles` times 64 columns.
+// Chunks of up to 16 rows: each wavefront forms its terms of v from the splits'
+// sums by itself, with no barrier. Larger ones: v is formed once for the block,
+// in LDS; wide: a lane reads and writes 16 neighbouring columns of a row (n a
+// multiple of 16, rows 16-byte aligned).
 template <typename T, int Q, int NJ>
 __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__restrict__ v, uint32_t splits, uint32_t m,
                                                                const uint16_t *__restrict__ b,
                                                                const float *__restrict__ scales, uint32_t n_adapters,
                                                                uint32_t rank, uint32_t n,
                                                                const uint32_t *__restrict__ adapters, const T *base,
-                                                               uint64_t base_ld, T *y, uint64_t y_ld, bool vec) {
-    constexpr int kLoads = 8;  // splits' sums requested together
+                                                               uint64_t base_ld, T *y, uint64_t y_ld, bool wide,
+                                                               uint32_t tiles) {
+    constexpr int kLoads = 4;                  // splits' sums requested together
+    constexpr int P = sizeof(T) == 2 ? 4 : 2;  // row tiles requested together
     __shared__ uint8_t lists[kLoraWaves][64];
     __shared__ uint64_t leads[Q];
     __shared__ __attribute__((aligned(16))) uint16_t vs[64 * (2 * 16 * NJ + 8)];
+    __shared__ __attribute__((aligned(16))) float tile[kLoraWaves][16][68];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.y * 64 * Q;
-    const uint32_t col0 = blockIdx.x * kLoraCols + wave * 64, vs_ld = 2 * rank + 8, quads = rank / 4;
+    const uint32_t c = lane & 15u, q = lane >> 4, vs_ld = 2 * rank + 8, quads = rank / 4;
+    const uint32_t col0 = (blockIdx.x * kLoraWaves + wave) * tiles * 64;
     const uint64_t split = static_cast<uint64_t>(m) * rank;
     const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
+    // the sums of 4 ranks of a row over the splits
+    auto add_splits = [&](const float *p, float (&f)[4]) {
+        f[0] = f[1] = f[2] = f[3] = 0.0f;
+        for (uint32_t u0 = 0; u0 < splits; u0 += kLoads) {
+            float4 part[kLoads];
+#pragma unroll
+            for (uint32_t u = 0; u < kLoads; ++u)
+                part[u] = *reinterpret_cast<const float4 *>(p + min(u0 + u, splits - 1) * split);
+#pragma unroll
+            for (uint32_t u = 0; u < kLoads; ++u)
+                if (u0 + u < splits) f[0] += part[u].x, f[1] += part[u].y, f[2] += part[u].z, f[3] += part[u].w;
+        }
+    };
     for (uint32_t item = blockIdx.z; item < o.chunks; item += gridDim.z) {
         uint32_t rows;
         const uint8_t *list = lists[wave];
         const uint32_t id = chunk_of<Q>(o, item, lane, lists[wave], rows);
         const float scale = scales[id];
+        const uint16_t *bu = b + static_cast<uint64_t>(id) * n * rank;
+        if (rows <= 16) {
+            if (col0 >= n) continue;
+            const uint32_t mine = row0 + list[min(c, rows - 1)];
+            uint4 vf[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t r = (2 * j + q / 2) * 8;
+                const float *p = v + static_cast<uint64_t>(mine) * rank + min(r, rank - 8);
+                float f[4], g[4];
+                add_splits(p, f);
+                add_splits(p + 4, g);
+                vf[j] = make_uint4(parts_of(f[0] * scale, f[1] * scale, q & 1), parts_of(f[2] * scale, f[3] * scale, q & 1),
+                                   parts_of(g[0] * scale, g[1] * scale, q & 1), parts_of(g[2] * scale, g[3] * scale, q & 1));
+                if (r >= rank) vf[j] = make_uint4(0, 0, 0, 0);
+            }
+            if (rows <= 4)
+                lora_up_rows<T, NJ, 4>(bu, vf, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave], lane);
+            else
+                lora_up_rows<T, NJ, 16>(bu, vf, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave], lane);
+            continue;
+        }
         for (uint32_t i = threadIdx.x; i < rows * quads; i += kLoraThreads) {
             const uint32_t member = i / quads, r = i % quads * 4;
-            const float *p = v + static_cast<uint64_t>(row0 + list[member]) * rank + r;
-            float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t u0 = 0; u0 < splits; u0 += kLoads) {
-                float4 part[kLoads];
+            float f[4];
+            add_splits(v + static_cast<uint64_t>(row0 + list[member]) * rank + r, f);
 #pragma unroll
-                for (uint32_t u = 0; u < kLoads; ++u)
-                    part[u] = *reinterpret_cast<const float4 *>(p + min(u0 + u, splits - 1) * split);
-#pragma unroll
-                for (uint32_t u = 0; u < kLoads; ++u)
-                    if (u0 + u < splits) f[0] += part[u].x, f[1] += part[u].y, f[2] += part[u].z, f[3] += part[u].w;
-            }
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float f0 = f[2 * e] * scale, f1 = f[2 * e + 1] * scale;
-                hi[e] = f32x2_to_bf16x2_rne(f0, f1);
-                // what the rounding lost; nothing where it is inf or NaN
-                const float h0 = bf(hi[e] & 0xFFFFu), h1 = bf(hi[e] >> 16);
-                lo[e] = f32x2_to_bf16x2_rne(fabsf(h0) < INFINITY ? f0 - h0 : 0.0f, fabsf(h1) < INFINITY ? f1 - h1 : 0.0f);
-            }
-            *reinterpret_cast<uint2 *>(vs + member * vs_ld + r) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2 *>(vs + member * vs_ld + rank + r) = make_uint2(lo[0], lo[1]);
+            for (uint32_t part = 0; part < 2; ++part)
+                *reinterpret_cast<uint2 *>(vs + member * vs_ld + part * rank + r) =
+                    make_uint2(parts_of(f[0] * scale, f[1] * scale, part), parts_of(f[2] * scale, f[3] * scale, part));
         }
-        const uint16_t *bu = b + static_cast<uint64_t>(id) * n * rank;
-        if (rows <= 16)
-            lora_up_chunk<T, 1, NJ>(bu, rank, n, base, base_ld, y, y_ld, vec, row0, rows, list, vs, vs_ld, col0, lane);
-        else
-            lora_up_chunk<T, 4, NJ>(bu, rank, n, base, base_ld, y, y_ld, vec, row0, rows, list, vs, vs_ld, col0, lane);
+        __syncthreads();
+        auto terms = [&](uint32_t member, uint4 (&vf)[NJ]) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t r = (2 * j + q / 2) * 8;
+                vf[j] = *reinterpret_cast<const uint4 *>(vs + min(member, rows - 1) * vs_ld + (q & 1) * rank +
+                                                         min(r, rank - 8));
+                if (r >= rank) vf[j] = make_uint4(0, 0, 0, 0);
+            }
+        };
+        if (!wide) {
+            for (uint32_t t = 0; t * 16 < rows && col0 < n; ++t) {
+                uint4 vf[NJ];
+                terms(t * 16 + c, vf);
+                lora_up_rows<T, NJ, 16>(bu, vf, rank, n, base, base_ld, y, y_ld, row0 + list[min(t * 16 + c, rows - 1)],
+                                        min(rows - t * 16, 16u), col0, tiles, tile[wave], lane);
+            }
+        } else {
+            for (uint32_t u = 0; u < tiles && col0 + u * 64 < n; ++u) {
+                uint4 bfr[4][NJ];
+                request_b<NJ, true>(bu, rank, n, col0 + u * 64, c, q, bfr);
+                const uint32_t col = min(col0 + u * 64 + q * 16, n - 16);  // the last ones twice where n ends before
+                for (uint32_t t0 = 0; t0 * 16 < rows; t0 += P) {
+                    Raw16<T> raw[P];
+#pragma unroll
+                    for (int t = 0; t < P; ++t)
+                        raw[t] = request16(base + static_cast<uint64_t>(row0 + list[min((t0 + t) * 16 + c, rows - 1)]) * base_ld +
+                                           col);
+#pragma unroll
+                    for (int t = 0; t < P; ++t) {
+                        const uint32_t member = (t0 + t) * 16 + c;
+                        uint4 vf[NJ];
+                        terms(member, vf);
+                        lo_f32x4_t acc[4];
+                        products<NJ>(bfr, vf, rank, q, acc);
+                        float f[16];
+                        floats16(raw[t], f);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) f[e] += acc[e / 4][e % 4];
+                        if (member < rows && col0 + u * 64 + q * 16 < n)
+                            store16(y + static_cast<uint64_t>(row0 + list[member]) * y_ld + col, f);
+                    }
+                }
+            }
+        }
         __syncthreads();  // vs is read
     }
     // rows without an adapter are base, where y is not
@@ -425,8 +519,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
         for (; bare; bare &= bare - 1, ++turn) {
             if (turn % gridDim.z != blockIdx.z) continue;
             const uint64_t row = row0 + w * 64 + __builtin_ctzll(bare);
-            for (uint32_t e = blockIdx.x * kLoraCols + threadIdx.x; e < min(n, (blockIdx.x + 1) * kLoraCols);
-                 e += kLoraThreads)
+            const uint32_t cols = kLoraWaves * tiles * 64;
+            for (uint32_t e = blockIdx.x * cols + threadIdx.x; e < min(n, (blockIdx.x + 1) * cols); e += kLoraThreads)
                 y[row * y_ld + e] = base[row * base_ld + e];
         }
     }
@@ -442,6 +536,7 @@ namespace {
 // `steps` x 32.
 struct Split {
     uint32_t quads, windows, splits, steps;
+    uint64_t chunks;  // expected
 };
 
 Split split_of(int64_t m, int64_t k) {
@@ -449,8 +544,10 @@ Split split_of(int64_t m, int64_t k) {
     s.quads = m > 64 && m <= kWideRows ? 4 : 1;
     s.windows = static_cast<uint32_t>((m + 64 * s.quads - 1) / (64 * s.quads));
     const uint64_t steps = (k + 31) / 32, least = kLoraWaves * kDownSteps;
-    const uint64_t want = std::max<uint64_t>(1, kDownBlocks / std::max<uint64_t>(1, (m + 63) / 64));
-    const uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>({want, (steps + least - 1) / least, kMaxSplits}));
+    // a few rows are mostly of different adapters, many mostly of the same
+    s.chunks = std::max<uint64_t>(1, m <= kWideRows ? m / 4 : (m + 63) / 64);
+    const uint64_t splits =
+        std::clamp<uint64_t>(std::min(kDownBlocks / s.chunks, (steps + least - 1) / least), 1, kMaxSplits);
     s.steps = static_cast<uint32_t>((steps + splits * kLoraWaves - 1) / (splits * kLoraWaves));
     s.splits = static_cast<uint32_t>((steps + s.steps * kLoraWaves - 1) / (s.steps * kLoraWaves));
     return s;
@@ -530,7 +627,9 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     const Split w = split_of(m, k);
     if (w.windows > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: m %lld", fn, (long long)m);
     if (int rc = set_current(dev, fn)) return rc;
-    const uint32_t cols = static_cast<uint32_t>((n + kLoraCols - 1) / kLoraCols);
+    const uint64_t tiles_of_all = w.chunks * ((n + 63) / 64);
+    const uint32_t tiles = static_cast<uint32_t>(std::clamp<uint64_t>(tiles_of_all / kUpWaves, 1, kMaxTiles));
+    const uint32_t cols = static_cast<uint32_t>((n + kLoraWaves * 64 * tiles - 1) / (kLoraWaves * 64 * tiles));
     // a window has at most as many chunks as rows
     const uint32_t most = static_cast<uint32_t>(std::min<int64_t>(m, 64 * w.quads));
     const uint32_t down_slots = std::clamp(kDownSlots / (w.windows * w.splits), 1u, most);
@@ -540,8 +639,8 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     float *v = static_cast<float *>(workspace);
     const uint32_t m32 = static_cast<uint32_t>(m), k32 = static_cast<uint32_t>(k), n32 = static_cast<uint32_t>(n);
     const uint32_t rank32 = static_cast<uint32_t>(rank), u32 = static_cast<uint32_t>(n_adapters);
-    const bool vec = ((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0 &&
-                     base_ld * elem % 16 == 0 && y_ld * elem % 16 == 0;
+    const bool wide = ((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0 &&
+                     base_ld * elem % 16 == 0 && y_ld * elem % 16 == 0 && n % 16 == 0;
     auto run_down = [&](auto kernel) {
         return dispatch(dev, fn, [&] {
             hipLaunchKernelGGL(kernel, down, threads, 0, dev->stream, x, m32, k32, static_cast<uint64_t>(x_ld), a, u32,
@@ -553,7 +652,7 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
         return dispatch(dev, fn, [&] {
             hipLaunchKernelGGL(kernel, up, threads, 0, dev->stream, v, w.splits, m32, b, scales, u32, rank32, n32,
                                adapters, static_cast<const T *>(base), static_cast<uint64_t>(base_ld),
-                               static_cast<T *>(y), static_cast<uint64_t>(y_ld), vec);
+                               static_cast<T *>(y), static_cast<uint64_t>(y_ld), wide, tiles);
         });
     };
     // rank tiles of 16: 1, 2, 4 or 8
