@@ -360,13 +360,13 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, const uint4 (&vf
     const uint32_t c = lane & 15u, q = lane >> 4;
     auto row = [&](int i) { return static_cast<uint64_t>(__builtin_amdgcn_readlane(mine, min(i, static_cast<int>(rows) - 1))); };
     auto request = [&](RowsTile<T, NJ, R> &x, uint32_t u) {
-        const uint32_t at = col0 + min(u, tiles - 1) * 64;
+        const uint32_t at = col0 + min(u, tiles - 1) * kLoraWaves * 64;
         request_b<NJ, false>(b, rank, n, at, c, q, x.b);
 #pragma unroll
         for (int i = 0; i < R; ++i) x.base[i] = (base + row(i) * base_ld)[min(at + lane, n - 1)];
     };
     auto finish = [&](const RowsTile<T, NJ, R> &x, uint32_t u) {
-        const uint32_t col = col0 + u * 64 + lane;
+        const uint32_t col = col0 + u * kLoraWaves * 64 + lane;
         lo_f32x4_t acc[4];
         products<NJ>(x.b, vf, rank, q, acc);
 #pragma unroll
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
     __shared__ __attribute__((aligned(16))) float tile[kLoraWaves][16][68];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.y * 64 * Q;
     const uint32_t c = lane & 15u, q = lane >> 4, vs_ld = 2 * rank + 8, quads = rank / 4;
-    const uint32_t col0 = (blockIdx.x * kLoraWaves + wave) * tiles * 64;
+    const uint32_t col0 = (blockIdx.x * tiles * kLoraWaves + wave) * 64;  // then every kLoraWaves-th tile
     const uint64_t split = static_cast<uint64_t>(m) * rank;
     const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
     // the sums of 4 ranks of a row over the splits
@@ -480,10 +480,12 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
                                         min(rows - t * 16, 16u), col0, tiles, tile[wave], lane);
             }
         } else {
-            for (uint32_t u = 0; u < tiles && col0 + u * 64 < n; ++u) {
+            for (uint32_t u = 0; u < tiles; ++u) {
+                const uint32_t first = col0 + u * kLoraWaves * 64;
+                if (first >= n) break;
                 uint4 bfr[4][NJ];
-                request_b<NJ, true>(bu, rank, n, col0 + u * 64, c, q, bfr);
-                const uint32_t col = min(col0 + u * 64 + q * 16, n - 16);  // the last ones twice where n ends before
+                request_b<NJ, true>(bu, rank, n, first, c, q, bfr);
+                const uint32_t col = min(first + q * 16, n - 16);  // the last ones twice where n ends before
                 for (uint32_t t0 = 0; t0 * 16 < rows; t0 += P) {
                     Raw16<T> raw[P];
 #pragma unroll
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
                         floats16(raw[t], f);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) f[e] += acc[e / 4][e % 4];
-                        if (member < rows && col0 + u * 64 + q * 16 < n)
+                        if (member < rows && first + q * 16 < n)
                             store16(y + static_cast<uint64_t>(row0 + list[member]) * y_ld + col, f);
                     }
                 }
