@@ -3,70 +3,183 @@
 
 namespace fh {
 
-// Tokens of one block: their counts and bias entries are a table in LDS.
-constexpr uint32_t kRuleChunk = 4096;
+// Bound by memory: the logits go through once, in pieces of 16 bytes where
+// their rows are so aligned (a row's first piece may begin before it). What a
+// token needs to know of the row's lists stands in LDS: a block takes a run of
+// up to kRuleTokens tokens, counts the whole history into a table of them, and
+// enters the bias list into another. Every block of a row reads its lists, from
+// the L2: runs are as long as the LDS and a filled GPU allow.
+constexpr uint32_t kRuleTokens = 2048;
+constexpr uint32_t kRuleThreads = 256;
+// Blocks that a launch aims for before runs get longer than the shortest, of
+// kRuleTokens / 4.
+constexpr uint32_t kRuleBlocks = 2048;
 
-// Block (chunk of tokens, row): the row's history is counted into the chunk's
-// table (bit 31: said at all; bits 0..30: times generated) and the row's bias
-// list entered into another (entry index + 1, the last of one id staying),
-// then each logit of the chunk goes through the rules. Whole-number LDS
-// atomics: the result does not depend on their order. Contraction is off, so
-// that each step is one fp32 rounding.
-template <typename T>
-__global__ __launch_bounds__(256) void logit_rules_kernel(const T *z, uint32_t n, fh_logit_rules rules, T *out) {
-#pragma clang fp contract(off)
-    __shared__ uint32_t said[kRuleChunk], entry[kRuleChunk];
-    const uint32_t r = blockIdx.y, lo = blockIdx.x * kRuleChunk, count = min(kRuleChunk, n - lo);
-    for (uint32_t i = threadIdx.x; i < kRuleChunk; i += 256) said[i] = entry[i] = 0;
-    __syncthreads();
-    if (rules.history) {
-        const uint32_t *ids = rules.history + static_cast<uint64_t>(r) * rules.history_ld;
-        const uint32_t used = min(rules.history_len[r], static_cast<uint32_t>(rules.history_ld));
-        const uint32_t prompt = rules.prompt_len ? rules.prompt_len[r] : 0;
-        for (uint32_t i = threadIdx.x; i < used; i += 256) {
-            const uint32_t at = ids[i] - lo;
-            if (ids[i] >= lo && at < count) {
-                atomicOr(&said[at], 0x80000000u);
-                if (i >= prompt) atomicAdd(&said[at], 1u);
+// Calls take(i, list[i]) for i < n: 16-byte loads where the list is aligned,
+// several requested together (the list's last words again past its end).
+template <typename Take>
+__device__ __forceinline__ void for_list(const uint32_t *list, uint32_t n, Take take) {
+    constexpr uint32_t kLoads = 4;
+    if (n == 0) return;
+    if ((reinterpret_cast<uintptr_t>(list) & 15u) == 0) {
+        const uint32_t quads = n / 4;
+        for (uint32_t q0 = threadIdx.x; q0 < quads; q0 += kRuleThreads * kLoads) {
+            uint4 v[kLoads];
+#pragma unroll
+            for (uint32_t u = 0; u < kLoads; ++u)
+                v[u] = reinterpret_cast<const uint4 *>(list)[min(q0 + u * kRuleThreads, quads - 1)];
+#pragma unroll
+            for (uint32_t u = 0; u < kLoads; ++u) {
+                const uint32_t i = (q0 + u * kRuleThreads) * 4;
+                if (q0 + u * kRuleThreads < quads) take(i, v[u].x), take(i + 1, v[u].y), take(i + 2, v[u].z), take(i + 3, v[u].w);
             }
         }
+        if (threadIdx.x < n % 4) take(quads * 4 + threadIdx.x, list[quads * 4 + threadIdx.x]);
+        return;
     }
-    if (rules.bias_ids) {
-        const uint32_t *ids = rules.bias_ids + static_cast<uint64_t>(r) * rules.bias_ld;
-        uint32_t used = static_cast<uint32_t>(rules.bias_ld);
-        if (rules.bias_len) used = min(used, rules.bias_len[r]);
-        for (uint32_t i = threadIdx.x; i < used; i += 256) {
-            const uint32_t at = ids[i] - lo;
-            if (ids[i] >= lo && at < count) atomicMax(&entry[at], i + 1);
-        }
+    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += kRuleThreads * kLoads) {
+        uint32_t v[kLoads];
+#pragma unroll
+        for (uint32_t u = 0; u < kLoads; ++u) v[u] = list[min(i0 + u * kRuleThreads, n - 1)];
+#pragma unroll
+        for (uint32_t u = 0; u < kLoads; ++u)
+            if (i0 + u * kRuleThreads < n) take(i0 + u * kRuleThreads, v[u]);
     }
-    __syncthreads();
+}
+
+// Block (run, row). said: bit 31 for an id of the prompt, the rest its count
+// among the generated. entry: a bias entry's index + 1, the last of one id
+// staying. Whole-number LDS atomics: their order does not matter. Contraction is
+// off, so that each step is one fp32 rounding.
+template <typename T>
+__global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(const T *z, uint32_t n, uint32_t run,
+                                                                   const fh_logit_rules rules, T *out) {
+#pragma clang fp contract(off)
+    constexpr uint32_t E = 16 / sizeof(T);  // logits of a piece
+    constexpr uint32_t kPieces = kRuleTokens / (kRuleThreads * E);
+    __shared__ __attribute__((aligned(16))) uint32_t said[kRuleTokens], entry[kRuleTokens];
+    const uint32_t r = blockIdx.y;
+    const T *from = z + static_cast<uint64_t>(r) * n;
+    T *to = out + static_cast<uint64_t>(r) * n;
+    // tokens before the row that its first piece begins with
+    const uint32_t before = (reinterpret_cast<uintptr_t>(from) & 15u) / sizeof(T);
+    const bool same = ((reinterpret_cast<uintptr_t>(from) ^ reinterpret_cast<uintptr_t>(to)) & 15u) == 0;
+    // this run: tokens lo .. lo + run - 1 (lo < 0 where the first piece begins before the row)
+    const int32_t lo = static_cast<int32_t>(blockIdx.x * run) - static_cast<int32_t>(before);
+    if (lo >= static_cast<int32_t>(n)) return;
+    const bool history = rules.history != nullptr, bias = rules.bias_ids != nullptr;
     const float rep = rules.repetition ? rules.repetition[r] : 1.0f;
     const float freq = rules.frequency ? rules.frequency[r] : 0.0f;
     const float pres = rules.presence ? rules.presence[r] : 0.0f;
-    const uint32_t words = (n + 31) / 32;
-    for (uint32_t i = threadIdx.x; i < count; i += 256) {
-        const uint64_t at = static_cast<uint64_t>(r) * n + lo + i;
-        float v;
-        if constexpr (sizeof(T) == 2)
-            v = bf(z[at]);
-        else
-            v = z[at];
-        const uint32_t s = said[i], times = s & 0x7FFFFFFFu;
+    const uint32_t said_len = history ? min(rules.history_len[r], static_cast<uint32_t>(rules.history_ld)) : 0;
+    const uint32_t prompt = history && rules.prompt_len ? rules.prompt_len[r] : 0;
+    const uint32_t bias_ld = static_cast<uint32_t>(rules.bias_ld);
+    const uint32_t bias_used = bias && rules.bias_len ? min(bias_ld, rules.bias_len[r]) : bias_ld;
+    const float *values = bias ? rules.bias_values + static_cast<uint64_t>(r) * rules.bias_ld : nullptr;
+    const uint32_t *mask = rules.mask ? rules.mask + static_cast<uint64_t>(r) * ((n + 31) / 32) : nullptr;
+    // the thread's whole pieces and their mask bits are requested before the lists are gone through
+    uint4 raw[kPieces];
+    uint32_t bits[kPieces][2];
+#pragma unroll
+    for (uint32_t p = 0; p < kPieces; ++p) {
+        const uint32_t at = (p * kRuleThreads + threadIdx.x) * E;
+        const int32_t j0 = lo + static_cast<int32_t>(at);
+        if (at < run && j0 >= 0 && j0 + E <= n) {
+            raw[p] = *reinterpret_cast<const uint4 *>(from + j0);
+            bits[p][0] = mask ? mask[j0 / 32] : ~0u;
+            bits[p][1] = mask ? mask[(j0 + E - 1) / 32] : ~0u;
+        }
+    }
+    for (uint32_t i = threadIdx.x * 4; i < run; i += kRuleThreads * 4) {
+        if (history) *reinterpret_cast<uint4 *>(said + i) = make_uint4(0, 0, 0, 0);
+        if (bias) *reinterpret_cast<uint4 *>(entry + i) = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    if (history)
+        for_list(rules.history + static_cast<uint64_t>(r) * rules.history_ld, said_len, [&](uint32_t i, uint32_t id) {
+            const uint32_t at = id - static_cast<uint32_t>(lo);
+            if (id >= n || at >= run) return;
+            if (i < prompt)
+                atomicOr(&said[at], 0x80000000u);
+            else
+                atomicAdd(&said[at], 1u);
+        });
+    if (bias)
+        for_list(rules.bias_ids + static_cast<uint64_t>(r) * rules.bias_ld, bias_used, [&](uint32_t i, uint32_t id) {
+            const uint32_t at = id - static_cast<uint32_t>(lo);
+            if (id < n && at < run) atomicMax(&entry[at], i + 1);
+        });
+    __syncthreads();
+    // one logit: s its word of said, e of entry
+    auto apply = [&](float v, uint32_t s, uint32_t e) {
+        const uint32_t times = s & 0x7FFFFFFFu;
         if (rules.repetition && s) v = v > 0.0f ? v / rep : v * rep;
         if (times) {
             if (rules.frequency) v = v - freq * static_cast<float>(times);
             if (rules.presence) v = v - pres;
         }
-        if (entry[i]) v = v + rules.bias_values[static_cast<uint64_t>(r) * rules.bias_ld + entry[i] - 1];
-        if (rules.mask) {
-            const uint32_t j = lo + i;
-            if (!(rules.mask[static_cast<uint64_t>(r) * words + j / 32] >> (j % 32) & 1u)) v = -INFINITY;
+        if (e) v = v + values[e - 1];
+        return v;
+    };
+#pragma unroll
+    for (uint32_t p = 0; p < kPieces; ++p) {
+        const uint32_t at = (p * kRuleThreads + threadIdx.x) * E;
+        const int32_t j0 = lo + static_cast<int32_t>(at);
+        if (at >= run || j0 >= static_cast<int32_t>(n)) break;
+        if (j0 >= 0 && j0 + E <= n) {
+            const uint32_t allow = (static_cast<uint64_t>(bits[p][1]) << 32 | bits[p][0]) >> (j0 % 32);
+            float v[E];
+            if constexpr (sizeof(T) == 2) {
+                unpack8(raw[p], v);
+            } else {
+                v[0] = __uint_as_float(raw[p].x), v[1] = __uint_as_float(raw[p].y);
+                v[2] = __uint_as_float(raw[p].z), v[3] = __uint_as_float(raw[p].w);
+            }
+            uint32_t s[E], e[E], any = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < E; i += 4) {
+                const uint4 a = history ? *reinterpret_cast<const uint4 *>(said + at + i) : make_uint4(0, 0, 0, 0);
+                const uint4 b = bias ? *reinterpret_cast<const uint4 *>(entry + at + i) : make_uint4(0, 0, 0, 0);
+                s[i] = a.x, s[i + 1] = a.y, s[i + 2] = a.z, s[i + 3] = a.w;
+                e[i] = b.x, e[i + 1] = b.y, e[i + 2] = b.z, e[i + 3] = b.w;
+                any |= a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w;
+            }
+            if (any)
+#pragma unroll
+                for (uint32_t i = 0; i < E; ++i) v[i] = apply(v[i], s[i], e[i]);
+#pragma unroll
+            for (uint32_t i = 0; i < E; ++i)
+                if (!(allow >> i & 1)) v[i] = -INFINITY;
+            uint4 o;
+            if constexpr (sizeof(T) == 2)
+                o = make_uint4(f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]),
+                               f32x2_to_bf16x2_rne(v[4], v[5]), f32x2_to_bf16x2_rne(v[6], v[7]));
+            else
+                o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            if (same) {
+                *reinterpret_cast<uint4 *>(to + j0) = o;
+            } else {
+                const T *x = reinterpret_cast<const T *>(&o);
+#pragma unroll
+                for (uint32_t i = 0; i < E; ++i) to[j0 + i] = x[i];
+            }
+            continue;
         }
-        if constexpr (sizeof(T) == 2)
-            out[at] = rne(v);
-        else
-            out[at] = v;
+        // the row's ends
+        for (int32_t j = max(j0, 0); j < min(j0 + static_cast<int32_t>(E), static_cast<int32_t>(n)); ++j) {
+            const uint32_t i = j - lo;
+            float v;
+            if constexpr (sizeof(T) == 2)
+                v = bf(from[j]);
+            else
+                v = from[j];
+            v = apply(v, history ? said[i] : 0, bias ? entry[i] : 0);
+            if (mask && !(mask[j / 32] >> (j % 32) & 1u)) v = -INFINITY;
+            if constexpr (sizeof(T) == 2)
+                to[j] = rne(v);
+            else
+                to[j] = v;
+        }
     }
 }
 
@@ -83,6 +196,7 @@ extern "C" int fh_logits_process(fh_device *dev, const void *logits, int dtype, 
     if (int rc = fh_check_dims(fn, {rows, n, u.history_ld, u.bias_ld})) return rc;
     if (dtype != FH_BF16 && dtype != FH_F32)
         return fail(FH_ERR_DTYPE, "%s: dtype %d is neither F32 nor BF16", fn, dtype);
+    if (n > 0x7FFFFFFFll - 2 * kRuleTokens) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: n %lld", fn, (long long)n);
     if (rows > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld rows exceed 65535", fn, (long long)rows);
     if ((u.history == nullptr) != (u.history_len == nullptr))
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: history and history_len go together", fn);
@@ -121,15 +235,18 @@ extern "C" int fh_logits_process(fh_device *dev, const void *logits, int dtype, 
     if (u.mask)
         if (int rc = check_range(dev, u.mask, r * ((n + 31) / 32) * 4, fn, "mask")) return rc;
     if (int rc = set_current(dev, fn)) return rc;
-    const dim3 grid(static_cast<uint32_t>((n + kRuleChunk - 1) / kRuleChunk), static_cast<uint32_t>(rows));
+    uint32_t run = kRuleTokens / 4;
+    while (run < kRuleTokens && r * ((n + run - 1) / run) > kRuleBlocks) run *= 2;
+    // a run may begin up to a piece before its row
+    const dim3 grid(static_cast<uint32_t>((n + 16 / elem - 1 + run - 1) / run), static_cast<uint32_t>(rows));
     return dispatch(dev, fn, [&] {
         if (dtype == FH_F32)
-            hipLaunchKernelGGL(logit_rules_kernel<float>, grid, dim3(256), 0, dev->stream,
-                               static_cast<const float *>(logits), static_cast<uint32_t>(n), u,
+            hipLaunchKernelGGL(logit_rules_kernel<float>, grid, dim3(kRuleThreads), 0, dev->stream,
+                               static_cast<const float *>(logits), static_cast<uint32_t>(n), run, u,
                                static_cast<float *>(out));
         else
-            hipLaunchKernelGGL(logit_rules_kernel<uint16_t>, grid, dim3(256), 0, dev->stream,
-                               static_cast<const uint16_t *>(logits), static_cast<uint32_t>(n), u,
+            hipLaunchKernelGGL(logit_rules_kernel<uint16_t>, grid, dim3(kRuleThreads), 0, dev->stream,
+                               static_cast<const uint16_t *>(logits), static_cast<uint32_t>(n), run, u,
                                static_cast<uint16_t *>(out));
     });
 }
