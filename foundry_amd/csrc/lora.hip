@@ -42,7 +42,7 @@ constexpr uint32_t kDownSlots = 512, kUpSlots = 2048;
 constexpr uint32_t kLoraThreads = 256;
 constexpr uint32_t kLoraWaves = kLoraThreads / 64;
 // Wavefronts that the up product aims for, and 64-column tiles of one at most.
-constexpr uint32_t kUpWaves = 1024, kMaxTiles = 8;
+constexpr uint32_t kUpWaves = 2048, kMaxTiles = 8;
 
 // The rows of a window and its chunks. A row's rank is the number of rows
 // before it with its adapter; rows of rank 0, 64, .. lead a chunk, and the
@@ -150,21 +150,36 @@ __device__ __forceinline__ uint32_t chunk_of(const Window<Q> &o, uint32_t item, 
     return id;
 }
 
-// Sums over k0 .. k1 - 1 of 16 rows (xr: lane's) by NR tiles of 16 ranks (ar:
-// lane's). A product has the ranks along its rows, so that a lane ends up with
-// 4 ranks of a row.
-template <int NR>
-__device__ __forceinline__ void lora_down_tile(const uint16_t *xr, const uint16_t *const (&ar)[NR], uint32_t k, uint32_t k0,
-                                               uint32_t k1, uint32_t q, lo_f32x4_t (&acc)[NR]) {
-    constexpr int U = NR >= 8 ? 2 : NR >= 4 ? 4 : 8;  // steps of 32 requested together
+// v[split][row][r] = sum over the split's k of x[row, k] A[r, k], for a chunk of
+// up to 16 RT rows. Each wavefront takes a quarter of the split's k for all the
+// rows, so that A's rows come once per chunk; they add up in LDS in their order.
+// A product has the ranks along its rows, so that a lane ends up with 4 ranks of
+// a row. (With 16 rows and all the k to a wavefront A came four times: 17 us for
+// 4096 packed rows of k 4096, rank 32, as much of it A's as x's.)
+template <int RT, int NR>
+__device__ __forceinline__ void lora_down_chunk(const uint16_t *x, uint32_t k, uint64_t x_ld, const uint16_t *a,
+                                                uint32_t rank, uint32_t k0, uint32_t k1, uint32_t row0, uint32_t rows,
+                                                const uint8_t *list, float4 *sums, float *v, uint32_t lane,
+                                                uint32_t wave) {
+    constexpr int U = RT + NR <= 2 ? 8 : RT + NR <= 6 ? 4 : RT + NR <= 9 ? 2 : 1;  // steps of 32 requested together
+    const uint32_t c = lane & 15u, q = lane >> 4;
+    const uint16_t *xr[RT], *ar[NR];
 #pragma unroll
-    for (int r = 0; r < NR; ++r) acc[r] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < RT; ++t) xr[t] = x + (row0 + list[min(t * 16 + c, rows - 1)]) * x_ld;
+#pragma unroll
+    for (int t = 0; t < NR; ++t) ar[t] = a + static_cast<uint64_t>(min(t * 16 + c, rank - 1)) * k;
+    lo_f32x4_t acc[RT][NR];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) acc[t][r] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t s = k0; s < k1; s += 32 * U) {
-        uint4 xf[U], af[U][NR];
+        uint4 xf[U][RT], af[U][NR];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t at = min(s + u * 32 + q * 8, k - 8);  // clamped: the pieces past k1 are zeroed below
-            xf[u] = *reinterpret_cast<const uint4 *>(xr + at);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) xf[u][t] = *reinterpret_cast<const uint4 *>(xr[t] + at);
 #pragma unroll
             for (int t = 0; t < NR; ++t) af[u][t] = *reinterpret_cast<const uint4 *>(ar[t] + at);
         }
@@ -172,7 +187,8 @@ __device__ __forceinline__ void lora_down_tile(const uint16_t *xr, const uint16_
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (s + u * 32 + q * 8 >= k1) {
-                    xf[u] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) xf[u][t] = make_uint4(0, 0, 0, 0);
 #pragma unroll
                     for (int t = 0; t < NR; ++t) af[u][t] = make_uint4(0, 0, 0, 0);
                 }
@@ -180,14 +196,34 @@ __device__ __forceinline__ void lora_down_tile(const uint16_t *xr, const uint16_
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int r = 0; r < NR; ++r) acc[r] = lo_mfma(af[u][r], xf[u], acc[r]);
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) acc[t][r] = lo_mfma(af[u][r], xf[u][t], acc[t][r]);
+    }
+    // wavefront w adds to what those before it left; the last one's sums go out
+    for (uint32_t w = 0; w < kLoraWaves; ++w) {
+        if (w == wave) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float4 f = make_float4(acc[t][r][0], acc[t][r][1], acc[t][r][2], acc[t][r][3]);
+                    if (w) {
+                        const float4 o = sums[(t * NR + r) * 64 + lane];
+                        f = make_float4(o.x + f.x, o.y + f.y, o.z + f.z, o.w + f.w);
+                    }
+                    if (w + 1 < kLoraWaves)
+                        sums[(t * NR + r) * 64 + lane] = f;
+                    else if (t * 16 + c < rows && r * 16 + q * 4 < rank)
+                        *reinterpret_cast<float4 *>(v + static_cast<uint64_t>(row0 + list[t * 16 + c]) * rank + r * 16 +
+                                                    q * 4) = f;
+                }
+        }
+        __syncthreads();
     }
 }
 
-// v[split][row][r] = sum over the split's k of x[row, k] A[r, k]. Block (split,
-// window, slot). Up to 16 rows of a chunk: each wavefront takes a quarter of
-// the split's k, and they add up in LDS in their order. More: each takes 16 of
-// the rows over all of the split's k.
+// Block (split, window, slot).
 template <int Q, int NR>
 __global__ __launch_bounds__(kLoraThreads) void lora_down_kernel(const uint16_t *__restrict__ x, uint32_t m, uint32_t k,
                                                                  uint64_t x_ld, const uint16_t *__restrict__ a,
@@ -196,55 +232,20 @@ __global__ __launch_bounds__(kLoraThreads) void lora_down_kernel(const uint16_t 
                                                                  float *__restrict__ v) {
     __shared__ uint8_t lists[kLoraWaves][64];
     __shared__ uint64_t leads[Q];
-    __shared__ float4 sums[NR * 64];
+    __shared__ float4 sums[4 * NR * 64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.y * 64 * Q;
-    const uint32_t c = lane & 15u, q = lane >> 4;
-    // steps: of 32 k, of a quarter of the split
-    const uint32_t k0 = min(blockIdx.x * kLoraWaves * steps * 32, k), k1 = min(k0 + kLoraWaves * steps * 32, k);
+    // steps: of 32 k, of each wavefront
+    const uint32_t k0 = min((blockIdx.x * kLoraWaves + wave) * steps * 32, k), k1 = min(k0 + steps * 32, k);
     v += static_cast<uint64_t>(blockIdx.x) * m * rank;
     const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
     for (uint32_t item = blockIdx.z; item < o.chunks; item += gridDim.z) {
         uint32_t rows;
         const uint32_t id = chunk_of<Q>(o, item, lane, lists[wave], rows);
-        const uint8_t *list = lists[wave];
-        const bool few = rows <= 16;
-        const uint32_t member = (few ? 0 : wave * 16) + c;
-        const uint16_t *ar[NR];
-#pragma unroll
-        for (int t = 0; t < NR; ++t) ar[t] = a + (static_cast<uint64_t>(id) * rank + min(t * 16 + c, rank - 1)) * k;
-        const uint16_t *xr = x + (row0 + list[min(member, rows - 1)]) * x_ld;
-        const uint32_t from = few ? min(k0 + wave * steps * 32, k1) : k0;
-        lo_f32x4_t acc[NR];
-        lora_down_tile<NR>(xr, ar, k, from, few ? min(from + steps * 32, k1) : wave * 16 < rows ? k1 : from, q, acc);
-        float *to = v + static_cast<uint64_t>(row0 + list[min(member, rows - 1)]) * rank;
-        if (!few) {
-            if (member < rows) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-                    if (r * 16 + q * 4 < rank)
-                        *reinterpret_cast<float4 *>(to + r * 16 + q * 4) =
-                            make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-            }
-            continue;
-        }
-        // wavefront w adds to what those before it left; the last one's sums go out
-        for (uint32_t w = 0; w < kLoraWaves; ++w) {
-            if (w == wave) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    float4 f = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-                    if (w) {
-                        const float4 p = sums[r * 64 + lane];
-                        f = make_float4(p.x + f.x, p.y + f.y, p.z + f.z, p.w + f.w);
-                    }
-                    if (w + 1 < kLoraWaves)
-                        sums[r * 64 + lane] = f;
-                    else if (member < rows && r * 16 + q * 4 < rank)
-                        *reinterpret_cast<float4 *>(to + r * 16 + q * 4) = f;
-                }
-            }
-            __syncthreads();
-        }
+        const uint16_t *au = a + static_cast<uint64_t>(id) * rank * k;
+        if (rows <= 16)
+            lora_down_chunk<1, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, lists[wave], sums, v, lane, wave);
+        else
+            lora_down_chunk<4, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, lists[wave], sums, v, lane, wave);
     }
 }
 
@@ -352,7 +353,7 @@ struct RowsTile {
     T base[R];
 };
 
-template <typename T, int NJ, int R>
+template <typename T, int NJ, int R, bool AHEAD>
 __device__ __forceinline__ void lora_up_rows(const uint16_t *b, const uint4 (&vf)[NJ], uint32_t rank, uint32_t n,
                                              const T *base, uint64_t base_ld, T *y, uint64_t y_ld, uint32_t mine,
                                              uint32_t rows, uint32_t col0, uint32_t tiles, float (*tile)[68],
@@ -378,6 +379,14 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, const uint4 (&vf
             if (i < static_cast<int>(rows) && col < n) (y + row(i) * y_ld)[col] = plus(x.base[i], tile[i][lane]);
         __builtin_amdgcn_wave_barrier();
     };
+    if constexpr (!AHEAD) {
+        for (uint32_t u = 0; u < tiles; ++u) {
+            RowsTile<T, NJ, R> x;
+            request(x, u);
+            finish(x, u);
+        }
+        return;
+    }
     RowsTile<T, NJ, R> one, two;
     request(one, 0);
     for (uint32_t u = 0; u < tiles; u += 2) {
@@ -394,7 +403,7 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, const uint4 (&vf
 // sums by itself, with no barrier. Larger ones: v is formed once for the block,
 // in LDS; wide: a lane reads and writes 16 neighbouring columns of a row (n a
 // multiple of 16, rows 16-byte aligned).
-template <typename T, int Q, int NJ>
+template <typename T, int Q, int NJ, bool PACKED>
 __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__restrict__ v, uint32_t splits, uint32_t m,
                                                                const uint16_t *__restrict__ b,
                                                                const float *__restrict__ scales, uint32_t n_adapters,
@@ -447,10 +456,10 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
                                    parts_of(g[0] * scale, g[1] * scale, q & 1), parts_of(g[2] * scale, g[3] * scale, q & 1));
                 if (r >= rank) vf[j] = make_uint4(0, 0, 0, 0);
             }
-            if (rows <= 4)
-                lora_up_rows<T, NJ, 4>(bu, vf, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave], lane);
+            if (!PACKED && rows <= 4)
+                lora_up_rows<T, NJ, 4, true>(bu, vf, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave], lane);
             else
-                lora_up_rows<T, NJ, 16>(bu, vf, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave], lane);
+                lora_up_rows<T, NJ, 16, !PACKED>(bu, vf, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave], lane);
             continue;
         }
         for (uint32_t i = threadIdx.x; i < rows * quads; i += kLoraThreads) {
@@ -476,7 +485,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
             for (uint32_t t = 0; t * 16 < rows && col0 < n; ++t) {
                 uint4 vf[NJ];
                 terms(t * 16 + c, vf);
-                lora_up_rows<T, NJ, 16>(bu, vf, rank, n, base, base_ld, y, y_ld, row0 + list[min(t * 16 + c, rows - 1)],
+                lora_up_rows<T, NJ, 16, !PACKED>(bu, vf, rank, n, base, base_ld, y, y_ld, row0 + list[min(t * 16 + c, rows - 1)],
                                         min(rows - t * 16, 16u), col0, tiles, tile[wave], lane);
             }
         } else {
@@ -661,8 +670,13 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     auto run = [&](auto q, auto tiles) {
         constexpr int Q = decltype(q)::value, N = decltype(tiles)::value;
         if (int rc = run_down(lora_down_kernel<Q, N>)) return rc;
-        return dtype == FH_F32 ? run_up(lora_up_kernel<float, Q, N>, static_cast<float *>(nullptr))
-                               : run_up(lora_up_kernel<uint16_t, Q, N>, static_cast<uint16_t *>(nullptr));
+        // windows of 64 rows past kWideRows rows: mostly whole chunks of 64
+        if constexpr (Q == 1)
+            if (m > kWideRows)
+                return dtype == FH_F32 ? run_up(lora_up_kernel<float, Q, N, true>, static_cast<float *>(nullptr))
+                                       : run_up(lora_up_kernel<uint16_t, Q, N, true>, static_cast<uint16_t *>(nullptr));
+        return dtype == FH_F32 ? run_up(lora_up_kernel<float, Q, N, false>, static_cast<float *>(nullptr))
+                               : run_up(lora_up_kernel<uint16_t, Q, N, false>, static_cast<uint16_t *>(nullptr));
     };
     auto by_rank = [&](auto q) {
         if (rank <= 16) return run(q, std::integral_constant<int, 1>{});
