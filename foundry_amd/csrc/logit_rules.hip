@@ -1,4 +1,6 @@
 // Penalties, biases and grammar masks on logits (fh_logits_process).
+#include <type_traits>
+
 #include "serving_checks.hpp"
 
 namespace fh {
@@ -6,14 +8,17 @@ namespace fh {
 // Bound by memory: the logits go through once, in pieces of 16 bytes where
 // their rows are so aligned (a row's first piece may begin before it). What a
 // token needs to know of the row's lists stands in LDS: a block takes a run of
-// up to kRuleTokens tokens, counts the whole history into a table of them, and
-// enters the bias list into another. Every block of a row reads its lists, from
+// tokens, enters the bias list into a table of them and counts the whole history
+// there too. Every block of a row reads its lists, from
 // the L2: runs are as long as the LDS and a filled GPU allow.
-constexpr uint32_t kRuleTokens = 2048;
+constexpr uint32_t kRuleTokens = 4096;
 constexpr uint32_t kRuleThreads = 256;
 // Blocks that a launch aims for before runs get longer than the shortest, of
-// kRuleTokens / 4.
+// kRuleTokens / 8.
 constexpr uint32_t kRuleBlocks = 2048;
+// A token's word: its count among the generated, then a bit for an id of the
+// prompt, then a bias entry's index + 1, for lists up to these lengths.
+constexpr uint32_t kCountBits = 20, kMaxCounted = (1u << kCountBits) - 1, kMaxBiases = (1u << (31 - kCountBits)) - 1;
 
 // Calls take(i, list[i]) for i < n: 16-byte loads where the list is aligned,
 // several requested together (the list's last words again past its end).
@@ -47,17 +52,21 @@ __device__ __forceinline__ void for_list(const uint32_t *list, uint32_t n, Take 
     }
 }
 
-// Block (run, row). said: bit 31 for an id of the prompt, the rest its count
-// among the generated. entry: a bias entry's index + 1, the last of one id
-// staying. Whole-number LDS atomics: their order does not matter. Contraction is
-// off, so that each step is one fp32 rounding.
-template <typename T>
+// Block (run, row). Of a bias id listed twice the last entry stays. TWO: lists
+// too long for one word: a table of counts (bit 31: an id of the prompt) and one
+// of bias entries, over half as many tokens. Whole-number LDS atomics: their
+// order does not matter. Contraction is off, so that each step is one fp32
+// rounding.
+template <typename T, bool TWO>
 __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(const T *z, uint32_t n, uint32_t run,
                                                                    const fh_logit_rules rules, T *out) {
 #pragma clang fp contract(off)
     constexpr uint32_t E = 16 / sizeof(T);  // logits of a piece
-    constexpr uint32_t kPieces = kRuleTokens / (kRuleThreads * E);
-    __shared__ __attribute__((aligned(16))) uint32_t said[kRuleTokens], entry[kRuleTokens];
+    constexpr uint32_t kMost = TWO ? kRuleTokens / 2 : kRuleTokens;
+    constexpr uint32_t kPieces = kMost / (kRuleThreads * E);
+    constexpr uint32_t kSaid = TWO ? 0x80000000u : 1u << kCountBits, kShift = TWO ? 0 : kCountBits + 1;
+    __shared__ __attribute__((aligned(16))) uint32_t said[kRuleTokens];
+    uint32_t *entry = TWO ? said + kMost : said;
     const uint32_t r = blockIdx.y;
     const T *from = z + static_cast<uint64_t>(r) * n;
     T *to = out + static_cast<uint64_t>(r) * n;
@@ -91,28 +100,32 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(const T *z, u
         }
     }
     for (uint32_t i = threadIdx.x * 4; i < run; i += kRuleThreads * 4) {
-        if (history) *reinterpret_cast<uint4 *>(said + i) = make_uint4(0, 0, 0, 0);
-        if (bias) *reinterpret_cast<uint4 *>(entry + i) = make_uint4(0, 0, 0, 0);
+        if (history || (bias && !TWO)) *reinterpret_cast<uint4 *>(said + i) = make_uint4(0, 0, 0, 0);
+        if (bias && TWO) *reinterpret_cast<uint4 *>(entry + i) = make_uint4(0, 0, 0, 0);
     }
     __syncthreads();
+    if (bias) {
+        for_list(rules.bias_ids + static_cast<uint64_t>(r) * rules.bias_ld, bias_used, [&](uint32_t i, uint32_t id) {
+            const uint32_t at = id - static_cast<uint32_t>(lo);
+            if (id < n && at < run) atomicMax(&entry[at], (i + 1) << kShift);
+        });
+        if (!TWO) __syncthreads();  // the entries are the words' largest part: before the counts
+    }
     if (history)
         for_list(rules.history + static_cast<uint64_t>(r) * rules.history_ld, said_len, [&](uint32_t i, uint32_t id) {
             const uint32_t at = id - static_cast<uint32_t>(lo);
             if (id >= n || at >= run) return;
             if (i < prompt)
-                atomicOr(&said[at], 0x80000000u);
+                atomicOr(&said[at], kSaid);
             else
                 atomicAdd(&said[at], 1u);
         });
-    if (bias)
-        for_list(rules.bias_ids + static_cast<uint64_t>(r) * rules.bias_ld, bias_used, [&](uint32_t i, uint32_t id) {
-            const uint32_t at = id - static_cast<uint32_t>(lo);
-            if (id < n && at < run) atomicMax(&entry[at], i + 1);
-        });
     __syncthreads();
-    // one logit: s its word of said, e of entry
+    const bool words = history || (bias && !TWO);
+    // one logit: s its word, e its entry's where that is another
     auto apply = [&](float v, uint32_t s, uint32_t e) {
-        const uint32_t times = s & 0x7FFFFFFFu;
+        if (!TWO) e = s >> kShift, s &= 2 * kSaid - 1;
+        const uint32_t times = s & (kSaid - 1);
         if (rules.repetition && s) v = v > 0.0f ? v / rep : v * rep;
         if (times) {
             if (rules.frequency) v = v - freq * static_cast<float>(times);
@@ -138,8 +151,8 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(const T *z, u
             uint32_t s[E], e[E], any = 0;
 #pragma unroll
             for (uint32_t i = 0; i < E; i += 4) {
-                const uint4 a = history ? *reinterpret_cast<const uint4 *>(said + at + i) : make_uint4(0, 0, 0, 0);
-                const uint4 b = bias ? *reinterpret_cast<const uint4 *>(entry + at + i) : make_uint4(0, 0, 0, 0);
+                const uint4 a = words ? *reinterpret_cast<const uint4 *>(said + at + i) : make_uint4(0, 0, 0, 0);
+                const uint4 b = bias && TWO ? *reinterpret_cast<const uint4 *>(entry + at + i) : make_uint4(0, 0, 0, 0);
                 s[i] = a.x, s[i + 1] = a.y, s[i + 2] = a.z, s[i + 3] = a.w;
                 e[i] = b.x, e[i + 1] = b.y, e[i + 2] = b.z, e[i + 3] = b.w;
                 any |= a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w;
@@ -173,7 +186,7 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(const T *z, u
                 v = bf(from[j]);
             else
                 v = from[j];
-            v = apply(v, history ? said[i] : 0, bias ? entry[i] : 0);
+            v = apply(v, words ? said[i] : 0, bias && TWO ? entry[i] : 0);
             if (mask && !(mask[j / 32] >> (j % 32) & 1u)) v = -INFINITY;
             if constexpr (sizeof(T) == 2)
                 to[j] = rne(v);
@@ -235,18 +248,21 @@ extern "C" int fh_logits_process(fh_device *dev, const void *logits, int dtype, 
     if (u.mask)
         if (int rc = check_range(dev, u.mask, r * ((n + 31) / 32) * 4, fn, "mask")) return rc;
     if (int rc = set_current(dev, fn)) return rc;
-    uint32_t run = kRuleTokens / 4;
-    while (run < kRuleTokens && r * ((n + run - 1) / run) > kRuleBlocks) run *= 2;
+    const bool two = (u.history && u.history_ld > kMaxCounted) || (u.bias_ids && u.bias_ld >= kMaxBiases);
+    const uint32_t longest = two ? kRuleTokens / 2 : kRuleTokens;
+    uint32_t run = kRuleTokens / 8;
+    while (run < longest && r * ((n + run - 1) / run) > kRuleBlocks) run *= 2;
     // a run may begin up to a piece before its row
     const dim3 grid(static_cast<uint32_t>((n + 16 / elem - 1 + run - 1) / run), static_cast<uint32_t>(rows));
-    return dispatch(dev, fn, [&] {
-        if (dtype == FH_F32)
-            hipLaunchKernelGGL(logit_rules_kernel<float>, grid, dim3(kRuleThreads), 0, dev->stream,
-                               static_cast<const float *>(logits), static_cast<uint32_t>(n), run, u,
-                               static_cast<float *>(out));
-        else
-            hipLaunchKernelGGL(logit_rules_kernel<uint16_t>, grid, dim3(kRuleThreads), 0, dev->stream,
-                               static_cast<const uint16_t *>(logits), static_cast<uint32_t>(n), run, u,
-                               static_cast<uint16_t *>(out));
-    });
+    auto launch = [&](auto kernel, auto *of) {
+        using T = std::remove_pointer_t<decltype(of)>;
+        return dispatch(dev, fn, [&] {
+            hipLaunchKernelGGL(kernel, grid, dim3(kRuleThreads), 0, dev->stream, static_cast<const T *>(logits),
+                               static_cast<uint32_t>(n), run, u, static_cast<T *>(out));
+        });
+    };
+    float *const f32 = nullptr;
+    uint16_t *const bf16 = nullptr;
+    if (dtype == FH_F32) return two ? launch(logit_rules_kernel<float, true>, f32) : launch(logit_rules_kernel<float, false>, f32);
+    return two ? launch(logit_rules_kernel<uint16_t, true>, bf16) : launch(logit_rules_kernel<uint16_t, false>, bf16);
 }

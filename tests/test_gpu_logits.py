@@ -128,6 +128,15 @@ def test_history_lengths(device, history):
     check(device, logits_of(8, 2, 3001, False), rules_of(history, 2, 3001, history, 0, False, ids_max=60))
 
 
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("history,bias", [(40, 3000), ((1 << 20) + 5, 20), (70, 2046), (70, 2047), (70, 2048)])
+def test_lists_that_need_a_table_each(device, history, bias, f32):
+    """Counts and bias entries share a word up to certain lengths of the lists."""
+    u = rules_of(bias, 2, 9001, history, bias, True, ids_max=50 if history > 1000 else None)
+    u["bias_len"][:] = [bias, bias // 2]
+    check(device, logits_of(24, 2, 9001, f32), u)
+
+
 def test_lengths_past_the_lists_and_prompts_past_the_history(device):
     u = rules_of(9, 4, 900, 30, 10, False)
     u["history_len"][:] = [0, 31, 0xFFFFFFFF, 30]
