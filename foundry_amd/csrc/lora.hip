@@ -17,8 +17,7 @@ namespace fh {
 // Grouping: rows come with their adapters in any order, so a block takes a
 // window of rows (64, or 256) and finds in it the groups of rows that share an
 // adapter, by ballots over the adapter ids; each group is cut into chunks of
-// up to 64 rows, and a block takes every (number of slots)-th chunk. Whatever
-// the order, the products run on the matrix cores with the adapter's rows read
+// up to 64 rows. Whatever the order, the products run on the matrix cores with the adapter's rows read
 // once for up to 64 rows (four tiles of 16).
 typedef __attribute__((ext_vector_type(8))) __bf16 lo_bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float lo_f32x4_t;
@@ -28,21 +27,38 @@ __device__ __forceinline__ lo_f32x4_t lo_mfma(uint4 a, uint4 b, lo_f32x4_t c) {
                                                    __builtin_bit_cast(lo_bf16x8_t, b), c, 0, 0, 0);
 }
 
-// Blocks of 64 rows and a range of k that the down product aims for, the ranges
-// at most, and the least steps of 32 k that a wavefront takes.
-constexpr uint32_t kDownBlocks = 512, kMaxSplits = 4, kDownSteps = 2;
+constexpr uint32_t kLoraThreads = 256;
+constexpr uint32_t kLoraWaves = kLoraThreads / 64;
 // Rows up to which a window is 256 rows (and an adapter that they share is
 // read once for all of them).
 constexpr uint32_t kWideRows = 1024;
-// Blocks that the chunks of the windows are spread over, down and up. Slots are
-// a grid's slowest dimension: a window has often fewer chunks than slots, and
-// neighbouring blocks run on different XCDs (with slots fastest, 4096 packed
-// rows ran on every second one: 62 us against 48).
-constexpr uint32_t kDownSlots = 512, kUpSlots = 2048;
-constexpr uint32_t kLoraThreads = 256;
-constexpr uint32_t kLoraWaves = kLoraThreads / 64;
-// Wavefronts that the up product aims for, and 64-column tiles of one at most.
-constexpr uint32_t kUpWaves = 2048, kMaxTiles = 8;
+// Blocks that the windows share, down and up. How many chunks a window has is
+// known on the device alone: there its blocks divide the chunks among
+// themselves, and each chunk's k (down, into kMaxSplits ranges at most and
+// kDownSteps steps of 32 per wavefront at least) or columns (up) as far as they
+// go round. With estimates of the host 1024 packed rows of rank 16 were left
+// to 40 blocks: 36 us against 24.
+constexpr uint32_t kDownBlocks = 512, kMaxSplits = 4, kDownSteps = 2;
+constexpr uint32_t kUpBlocks = 768, kUpPacked = 512;
+// (Up, as many as the GPU holds at once: 200 rows of 48 adapters 28 us at 768
+// blocks, 31.8 at 512, 32.7 at 1024; 4096 packed rows 36.8 at 512, 40.1 at 768.)
+
+// The ranges of k of a window with `chunks` chunks and `blocks` blocks: `splits`
+// of them, of kLoraWaves x `steps` x 32.
+struct Ranges {
+    uint32_t splits, steps;
+};
+
+__host__ __device__ __forceinline__ uint32_t most_splits(uint32_t k) {
+    const uint32_t n = ((k + 31) / 32 + kLoraWaves * kDownSteps - 1) / (kLoraWaves * kDownSteps);
+    return n < kMaxSplits ? n : kMaxSplits;
+}
+
+__device__ __forceinline__ Ranges ranges_of(uint32_t k, uint32_t chunks, uint32_t blocks) {
+    const uint32_t all = (k + 31) / 32, want = min(max(blocks / max(chunks, 1u), 1u), most_splits(k));
+    const uint32_t steps = (all + want * kLoraWaves - 1) / (want * kLoraWaves);
+    return {(all + steps * kLoraWaves - 1) / (steps * kLoraWaves), steps};
+}
 
 // The rows of a window and its chunks. A row's rank is the number of rows
 // before it with its adapter; rows of rank 0, 64, .. lead a chunk, and the
@@ -223,29 +239,32 @@ __device__ __forceinline__ void lora_down_chunk(const uint16_t *x, uint32_t k, u
     }
 }
 
-// Block (split, window, slot).
+// Grid (windows, blocks of a window): neighbouring blocks run on different XCDs,
+// and a window may have fewer units than blocks (the other way round 4096 packed
+// rows' down products ran on 4 of 8).
 template <int Q, int NR>
 __global__ __launch_bounds__(kLoraThreads) void lora_down_kernel(const uint16_t *__restrict__ x, uint32_t m, uint32_t k,
                                                                  uint64_t x_ld, const uint16_t *__restrict__ a,
                                                                  uint32_t n_adapters, uint32_t rank,
-                                                                 const uint32_t *__restrict__ adapters, uint32_t steps,
+                                                                 const uint32_t *__restrict__ adapters,
                                                                  float *__restrict__ v) {
     __shared__ uint8_t lists[kLoraWaves][64];
     __shared__ uint64_t leads[Q];
     __shared__ float4 sums[4 * NR * 64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.y * 64 * Q;
-    // steps: of 32 k, of each wavefront
-    const uint32_t k0 = min((blockIdx.x * kLoraWaves + wave) * steps * 32, k), k1 = min(k0 + steps * 32, k);
-    v += static_cast<uint64_t>(blockIdx.x) * m * rank;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.x * 64 * Q;
     const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
-    for (uint32_t item = blockIdx.z; item < o.chunks; item += gridDim.z) {
+    const Ranges g = ranges_of(k, o.chunks, gridDim.y);
+    for (uint32_t unit = blockIdx.y; unit < o.chunks * g.splits; unit += gridDim.y) {
+        const uint32_t split = unit % g.splits;
+        const uint32_t k0 = min((split * kLoraWaves + wave) * g.steps * 32, k), k1 = min(k0 + g.steps * 32, k);
+        float *to = v + static_cast<uint64_t>(split) * m * rank;
         uint32_t rows;
-        const uint32_t id = chunk_of<Q>(o, item, lane, lists[wave], rows);
+        const uint32_t id = chunk_of<Q>(o, unit / g.splits, lane, lists[wave], rows);
         const uint16_t *au = a + static_cast<uint64_t>(id) * rank * k;
         if (rows <= 16)
-            lora_down_chunk<1, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, lists[wave], sums, v, lane, wave);
+            lora_down_chunk<1, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, lists[wave], sums, to, lane, wave);
         else
-            lora_down_chunk<4, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, lists[wave], sums, v, lane, wave);
+            lora_down_chunk<4, NR>(x, k, x_ld, au, rank, k0, k1, row0, rows, lists[wave], sums, to, lane, wave);
     }
 }
 
@@ -345,20 +364,22 @@ __device__ __forceinline__ T plus(T base, float d) {
 
 // Up to R rows of a chunk through LDS (tile: this wavefront's), `tiles` times 64
 // columns: a lane has one column of each row, so that rows are read and written
-// in whole lines whatever their alignment and however few they are. The next 64
-// columns are requested before a tile's products.
+// in whole lines whatever their alignment and however few they are. The first 64
+// columns are requested before terms() forms the lane's terms of v, with AHEAD
+// the next 64 before a tile's products.
 template <typename T, int NJ, int R>
 struct RowsTile {
     uint4 b[4][NJ];
     T base[R];
 };
 
-template <typename T, int NJ, int R, bool AHEAD>
-__device__ __forceinline__ void lora_up_rows(const uint16_t *b, const uint4 (&vf)[NJ], uint32_t rank, uint32_t n,
-                                             const T *base, uint64_t base_ld, T *y, uint64_t y_ld, uint32_t mine,
-                                             uint32_t rows, uint32_t col0, uint32_t tiles, float (*tile)[68],
-                                             uint32_t lane) {
+template <typename T, int NJ, int R, bool AHEAD, typename Terms>
+__device__ __forceinline__ void lora_up_rows(const uint16_t *b, uint32_t rank, uint32_t n, const T *base,
+                                             uint64_t base_ld, T *y, uint64_t y_ld, uint32_t mine, uint32_t rows,
+                                             uint32_t col0, uint32_t tiles, float (*tile)[68], uint32_t lane,
+                                             Terms terms) {
     const uint32_t c = lane & 15u, q = lane >> 4;
+    uint4 vf[NJ];
     auto row = [&](int i) { return static_cast<uint64_t>(__builtin_amdgcn_readlane(mine, min(i, static_cast<int>(rows) - 1))); };
     auto request = [&](RowsTile<T, NJ, R> &x, uint32_t u) {
         const uint32_t at = col0 + min(u, tiles - 1) * kLoraWaves * 64;
@@ -379,16 +400,16 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, const uint4 (&vf
             if (i < static_cast<int>(rows) && col < n) (y + row(i) * y_ld)[col] = plus(x.base[i], tile[i][lane]);
         __builtin_amdgcn_wave_barrier();
     };
+    RowsTile<T, NJ, R> one, two;
+    request(one, 0);
+    terms(vf);
     if constexpr (!AHEAD) {
         for (uint32_t u = 0; u < tiles; ++u) {
-            RowsTile<T, NJ, R> x;
-            request(x, u);
-            finish(x, u);
+            if (u) request(one, u);
+            finish(one, u);
         }
         return;
     }
-    RowsTile<T, NJ, R> one, two;
-    request(one, 0);
     for (uint32_t u = 0; u < tiles; u += 2) {
         request(two, u + 1);
         finish(one, u);
@@ -398,96 +419,101 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, const uint4 (&vf
     }
 }
 
-// Block (columns, window, slot); a wavefront takes `tiles` times 64 columns.
-// Chunks of up to 16 rows: each wavefront forms its terms of v from the splits'
-// sums by itself, with no barrier. Larger ones: v is formed once for the block,
-// in LDS; wide: a lane reads and writes 16 neighbouring columns of a row (n a
-// multiple of 16, rows 16-byte aligned).
+// Grid (windows, blocks of a window): neighbouring blocks run on different XCDs,
+// and a window may have fewer units than blocks (the other way round 4096 packed
+// rows' down products ran on 4 of 8). v is formed in LDS from the splits' sums:
+// for a chunk of up to 16 rows by each wavefront for itself, with no barrier,
+// else once for the block. wide: there a lane reads and writes 16 neighbouring
+// columns of a row (n a multiple of 16, rows 16-byte aligned).
 template <typename T, int Q, int NJ, bool PACKED>
-__global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__restrict__ v, uint32_t splits, uint32_t m,
-                                                               const uint16_t *__restrict__ b,
+__global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__restrict__ v, uint32_t down_blocks,
+                                                               uint32_t m, uint32_t k, const uint16_t *__restrict__ b,
                                                                const float *__restrict__ scales, uint32_t n_adapters,
                                                                uint32_t rank, uint32_t n,
                                                                const uint32_t *__restrict__ adapters, const T *base,
-                                                               uint64_t base_ld, T *y, uint64_t y_ld, bool wide,
-                                                               uint32_t tiles) {
-    constexpr int kLoads = 4;                  // splits' sums requested together
-    constexpr int P = sizeof(T) == 2 ? 4 : 2;  // row tiles requested together
+                                                               uint64_t base_ld, T *y, uint64_t y_ld, bool wide) {
+    constexpr int kLoads = 4;                       // splits' sums requested together
+    constexpr int P = sizeof(T) == 2 ? 4 : 2;       // row tiles requested together
+    constexpr bool kAhead = !PACKED && NJ <= 2;     // the registers hold two tiles of B
     __shared__ uint8_t lists[kLoraWaves][64];
     __shared__ uint64_t leads[Q];
     __shared__ __attribute__((aligned(16))) uint16_t vs[64 * (2 * 16 * NJ + 8)];
     __shared__ __attribute__((aligned(16))) float tile[kLoraWaves][16][68];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.y * 64 * Q;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.x * 64 * Q;
     const uint32_t c = lane & 15u, q = lane >> 4, vs_ld = 2 * rank + 8, quads = rank / 4;
-    const uint32_t col0 = (blockIdx.x * tiles * kLoraWaves + wave) * 64;  // then every kLoraWaves-th tile
     const uint64_t split = static_cast<uint64_t>(m) * rank;
     const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
-    // the sums of 4 ranks of a row over the splits
-    auto add_splits = [&](const float *p, float (&f)[4]) {
-        f[0] = f[1] = f[2] = f[3] = 0.0f;
-        for (uint32_t u0 = 0; u0 < splits; u0 += kLoads) {
-            float4 part[kLoads];
-#pragma unroll
-            for (uint32_t u = 0; u < kLoads; ++u)
-                part[u] = *reinterpret_cast<const float4 *>(p + min(u0 + u, splits - 1) * split);
-#pragma unroll
-            for (uint32_t u = 0; u < kLoads; ++u)
-                if (u0 + u < splits) f[0] += part[u].x, f[1] += part[u].y, f[2] += part[u].z, f[3] += part[u].w;
-        }
-    };
-    for (uint32_t item = blockIdx.z; item < o.chunks; item += gridDim.z) {
+    const uint32_t splits = ranges_of(k, o.chunks, down_blocks).splits;
+    // a chunk's columns in `parts` parts of `tiles` times 64 per wavefront
+    const uint32_t all = (n + kLoraWaves * 64 - 1) / (kLoraWaves * 64);
+    const uint32_t tiles = (all + min(max(gridDim.y / max(o.chunks, 1u), 1u), all) - 1) /
+                           min(max(gridDim.y / max(o.chunks, 1u), 1u), all);
+    const uint32_t parts = (all + tiles - 1) / tiles;
+    for (uint32_t unit = blockIdx.y; unit < o.chunks * parts; unit += gridDim.y) {
+        const uint32_t col0 = (unit % parts * tiles * kLoraWaves + wave) * 64;  // then every kLoraWaves-th tile
         uint32_t rows;
         const uint8_t *list = lists[wave];
-        const uint32_t id = chunk_of<Q>(o, item, lane, lists[wave], rows);
+        const uint32_t id = chunk_of<Q>(o, unit / parts, lane, lists[wave], rows);
         const float scale = scales[id];
         const uint16_t *bu = b + static_cast<uint64_t>(id) * n * rank;
-        if (rows <= 16) {
-            if (col0 >= n) continue;
-            const uint32_t mine = row0 + list[min(c, rows - 1)];
-            uint4 vf[NJ];
+        const bool few = rows <= 16;
+        uint16_t *terms_of = few ? vs + wave * 16 * vs_ld : vs;
+        if (!few) __syncthreads();  // other wavefronts may still read theirs, of a chunk before
+        auto fill = [&](uint32_t from, uint32_t by) {
+            for (uint32_t i = from; i < rows * quads; i += by) {
+                const uint32_t member = i / quads, r = i % quads * 4;
+                const float *p = v + static_cast<uint64_t>(row0 + list[member]) * rank + r;
+                float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float4 part[kLoads];
+                static_assert(kLoads == kMaxSplits, "one round of loads");
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const uint32_t r = (2 * j + q / 2) * 8;
-                const float *p = v + static_cast<uint64_t>(mine) * rank + min(r, rank - 8);
-                float f[4], g[4];
-                add_splits(p, f);
-                add_splits(p + 4, g);
-                vf[j] = make_uint4(parts_of(f[0] * scale, f[1] * scale, q & 1), parts_of(f[2] * scale, f[3] * scale, q & 1),
-                                   parts_of(g[0] * scale, g[1] * scale, q & 1), parts_of(g[2] * scale, g[3] * scale, q & 1));
-                if (r >= rank) vf[j] = make_uint4(0, 0, 0, 0);
+                for (uint32_t u = 0; u < kLoads; ++u)
+                    part[u] = *reinterpret_cast<const float4 *>(p + min(u, splits - 1) * split);
+#pragma unroll
+                for (uint32_t u = 0; u < kLoads; ++u)
+                    if (u < splits) f[0] += part[u].x, f[1] += part[u].y, f[2] += part[u].z, f[3] += part[u].w;
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+                    *reinterpret_cast<uint2 *>(terms_of + member * vs_ld + h * rank + r) =
+                        make_uint2(parts_of(f[0] * scale, f[1] * scale, h), parts_of(f[2] * scale, f[3] * scale, h));
             }
-            if (!PACKED && rows <= 4)
-                lora_up_rows<T, NJ, 4, true>(bu, vf, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave], lane);
-            else
-                lora_up_rows<T, NJ, 16, !PACKED>(bu, vf, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave], lane);
-            continue;
-        }
-        for (uint32_t i = threadIdx.x; i < rows * quads; i += kLoraThreads) {
-            const uint32_t member = i / quads, r = i % quads * 4;
-            float f[4];
-            add_splits(v + static_cast<uint64_t>(row0 + list[member]) * rank + r, f);
-#pragma unroll
-            for (uint32_t part = 0; part < 2; ++part)
-                *reinterpret_cast<uint2 *>(vs + member * vs_ld + part * rank + r) =
-                    make_uint2(parts_of(f[0] * scale, f[1] * scale, part), parts_of(f[2] * scale, f[3] * scale, part));
-        }
-        __syncthreads();
+        };
         auto terms = [&](uint32_t member, uint4 (&vf)[NJ]) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const uint32_t r = (2 * j + q / 2) * 8;
-                vf[j] = *reinterpret_cast<const uint4 *>(vs + min(member, rows - 1) * vs_ld + (q & 1) * rank +
+                vf[j] = *reinterpret_cast<const uint4 *>(terms_of + min(member, rows - 1) * vs_ld + (q & 1) * rank +
                                                          min(r, rank - 8));
                 if (r >= rank) vf[j] = make_uint4(0, 0, 0, 0);
             }
         };
-        if (!wide) {
-            for (uint32_t t = 0; t * 16 < rows && col0 < n; ++t) {
-                uint4 vf[NJ];
-                terms(t * 16 + c, vf);
-                lora_up_rows<T, NJ, 16, !PACKED>(bu, vf, rank, n, base, base_ld, y, y_ld, row0 + list[min(t * 16 + c, rows - 1)],
-                                        min(rows - t * 16, 16u), col0, tiles, tile[wave], lane);
-            }
+        if (few) {
+            if (col0 >= n) continue;
+            const uint32_t mine = row0 + list[min(c, rows - 1)];
+            auto form = [&](uint4 (&vf)[NJ]) {
+                fill(lane, 64);
+                __builtin_amdgcn_wave_barrier();
+                terms(c, vf);
+                __builtin_amdgcn_wave_barrier();
+            };
+            if (!PACKED && rows <= 4)
+                lora_up_rows<T, NJ, 4, kAhead>(bu, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave],
+                                               lane, form);
+            else if (!PACKED && rows <= 8)
+                lora_up_rows<T, NJ, 8, kAhead>(bu, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave],
+                                               lane, form);
+            else
+                lora_up_rows<T, NJ, 16, false>(bu, rank, n, base, base_ld, y, y_ld, mine, rows, col0, tiles, tile[wave],
+                                               lane, form);
+            continue;
+        }
+        fill(threadIdx.x, kLoraThreads);
+        __syncthreads();
+        if (!PACKED || !wide) {
+            for (uint32_t t = 0; t * 16 < rows && col0 < n; ++t)
+                lora_up_rows<T, NJ, 16, false>(bu, rank, n, base, base_ld, y, y_ld, row0 + list[min(t * 16 + c, rows - 1)],
+                                               min(rows - t * 16, 16u), col0, tiles, tile[wave], lane,
+                                               [&](uint4 (&vf)[NJ]) { terms(t * 16 + c, vf); });
         } else {
             for (uint32_t u = 0; u < tiles; ++u) {
                 const uint32_t first = col0 + u * kLoraWaves * 64;
@@ -520,51 +546,36 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
         }
         __syncthreads();  // vs is read
     }
-    // rows without an adapter are base, where y is not
+    // rows without an adapter are base, where y is not: in runs of kBareCols columns, to the blocks in turn
+    // from the last one on, which have the fewest units
     if (y == base) return;
-    uint32_t turn = 0;
+    constexpr uint32_t kBareLoads = 8, kBareCols = kBareLoads * kLoraThreads;
+    const uint32_t runs = (n + kBareCols - 1) / kBareCols;
+    uint32_t turn = gridDim.y - 1 - blockIdx.y;  // this block's next run
 #pragma unroll
     for (int w = 0; w < Q; ++w) {
         const uint32_t here = m - row0 > w * 64u ? min(m - row0 - w * 64u, 64u) : 0;
-        uint64_t bare = ~o.live[w] & (here < 64 ? (1ull << here) - 1 : ~0ull);
-        for (; bare; bare &= bare - 1, ++turn) {
-            if (turn % gridDim.z != blockIdx.z) continue;
-            const uint64_t row = row0 + w * 64 + __builtin_ctzll(bare);
-            const uint32_t cols = kLoraWaves * tiles * 64;
-            for (uint32_t e = blockIdx.x * cols + threadIdx.x; e < min(n, (blockIdx.x + 1) * cols); e += kLoraThreads)
-                y[row * y_ld + e] = base[row * base_ld + e];
+        const uint64_t bare = ~o.live[w] & (here < 64 ? (1ull << here) - 1 : ~0ull);
+        const uint32_t turns = __builtin_popcountll(bare) * runs;
+        for (; turn < turns; turn += gridDim.y) {
+            uint64_t left = bare;
+            for (uint32_t i = 0; i < turn / runs; ++i) left &= left - 1;
+            const uint64_t row = row0 + w * 64 + __builtin_ctzll(left);
+            const uint32_t at = turn % runs * kBareCols + threadIdx.x;
+            T held[kBareLoads];
+#pragma unroll
+            for (uint32_t i = 0; i < kBareLoads; ++i) held[i] = base[row * base_ld + min(at + i * kLoraThreads, n - 1)];
+#pragma unroll
+            for (uint32_t i = 0; i < kBareLoads; ++i)
+                if (at + i * kLoraThreads < n) y[row * y_ld + at + i * kLoraThreads] = held[i];
         }
+        turn -= turns;
     }
 }
 
 }  // namespace fh
 
 using namespace fh;
-
-namespace {
-
-// Windows of 64 * quads rows, and k cut into `splits` ranges of 4 wavefronts x
-// `steps` x 32.
-struct Split {
-    uint32_t quads, windows, splits, steps;
-    uint64_t chunks;  // expected
-};
-
-Split split_of(int64_t m, int64_t k) {
-    Split s;
-    s.quads = m > 64 && m <= kWideRows ? 4 : 1;
-    s.windows = static_cast<uint32_t>((m + 64 * s.quads - 1) / (64 * s.quads));
-    const uint64_t steps = (k + 31) / 32, least = kLoraWaves * kDownSteps;
-    // a few rows are mostly of different adapters, many mostly of the same
-    s.chunks = std::max<uint64_t>(1, m <= kWideRows ? m / 4 : (m + 63) / 64);
-    const uint64_t splits =
-        std::clamp<uint64_t>(std::min(kDownBlocks / s.chunks, (steps + least - 1) / least), 1, kMaxSplits);
-    s.steps = static_cast<uint32_t>((steps + splits * kLoraWaves - 1) / (splits * kLoraWaves));
-    s.splits = static_cast<uint32_t>((steps + s.steps * kLoraWaves - 1) / (s.steps * kLoraWaves));
-    return s;
-}
-
-}  // namespace
 
 extern "C" int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *bytes) {
     const char *fn = "fh_lora_workspace";
@@ -574,7 +585,7 @@ extern "C" int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *b
         return fail(FH_ERR_UNSUPPORTED, "%s: rank %lld must be a multiple of 8, at most 128", fn, (long long)rank);
     if (k < 8 || k % 8 != 0)
         return fail(FH_ERR_UNSUPPORTED, "%s: k %lld must be a multiple of 8", fn, (long long)k);
-    *bytes = static_cast<uint64_t>(split_of(m, k).splits) * m * rank * 4 + 16;
+    *bytes = static_cast<uint64_t>(most_splits(static_cast<uint32_t>(k))) * m * rank * 4 + 16;
     return FH_OK;
 }
 
@@ -635,18 +646,17 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     }
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "y", y, y_bytes)) return rc;
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "base", base, base_bytes)) return rc;
-    const Split w = split_of(m, k);
-    if (w.windows > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: m %lld", fn, (long long)m);
+    const uint32_t quads = m > 64 && m <= kWideRows ? 4 : 1, rows_of = 64 * quads;
+    const uint64_t windows = (rows + rows_of - 1) / rows_of, cols = (n + kLoraWaves * 64 - 1) / (kLoraWaves * 64);
+    if (windows > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: m %lld", fn, (long long)m);
     if (int rc = set_current(dev, fn)) return rc;
-    const uint64_t tiles_of_all = w.chunks * ((n + 63) / 64);
-    const uint32_t tiles = static_cast<uint32_t>(std::clamp<uint64_t>(tiles_of_all / kUpWaves, 1, kMaxTiles));
-    const uint32_t cols = static_cast<uint32_t>((n + kLoraWaves * 64 * tiles - 1) / (kLoraWaves * 64 * tiles));
     // a window has at most as many chunks as rows
-    const uint32_t most = static_cast<uint32_t>(std::min<int64_t>(m, 64 * w.quads));
-    const uint32_t down_slots = std::clamp(kDownSlots / (w.windows * w.splits), 1u, most);
-    const uint32_t up_slots = std::clamp(static_cast<uint32_t>(kUpSlots / (static_cast<uint64_t>(w.windows) * cols)), 1u,
-                                         most);
-    const dim3 down(w.splits, w.windows, down_slots), up(cols, w.windows, up_slots), threads(kLoraThreads);
+    const uint64_t most = std::min<uint64_t>(rows, rows_of);
+    const uint32_t down_blocks = static_cast<uint32_t>(
+        std::clamp<uint64_t>(kDownBlocks / windows, 1, most * most_splits(static_cast<uint32_t>(k))));
+    const uint32_t up_blocks = static_cast<uint32_t>(std::clamp<uint64_t>((m > kWideRows ? kUpPacked : kUpBlocks) / windows, 1, most * cols));
+    const dim3 down(static_cast<uint32_t>(windows), down_blocks), up(static_cast<uint32_t>(windows), up_blocks);
+    const dim3 threads(kLoraThreads);
     float *v = static_cast<float *>(workspace);
     const uint32_t m32 = static_cast<uint32_t>(m), k32 = static_cast<uint32_t>(k), n32 = static_cast<uint32_t>(n);
     const uint32_t rank32 = static_cast<uint32_t>(rank), u32 = static_cast<uint32_t>(n_adapters);
@@ -655,15 +665,15 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     auto run_down = [&](auto kernel) {
         return dispatch(dev, fn, [&] {
             hipLaunchKernelGGL(kernel, down, threads, 0, dev->stream, x, m32, k32, static_cast<uint64_t>(x_ld), a, u32,
-                               rank32, adapters, w.steps, v);
+                               rank32, adapters, v);
         });
     };
     auto run_up = [&](auto kernel, auto *of) {
         using T = std::remove_pointer_t<decltype(of)>;
         return dispatch(dev, fn, [&] {
-            hipLaunchKernelGGL(kernel, up, threads, 0, dev->stream, v, w.splits, m32, b, scales, u32, rank32, n32,
+            hipLaunchKernelGGL(kernel, up, threads, 0, dev->stream, v, down_blocks, m32, k32, b, scales, u32, rank32, n32,
                                adapters, static_cast<const T *>(base), static_cast<uint64_t>(base_ld),
-                               static_cast<T *>(y), static_cast<uint64_t>(y_ld), wide, tiles);
+                               static_cast<T *>(y), static_cast<uint64_t>(y_ld), wide);
         });
     };
     // rank tiles of 16: 1, 2, 4 or 8
@@ -684,5 +694,5 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
         if (rank <= 64) return run(q, std::integral_constant<int, 4>{});
         return run(q, std::integral_constant<int, 8>{});
     };
-    return w.quads == 4 ? by_rank(std::integral_constant<int, 4>{}) : by_rank(std::integral_constant<int, 1>{});
+    return quads == 4 ? by_rank(std::integral_constant<int, 4>{}) : by_rank(std::integral_constant<int, 1>{});
 }
