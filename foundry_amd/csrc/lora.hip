@@ -314,19 +314,37 @@ __device__ __forceinline__ void store16(T *p, const float (&f)[16]) {
     }
 }
 
-// Two parts of a value in bf16: rounded, and what the rounding lost (nothing of
-// an inf or NaN). part: 0 the first, 1 the second, of two values.
+// Parts of two values in bf16: 0 the values rounded, 1 and 2 what the parts before
+// have lost, rounded (nothing of an inf or NaN).
 __device__ __forceinline__ uint32_t parts_of(float x, float y, uint32_t part) {
-    const uint32_t hi = f32x2_to_bf16x2_rne(x, y);
-    const float h0 = bf(hi & 0xFFFFu), h1 = bf(hi >> 16);
-    const uint32_t lo = f32x2_to_bf16x2_rne(fabsf(h0) < INFINITY ? x - h0 : 0.0f, fabsf(h1) < INFINITY ? y - h1 : 0.0f);
-    return part ? lo : hi;
+    uint32_t p = f32x2_to_bf16x2_rne(x, y);
+#pragma unroll
+    for (uint32_t i = 1; i <= 2; ++i) {
+        if (i > part) break;
+        const float x0 = bf(p & 0xFFFFu), y0 = bf(p >> 16);
+        x = fabsf(x0) < INFINITY ? x - x0 : 0.0f;
+        y = fabsf(y0) < INFINITY ? y - y0 : 0.0f;
+        p = f32x2_to_bf16x2_rne(x, y);
+    }
+    return p;
 }
+
+// A lane's terms of v: of each 16 ranks its 8 as part 0 or 1 (q & 1), and for
+// f32 results part 2 (as the second product of the same B; zero where q & 1).
+// bf16 results take 16 bits of v, f32 ones 24.
+template <typename T, int NJ>
+struct Terms {
+    uint4 v[NJ];
+    uint4 low[sizeof(T) == 4 ? NJ : 1];
+};
+
+template <typename T>
+constexpr uint32_t kParts = sizeof(T) == 4 ? 3 : 2;
 
 // v B^T of 16 rows and 64 columns. A product has 16 of the columns along its
 // rows and the rows along its columns, so that a lane holds 4 columns of row c
 // per product; along its 32 terms lie 16 ranks, 8 at a time as (first part,
-// second part) of v, so that 16 bits of v take part. WIDE: the columns of the
+// second part) of v. WIDE: the columns of the
 // four products are taken so that a lane's 16 are neighbours (from q * 16 on),
 // else product t has columns 16 t .. 16 t + 15 and a lane 4 from t * 16 + q * 4.
 template <int NJ, bool WIDE>
@@ -341,17 +359,19 @@ __device__ __forceinline__ void request_b(const uint16_t *b, uint32_t rank, uint
     }
 }
 
-// vf: lane's terms of v, zero past the rank.
-template <int NJ>
-__device__ __forceinline__ void products(const uint4 (&bfr)[4][NJ], const uint4 (&vf)[NJ], uint32_t rank, uint32_t q,
+template <typename T, int NJ>
+__device__ __forceinline__ void products(const uint4 (&bfr)[4][NJ], const Terms<T, NJ> &vf, uint32_t rank, uint32_t q,
                                          lo_f32x4_t (&acc)[4]) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) acc[u] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            acc[u] = lo_mfma((2 * j + q / 2) * 8 < rank ? bfr[u][j] : make_uint4(0, 0, 0, 0), vf[j], acc[u]);
+        for (int u = 0; u < 4; ++u) {
+            const uint4 f = (2 * j + q / 2) * 8 < rank ? bfr[u][j] : make_uint4(0, 0, 0, 0);
+            if constexpr (sizeof(T) == 4) acc[u] = lo_mfma(f, vf.low[j], acc[u]);
+            acc[u] = lo_mfma(f, vf.v[j], acc[u]);
+        }
 }
 
 template <typename T>
@@ -373,13 +393,13 @@ struct RowsTile {
     T base[R];
 };
 
-template <typename T, int NJ, int R, bool AHEAD, typename Terms>
+template <typename T, int NJ, int R, bool AHEAD, typename Form>
 __device__ __forceinline__ void lora_up_rows(const uint16_t *b, uint32_t rank, uint32_t n, const T *base,
                                              uint64_t base_ld, T *y, uint64_t y_ld, uint32_t mine, uint32_t rows,
                                              uint32_t col0, uint32_t tiles, float (*tile)[68], uint32_t lane,
-                                             Terms terms) {
+                                             Form terms) {
     const uint32_t c = lane & 15u, q = lane >> 4;
-    uint4 vf[NJ];
+    Terms<T, NJ> vf;
     auto row = [&](int i) { return static_cast<uint64_t>(__builtin_amdgcn_readlane(mine, min(i, static_cast<int>(rows) - 1))); };
     auto request = [&](RowsTile<T, NJ, R> &x, uint32_t u) {
         const uint32_t at = col0 + min(u, tiles - 1) * kLoraWaves * 64;
@@ -390,15 +410,21 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, uint32_t rank, u
     auto finish = [&](const RowsTile<T, NJ, R> &x, uint32_t u) {
         const uint32_t col = col0 + u * kLoraWaves * 64 + lane;
         lo_f32x4_t acc[4];
-        products<NJ>(x.b, vf, rank, q, acc);
+        products<T, NJ>(x.b, vf, rank, q, acc);
+        // 8 rows at a time
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-            *reinterpret_cast<lo_f32x4_t *>(&tile[c][t * 16 + q * 4]) = acc[t];
-        __builtin_amdgcn_wave_barrier();
+        for (int h = 0; h < R; h += 8) {
+            if (h >= static_cast<int>(rows)) break;
+            if (c / 8 == h / 8)
 #pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (i < static_cast<int>(rows) && col < n) (y + row(i) * y_ld)[col] = plus(x.base[i], tile[i][lane]);
-        __builtin_amdgcn_wave_barrier();
+                for (int t = 0; t < 4; ++t)
+                    *reinterpret_cast<lo_f32x4_t *>(&tile[c % 8][t * 16 + q * 4]) = acc[t];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = h; i < h + 8 && i < R; ++i)
+                if (i < static_cast<int>(rows) && col < n) (y + row(i) * y_ld)[col] = plus(x.base[i], tile[i - h][lane]);
+            __builtin_amdgcn_wave_barrier();
+        }
     };
     RowsTile<T, NJ, R> one, two;
     request(one, 0);
@@ -437,10 +463,10 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
     constexpr bool kAhead = !PACKED && NJ <= 2;     // the registers hold two tiles of B
     __shared__ uint8_t lists[kLoraWaves][64];
     __shared__ uint64_t leads[Q];
-    __shared__ __attribute__((aligned(16))) uint16_t vs[64 * (2 * 16 * NJ + 8)];
-    __shared__ __attribute__((aligned(16))) float tile[kLoraWaves][16][68];
+    __shared__ __attribute__((aligned(16))) uint16_t vs[64 * (kParts<T> * 16 * NJ + 8)];
+    __shared__ __attribute__((aligned(16))) float tile[kLoraWaves][8][68];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.x * 64 * Q;
-    const uint32_t c = lane & 15u, q = lane >> 4, vs_ld = 2 * rank + 8, quads = rank / 4;
+    const uint32_t c = lane & 15u, q = lane >> 4, vs_ld = kParts<T> * rank + 8, quads = rank / 4;
     const uint64_t split = static_cast<uint64_t>(m) * rank;
     const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
     const uint32_t splits = ranges_of(k, o.chunks, down_blocks).splits;
@@ -473,24 +499,28 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
                 for (uint32_t u = 0; u < kLoads; ++u)
                     if (u < splits) f[0] += part[u].x, f[1] += part[u].y, f[2] += part[u].z, f[3] += part[u].w;
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
+                for (uint32_t h = 0; h < kParts<T>; ++h)
                     *reinterpret_cast<uint2 *>(terms_of + member * vs_ld + h * rank + r) =
                         make_uint2(parts_of(f[0] * scale, f[1] * scale, h), parts_of(f[2] * scale, f[3] * scale, h));
             }
         };
-        auto terms = [&](uint32_t member, uint4 (&vf)[NJ]) {
+        auto terms = [&](uint32_t member, Terms<T, NJ> &vf) {
+            const uint16_t *of = terms_of + min(member, rows - 1) * vs_ld;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                const uint32_t r = (2 * j + q / 2) * 8;
-                vf[j] = *reinterpret_cast<const uint4 *>(terms_of + min(member, rows - 1) * vs_ld + (q & 1) * rank +
-                                                         min(r, rank - 8));
-                if (r >= rank) vf[j] = make_uint4(0, 0, 0, 0);
+                const uint32_t r = (2 * j + q / 2) * 8, at = min(r, rank - 8);
+                vf.v[j] = *reinterpret_cast<const uint4 *>(of + (q & 1) * rank + at);
+                if (r >= rank) vf.v[j] = make_uint4(0, 0, 0, 0);
+                if constexpr (sizeof(T) == 4) {
+                    vf.low[j] = *reinterpret_cast<const uint4 *>(of + 2 * rank + at);
+                    if (r >= rank || (q & 1)) vf.low[j] = make_uint4(0, 0, 0, 0);
+                }
             }
         };
         if (few) {
             if (col0 >= n) continue;
             const uint32_t mine = row0 + list[min(c, rows - 1)];
-            auto form = [&](uint4 (&vf)[NJ]) {
+            auto form = [&](Terms<T, NJ> &vf) {
                 fill(lane, 64);
                 __builtin_amdgcn_wave_barrier();
                 terms(c, vf);
@@ -509,11 +539,11 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
         }
         fill(threadIdx.x, kLoraThreads);
         __syncthreads();
-        if (!PACKED || !wide) {
+        if (!wide || (!PACKED && NJ == 1)) {
             for (uint32_t t = 0; t * 16 < rows && col0 < n; ++t)
                 lora_up_rows<T, NJ, 16, false>(bu, rank, n, base, base_ld, y, y_ld, row0 + list[min(t * 16 + c, rows - 1)],
                                                min(rows - t * 16, 16u), col0, tiles, tile[wave], lane,
-                                               [&](uint4 (&vf)[NJ]) { terms(t * 16 + c, vf); });
+                                               [&](Terms<T, NJ> &vf) { terms(t * 16 + c, vf); });
         } else {
             for (uint32_t u = 0; u < tiles; ++u) {
                 const uint32_t first = col0 + u * kLoraWaves * 64;
@@ -530,10 +560,10 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
 #pragma unroll
                     for (int t = 0; t < P; ++t) {
                         const uint32_t member = (t0 + t) * 16 + c;
-                        uint4 vf[NJ];
+                        Terms<T, NJ> vf;
                         terms(member, vf);
                         lo_f32x4_t acc[4];
-                        products<NJ>(bfr, vf, rank, q, acc);
+                        products<T, NJ>(bfr, vf, rank, q, acc);
                         float f[16];
                         floats16(raw[t], f);
 #pragma unroll

@@ -3,8 +3,8 @@
 Bounds: y is rounded once, by at most half a step of its dtype (2^-8 of the
 value in bf16, 2^-24 in fp32), and base + delta once more in fp32. Behind that,
 x . A^T is an fp32 sum of k exact products in some order (k * 2^-24 of sum
-|x||A|), scaled once; v . B^T has v as two bf16 parts (2^-16 of it) and is a
-sum of 2 rank products.
+|x||A|), scaled once; v . B^T has v as two bf16 parts (2^-16 of it), for fp32
+results as three (2^-23), and is a sum of 2 or 3 rank products.
 """
 import ctypes
 
@@ -80,7 +80,7 @@ class Case:
                                self.ids, val(base))
         half = 2.0 ** -24 if self.f32 else 2.0 ** -8
         bound = half * np.abs(ref) + 2.0 ** -24 * (np.abs(ref) + np.abs(val(base))) + (k + 2) * 2.0 ** -24 * mag
-        bound += (2.0 ** -16 + 2 * rank * 2.0 ** -24) * low
+        bound += ((2.0 ** -23 if self.f32 else 2.0 ** -16) + 3 * rank * 2.0 ** -24) * low
         assert (np.abs(val(got) - ref) <= bound * (1 + 2.0 ** -20)).all()
         bare = self.ids >= self.dims[4]
         assert np.array_equal(got[bare], base[bare]), "a row without an adapter is base"
