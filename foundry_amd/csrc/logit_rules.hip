@@ -10,7 +10,9 @@ namespace fh {
 // token needs to know of the row's lists stands in LDS: a block takes a run of
 // tokens, enters the bias list into a table of them and counts the whole history
 // there too. Every block of a row reads its lists, from
-// the L2: runs are as long as the LDS and a filled GPU allow.
+// the L2: runs are as long as the LDS and a filled GPU allow. 64 rows of 128256
+// bf16 take 6.7 us with no rule (4.9 TB/s), 12.5 with histories to 8192 and a
+// mask, 14.5 with 300 biases a row as well: the lists' latency and the tables.
 constexpr uint32_t kRuleTokens = 4096;
 constexpr uint32_t kRuleThreads = 256;
 // Blocks that a launch aims for before runs get longer than the shortest, of
@@ -36,7 +38,12 @@ __device__ __forceinline__ void for_list(const uint32_t *list, uint32_t n, Take 
 #pragma unroll
             for (uint32_t u = 0; u < kLoads; ++u) {
                 const uint32_t i = (q0 + u * kRuleThreads) * 4;
-                if (q0 + u * kRuleThreads < quads) take(i, v[u].x), take(i + 1, v[u].y), take(i + 2, v[u].z), take(i + 3, v[u].w);
+                if (q0 + u * kRuleThreads < quads) {
+                    take(i, v[u].x);
+                    take(i + 1, v[u].y);
+                    take(i + 2, v[u].z);
+                    take(i + 3, v[u].w);
+                }
             }
         }
         if (threadIdx.x < n % 4) take(quads * 4 + threadIdx.x, list[quads * 4 + threadIdx.x]);
@@ -168,7 +175,8 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(const T *z, u
                 o = make_uint4(f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]),
                                f32x2_to_bf16x2_rne(v[4], v[5]), f32x2_to_bf16x2_rne(v[6], v[7]));
             else
-                o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                               __float_as_uint(v[3]));
             if (same) {
                 *reinterpret_cast<uint4 *>(to + j0) = o;
             } else {
@@ -263,6 +271,7 @@ extern "C" int fh_logits_process(fh_device *dev, const void *logits, int dtype, 
     };
     float *const f32 = nullptr;
     uint16_t *const bf16 = nullptr;
-    if (dtype == FH_F32) return two ? launch(logit_rules_kernel<float, true>, f32) : launch(logit_rules_kernel<float, false>, f32);
+    if (dtype == FH_F32)
+        return two ? launch(logit_rules_kernel<float, true>, f32) : launch(logit_rules_kernel<float, false>, f32);
     return two ? launch(logit_rules_kernel<uint16_t, true>, bf16) : launch(logit_rules_kernel<uint16_t, false>, bf16);
 }

@@ -16,9 +16,15 @@ namespace fh {
 //
 // Grouping: rows come with their adapters in any order, so a block takes a
 // window of rows (64, or 256) and finds in it the groups of rows that share an
-// adapter, by ballots over the adapter ids; each group is cut into chunks of
-// up to 64 rows. Whatever the order, the products run on the matrix cores with the adapter's rows read
-// once for up to 64 rows (four tiles of 16).
+// adapter, by ballots over the adapter ids; each group is cut into chunks of up
+// to 64 rows. Whatever the order, the products run on the matrix cores with the
+// adapter's rows read once for up to 64 rows (four tiles of 16).
+//
+// Measured (down + up): 8 rows of 8 adapters, k 4096, n 6144, rank 16: 8.4 us,
+// of which each launch has 4 at least; 200 rows of 48 adapters, n 28672, rank
+// 16, f32 (98 MB): 28 us, 3.5 TB/s, a wavefront's few loads per 64 columns in
+// flight; 4096 packed rows, n 4096, rank 32 (103 MB): 37 us, 2.8 TB/s, the
+// latencies from ids to chunk to x or v before the stream begins.
 typedef __attribute__((ext_vector_type(8))) __bf16 lo_bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float lo_f32x4_t;
 
@@ -39,9 +45,10 @@ constexpr uint32_t kWideRows = 1024;
 // go round. With estimates of the host 1024 packed rows of rank 16 were left
 // to 40 blocks: 36 us against 24.
 constexpr uint32_t kDownBlocks = 512, kMaxSplits = 4, kDownSteps = 2;
+// Up, what the GPU holds of each form at once: 200 rows of 48 adapters take 28 us
+// at 768 blocks, 31.8 at 512, 32.7 at 1024; 4096 packed rows 36.8 at 512, 40.1 at
+// 768.
 constexpr uint32_t kUpBlocks = 768, kUpPacked = 512;
-// (Up, as many as the GPU holds at once: 200 rows of 48 adapters 28 us at 768
-// blocks, 31.8 at 512, 32.7 at 1024; 4096 packed rows 36.8 at 512, 40.1 at 768.)
 
 // The ranges of k of a window with `chunks` chunks and `blocks` blocks: `splits`
 // of them, of kLoraWaves x `steps` x 32.
@@ -64,7 +71,8 @@ __device__ __forceinline__ Ranges ranges_of(uint32_t k, uint32_t chunks, uint32_
 // before it with its adapter; rows of rank 0, 64, .. lead a chunk, and the
 // chunks are numbered by their leaders' order. Ranks come from match masks,
 // formed bit by bit of the ids: a ballot per bit and 64 rows, instead of a
-// round per adapter (48 adapters in 256 rows: 6 us a block).
+// round per adapter (200 rows of 48 adapters: 181 -> 55 us, with the splits'
+// sums requested together).
 template <int Q>
 struct Window {
     uint32_t id[Q];     // lane's rows' adapters
@@ -170,8 +178,8 @@ __device__ __forceinline__ uint32_t chunk_of(const Window<Q> &o, uint32_t item, 
 // up to 16 RT rows. Each wavefront takes a quarter of the split's k for all the
 // rows, so that A's rows come once per chunk; they add up in LDS in their order.
 // A product has the ranks along its rows, so that a lane ends up with 4 ranks of
-// a row. (With 16 rows and all the k to a wavefront A came four times: 17 us for
-// 4096 packed rows of k 4096, rank 32, as much of it A's as x's.)
+// a row. (With 16 rows and all the k to a wavefront A comes four times: 16.9 us
+// against 15.5 for 4096 packed rows of k 4096, rank 32.)
 template <int RT, int NR>
 __device__ __forceinline__ void lora_down_chunk(const uint16_t *x, uint32_t k, uint64_t x_ld, const uint16_t *a,
                                                 uint32_t rank, uint32_t k0, uint32_t k1, uint32_t row0, uint32_t rows,
@@ -355,7 +363,8 @@ __device__ __forceinline__ void request_b(const uint16_t *b, uint32_t rank, uint
         const uint32_t col = min(col0 + (WIDE ? c / 4 * 16 + t * 4 + c % 4 : t * 16 + c), n - 1);
         const uint16_t *br = b + static_cast<uint64_t>(col) * rank;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) f[t][j] = *reinterpret_cast<const uint4 *>(br + min((2 * j + q / 2) * 8, rank - 8));
+        for (int j = 0; j < NJ; ++j)
+            f[t][j] = *reinterpret_cast<const uint4 *>(br + min((2 * j + q / 2) * 8, rank - 8));
     }
 }
 
@@ -400,7 +409,9 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, uint32_t rank, u
                                              Form terms) {
     const uint32_t c = lane & 15u, q = lane >> 4;
     Terms<T, NJ> vf;
-    auto row = [&](int i) { return static_cast<uint64_t>(__builtin_amdgcn_readlane(mine, min(i, static_cast<int>(rows) - 1))); };
+    auto row = [&](int i) {
+        return static_cast<uint64_t>(__builtin_amdgcn_readlane(mine, min(i, static_cast<int>(rows) - 1)));
+    };
     auto request = [&](RowsTile<T, NJ, R> &x, uint32_t u) {
         const uint32_t at = col0 + min(u, tiles - 1) * kLoraWaves * 64;
         request_b<NJ, false>(b, rank, n, at, c, q, x.b);
@@ -422,7 +433,8 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, uint32_t rank, u
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int i = h; i < h + 8 && i < R; ++i)
-                if (i < static_cast<int>(rows) && col < n) (y + row(i) * y_ld)[col] = plus(x.base[i], tile[i - h][lane]);
+                if (i < static_cast<int>(rows) && col < n)
+                    (y + row(i) * y_ld)[col] = plus(x.base[i], tile[i - h][lane]);
             __builtin_amdgcn_wave_barrier();
         }
     };
@@ -541,8 +553,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
         __syncthreads();
         if (!wide || (!PACKED && NJ == 1)) {
             for (uint32_t t = 0; t * 16 < rows && col0 < n; ++t)
-                lora_up_rows<T, NJ, 16, false>(bu, rank, n, base, base_ld, y, y_ld, row0 + list[min(t * 16 + c, rows - 1)],
-                                               min(rows - t * 16, 16u), col0, tiles, tile[wave], lane,
+                lora_up_rows<T, NJ, 16, false>(bu, rank, n, base, base_ld, y, y_ld,
+                                               row0 + list[min(t * 16 + c, rows - 1)], min(rows - t * 16, 16u), col0, tiles, tile[wave], lane,
                                                [&](Terms<T, NJ> &vf) { terms(t * 16 + c, vf); });
         } else {
             for (uint32_t u = 0; u < tiles; ++u) {
@@ -554,9 +566,10 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
                 for (uint32_t t0 = 0; t0 * 16 < rows; t0 += P) {
                     Raw16<T> raw[P];
 #pragma unroll
-                    for (int t = 0; t < P; ++t)
-                        raw[t] = request16(base + static_cast<uint64_t>(row0 + list[min((t0 + t) * 16 + c, rows - 1)]) * base_ld +
-                                           col);
+                    for (int t = 0; t < P; ++t) {
+                        const uint64_t row = row0 + list[min((t0 + t) * 16 + c, rows - 1)];
+                        raw[t] = request16(base + row * base_ld + col);
+                    }
 #pragma unroll
                     for (int t = 0; t < P; ++t) {
                         const uint32_t member = (t0 + t) * 16 + c;
@@ -684,7 +697,8 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     const uint64_t most = std::min<uint64_t>(rows, rows_of);
     const uint32_t down_blocks = static_cast<uint32_t>(
         std::clamp<uint64_t>(kDownBlocks / windows, 1, most * most_splits(static_cast<uint32_t>(k))));
-    const uint32_t up_blocks = static_cast<uint32_t>(std::clamp<uint64_t>((m > kWideRows ? kUpPacked : kUpBlocks) / windows, 1, most * cols));
+    const uint64_t up_all = m > kWideRows ? kUpPacked : kUpBlocks;
+    const uint32_t up_blocks = static_cast<uint32_t>(std::clamp<uint64_t>(up_all / windows, 1, most * cols));
     const dim3 down(static_cast<uint32_t>(windows), down_blocks), up(static_cast<uint32_t>(windows), up_blocks);
     const dim3 threads(kLoraThreads);
     float *v = static_cast<float *>(workspace);
@@ -701,8 +715,8 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     auto run_up = [&](auto kernel, auto *of) {
         using T = std::remove_pointer_t<decltype(of)>;
         return dispatch(dev, fn, [&] {
-            hipLaunchKernelGGL(kernel, up, threads, 0, dev->stream, v, down_blocks, m32, k32, b, scales, u32, rank32, n32,
-                               adapters, static_cast<const T *>(base), static_cast<uint64_t>(base_ld),
+            hipLaunchKernelGGL(kernel, up, threads, 0, dev->stream, v, down_blocks, m32, k32, b, scales, u32, rank32,
+                               n32, adapters, static_cast<const T *>(base), static_cast<uint64_t>(base_ld),
                                static_cast<T *>(y), static_cast<uint64_t>(y_ld), wide);
         });
     };

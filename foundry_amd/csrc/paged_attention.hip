@@ -13,12 +13,12 @@ namespace fh {
 // joined over disjoint key ranges by the same rule. Exponentials are taken as
 // powers of two of scores scaled by log2 e.
 //
-// The split: a block of four wavefronts takes one part of a sequence (whole
-// steps of kStepKeys keys) for one KV head and up to 8 of the query heads that
-// share it; each wavefront streams its quarter of the part's keys, 32 at a
-// time, and the four join in LDS. The parts of all sequences are laid out from
-// the positions on the device (see find_part), so the same launch serves one
-// long context and a ragged batch, and may be captured.
+// The split: a block of four wavefronts takes a part of the batch's keys (whole
+// steps of kStepKeys) for one KV head and up to 8 of the query heads that share
+// it; of each sequence in its part every wavefront streams a quarter of the
+// keys, 32 at a time, and the four join in LDS. The parts are laid out from
+// the positions on the device (see Layout), so the same launch serves one long
+// context and a ragged batch, and may be captured.
 //
 // Per 32 keys the scores are S^T = K Q^T on the matrix cores
 // (v_mfma_f32_16x16x32_bf16, 16 keys x 16 columns): a lane ends up with its
@@ -29,10 +29,17 @@ namespace fh {
 // columns are 8 heads twice: columns 0..7 hold the probabilities rounded to
 // bf16, columns 8..15 what that rounding lost, so that P V has 16 bits of P at
 // the cost of none (the columns would idle).
+//
+// Bound by memory: K and V come once, with the nontemporal hint (131077 keys of
+// 8 KV heads of 128: 104 us without, 90 with), the next tile's K in flight behind
+// a tile's softmax, its V behind the next one's. 131077 keys (537 MB) take 91 us
+// with the join (5.9 TB/s; the parts alone 80, 6.7 TB/s), 96 ragged sequences of
+// 17 to 16384 keys (950 MB) 161 (5.9 TB/s), 8 of 1900 to 4111 (97 MB) 24.
 constexpr uint32_t kPagedThreads = 256;
 constexpr uint32_t kStepKeys = 128;
 constexpr uint32_t kHeadTile = 8;
-// Blocks of a launch: what the GPU holds at once.
+// Blocks of a launch: what the GPU holds at once (2 per CU). 8 sequences, 96,
+// one of 131077 keys: 24.0, 161, 91.9 us with 512; 29.0, 169, 92.3 with 768.
 constexpr uint32_t kPartBlocks = 512;
 // Tables of so few positions (times head_dim) take one block per sequence, of 8
 // wavefronts (4 at head_dim 256), and no join: one launch. One sequence of 500
@@ -169,7 +176,8 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
         const uint32_t keys = count ? a.positions[seq] + 1 : 0;
         // this wavefront's keys: from .. to, in tiles of 32
         const uint32_t share = (count * (kStepKeys / 32) + W - 1) / W * 32;
-        const uint32_t from = first * kStepKeys + wave * share, to = min(from + share, min(keys, (first + count) * kStepKeys));
+        const uint32_t from = first * kStepKeys + wave * share;
+        const uint32_t to = min(from + share, min(keys, (first + count) * kStepKeys));
         const uint32_t n_tiles = from < to ? (to - from + 31) / 32 : 0;
 
         uint4 qf[KC];
@@ -206,7 +214,8 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
                 for (int h = 0; h < 2; ++h) {
                     const uint16_t *src = a.k_pages + group_at(t, h) + c * 32 + q * 8;
 #pragma unroll
-                    for (int s = 0; s < KC; ++s) kf[h][s] = load_stream16(reinterpret_cast<const uint4 *>(src + s * 512));
+                    for (int s = 0; s < KC; ++s)
+                        kf[h][s] = load_stream16(reinterpret_cast<const uint4 *>(src + s * 512));
                 }
             };
             auto load_v = [&](uint32_t t) {
@@ -238,7 +247,8 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
                 float s[8];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[i] = s0[i] * scale2, s[4 + i] = s1[i] * scale2;
-                const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2), w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
+                const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2);
+                const uint32_t w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
                 const uint32_t key0 = from + (t0 + t) * 32;
                 if (w0 == ~0u || w1 == ~0u || key0 + 32 > to) {
                     // keys past the position or of no page: no score, and no value, whatever lies there
@@ -255,7 +265,8 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
                 } else {
                     any = true;
                 }
-                float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+                float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                                  fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
                 const float next = fmaxf(m, top);
@@ -270,7 +281,8 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
                 uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p0 = __builtin_amdgcn_exp2f(s[2 * i] - ref), p1 = __builtin_amdgcn_exp2f(s[2 * i + 1] - ref);
+                    const float p0 = __builtin_amdgcn_exp2f(s[2 * i] - ref);
+                    const float p1 = __builtin_amdgcn_exp2f(s[2 * i + 1] - ref);
                     l += p0 + p1;
                     const uint32_t hi = f32x2_to_bf16x2_rne(p0, p1);
                     // what the rounding lost; nothing of an inf or NaN
@@ -288,8 +300,8 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
                         return d / 2 == 0 ? v.x : d / 2 == 1 ? v.y : d / 2 == 2 ? v.z : v.w;
                     };
                     const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
-                    const uint4 f = make_uint4(__builtin_amdgcn_perm(word(1), word(0), sel), __builtin_amdgcn_perm(word(3), word(2), sel),
-                                               __builtin_amdgcn_perm(word(5), word(4), sel), __builtin_amdgcn_perm(word(7), word(6), sel));
+                    auto pair = [&](int i) { return __builtin_amdgcn_perm(word(i + 1), word(i), sel); };
+                    const uint4 f = make_uint4(pair(0), pair(2), pair(4), pair(6));
                     acc[t] = pa_mfma(f, pf, acc[t]);
                 }
             };
@@ -469,6 +481,10 @@ int check_shape(const char *fn, int64_t batch, int64_t n_heads, int64_t n_kv, in
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: %lld heads do not share %lld KV heads", fn, (long long)n_heads,
                     (long long)n_kv);
     if (batch > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: batch %lld exceeds 65535", fn, (long long)batch);
+    // the steps of all sequences are counted in 32 bits (pages may be shared, so their number bounds nothing)
+    if (batch * (max_pages * page_size / kStepKeys + 1) > 0x7FFFFFFFll)
+        return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld sequences of %lld positions", fn, (long long)batch,
+                    (long long)(max_pages * page_size));
     return FH_OK;
 }
 

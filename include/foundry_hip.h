@@ -549,7 +549,8 @@ int fh_paged_attention_workspace(int64_t batch, int64_t n_heads, int64_t n_kv, i
  * are left out; a sequence left with no key gets zeros. What lies in a page
  * behind the position is not used, whatever its bits. A row whose every score
  * is -inf is NaN. head_dim is 64, 128 or 256; any n_heads / n_kv; batch at
- * most 65535; out does not overlap the inputs. workspace: at least
+ * most 65535, and batch * (max_pages * page_size / 128 + 1) at most 2^31 - 1;
+ * out does not overlap the inputs. workspace: at least
  * fh_paged_attention_workspace() bytes, 16-byte aligned, no initial contents;
  * calls that share a workspace must not run concurrently. */
 int fh_paged_attention(fh_device *dev, const uint16_t *q, int64_t batch, int64_t n_heads,

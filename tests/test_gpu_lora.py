@@ -137,6 +137,21 @@ def test_a_prompt_batch(device):
     Case(device, 9, len(ids), 1024, 384, 32, 3, ids).check()
 
 
+@pytest.mark.parametrize("n", [96, 101])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("rank", [16, 40, 128])
+def test_more_rows_than_a_wide_window_holds(device, rank, f32, n):
+    """Past 1024 rows: packed requests from one row to hundreds, rows with no adapter among them."""
+    ids = np.repeat([1, NONE, 0, 3, 2, NONE, 4, 0, 1], [500, 70, 1, 15, 64, 3, 33, 400, 130])
+    c = Case(device, rank + n, len(ids), 136, n, rank, 5, ids, f32)
+    assert np.array_equal(c.check(), c.run(in_place=True))
+
+
+def test_many_rows_in_no_order(device):
+    ids = np.random.default_rng(3).integers(0, 40, 1500)
+    Case(device, 11, len(ids), 200, 80, 16, 39, np.where(ids == 39, NONE, ids)).check()
+
+
 def test_special_values_stay_in_their_rows(device):
     """An inf or NaN of one row's x or base does not reach rows beside it,
     nor an adapter's NaN the rows of others."""

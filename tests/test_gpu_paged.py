@@ -200,9 +200,25 @@ def test_attention_split_over_the_context(device, heads, kv, hd, page, lens):
     check_attention(device, *cache(sum(lens) + hd, lens, heads, kv, hd, page), hd ** -0.5)
 
 
-def test_attention_many_ragged_sequences(device):
+@pytest.mark.parametrize("width", [46, 80])
+def test_attention_many_ragged_sequences(device, width):
+    """A block per sequence, and (past the positions that this is for) parts
+    laid out over more than 64 sequences."""
     lens = [(i * 7919) % 700 if i % 9 else 0 for i in range(300)]
-    check_attention(device, *cache(77, lens, 4, 1, 64, 16), 64 ** -0.5)
+    check_attention(device, *cache(77, lens, 4, 1, 64, 16, width=width), 64 ** -0.5)
+
+
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+def test_attention_short_contexts_of_wide_tables(device, heads, kv, hd):
+    """The parts' layout where every sequence is shorter than a step or ends near one."""
+    lens = [1, 0, 17, 127, 128, 129, 255, 256, 257, 0, 0, 31, 300]
+    check_attention(device, *cache(heads + hd, lens, heads, kv, hd, 16, width=100), hd ** -0.5)
+
+
+def test_attention_idle_runs_of_a_large_batch(device):
+    """Whole groups of 64 sequences idle, at the start, between and at the end."""
+    lens = [0] * 70 + [40, 900] + [0] * 130 + [5] * 3 + [0] * 80
+    check_attention(device, *cache(80, lens, 4, 2, 64, 16, width=80), 64 ** -0.5)
 
 
 @pytest.mark.parametrize("width", [8, 80])

@@ -39,6 +39,8 @@ def test_paged_attention_workspace():
     refused(_lib.ERR_UNSUPPORTED, name, 1, 4, 2, 96, 16, 4)
     refused(_lib.ERR_INDEX_TOO_LARGE, name, 65536, 4, 2, 64, 16, 4)
     refused(_lib.ERR_INDEX_TOO_LARGE, name, 1, 4, 2, 64, 16, 1 << 27)
+    # more steps than 32 bits count, over pages that sequences share
+    refused(_lib.ERR_INDEX_TOO_LARGE, name, 1024, 4, 2, 64, 1 << 30, 1)
     assert _lib.load().fh_paged_attention_workspace(1, 4, 2, 64, 16, 4, None) == bad
 
 
