@@ -11,8 +11,9 @@ namespace fh {
 // tokens, enters the bias list into a table of them and counts the whole history
 // there too. Every block of a row reads its lists, from
 // the L2: runs are as long as the LDS and a filled GPU allow. 64 rows of 128256
-// bf16 take 6.7 us with no rule (4.9 TB/s), 12.5 with histories to 8192 and a
-// mask, 14.5 with 300 biases a row as well: the lists' latency and the tables.
+// bf16 take 6.7 us with no rule (4.9 TB/s), 11.0 with histories to 500, 13.3 with
+// histories to 8192, 14.5 with a mask and 300 biases a row as well: the lists'
+// latency and the tables.
 constexpr uint32_t kRuleTokens = 4096;
 constexpr uint32_t kRuleThreads = 256;
 // Blocks that a launch aims for before runs get longer than the shortest, of
