@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void paged_rope_kv_kernel(
             to = keys + k_offset(slot, d, page_size, head_dim);
             to2 = keys + k_offset(slot, half + d, page_size, head_dim);
         } else {
-            to = v_pages + base + (h - n_heads - n_kv) * region + slot * head_dim + d;
+            to = v_pages + base + (h - n_heads - n_kv) * region + static_cast<uint64_t>(slot) * head_dim + d;
             to2 = to + half;
         }
         put16<STREAM>(to, x);

@@ -357,6 +357,33 @@ def test_attention_a_pool_past_4_gib(device):
     assert np.array_equal(tail[:, :63], v[0][:, :63])
 
 
+def test_append_into_a_page_past_2_32_elements(device):
+    """One long page (a cache that is not cut): the row of its last position
+    begins past 2^32 elements, and the rows that the low 32 bits would name stay."""
+    heads, kv, hd, page = 1, 1, 256, (1 << 24) + 16
+    pool = [device.zeros(page * hd * 2) for _ in range(2)]
+    table = device.zeros(page * hd * 2)  # cos and sin: both zero but for the last position's cos
+    ones = np.full(hd, 0x3F80, np.uint16)
+    last = page - 1
+    _lib.call("fh_upload", device.handle, p(table, last * hd * 2), ones.ctypes.data_as(ctypes.c_void_p), ones.nbytes)
+    sin = device.zeros(page * hd * 2)
+    qkv = synth.bf16_normal(5, (1, 3 * hd))
+    s_qkv, s_pos, s_t, out = up(device, qkv), up(device, np.array([last], np.uint32)), device.zeros(4), device.empty(hd * 2)
+    _lib.call("fh_paged_rope_kv", device.handle, p(s_qkv), 1, heads, kv, hd, p(table), p(sin), page, None, p(s_pos),
+              p(s_t), 1, 1, p(pool[0]), p(pool[1]), 1, page, p(out))
+    q, k, v = qkv.reshape(3, hd)
+    assert np.array_equal(down(device, out, np.uint16, (hd,)), q)  # cos 1, sin 0
+    for st, row, is_k in ((pool[0], k, True), (pool[1], v, False)):
+        group, head = np.empty((2, 16, hd), np.uint16)
+        _lib.call("fh_download", device.handle, group.ctypes.data_as(ctypes.c_void_p), p(st, (page - 16) * hd * 2),
+                  group.nbytes)
+        _lib.call("fh_download", device.handle, head.ctypes.data_as(ctypes.c_void_p), p(st), head.nbytes)
+        want = np.zeros((16, hd), np.uint16)
+        want[15] = row
+        assert np.array_equal(group, tile_k(want[None, None])[0, 0].reshape(16, hd) if is_k else want)
+        assert not head.any()
+
+
 # ----------------------------------------------------------------- refusals
 
 def refused(status, name, *args, match=""):
