@@ -1,4 +1,6 @@
 // Appending to a paged cache with the rotation on the way (fh_paged_rope_kv).
+#include <tuple>
+
 #include "paged_cache.hpp"
 
 namespace fh {
@@ -105,6 +107,8 @@ extern "C" int fh_paged_rope_kv(fh_device *dev, const uint16_t *qkv, int64_t tok
                     (long long)n_kv);
     if (n_seqs < 1 || table_len < 1)
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: n_seqs and table_len must be at least 1", fn);
+    // a launch has fewer than 2^32 threads
+    if (tokens > 0xFFFFFF) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld tokens exceed 2^24 - 1", fn, (long long)tokens);
     if (sequences == nullptr && tokens > n_seqs)
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: %lld tokens of %lld sequences need their sequences named", fn,
                     (long long)tokens, (long long)n_seqs);
@@ -127,11 +131,20 @@ extern "C" int fh_paged_rope_kv(fh_device *dev, const uint16_t *qkv, int64_t tok
     if (int rc = check_range(dev, q_out, t * n_heads * head_dim * 2, fn, "q_out")) return rc;
     const uint64_t q_bytes = t * n_heads * head_dim * 2;
     if (int rc = refuse_overlap(fn, "v_pages", v_pages, pool, "k_pages", k_pages, pool)) return rc;
-    if (int rc = refuse_overlap(fn, "q_out", q_out, q_bytes, "qkv", qkv, t * width * 2)) return rc;
     if (int rc = refuse_overlap(fn, "q_out", q_out, q_bytes, "k_pages", k_pages, pool)) return rc;
     if (int rc = refuse_overlap(fn, "q_out", q_out, q_bytes, "v_pages", v_pages, pool)) return rc;
-    if (int rc = refuse_overlap(fn, "k_pages", k_pages, pool, "qkv", qkv, t * width * 2)) return rc;
-    if (int rc = refuse_overlap(fn, "v_pages", v_pages, pool, "qkv", qkv, t * width * 2)) return rc;
+    const uint64_t entries = static_cast<uint64_t>(n_seqs) * max_pages * 4;
+    for (const auto &[what, ptr, size] : {std::tuple{"q_out", static_cast<const void *>(q_out), q_bytes},
+                                          std::tuple{"k_pages", static_cast<const void *>(k_pages), pool},
+                                          std::tuple{"v_pages", static_cast<const void *>(v_pages), pool}}) {
+        if (int rc = refuse_overlap(fn, what, ptr, size, "qkv", qkv, t * width * 2)) return rc;
+        if (int rc = refuse_overlap(fn, what, ptr, size, "cos_tab", cos_tab, table)) return rc;
+        if (int rc = refuse_overlap(fn, what, ptr, size, "sin_tab", sin_tab, table)) return rc;
+        if (int rc = refuse_overlap(fn, what, ptr, size, "positions", positions, t * 4)) return rc;
+        if (int rc = refuse_overlap(fn, what, ptr, size, "page_table", page_table, entries)) return rc;
+        if (sequences)
+            if (int rc = refuse_overlap(fn, what, ptr, size, "sequences", sequences, t * 4)) return rc;
+    }
     if (int rc = set_current(dev, fn)) return rc;
     // what 8 XCDs' L2s do not hold anyway goes past them: 8192 tokens of 32 and 8
     // heads of 128 (100 MB) 40.3 -> 35.1 us (5.8 TB/s); no difference at 61 tokens

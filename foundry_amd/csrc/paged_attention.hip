@@ -554,6 +554,11 @@ extern "C" int fh_paged_attention(fh_device *dev, const uint16_t *q, int64_t bat
         if (int rc = refuse_overlap(fn, what, ptr, size, "q", q, rows)) return rc;
         if (int rc = refuse_overlap(fn, what, ptr, size, "k_pages", k_pages, pool)) return rc;
         if (int rc = refuse_overlap(fn, what, ptr, size, "v_pages", v_pages, pool)) return rc;
+        if (int rc = refuse_overlap(fn, what, ptr, size, "page_table", page_table,
+                                    static_cast<uint64_t>(batch) * max_pages * 4))
+            return rc;
+        if (int rc = refuse_overlap(fn, what, ptr, size, "positions", positions, static_cast<uint64_t>(batch) * 4))
+            return rc;
     }
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "out", out, rows)) return rc;
     if (int rc = set_current(dev, fn)) return rc;

@@ -520,13 +520,14 @@ int fh_append_token_advance(fh_device *dev, const uint32_t *token, int64_t rows,
  * qkv: [tokens, (n_heads + 2 n_kv) * head_dim]; cos_tab / sin_tab:
  * [table_len, head_dim]; sequences: u32 [tokens], or null where token t is of
  * sequence t (tokens <= n_seqs); positions: u32 [tokens]; q_out: [tokens,
- * n_heads, head_dim], not overlapping qkv. A token whose position is >=
- * max_pages * page_size or >= table_len, whose sequence is >= n_seqs or whose
- * page is >= n_pages writes nothing, neither to the pools nor to q_out (a
- * padded row takes a position past the pages, far enough below 2^32 where
- * fh_advance_positions moves it on). Two tokens of one sequence and position
- * leave the values of either in each 16-byte piece. head_dim is a multiple of
- * 32, at most 256. */
+ * n_heads, head_dim]. q_out and the pools overlap neither each other nor the
+ * inputs. A token whose position is >= max_pages * page_size or >= table_len,
+ * whose sequence is >= n_seqs or whose page is >= n_pages writes nothing,
+ * neither to the pools nor to q_out (a padded row takes a position past the
+ * pages, far enough below 2^32 where fh_advance_positions moves it on). Two
+ * tokens of one sequence and position leave the values of either in each
+ * 16-byte piece. head_dim is a multiple of 32, at most 256, tokens at most
+ * 2^24 - 1. */
 int fh_paged_rope_kv(fh_device *dev, const uint16_t *qkv, int64_t tokens, int64_t n_heads,
                      int64_t n_kv, int64_t head_dim, const uint16_t *cos_tab,
                      const uint16_t *sin_tab, int64_t table_len, const uint32_t *sequences,

@@ -466,3 +466,41 @@ def test_attention_refusals(device):
     refused(_lib.ERR_INDEX_TOO_LARGE, name, *args(batch=65536))
     refused(_lib.ERR_OUT_OF_BOUNDS, name, *args(n_pages=1 << 20))
     refused(_lib.ERR_FOREIGN_STORAGE, name, *args(k=ctypes.c_void_p(4096)))
+
+
+def test_append_refuses_outputs_over_its_device_lists(device):
+    """The lists steer addresses: no output may change them under way."""
+    heads, kv, hd, page, t = 4, 2, 64, 16, 3
+    big = {k: device.zeros(1 << 16) for k in ("qkv", "cos", "sin", "seq", "pos", "table", "k", "v", "q")}
+
+    def args(**o):
+        a = dict(dev=device.handle, qkv=p(big["qkv"]), tokens=t, heads=heads, kv=kv, hd=hd, cos=p(big["cos"]),
+                 sin=p(big["sin"]), table_len=32, seq=p(big["seq"]), pos=p(big["pos"]), table=p(big["table"]), n_seqs=2,
+                 max_pages=2, k=p(big["k"]), v=p(big["v"]), n_pages=4, page=page, q=p(big["q"]))
+        return list((a | o).values())
+
+    bad, name = _lib.ERR_INVALID_ARGUMENT, "fh_paged_rope_kv"
+    _lib.call(name, *args())
+    for of in ("q", "k", "v"):
+        for over in ("qkv", "cos", "sin", "seq", "pos", "table"):
+            refused(bad, name, *args(**{of: p(big[over])}), match="overlap")
+    refused(_lib.ERR_INDEX_TOO_LARGE, name, *args(tokens=1 << 24), match="tokens")
+
+
+def test_attention_refuses_outputs_over_its_device_lists(device):
+    b, heads, kv, hd, page, width = 2, 4, 2, 64, 16, 2
+    nbytes = _lib.paged_attention_workspace_bytes(b, heads, kv, hd, page, width)
+    assert nbytes <= 1 << 16
+    big = {k: device.zeros(1 << 16) for k in ("q", "k", "v", "table", "pos", "ws", "out")}
+
+    def args(**o):
+        a = dict(dev=device.handle, q=p(big["q"]), batch=b, heads=heads, kv=kv, hd=hd, k=p(big["k"]), v=p(big["v"]),
+                 n_pages=4, page=page, table=p(big["table"]), max_pages=width, pos=p(big["pos"]),
+                 scale=ctypes.c_float(1.0), ws=p(big["ws"]), nbytes=nbytes, out=p(big["out"]))
+        return list((a | o).values())
+
+    bad, name = _lib.ERR_INVALID_ARGUMENT, "fh_paged_attention"
+    _lib.call(name, *args())
+    for of in ("ws", "out"):
+        for over in ("q", "k", "v", "table", "pos"):
+            refused(bad, name, *args(**{of: p(big[over])}), match="overlap")
