@@ -1,4 +1,5 @@
 // Penalties, biases and grammar masks on logits (fh_logits_process).
+#include <tuple>
 #include <type_traits>
 
 #include "serving_checks.hpp"
@@ -236,26 +237,22 @@ extern "C" int fh_logits_process(fh_device *dev, const void *logits, int dtype, 
     if (int rc = check_range(dev, out, bytes, fn, "out")) return rc;
     if (logits != out)
         if (int rc = refuse_overlap(fn, "out", out, bytes, "logits", logits, bytes)) return rc;
-    if (u.history) {
-        if (int rc = check_range(dev, u.history, r * u.history_ld * 4, fn, "history")) return rc;
-        if (int rc = check_range(dev, u.history_len, r * 4, fn, "history_len")) return rc;
+    const uint64_t each = r * 4;
+    for (const auto &[what, ptr, size] :
+         {std::tuple{"history", static_cast<const void *>(u.history), each * u.history_ld},
+          std::tuple{"history_len", static_cast<const void *>(u.history_len), each},
+          std::tuple{"prompt_len", static_cast<const void *>(u.prompt_len), each},
+          std::tuple{"repetition", static_cast<const void *>(u.repetition), each},
+          std::tuple{"frequency", static_cast<const void *>(u.frequency), each},
+          std::tuple{"presence", static_cast<const void *>(u.presence), each},
+          std::tuple{"bias_ids", static_cast<const void *>(u.bias_ids), each * u.bias_ld},
+          std::tuple{"bias_values", static_cast<const void *>(u.bias_values), each * u.bias_ld},
+          std::tuple{"bias_len", static_cast<const void *>(u.bias_ids ? u.bias_len : nullptr), each},
+          std::tuple{"mask", static_cast<const void *>(u.mask), each * ((n + 31) / 32)}}) {
+        if (ptr == nullptr) continue;
+        if (int rc = check_range(dev, ptr, size, fn, what)) return rc;
+        if (int rc = refuse_overlap(fn, "out", out, bytes, what, ptr, size)) return rc;
     }
-    if (u.bias_ids) {
-        if (int rc = check_range(dev, u.bias_ids, r * u.bias_ld * 4, fn, "bias_ids")) return rc;
-        if (int rc = check_range(dev, u.bias_values, r * u.bias_ld * 4, fn, "bias_values")) return rc;
-        if (u.bias_len)
-            if (int rc = check_range(dev, u.bias_len, r * 4, fn, "bias_len")) return rc;
-    }
-    if (u.prompt_len)
-        if (int rc = check_range(dev, u.prompt_len, r * 4, fn, "prompt_len")) return rc;
-    if (u.repetition)
-        if (int rc = check_range(dev, u.repetition, r * 4, fn, "repetition")) return rc;
-    if (u.frequency)
-        if (int rc = check_range(dev, u.frequency, r * 4, fn, "frequency")) return rc;
-    if (u.presence)
-        if (int rc = check_range(dev, u.presence, r * 4, fn, "presence")) return rc;
-    if (u.mask)
-        if (int rc = check_range(dev, u.mask, r * ((n + 31) / 32) * 4, fn, "mask")) return rc;
     if (int rc = set_current(dev, fn)) return rc;
     const bool two = (u.history && u.history_ld > kMaxCounted) || (u.bias_ids && u.bias_ld >= kMaxBiases);
     const uint32_t longest = two ? kRuleTokens / 2 : kRuleTokens;

@@ -686,6 +686,8 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
         if (int rc = refuse_overlap(fn, what, ptr, size, "a", a, a_bytes)) return rc;
         if (int rc = refuse_overlap(fn, what, ptr, size, "b", b, b_bytes)) return rc;
         if (int rc = refuse_overlap(fn, what, ptr, size, "adapters", adapters, rows * 4)) return rc;
+        if (int rc = refuse_overlap(fn, what, ptr, size, "scales", scales, static_cast<uint64_t>(n_adapters) * 4))
+            return rc;
     }
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "y", y, y_bytes)) return rc;
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "base", base, base_bytes)) return rc;

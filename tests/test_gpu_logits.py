@@ -246,3 +246,19 @@ def test_refusals(device):
     refused(_lib.ERR_OUT_OF_BOUNDS, rules=dict(history=a["ids"], history_ld=9, history_len=a["len"]))
     refused(_lib.ERR_OUT_OF_BOUNDS, rules=dict(mask=a["mask"] + 8))
     refused(_lib.ERR_FOREIGN_STORAGE, rules=dict(mask=4096))
+
+
+def test_refuses_out_over_a_rule(device):
+    rows, n, ld = 2, 64, 8
+    st = {k: device.zeros(4096) for k in ("z", "history", "history_len", "prompt_len", "repetition", "frequency",
+                                          "presence", "bias_ids", "bias_values", "bias_len", "mask")}
+    rules = {k: s.ptr for k, s in st.items() if k != "z"} | dict(history_ld=ld, bias_ld=ld)
+    u = _lib.LogitRules(**rules)
+    for dtype in (_lib.F32, _lib.BF16):
+        _lib.call("fh_logits_process", device.handle, p(st["z"]), dtype, rows, n, ctypes.byref(u), p(st["z"]))
+        for k in rules:
+            if k.endswith("_ld"):
+                continue
+            with pytest.raises(_lib.HipError, match="overlap") as e:
+                _lib.call("fh_logits_process", device.handle, p(st["z"]), dtype, rows, n, ctypes.byref(u), p(st[k]))
+            assert e.value.status == _lib.ERR_INVALID_ARGUMENT

@@ -235,3 +235,22 @@ def test_refusals(device):
     refused(_lib.ERR_OUT_OF_BOUNDS, u=3)
     refused(_lib.ERR_OUT_OF_BOUNDS, n=n + 8, base_ld=n + 8, y_ld=n + 8)
     refused(_lib.ERR_FOREIGN_STORAGE, b=ctypes.c_void_p(4096))
+
+
+def test_refuses_outputs_over_every_operand(device):
+    m, k, n, rank, u = 4, 64, 48, 16, 2
+    nbytes = _lib.lora_workspace_bytes(m, k, rank)
+    st = {key: device.zeros(1 << 15) for key in ("x", "a", "b", "s", "ids", "base", "y", "ws")}
+    assert nbytes <= 1 << 15
+
+    def run(y, ws):
+        _lib.call("fh_lora_add", device.handle, p(st["x"]), m, k, k, p(st["a"]), p(st["b"]), p(st["s"]), u, rank, n,
+                  p(st["ids"]), p(st["base"]), n, p(st[y]), n, _lib.BF16, p(st[ws]), nbytes)
+
+    run("y", "ws")
+    run("base", "ws")
+    for y, ws in [(o, "ws") for o in ("x", "a", "b", "s", "ids")] + \
+                 [("y", o) for o in ("x", "a", "b", "s", "ids", "base", "y")]:
+        with pytest.raises(_lib.HipError, match="overlap") as e:
+            run(y, ws)
+        assert e.value.status == _lib.ERR_INVALID_ARGUMENT
