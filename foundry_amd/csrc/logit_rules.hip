@@ -10,16 +10,16 @@ namespace fh {
 // their rows are so aligned (a row's first piece may begin before it). What a
 // token needs to know of the row's lists stands in LDS: a block takes a run of
 // tokens, enters the bias list into a table of them and counts the whole history
-// there too. Every block of a row reads its lists, from
-// the L2: runs are as long as the LDS and a filled GPU allow. 64 rows of 128256
-// bf16 take 6.7 us with no rule (4.9 TB/s), 11.0 with histories to 500, 13.3 with
-// histories to 8192, 14.5 with a mask and 300 biases a row as well: the lists'
-// latency and the tables.
-constexpr uint32_t kRuleTokens = 4096;
-constexpr uint32_t kRuleThreads = 256;
-// Blocks that a launch aims for before runs get longer than the shortest, of
-// kRuleTokens / 8.
-constexpr uint32_t kRuleBlocks = 2048;
+// there too. Every block of a row reads its lists, from the L2: runs are as long
+// as the LDS and a filled GPU allow. 64 rows of 128256 bf16 take 6.7 us with no
+// rule (4.9 TB/s), 10.1 with histories to 500, 12.7 with histories to 8192, 13.5
+// with a mask and 300 biases a row as well: the lists' latency and the tables. (256 threads with runs of 4096: 14.5; 512 with 4096:
+// 15.5; 1024 with 8192: 16.0, with 16384: 13.8.)
+constexpr uint32_t kRuleTokens = 8192;
+constexpr uint32_t kRuleThreads = 512;
+// The shortest run, and the blocks that a launch aims for before runs get longer.
+constexpr uint32_t kRuleLeast = 512;
+constexpr uint32_t kRuleBlocks = 1024;
 // A token's word: its count among the generated, then a bit for an id of the
 // prompt, then a bias entry's index + 1, for lists up to these lengths.
 constexpr uint32_t kCountBits = 20, kMaxCounted = (1u << kCountBits) - 1, kMaxBiases = (1u << (31 - kCountBits)) - 1;
@@ -63,19 +63,17 @@ __device__ __forceinline__ void for_list(const uint32_t *list, uint32_t n, Take 
 
 // Block (run, row). Of a bias id listed twice the last entry stays. TWO: lists
 // too long for one word: a table of counts (bit 31: an id of the prompt) and one
-// of bias entries, over half as many tokens. Whole-number LDS atomics: their
-// order does not matter. Contraction is off, so that each step is one fp32
-// rounding.
+// of bias entries. Whole-number LDS atomics: their order does not matter.
+// Contraction is off, so that each step is one fp32 rounding.
 template <typename T, bool TWO>
 __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(const T *z, uint32_t n, uint32_t run,
                                                                    const fh_logit_rules rules, T *out) {
 #pragma clang fp contract(off)
     constexpr uint32_t E = 16 / sizeof(T);  // logits of a piece
-    constexpr uint32_t kMost = TWO ? kRuleTokens / 2 : kRuleTokens;
-    constexpr uint32_t kPieces = kMost / (kRuleThreads * E);
+    constexpr uint32_t kPieces = kRuleTokens / (kRuleThreads * E);
     constexpr uint32_t kSaid = TWO ? 0x80000000u : 1u << kCountBits, kShift = TWO ? 0 : kCountBits + 1;
-    __shared__ __attribute__((aligned(16))) uint32_t said[kRuleTokens];
-    uint32_t *entry = TWO ? said + kMost : said;
+    __shared__ __attribute__((aligned(16))) uint32_t said[TWO ? 2 * kRuleTokens : kRuleTokens];
+    uint32_t *entry = TWO ? said + kRuleTokens : said;
     const uint32_t r = blockIdx.y;
     const T *from = z + static_cast<uint64_t>(r) * n;
     T *to = out + static_cast<uint64_t>(r) * n;
@@ -255,9 +253,8 @@ extern "C" int fh_logits_process(fh_device *dev, const void *logits, int dtype, 
     }
     if (int rc = set_current(dev, fn)) return rc;
     const bool two = (u.history && u.history_ld > kMaxCounted) || (u.bias_ids && u.bias_ld >= kMaxBiases);
-    const uint32_t longest = two ? kRuleTokens / 2 : kRuleTokens;
-    uint32_t run = kRuleTokens / 8;
-    while (run < longest && r * ((n + run - 1) / run) > kRuleBlocks) run *= 2;
+    uint32_t run = kRuleLeast;
+    while (run < kRuleTokens && r * ((n + run - 1) / run) > kRuleBlocks) run *= 2;
     // a run may begin up to a piece before its row
     const dim3 grid(static_cast<uint32_t>((n + 16 / elem - 1 + run - 1) / run), static_cast<uint32_t>(rows));
     auto launch = [&](auto kernel, auto *of) {
