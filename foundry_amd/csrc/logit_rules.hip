@@ -14,8 +14,8 @@ namespace fh {
 // as the LDS and a filled GPU allow. 64 rows of 128256 bf16 take 6.7 us with no
 // rule (4.9 TB/s), 10.1 with histories to 500, 12.7 with histories to 8192, 13.5
 // with a mask and 300 biases a row as well: the lists' latency and the tables.
-// (256 threads with runs of 4096: 14.5; 512 with 4096:
-// 15.5; 1024 with 8192: 16.0, with 16384: 13.8.)
+// (256 threads with runs of 4096: 14.5; 512 with 4096: 15.5; 1024 with 8192:
+// 16.0, with 16384: 13.8.)
 constexpr uint32_t kRuleTokens = 8192;
 constexpr uint32_t kRuleThreads = 512;
 // The shortest run, and the blocks that a launch aims for before runs get longer.
