@@ -40,11 +40,13 @@ constexpr uint32_t kLoraWaves = kLoraThreads / 64;
 constexpr uint32_t kWideRows = 1024;
 // Blocks that the windows share, down and up. How many chunks a window has is
 // known on the device alone: there its blocks divide the chunks among
-// themselves, and each chunk's k (down, into kMaxSplits ranges at most and
-// kDownSteps steps of 32 per wavefront at least) or columns (up) as far as they
-// go round. With estimates of the host 1024 packed rows of rank 16 were left
-// to 40 blocks: 36 us against 24.
-constexpr uint32_t kDownBlocks = 512, kMaxSplits = 4, kDownSteps = 2;
+// themselves, and each chunk's k (down) or columns (up) as far as they go round.
+// With estimates of the host 1024 packed rows of rank 16 were left to 40 blocks:
+// 36 us against 24. k is cut into kMaxSplits ranges at most, of kDownSteps steps
+// of 32 per wavefront at least, a long one of up to kWideRows rows into more, of
+// kLongSteps: k 14336, 71 rows of 5 adapters of rank 128: 51 -> 38 us, 8 rows of 8
+// of rank 16: 11.7 -> 10.0; 1820 rows of 3 of rank 32: 39.2 -> 41.8, so not there.
+constexpr uint32_t kDownBlocks = 512, kMaxSplits = 4, kDownSteps = 2, kLongSplits = 8, kLongSteps = 8;
 // Up, what the GPU holds of each form at once: 200 rows of 48 adapters take 28 us
 // at 768 blocks, 31.8 at 512, 32.7 at 1024; 4096 packed rows 36.8 at 512, 40.1 at
 // 768.
@@ -56,13 +58,16 @@ struct Ranges {
     uint32_t splits, steps;
 };
 
-__host__ __device__ __forceinline__ uint32_t most_splits(uint32_t k) {
-    const uint32_t n = ((k + 31) / 32 + kLoraWaves * kDownSteps - 1) / (kLoraWaves * kDownSteps);
+__host__ __device__ __forceinline__ uint32_t most_splits(uint32_t k, uint32_t m) {
+    const uint32_t all = (k + 31) / 32;
+    const uint32_t n = (all + kLoraWaves * kDownSteps - 1) / (kLoraWaves * kDownSteps);
+    const uint32_t more = m > kWideRows ? 0 : all / (kLoraWaves * kLongSteps);
+    if (more > kMaxSplits) return more < kLongSplits ? more : kLongSplits;
     return n < kMaxSplits ? n : kMaxSplits;
 }
 
-__device__ __forceinline__ Ranges ranges_of(uint32_t k, uint32_t chunks, uint32_t blocks) {
-    const uint32_t all = (k + 31) / 32, want = min(max(blocks / max(chunks, 1u), 1u), most_splits(k));
+__device__ __forceinline__ Ranges ranges_of(uint32_t k, uint32_t m, uint32_t chunks, uint32_t blocks) {
+    const uint32_t all = (k + 31) / 32, want = min(max(blocks / max(chunks, 1u), 1u), most_splits(k, m));
     const uint32_t steps = (all + want * kLoraWaves - 1) / (want * kLoraWaves);
     return {(all + steps * kLoraWaves - 1) / (steps * kLoraWaves), steps};
 }
@@ -261,7 +266,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_down_kernel(const uint16_t 
     __shared__ float4 sums[4 * NR * 64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row0 = blockIdx.x * 64 * Q;
     const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
-    const Ranges g = ranges_of(k, o.chunks, gridDim.y);
+    const Ranges g = ranges_of(k, m, o.chunks, gridDim.y);
     for (uint32_t unit = blockIdx.y; unit < o.chunks * g.splits; unit += gridDim.y) {
         const uint32_t split = unit % g.splits;
         const uint32_t k0 = min((split * kLoraWaves + wave) * g.steps * 32, k), k1 = min(k0 + g.steps * 32, k);
@@ -462,15 +467,15 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, uint32_t rank, u
 // rows' down products ran on 4 of 8). v is formed in LDS from the splits' sums:
 // for a chunk of up to 16 rows by each wavefront for itself, with no barrier,
 // else once for the block. wide: there a lane reads and writes 16 neighbouring
-// columns of a row (n a multiple of 16, rows 16-byte aligned).
-template <typename T, int Q, int NJ, bool PACKED>
+// columns of a row (n a multiple of 16, rows 16-byte aligned). SPLITS: as many
+// as k has at most, whose sums are requested together.
+template <typename T, int Q, int NJ, bool PACKED, uint32_t SPLITS>
 __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__restrict__ v, uint32_t down_blocks,
                                                                uint32_t m, uint32_t k, const uint16_t *__restrict__ b,
                                                                const float *__restrict__ scales, uint32_t n_adapters,
                                                                uint32_t rank, uint32_t n,
                                                                const uint32_t *__restrict__ adapters, const T *base,
                                                                uint64_t base_ld, T *y, uint64_t y_ld, bool wide) {
-    constexpr int kLoads = 4;                       // splits' sums requested together
     constexpr int P = sizeof(T) == 2 ? 4 : 2;       // row tiles requested together
     constexpr bool kAhead = !PACKED && NJ <= 2;     // the registers hold two tiles of B
     __shared__ uint8_t lists[kLoraWaves][64];
@@ -481,7 +486,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
     const uint32_t c = lane & 15u, q = lane >> 4, vs_ld = kParts<T> * rank + 8, quads = rank / 4;
     const uint64_t split = static_cast<uint64_t>(m) * rank;
     const Window<Q> o = window_of<Q>(adapters, row0, m, n_adapters, lane, wave, leads);
-    const uint32_t splits = ranges_of(k, o.chunks, down_blocks).splits;
+    const uint32_t splits = ranges_of(k, m, o.chunks, down_blocks).splits;
     // a chunk's columns in `parts` parts of `tiles` times 64 per wavefront
     const uint32_t all = (n + kLoraWaves * 64 - 1) / (kLoraWaves * 64);
     const uint32_t tiles = (all + min(max(gridDim.y / max(o.chunks, 1u), 1u), all) - 1) /
@@ -502,13 +507,12 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
                 const uint32_t member = i / quads, r = i % quads * 4;
                 const float *p = v + static_cast<uint64_t>(row0 + list[member]) * rank + r;
                 float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                float4 part[kLoads];
-                static_assert(kLoads == kMaxSplits, "one round of loads");
+                float4 part[SPLITS];
 #pragma unroll
-                for (uint32_t u = 0; u < kLoads; ++u)
+                for (uint32_t u = 0; u < SPLITS; ++u)
                     part[u] = *reinterpret_cast<const float4 *>(p + min(u, splits - 1) * split);
 #pragma unroll
-                for (uint32_t u = 0; u < kLoads; ++u)
+                for (uint32_t u = 0; u < SPLITS; ++u)
                     if (u < splits) f[0] += part[u].x, f[1] += part[u].y, f[2] += part[u].z, f[3] += part[u].w;
 #pragma unroll
                 for (uint32_t h = 0; h < kParts<T>; ++h)
@@ -628,7 +632,11 @@ extern "C" int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *b
         return fail(FH_ERR_UNSUPPORTED, "%s: rank %lld must be a multiple of 8, at most 128", fn, (long long)rank);
     if (k < 8 || k % 8 != 0)
         return fail(FH_ERR_UNSUPPORTED, "%s: k %lld must be a multiple of 8", fn, (long long)k);
-    *bytes = static_cast<uint64_t>(most_splits(static_cast<uint32_t>(k))) * m * rank * 4 + 16;
+    // fewer rows never need more: what serves the largest batch serves them all
+    const uint32_t m32 = static_cast<uint32_t>(m), k32 = static_cast<uint32_t>(k), wide = std::min(m32, kWideRows);
+    const uint64_t rows = std::max<uint64_t>(static_cast<uint64_t>(most_splits(k32, m32)) * m32,
+                                             static_cast<uint64_t>(most_splits(k32, wide)) * wide);
+    *bytes = rows * rank * 4 + 16;
     return FH_OK;
 }
 
@@ -695,16 +703,17 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     const uint64_t windows = (rows + rows_of - 1) / rows_of, cols = (n + kLoraWaves * 64 - 1) / (kLoraWaves * 64);
     if (windows > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: m %lld", fn, (long long)m);
     if (int rc = set_current(dev, fn)) return rc;
+    const uint32_t m32 = static_cast<uint32_t>(m), k32 = static_cast<uint32_t>(k);
     // a window has at most as many chunks as rows
     const uint64_t most = std::min<uint64_t>(rows, rows_of);
     const uint32_t down_blocks = static_cast<uint32_t>(
-        std::clamp<uint64_t>(kDownBlocks / windows, 1, most * most_splits(static_cast<uint32_t>(k))));
+        std::clamp<uint64_t>(kDownBlocks / windows, 1, most * most_splits(k32, m32)));
     const uint64_t up_all = m > kWideRows ? kUpPacked : kUpBlocks;
     const uint32_t up_blocks = static_cast<uint32_t>(std::clamp<uint64_t>(up_all / windows, 1, most * cols));
     const dim3 down(static_cast<uint32_t>(windows), down_blocks), up(static_cast<uint32_t>(windows), up_blocks);
     const dim3 threads(kLoraThreads);
     float *v = static_cast<float *>(workspace);
-    const uint32_t m32 = static_cast<uint32_t>(m), k32 = static_cast<uint32_t>(k), n32 = static_cast<uint32_t>(n);
+    const uint32_t n32 = static_cast<uint32_t>(n);
     const uint32_t rank32 = static_cast<uint32_t>(rank), u32 = static_cast<uint32_t>(n_adapters);
     const bool wide = ((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0 &&
                      base_ld * elem % 16 == 0 && y_ld * elem % 16 == 0 && n % 16 == 0;
@@ -726,13 +735,18 @@ extern "C" int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t
     auto run = [&](auto q, auto tiles) {
         constexpr int Q = decltype(q)::value, N = decltype(tiles)::value;
         if (int rc = run_down(lora_down_kernel<Q, N>)) return rc;
+        auto run_as = [&](auto packed, auto splits) {
+            constexpr bool P = decltype(packed)::value;
+            constexpr uint32_t S = decltype(splits)::value;
+            return dtype == FH_F32 ? run_up(lora_up_kernel<float, Q, N, P, S>, static_cast<float *>(nullptr))
+                                   : run_up(lora_up_kernel<uint16_t, Q, N, P, S>, static_cast<uint16_t *>(nullptr));
+        };
+        constexpr std::integral_constant<uint32_t, kMaxSplits> few{};
+        constexpr std::integral_constant<uint32_t, kLongSplits> many{};
         // windows of 64 rows past kWideRows rows: mostly whole chunks of 64
         if constexpr (Q == 1)
-            if (m > kWideRows)
-                return dtype == FH_F32 ? run_up(lora_up_kernel<float, Q, N, true>, static_cast<float *>(nullptr))
-                                       : run_up(lora_up_kernel<uint16_t, Q, N, true>, static_cast<uint16_t *>(nullptr));
-        return dtype == FH_F32 ? run_up(lora_up_kernel<float, Q, N, false>, static_cast<float *>(nullptr))
-                               : run_up(lora_up_kernel<uint16_t, Q, N, false>, static_cast<uint16_t *>(nullptr));
+            if (m > kWideRows) return run_as(std::true_type{}, few);
+        return most_splits(k32, m32) > kMaxSplits ? run_as(std::false_type{}, many) : run_as(std::false_type{}, few);
     };
     auto by_rank = [&](auto q) {
         if (rank <= 16) return run(q, std::integral_constant<int, 1>{});

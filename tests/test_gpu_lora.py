@@ -111,6 +111,19 @@ def test_inner_sizes(device, k):
     Case(device, k, 20, k, 64, 16, 3, [i % 4 if i % 4 < 3 else NONE for i in range(20)]).check()
 
 
+@pytest.mark.parametrize("rank,f32", [(16, False), (40, True), (128, True), (128, False)])
+@pytest.mark.parametrize("m,k", [(3, 5120), (9, 6664), (40, 14336), (70, 10248)])
+def test_long_inner_sizes(device, m, k, rank, f32):
+    """k in more ranges than a short one's."""
+    Case(device, m + k, m, k, 144, rank, 4, [i % 5 for i in range(m)], f32).check()
+    Case(device, m + k + 1, m, k, 33, rank, 2, [0] * m, f32).check()
+
+
+@pytest.mark.parametrize("m", [1024, 1025])
+def test_long_inner_sizes_where_windows_change(device, m):
+    Case(device, m, m, 8200, 48, 16, 3, [i // 200 % 4 for i in range(m)]).check()
+
+
 @pytest.mark.parametrize("n", [1, 3, 63, 64, 65, 255, 257, 1001])
 @pytest.mark.parametrize("f32", [False, True])
 def test_odd_widths(device, n, f32):

@@ -55,6 +55,12 @@ def test_lora_workspace():
     assert _lib.load().fh_lora_workspace(1, 64, 8, None) == _lib.ERR_INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("k", [64, 4096, 14336])
+def test_lora_workspace_of_the_most_rows_serves_fewer(k):
+    sizes = [_lib.lora_workspace_bytes(m, k, 16) for m in (0, 1, 64, 65, 1000, 1024, 1025, 1100, 2047, 2049, 4096)]
+    assert sizes == sorted(sizes)
+
+
 def test_calls_without_a_device():
     lib, f = _lib.load(), ctypes.c_float(1)
     rules = _lib.LogitRules()
