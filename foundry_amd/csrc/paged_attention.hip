@@ -500,8 +500,10 @@ Plan plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_
     const uint64_t tiles = n_kv * ((n_heads / n_kv + kHeadTile - 1) / kHeadTile);
     const uint64_t capacity = static_cast<uint64_t>(max_pages) * page_size;
     const bool whole = capacity * head_dim <= kWholeElements;
-    if (batch > kPlanBatch || whole)
-        return {0, static_cast<uint32_t>(batch), static_cast<uint32_t>(tiles), 16, whole};
+    if (whole) return {0, static_cast<uint32_t>(batch), static_cast<uint32_t>(tiles), 16, true};
+    if (batch > kPlanBatch)  // what serves the largest batch serves smaller ones: the bytes of those that are split
+        return {0, static_cast<uint32_t>(batch), static_cast<uint32_t>(tiles),
+                plan(kPlanBatch, n_heads, n_kv, head_dim, page_size, max_pages).bytes, false};
     // a table of few steps has no use for more parts than steps
     const uint64_t steps = (capacity + kStepKeys - 1) / kStepKeys;
     const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>(kPartBlocks / tiles, batch * steps));

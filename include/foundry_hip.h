@@ -535,7 +535,8 @@ int fh_paged_rope_kv(fh_device *dev, const uint16_t *qkv, int64_t tokens, int64_
                      int64_t max_pages, uint16_t *k_pages, uint16_t *v_pages, int64_t n_pages,
                      int64_t page_size, uint16_t *q_out);
 
-/* Bytes of device workspace fh_paged_attention needs for these sizes. */
+/* Bytes of device workspace fh_paged_attention needs for these sizes, never
+ * less for a larger batch. */
 int fh_paged_attention_workspace(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
                                  int64_t page_size, int64_t max_pages, uint64_t *bytes);
 
@@ -560,7 +561,8 @@ int fh_paged_attention(fh_device *dev, const uint16_t *q, int64_t batch, int64_t
                        const uint32_t *page_table, int64_t max_pages, const uint32_t *positions,
                        float scale, void *workspace, uint64_t workspace_bytes, uint16_t *out);
 
-/* Bytes of device workspace fh_lora_add needs for these sizes. */
+/* Bytes of device workspace fh_lora_add needs for these sizes, never less for
+ * more rows. */
 int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *bytes);
 
 /* The low-rank adapters of many requests beside a shared projection (base,

@@ -44,6 +44,14 @@ def test_paged_attention_workspace():
     assert _lib.load().fh_paged_attention_workspace(1, 4, 2, 64, 16, 4, None) == bad
 
 
+@pytest.mark.parametrize("heads,kv,hd,page,width", [(32, 8, 128, 16, 8), (32, 8, 128, 64, 128), (24, 8, 128, 16, 2048),
+                                                    (8, 1, 256, 32, 33)])
+def test_attention_workspace_of_the_largest_batch_serves_smaller_ones(heads, kv, hd, page, width):
+    sizes = [_lib.paged_attention_workspace_bytes(b, heads, kv, hd, page, width)
+             for b in (0, 1, 2, 7, 64, 65, 512, 1023, 1024, 1025, 5000, 16000)]
+    assert sizes == sorted(sizes)
+
+
 def test_lora_workspace():
     assert _lib.lora_workspace_bytes(1, 64, 8) > 0
     assert _lib.lora_workspace_bytes(0, 64, 8) >= 0
