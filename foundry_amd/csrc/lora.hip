@@ -373,19 +373,42 @@ __device__ __forceinline__ void request_b(const uint16_t *b, uint32_t rank, uint
     }
 }
 
-template <typename T, int NJ>
-__device__ __forceinline__ void products(const uint4 (&bfr)[4][NJ], const Terms<T, NJ> &vf, uint32_t rank, uint32_t q,
-                                         lo_f32x4_t (&acc)[4]) {
+// APART: infs and NaNs of B meet v's first part alone (a rest has the other sign,
+// or is 0, as it falls: with it an infinite sum would be NaN), and none that lies
+// past the ranks, where v is 0 and what stands for B need not be.
+template <bool APART, typename T, int NJ>
+__device__ __forceinline__ void sum_products(const uint4 (&bfr)[4][NJ], const Terms<T, NJ> &vf, uint32_t rank,
+                                             uint32_t q, lo_f32x4_t (&acc)[4]) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) acc[u] = lo_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const uint4 f = (2 * j + q / 2) * 8 < rank ? bfr[u][j] : make_uint4(0, 0, 0, 0);
-            if constexpr (sizeof(T) == 4) acc[u] = lo_mfma(f, vf.low[j], acc[u]);
+            uint4 f = bfr[u][j], rest = f;
+            if constexpr (APART) {
+                // here and now, one after the other: ahead of the loops around it would take twice B's registers
+                asm volatile("" : "+v"(rest.x), "+v"(rest.y), "+v"(rest.z), "+v"(rest.w));
+                __builtin_amdgcn_sched_barrier(0);
+                clear_specials(rest);
+                if ((q & 1) || (2 * j + q / 2) * 8 >= rank) f = rest;
+            }
+            if constexpr (sizeof(T) == 4) acc[u] = lo_mfma(rest, vf.low[j], acc[u]);
             acc[u] = lo_mfma(f, vf.v[j], acc[u]);
         }
+}
+
+// Infs and NaNs of B are looked for in the sums, fewer than its entries: an inf or
+// NaN among a wavefront's, or sums that large, and they are formed again, apart
+// (finite ones are the same again).
+template <typename T, int NJ>
+__device__ __forceinline__ void products(const uint4 (&bfr)[4][NJ], const Terms<T, NJ> &vf, uint32_t rank, uint32_t q,
+                                         lo_f32x4_t (&acc)[4]) {
+    sum_products<false>(bfr, vf, rank, q, acc);
+    float all = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) all += (fabsf(acc[u][0]) + fabsf(acc[u][1])) + (fabsf(acc[u][2]) + fabsf(acc[u][3]));
+    if (__any(!(all < INFINITY))) sum_products<true>(bfr, vf, rank, q, acc);
 }
 
 template <typename T>
@@ -426,7 +449,7 @@ __device__ __forceinline__ void lora_up_rows(const uint16_t *b, uint32_t rank, u
     auto finish = [&](const RowsTile<T, NJ, R> &x, uint32_t u) {
         const uint32_t col = col0 + u * kLoraWaves * 64 + lane;
         lo_f32x4_t acc[4];
-        products<T, NJ>(x.b, vf, rank, q, acc);
+        products(x.b, vf, rank, q, acc);
         // 8 rows at a time
 #pragma unroll
         for (int h = 0; h < R; h += 8) {
@@ -580,7 +603,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
                         Terms<T, NJ> vf;
                         terms(member, vf);
                         lo_f32x4_t acc[4];
-                        products<T, NJ>(bfr, vf, rank, q, acc);
+                        products(bfr, vf, rank, q, acc);
                         float f[16];
                         floats16(raw[t], f);
 #pragma unroll

@@ -201,6 +201,39 @@ def test_infinite_down_products(device):
     assert np.array_equal(got[0], np.where(sign > 0, np.inf, -np.inf)) and np.isfinite(got[1:]).all()
 
 
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("m,k,n,rank", [(1, 64, 33, 8), (3, 64, 32, 16), (12, 72, 100, 40), (40, 128, 100, 16),
+                                        (40, 64, 64, 24), (200, 64, 144, 40), (90, 64, 48, 128), (1100, 136, 96, 32),
+                                        (1100, 136, 101, 128), (1100, 64, 64, 16)])
+def test_infinities_and_nans_of_b(device, m, k, n, rank, f32):
+    """An infinite entry of B makes its column infinite, by the signs of v and
+    of the entry (NaN where two of them disagree), and no other column; a NaN
+    makes its column NaN. Rows of the other adapter stay as they are."""
+    c = Case(device, m + rank, m, k, n, rank, 2, [i * 7 // m % 2 for i in range(m)], f32)
+    clean = c.run()
+    b = c.b.copy()
+    b[0, 2, 3], b[0, 9, 0], b[0, n - 1, rank - 1] = 0x7F80, 0xFF80, 0x7F80
+    b[0, 17, 1], b[0, 17, 6] = 0x7F80, 0xFF80
+    b[0, 30, 5] = 0x7FC0
+    c.st[2] = up(device, b)
+    got = c.run().astype(np.float64) if f32 else S.f64(c.run())
+    val = clean.astype(np.float64) if f32 else S.f64(clean)
+    hit = np.isin(np.arange(n), [2, 9, 17, 30, n - 1])
+    mine = c.ids == 0
+    assert np.array_equal(got[~mine], val[~mine]) and np.array_equal(got[:, ~hit], val[:, ~hit])
+    x, a = S.f64(c.x[mine]), S.f64(c.a[0])
+    v = x @ a.T * c.scales[0]
+    # rows whose v at these entries are not so near 0 that the kernel's sums may have another sign
+    sure = np.abs(v) > (k + 2) * 2.0 ** -24 * (np.abs(x) @ np.abs(a).T) * abs(c.scales[0])
+    sure = sure[:, [0, 1, 3, 5, 6, rank - 1]].all(1)
+    assert sure.mean() > 0.9
+    for col in np.flatnonzero(hit):
+        with np.errstate(invalid="ignore"):
+            want = (v * S.f64(b[0, col])).sum(-1)
+        assert not np.isfinite(got[mine, col]).any() and not np.isfinite(want).any()
+        assert np.array_equal(got[mine, col][sure], want[sure], equal_nan=True)
+
+
 def test_refusals(device):
     m, k, n, rank, u = 4, 64, 48, 16, 2
     nbytes = _lib.lora_workspace_bytes(m, k, rank)
