@@ -328,9 +328,12 @@ __device__ __forceinline__ void store16(T *p, const float (&f)[16]) {
 }
 
 // Parts of two values in bf16: 0 the values rounded, 1 and 2 what the parts before
-// have lost, rounded (nothing of an inf or NaN).
+// have lost, rounded (nothing of an inf or NaN). A finite value past the largest bf16
+// begins with that one, as its rounding would be inf.
 __device__ __forceinline__ uint32_t parts_of(float x, float y, uint32_t part) {
-    uint32_t p = f32x2_to_bf16x2_rne(x, y);
+    constexpr float kLargest = 0x1.FEp127f;
+    auto first = [](float v) { return fabsf(v) < INFINITY ? fminf(fmaxf(v, -kLargest), kLargest) : v; };
+    uint32_t p = f32x2_to_bf16x2_rne(first(x), first(y));
 #pragma unroll
     for (uint32_t i = 1; i <= 2; ++i) {
         if (i > part) break;

@@ -234,6 +234,21 @@ def test_infinities_and_nans_of_b(device, m, k, n, rank, f32):
         assert np.array_equal(got[mine, col][sure], want[sure], equal_nan=True)
 
 
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("m", [3, 40])
+def test_v_between_the_largest_bf16_and_the_largest_f32(device, m, f32):
+    """A finite v that bf16 would round to inf, times small entries of B."""
+    c = Case(device, m, m, 64, 48, 8, 1, [0] * m, f32)
+    x, a = np.zeros_like(c.x), np.zeros_like(c.a)
+    x[:, 0] = np.where(np.arange(m) % 2, 0xFF7F, 0x7F7F)  # the largest bf16, 3.3895e38
+    a[0, [0, 5], 0] = 0x3F80
+    b = synth.bf16_rne((S.f64(c.b) * 2.0 ** -100).astype(np.float32))
+    c.scales[:] = 1.0035  # v = 3.4014e38, past where bf16 rounds to inf (3.3962e38)
+    c.x, c.a, c.b = x, a, b
+    c.st[:4] = [up(device, v) for v in (x, a, b, c.scales)]
+    assert np.isfinite(c.check().astype(np.float64) if f32 else S.f64(c.check())).all()
+
+
 def test_refusals(device):
     m, k, n, rank, u = 4, 64, 48, 16, 2
     nbytes = _lib.lora_workspace_bytes(m, k, rank)
