@@ -11,7 +11,8 @@ namespace fh {
 // sum l and weighted values o of each query head,
 //   m' = max(m, s), l' = l e^(m - m') + e^(s - m'), o' = o e^(m - m') + e^(s - m') v,
 // joined over disjoint key ranges by the same rule. Exponentials are taken as
-// powers of two of scores scaled by log2 e.
+// powers of two, their exponents scaled by log2 e after the maximum is taken off:
+// any finite score has a finite weight.
 //
 // The split: a block of four wavefronts takes a part of the batch's keys (whole
 // steps of kStepKeys) for one KV head and up to 8 of the query heads that share
@@ -57,6 +58,8 @@ __device__ __forceinline__ pa_f32x4_t pa_mfma(uint4 a, uint4 b, pa_f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8_t, a),
                                                    __builtin_bit_cast(pa_bf16x8_t, b), c, 0, 0, 0);
 }
+
+__device__ __forceinline__ float pa_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
 struct PagedArgs {
     const uint16_t *q, *k_pages, *v_pages;
@@ -148,7 +151,6 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
     const uint32_t group = a.n_heads / a.n_kv, tiles = (group + kHeadTile - 1) / kHeadTile;
     const uint32_t kv = blockIdx.y / tiles, head0 = (blockIdx.y % tiles) * kHeadTile;
     const uint32_t heads = min(kHeadTile, group - head0);  // this block's, from kv * group + head0
-    const float scale2 = a.scale * 1.4426950408889634f;
     const uint32_t groups_pp = a.page_size / 16;
     Layout y;
     uint32_t at = 0, end = 1;
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
             auto weigh = [&](uint32_t t) {
                 float s[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[i] = s0[i] * scale2, s[4 + i] = s1[i] * scale2;
+                for (int i = 0; i < 4; ++i) s[i] = s0[i] * a.scale, s[4 + i] = s1[i] * a.scale;
                 const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2);
                 const uint32_t w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
                 const uint32_t key0 = from + (t0 + t) * 32;
@@ -272,7 +274,7 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
                 const float next = fmaxf(m, top);
                 const float ref = next == -INFINITY ? 0.0f : next;
                 if (__any(next != m)) {
-                    const float keep = __builtin_amdgcn_exp2f(m - ref);
+                    const float keep = pa_exp(m - ref);
                     l *= keep;
 #pragma unroll
                     for (int t = 0; t < VT; ++t) acc[t] *= keep;
@@ -281,8 +283,8 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
                 uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p0 = __builtin_amdgcn_exp2f(s[2 * i] - ref);
-                    const float p1 = __builtin_amdgcn_exp2f(s[2 * i + 1] - ref);
+                    const float p0 = pa_exp(s[2 * i] - ref);
+                    const float p1 = pa_exp(s[2 * i + 1] - ref);
                     l += p0 + p1;
                     const uint32_t hi = f32x2_to_bf16x2_rne(p0, p1);
                     // what the rounding lost; nothing of an inf or NaN
@@ -356,7 +358,7 @@ __global__ __launch_bounds__(64 * W, HD == 256 ? 1 : 2) void paged_part_kernel(c
         for (int d = 0; d < DT; ++d) o[d] = 0.0f;
 #pragma unroll
         for (uint32_t w = 0; w < W; ++w) {
-            const float f = __builtin_amdgcn_exp2f(part_ml[w][0][h] - ref);
+            const float f = pa_exp(part_ml[w][0][h] - ref);
             sum = fmaf(f, part_ml[w][1][h], sum);
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part_o[w][h][d0 + d], o[d]);
@@ -431,13 +433,13 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedAr
             if (i0 + u * kRows >= pieces) pm[u] = -INFINITY;
             next = fmaxf(next, pm[u]);
         }
-        const float ref = next == -INFINITY ? 0.0f : next, f = __builtin_amdgcn_exp2f(m - ref);
+        const float ref = next == -INFINITY ? 0.0f : next, f = pa_exp(m - ref);
         m = next;
         l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
 #pragma unroll
         for (int u = 0; u < kJoinLoads; ++u)
             if (i0 + u * kRows < pieces) {
-                const float g = __builtin_amdgcn_exp2f(pm[u] - ref);
+                const float g = pa_exp(pm[u] - ref);
                 some = fmaxf(some, ps[u]);
                 l = fmaf(pl[u], g, l);
                 o.x = fmaf(v[u].x, g, o.x), o.y = fmaf(v[u].y, g, o.y);
@@ -454,7 +456,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedAr
     o = make_float4(0, 0, 0, 0);
 #pragma unroll
     for (uint32_t r = 0; r < kRows; ++r) {
-        const float f = __builtin_amdgcn_exp2f(rows_ml[r][0] - ref);
+        const float f = pa_exp(rows_ml[r][0] - ref);
         const float4 v = *reinterpret_cast<const float4 *>(&rows_o[r][d]);
         l = fmaf(f, rows_ml[r][1], l);
         some = fmaxf(some, rows_ml[r][2]);

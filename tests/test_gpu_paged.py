@@ -294,6 +294,31 @@ def test_attention_lowest_and_infinite_scores(device):
     assert (np.abs(got - ref)[:2] <= 2.0 ** -8 * np.abs(ref[:2]) + 2.0 ** -15 * weight[:2]).all()
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(2, 1, 64), (8, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("width", [17, 600])
+def test_attention_finite_scores_up_to_the_largest_f32(device, heads, kv, hd, width):
+    """Finite scores whose multiples by log2 e are not: rows whose every score
+    is the type's lowest, the largest for one key or for a few, and both; at
+    once for a block of its own and (the wide table) split and joined."""
+    lens = [250, 250, 250, 250, 40]
+    q, k, v, table, pos = cache(hd + width, lens, heads, kv, hd, 16, width=width)
+    q[:], k[:] = 0, 0
+    q[:, :, 0] = 0x3F80                      # 1.0: the score is the key's dim 0
+    kk = k.reshape(-1, 16, hd)
+    low, high = 0xFF7F, 0x7F7F               # -3.3895e38, 3.3895e38
+    rows = [lambda j: low, lambda j: high if j == 201 else 0x3F80, lambda j: high if j % 100 == 3 else low,
+            lambda j: 0xFF80 if j % 3 else low, lambda j: high]
+    for s, of in enumerate(rows):
+        for j in range(lens[s]):
+            kk[table[s, j // 16], j % 16, 0] = of(j)
+    kk = kk.reshape(k.shape)
+    got = S.f64(attention(device, q, kk, v, table, pos, 1.0))
+    ref, weight, _ = S.attend(S.f64(q), S.f64(kk), S.f64(v), table, pos, 1.0)
+    # equal scores or none that counts: what is left is 2^-16 of p's parts, the exponentials' and the sums' roundings
+    bound = 2.0 ** -8 * np.abs(ref) + (2.0 ** -16 + 2.0 ** -22 + 2 * 250 * 2.0 ** -24) * weight
+    assert np.isfinite(ref).all() and (np.abs(got - ref) <= bound).all()
+
+
 def test_attention_infinite_and_nan_values_of_used_keys(device):
     q, k, v, table, pos = cache(19, [50, 50], 4, 1, 128, 16)
     vv = v.reshape(-1, 16, 128)
