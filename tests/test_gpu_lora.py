@@ -249,6 +249,46 @@ def test_v_between_the_largest_bf16_and_the_largest_f32(device, m, f32):
     assert np.isfinite(c.check().astype(np.float64) if f32 else S.f64(c.check())).all()
 
 
+@pytest.mark.parametrize("rank", [8, 40, 128])
+@pytest.mark.parametrize("m,n", [(3, 100), (40, 64), (200, 144), (1100, 96), (1100, 101)])
+def test_f32_results_take_24_bits_of_v(device, m, n, rank):
+    """v = scale * (power of two), so with 24 bits, times one power of two per
+    column: nothing is off but three roundings. v: the product of x . A^T (one
+    exact product) and scale, 2^-24. Its parts: each half a bf16 step, 2^-8, of
+    what the part before lost: 2^-24. Their products are exact, the two sums of
+    them within 2^-23 each (whole steps, however the matrix cores round)."""
+    k, u = 8, 7
+    c = Case(device, m + rank, m, k, n, rank, u, [i * u // m for i in range(m)], f32=True)
+    rng = np.random.default_rng(rank + n)
+    x, a, b = np.zeros((m, k)), np.zeros((u, rank, k)), np.zeros((u, n, rank))
+    x[:, 3] = 2.0 ** rng.integers(-3, 4, m)
+    a[:, :, 3] = 2.0 ** rng.integers(-3, 4, (u, rank))
+    b[:, np.arange(n), rng.integers(0, rank, n)] = 2.0 ** rng.integers(-3, 4, n)
+    c.base[:] = 0
+    bits = [synth.bf16_rne(t.astype(np.float32)) for t in (x, a, b)]
+    c.st[:3] = [up(device, t) for t in bits]
+    got = c.run().astype(np.float64)
+    ref, _, _ = S.lora(x, a, b, c.scales.astype(np.float64), c.ids, np.zeros((m, n)))
+    bound = (1 + 1 + 4) * 2.0 ** -24 * np.abs(ref)
+    assert (np.abs(got - ref) <= bound).all()
+    # two parts (16 bits) would not do: v is its scale times a power of two
+    v = c.scales
+    hi = S.f64(synth.bf16_rne(v))
+    two = hi + S.f64(synth.bf16_rne((v - hi).astype(np.float32)))
+    assert (np.abs(two - v) > 2 * 6 * 2.0 ** -24 * np.abs(v)).any()
+
+
+@pytest.mark.parametrize("rank", [24, 40, 128])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("n,y_ld", [(144, None), (96, 112), (100, None)])
+def test_chunks_of_many_rows_in_windows_of_256(device, rank, f32, n, y_ld):
+    """65 to 1024 rows that share two adapters: chunks of 64 and their rests,
+    in whole pieces of 16 columns or not, in base's place or not."""
+    ids = [NONE if i % 41 == 7 else i // 3 % 2 for i in range(300)]
+    c = Case(device, rank + n, 300, 136, n, rank, 2, ids, f32, y_ld=y_ld)
+    assert np.array_equal(c.check(), c.run(in_place=True))
+
+
 def test_refusals(device):
     m, k, n, rank, u = 4, 64, 48, 16, 2
     nbytes = _lib.lora_workspace_bytes(m, k, rank)

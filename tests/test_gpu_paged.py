@@ -228,6 +228,14 @@ def test_attention_more_sequences_than_one_layout_holds(device, width):
     check_attention(device, *cache(79, lens, 2, 1, 64, 16, width=width), 64 ** -0.5)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(2, 1, 64), (3, 3, 128)])
+def test_attention_a_long_context_among_more_sequences_than_one_layout_holds(device, heads, kv, hd):
+    """Past 1024 sequences, where none is split: a long one at the start, in the middle, and an idle last one."""
+    lens = [(i * 31) % 40 if i % 13 else 0 for i in range(1030)]
+    lens[0], lens[500], lens[1029] = 5000, 3001, 0
+    check_attention(device, *cache(81, lens, heads, kv, hd, 16), hd ** -0.5)
+
+
 def test_attention_a_wide_table_of_short_sequences(device):
     """A capacity far past what the sequences use."""
     check_attention(device, *cache(78, [40, 1, 90], 4, 2, 128, 16, width=5000), 128 ** -0.5)
