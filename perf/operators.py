@@ -7,6 +7,10 @@ projection, and penalties, biases and grammar masks on the logits.
 pass: with `own` through the library's entry points, else in plain torch (32
 bits inside, each output rounded once). `exact` restates the result in 64 bits.
 
+With `own` the work is queued on the library's stream, which torch's streams do
+not wait for: synchronise the device before a result is read. Results are the
+state's own buffers, which its next pass writes again.
+
 Shapes are those of the decoders the library is configured for (8 KV heads of
 128 or of 64) and generic ones.
 """
