@@ -20,11 +20,14 @@ namespace fh {
 // to 64 rows. Whatever the order, the products run on the matrix cores with the
 // adapter's rows read once for up to 64 rows (four tiles of 16).
 //
-// Measured (down + up): 8 rows of 8 adapters, k 4096, n 6144, rank 16: 8.4 us,
+// Measured (down + up): 8 rows of 8 adapters, k 4096, n 6144, rank 16: 9.1 us,
 // of which each launch has 4 at least; 200 rows of 48 adapters, n 28672, rank
 // 16, f32 (98 MB): 28 us, 3.5 TB/s, a wavefront's few loads per 64 columns in
 // flight; 4096 packed rows, n 4096, rank 32 (103 MB): 37 us, 2.8 TB/s, the
-// latencies from ids to chunk to x or v before the stream begins.
+// latencies from ids to chunk to x or v before the stream begins; 754 packed
+// rows, n 16384, rank 128, f32 (121 MB): 89 us (down 22, up 70), 1.4 TB/s, one
+// wavefront per SIMD; 2000 rows of 40 adapters of rank 16, n 4096: 32 us by
+// request, 84 in no order, as past kWideRows rows each 64 read their own.
 typedef __attribute__((ext_vector_type(8))) __bf16 lo_bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float lo_f32x4_t;
 
@@ -47,9 +50,10 @@ constexpr uint32_t kWideRows = 1024;
 // kLongSteps: k 14336, 71 rows of 5 adapters of rank 128: 51 -> 38 us, 8 rows of 8
 // of rank 16: 11.7 -> 10.0; 1820 rows of 3 of rank 32: 39.2 -> 41.8, so not there.
 constexpr uint32_t kDownBlocks = 512, kMaxSplits = 4, kDownSteps = 2, kLongSplits = 8, kLongSteps = 8;
-// Up, what the GPU holds of each form at once: 200 rows of 48 adapters take 28 us
-// at 768 blocks, 31.8 at 512, 32.7 at 1024; 4096 packed rows 36.8 at 512, 40.1 at
-// 768.
+// Up: 200 rows of 48 adapters of rank 16, of which the GPU holds 3 blocks per CU,
+// take 28 us at 768 blocks, 31.8 at 512, 32.7 at 1024; 4096 packed rows of rank 32
+// (2 per CU) 36.8 at 512, 40.1 at 768. Higher ranks take the same numbers: 1 per CU
+// is held of most forms past rank 32, which run in up to three rounds.
 constexpr uint32_t kUpBlocks = 768, kUpPacked = 512;
 
 // The ranges of k of a window with `chunks` chunks and `blocks` blocks: `splits`
@@ -347,7 +351,9 @@ __device__ __forceinline__ uint32_t parts_of(float x, float y, uint32_t part) {
 
 // A lane's terms of v: of each 16 ranks its 8 as part 0 or 1 (q & 1), and for
 // f32 results part 2 (as the second product of the same B; zero where q & 1).
-// bf16 results take 16 bits of v, f32 ones 24.
+// f32 results take 24 bits of v. bf16 ones take 16: what those lose, 2^-16 of a
+// term, is far below the half step of 2^-8 that B's own entry is off by, and with
+// 24 2000 packed rows of rank 64 took 42 us instead of 32, others 5% less to 14% more.
 template <typename T, int NJ>
 struct Terms {
     uint4 v[NJ];
@@ -584,7 +590,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_up_kernel(const float *__re
         if (!wide || (!PACKED && NJ == 1)) {
             for (uint32_t t = 0; t * 16 < rows && col0 < n; ++t)
                 lora_up_rows<T, NJ, 16, false>(bu, rank, n, base, base_ld, y, y_ld,
-                                               row0 + list[min(t * 16 + c, rows - 1)], min(rows - t * 16, 16u), col0, tiles, tile[wave], lane,
+                                               row0 + list[min(t * 16 + c, rows - 1)], min(rows - t * 16, 16u), col0,
+                                               tiles, tile[wave], lane,
                                                [&](Terms<T, NJ> &vf) { terms(t * 16 + c, vf); });
         } else {
             for (uint32_t u = 0; u < tiles; ++u) {

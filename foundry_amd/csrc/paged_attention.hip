@@ -29,26 +29,36 @@ namespace fh {
 // as they lie, become V^T fragments by byte permutes within a lane. The 16
 // columns are 8 heads twice: columns 0..7 hold the probabilities rounded to
 // bf16, columns 8..15 what that rounding lost, so that P V has 16 bits of P at
-// the cost of none (the columns would idle).
+// the cost of none (the columns would idle). What 16 bits lose, 2^-16 of a term,
+// is far below the half step of 2^-8 that bf16 V is off by itself; p's sum, the
+// maximum and all sums of values are fp32.
 //
 // Bound by memory: K and V come once, with the nontemporal hint (131077 keys of
 // 8 KV heads of 128: 104 us without, 90 with), the next tile's K in flight behind
-// a tile's softmax, its V behind the next one's. 131077 keys (537 MB) take 91 us
-// with the join (5.9 TB/s; the parts alone 80, 6.7 TB/s), 96 ragged sequences of
-// 17 to 16384 keys (950 MB) 161 (5.9 TB/s), 8 of 1900 to 4111 (97 MB) 24.
+// a tile's softmax, its V behind the next one's. 131077 keys (537 MB) take 92 us
+// with the join (5.9 TB/s; the parts alone 89, 6.0 TB/s), 96 ragged sequences of
+// 17 to 16384 keys (949 MB) 161 (5.9 TB/s; the parts 152), 8 of 1900 to 4111 (97
+// MB) 24 (the parts 20, 4.8 TB/s). 8 KV heads of 64: 48 us (268 MB, 5.6 TB/s), 89
+// (480 MB, 5.4), 16.4 (48 MB); one of 256 with 8 heads: 53 (134 MB, 2.5 TB/s; the
+// parts 38, the join's 8 blocks 15), 63 (241 MB, 3.8), 15.6 (24 MB).
 constexpr uint32_t kPagedThreads = 256;
 constexpr uint32_t kStepKeys = 128;
 constexpr uint32_t kHeadTile = 8;
-// Blocks of a launch: what the GPU holds at once (2 per CU). 8 sequences, 96,
-// one of 131077 keys: 24.0, 161, 91.9 us with 512; 29.0, 169, 92.3 with 768.
+// Blocks of a launch: with heads of 128 what the GPU holds at once, 2 per CU (of
+// 64 it holds 4, of 256 one; their number was not measured apart). 8 sequences, 96,
+// one of 131077 keys of 128: 24.0, 161, 91.9 us with 512; 29.0, 169, 92.3 with 768.
 constexpr uint32_t kPartBlocks = 512;
 // Tables of so few positions (times head_dim) take one block per sequence, of 8
 // wavefronts (4 at head_dim 256), and no join: one launch. One sequence of 500
 // keys of 128: 8.5 us against 10.1 split, of 1000: 14.2 against 10.7; of 1000
 // keys of 64: 9.1 against 9.2, of 1500: 11.3 against 9.2; of 300 of 256: 11.2
-// against 12.3, of 500: 13.3 against 12.6. 48 sequences: even up to 4000 keys.
+// against 12.3, of 500: 13.3 against 12.6. 48 sequences: even up to 4000 keys. The
+// table's width decides, not the positions, which the host does not know: 300 keys
+// of 128 take 8.0 us, behind a table of 8000 pages 12.3.
 constexpr uint32_t kWholeElements = 65536;
-// Larger batches take one part per sequence, laid out without a search.
+// Larger batches take one part per sequence, as every block would lay them all out:
+// for 1024 sequences (one of 131077 keys, the others of 100) that makes 0.2 of the
+// two launches' 0.42 ms. Unsplit, as with 1025, they take 1.23 ms.
 constexpr uint32_t kPlanBatch = 1024;
 
 typedef __attribute__((ext_vector_type(8))) __bf16 pa_bf16x8_t;

@@ -496,8 +496,9 @@ int fh_append_token_advance(fh_device *dev, const uint32_t *token, int64_t rows,
  * logit rules. No counterpart in the reference, which decodes equal-length
  * sequences over one static cache each (src/nn/kv_cache.rs:13-39), with one
  * set of weights, greedily. Unlike the decoder-step ops above, which round
- * where the reference's op sequence rounds, these keep fp32 inside and round
- * each output once.
+ * where the reference's op sequence rounds, these keep every sum and the
+ * softmax's maximum and sum in fp32 and round each output once; a factor that
+ * they hold in fewer bits on the way is named at its call.
  *
  * A paged cache is a pool of n_pages pages of page_size tokens (a multiple of
  * 16). Page p of the K pool and of the V pool holds n_kv regions of page_size
@@ -544,15 +545,18 @@ int fh_paged_attention_workspace(int64_t batch, int64_t n_heads, int64_t n_kv, i
  * keys and values (the new token's among them) fh_paged_rope_kv has written:
  *   s_j = scale * (q . k_j), j = 0..positions[b],
  *   out[b] = RNE(sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s))
- * with fp32 sums. q, out: [batch, n_heads * head_dim]; row b of page_table
- * and positions[b] belong to sequence b; query head h uses KV head h /
- * (n_heads / n_kv). A sequence whose position is >= max_pages * page_size is
- * idle: zeros to its rows of out. Keys of a table entry that names no page
- * are left out; a sequence left with no key gets zeros. What lies in a page
- * behind the position is not used, whatever its bits. A row whose every score
- * is -inf is NaN. head_dim is 64, 128 or 256; any n_heads / n_kv; batch at
- * most 65535, and batch * (max_pages * page_size / 128 + 1) at most 2^31 - 1;
- * out does not overlap the inputs. workspace: at least
+ * with fp32 sums; exp(..) as v's factor has 16 bits (off by 2^-16 of a term
+ * at most). q, out: [batch, n_heads * head_dim]; row b of page_table and
+ * positions[b] belong to sequence b; query head h uses KV head h / (n_heads /
+ * n_kv). A sequence whose position is >= max_pages * page_size is idle: zeros
+ * to its rows of out. Keys of a table entry that names no page are left out; a
+ * sequence left with no key gets zeros. What lies in a page behind the
+ * position is not used, whatever its bits. A row whose every score is -inf is
+ * NaN. Up to 1024 sequences share the GPU by their lengths; in a larger batch
+ * each has one block per KV head and 8 query heads, so a long one among them
+ * is faster in a call of its own. head_dim is 64, 128 or 256; any n_heads /
+ * n_kv; batch at most 65535, and batch * (max_pages * page_size / 128 + 1) at
+ * most 2^31 - 1; out does not overlap the inputs. workspace: at least
  * fh_paged_attention_workspace() bytes, 16-byte aligned, no initial contents;
  * calls that share a workspace must not run concurrently. */
 int fh_paged_attention(fh_device *dev, const uint16_t *q, int64_t batch, int64_t n_heads,
@@ -569,16 +573,18 @@ int fh_lora_workspace(int64_t m, int64_t k, int64_t rank, uint64_t *bytes);
  * what fh_q4_matmul gave for the same x):
  *   y[i, :] = RNE(base[i, :] + scales[a] * (x[i, :] . A_a^T) . B_a^T),
  *   a = adapters[i],
- * with fp32 sums. x: bf16 [m, k] with row stride x_ld (a multiple of 8, >= k);
- * a: bf16 [n_adapters, rank, k]; b: bf16 [n_adapters, n, rank]; scales: f32
- * [n_adapters]; adapters: u32 [m], in any order, a row of a value >=
- * n_adapters taking no adapter (y = base there). An adapter of a lower rank
- * is filled up with zeros. base, y: [m, n] of `dtype` (FH_BF16 or FH_F32)
- * with row strides base_ld, y_ld >= n; y is base itself (the same pointer and
- * stride) or does not overlap the operands. rank and k are multiples of 8,
- * rank at most 128; n is any, m at most 4194240; x, a, b 16-byte aligned. workspace: at least
- * fh_lora_workspace() bytes, 16-byte aligned, no initial contents; calls that
- * share a workspace must not run concurrently. */
+ * with fp32 sums; scales[a] * (x . A_a^T) as B's factor has 16 bits for bf16
+ * results (off by 2^-16 of a term at most), 24 for f32. x: bf16 [m, k] with
+ * row stride x_ld (a multiple of 8, >= k); a: bf16 [n_adapters, rank, k]; b:
+ * bf16 [n_adapters, n, rank]; scales: f32 [n_adapters]; adapters: u32 [m], in
+ * any order, a row of a value >= n_adapters taking no adapter (y = base
+ * there). An adapter of a lower rank is filled up with zeros. base, y: [m, n]
+ * of `dtype` (FH_BF16 or FH_F32) with row strides base_ld, y_ld >= n; y is
+ * base itself (the same pointer and stride) or does not overlap the operands.
+ * rank and k are multiples of 8, rank at most 128; n is any, m at most
+ * 4194240; x, a, b 16-byte aligned. workspace: at least fh_lora_workspace()
+ * bytes, 16-byte aligned, no initial contents; calls that share a workspace
+ * must not run concurrently. */
 int fh_lora_add(fh_device *dev, const uint16_t *x, int64_t m, int64_t k, int64_t x_ld,
                 const uint16_t *a, const uint16_t *b, const float *scales, int64_t n_adapters,
                 int64_t rank, int64_t n, const uint32_t *adapters, const void *base,
