@@ -100,6 +100,19 @@ class LogitRules(ctypes.Structure):
                 ("bias_ld", ctypes.c_int64), ("bias_len", ctypes.c_void_p), ("mask", ctypes.c_void_p)]
 
 
+class PagedPool(ctypes.Structure):
+    """fh_paged_pool: one layer's pools of a paged cache."""
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p)]
+
+
+class PagedCache(ctypes.Structure):
+    """fh_paged_cache: a paged cache of all layers (pools is a host array)."""
+    _fields_ = [("pools", ctypes.POINTER(PagedPool)), ("n_layers", ctypes.c_int64), ("n_kv", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("n_pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+                ("page_table", ctypes.c_void_p), ("n_seqs", ctypes.c_int64), ("max_pages", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("refs", ctypes.c_void_p)]
+
+
 _I64x4 = ctypes.c_int64 * 4
 
 
@@ -187,6 +200,19 @@ SIGNATURES = {
     "fh_lora_add": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _int, _vp,
                     ctypes.c_uint64],
     "fh_logits_process": [_vp, _vp, _int, _i64, _i64, ctypes.POINTER(LogitRules), _vp],
+    "fh_paged_norm_rope_kv": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _vp, _i64, _vp, _vp, _vp,
+                              _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp],
+    "fh_paged_tree_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(ctypes.c_uint64)],
+    "fh_paged_tree_attention": [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp,
+                                ctypes.c_float, _vp, ctypes.c_uint64, _vp],
+    "fh_logits_probs_workspace": [_i64, _i64, ctypes.POINTER(ctypes.c_uint64)],
+    "fh_logits_probs": [_vp, _vp, _int, _i64, _i64, _vp, _vp, ctypes.c_uint64, _vp],
+    "fh_verify_draft_workspace": [_i64, _i64, _i64, ctypes.POINTER(ctypes.c_uint64)],
+    "fh_verify_draft": [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, ctypes.c_uint64, _vp, _vp, _vp],
+    "fh_paged_reserve": [_vp, ctypes.POINTER(PagedCache), _vp, _vp],
+    "fh_paged_fork": [_vp, ctypes.POINTER(PagedCache), _vp, _vp, _i64, _vp],
+    "fh_paged_free": [_vp, ctypes.POINTER(PagedCache), _vp, _i64],
+    "fh_paged_compact": [_vp, ctypes.POINTER(PagedCache), _vp, _vp, _i64, _vp],
     "fh_llama_forward": [_vp, _vp, _i64, _vp, _vp, _vp],
     "fh_copy_strided": [_vp, _int, _vp, ctypes.POINTER(View), _vp],
     "fh_to_dtype": [_vp, _int, _vp, ctypes.POINTER(View), _int, _vp],
@@ -255,6 +281,26 @@ def paged_attention_workspace_bytes(batch: int, n_heads: int, n_kv: int, head_di
 def lora_workspace_bytes(m: int, k: int, rank: int) -> int:
     out = ctypes.c_uint64()
     call("fh_lora_workspace", m, k, rank, ctypes.byref(out))
+    return out.value
+
+
+def paged_tree_attention_workspace_bytes(batch: int, width: int, n_heads: int, n_kv: int, head_dim: int,
+                                         page_size: int, max_pages: int) -> int:
+    out = ctypes.c_uint64()
+    call("fh_paged_tree_attention_workspace", batch, width, n_heads, n_kv, head_dim, page_size, max_pages,
+         ctypes.byref(out))
+    return out.value
+
+
+def logits_probs_workspace_bytes(rows: int, n: int) -> int:
+    out = ctypes.c_uint64()
+    call("fh_logits_probs_workspace", rows, n, ctypes.byref(out))
+    return out.value
+
+
+def verify_draft_workspace_bytes(batch: int, width: int, n: int) -> int:
+    out = ctypes.c_uint64()
+    call("fh_verify_draft_workspace", batch, width, n, ctypes.byref(out))
     return out.value
 
 

@@ -623,6 +623,189 @@ int fh_logits_process(fh_device *dev, const void *logits, int dtype, int64_t row
                       const fh_logit_rules *rules, void *out);
 
 /* ======================================================================
+ * Drafting several tokens ahead: each step runs a tree of drafted tokens (or a
+ * chain) through the model at once and keeps the branch that the target's
+ * distributions accept. No counterpart in the reference, which decodes one
+ * token at a time (src/generate/mod.rs:150-204). A sequence b with lengths[b]
+ * tokens in the paged cache above has its tree's nodes at the places lengths[b]
+ * + 0, 1, ..: node 0, the root, is the last token emitted, whose key and value
+ * the cache does not hold yet; a node's parent comes before it. What holds for
+ * the serving calls above (device data that names nothing, alignment, sums in
+ * fp32, one rounding of each output) holds here. A step is
+ *   fh_paged_reserve        pages for the nodes
+ *   fh_paged_norm_rope_kv   each layer's k and v of the nodes, at their places
+ *   fh_paged_tree_attention each layer's attention of the nodes
+ *   fh_logits_probs         the distribution behind each node
+ *   fh_verify_draft         the accepted path and the token after it
+ *   fh_paged_compact        the path's keys and values to the front, new lengths
+ * and may be captured as a whole.
+ * ====================================================================== */
+
+/* fh_paged_rope_kv with a norm of each q and k head before the rotation and
+ * places apart from the positions:
+ *   q' = RNE(n * cos + rot(n) * sin), n = q * w / sqrt(sum(q^2) / head_dim + eps),
+ * w = q_norm for q's heads, k_norm for k's (bf16 [head_dim]; null: n = q, n =
+ * k); v as it is. The sum of squares, n and the rotation are fp32 (squares past
+ * fp32's largest make n zero). positions (u32 [tokens]) give the rotation,
+ * slots (u32 [tokens], null: the positions) the place in the sequence: the nodes
+ * of a tree share positions. A token whose position is >= table_len, whose slot
+ * is >= max_pages * page_size, whose sequence is >= n_seqs or whose page is >=
+ * n_pages writes nothing. eps >= 0; the rest is as for fh_paged_rope_kv. */
+int fh_paged_norm_rope_kv(fh_device *dev, const uint16_t *qkv, int64_t tokens, int64_t n_heads,
+                          int64_t n_kv, int64_t head_dim, const uint16_t *q_norm,
+                          const uint16_t *k_norm, float eps, const uint16_t *cos_tab,
+                          const uint16_t *sin_tab, int64_t table_len, const uint32_t *sequences,
+                          const uint32_t *positions, const uint32_t *slots,
+                          const uint32_t *page_table, int64_t n_seqs, int64_t max_pages,
+                          uint16_t *k_pages, uint16_t *v_pages, int64_t n_pages, int64_t page_size,
+                          uint16_t *q_out);
+
+/* Bytes of device workspace fh_paged_tree_attention needs for these sizes,
+ * never less for a larger batch. */
+int fh_paged_tree_attention_workspace(int64_t batch, int64_t width, int64_t n_heads, int64_t n_kv,
+                                      int64_t head_dim, int64_t page_size, int64_t max_pages,
+                                      uint64_t *bytes);
+
+/* Attention of each sequence's nodes over its cached tokens and its tree (keys
+ * and values of both are in the paged cache): node i of sequence b sees keys 0
+ * .. lengths[b] - 1, and key lengths[b] + j for each j < counts[b] whose bit (bit
+ * j % 32 of word j / 32) in masks[b, i] is set, whether that is i itself or not:
+ *   s_j = scale * (q . k_j), out[b, i] = RNE(sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s))
+ * q, out: [batch, width, n_heads * head_dim]; lengths: u32 [batch]; counts: u32
+ * [batch], nodes in use (more than width count as width; null: width); masks:
+ * u32 [batch, width, ceil(width / 32)], or null for chains (node i sees nodes 0
+ * .. i). A row past a sequence's nodes, one that sees no key and those of a
+ * sequence whose nodes do not fit its table (lengths[b] + counts[b] > max_pages
+ * * page_size: idle) are zeros. Keys of a table entry that names no page are
+ * left out. What lies at places that a row does not see is not used for it,
+ * whatever its bits. A row whose every score is -inf is NaN. exp(..) as v's
+ * factor has 16 bits (off by 2^-16 of a term at most). head_dim is 64, 128 or
+ * 256, any n_heads / n_kv; width is 1 to 1024, batch at most 65535, scale finite
+ * and above 0; out does not overlap the inputs. workspace: as for
+ * fh_paged_attention, at least fh_paged_tree_attention_workspace() bytes. */
+int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_t batch, int64_t width,
+                            int64_t n_heads, int64_t n_kv, int64_t head_dim,
+                            const uint16_t *k_pages, const uint16_t *v_pages, int64_t n_pages,
+                            int64_t page_size, const uint32_t *page_table, int64_t max_pages,
+                            const uint32_t *lengths, const uint32_t *counts, const uint32_t *masks,
+                            float scale, void *workspace, uint64_t workspace_bytes, uint16_t *out);
+
+/* Bytes of device workspace fh_logits_probs needs for these sizes, never less
+ * for more rows. */
+int fh_logits_probs_workspace(int64_t rows, int64_t n, uint64_t *bytes);
+
+/* The distribution of each row of logits at its temperature:
+ *   probs[r, j] = exp((z_j - max z) / t) / sum_j exp((z_j - max z) / t), t = temperatures[r]
+ * logits: [rows, n] of `dtype` (FH_BF16 or FH_F32); temperatures: f32 [rows],
+ * null for 1. A temperature that is not above 0 is a greedy request's: 1 at the
+ * row's largest logit (the first of equals), 0 elsewhere. Others count as at
+ * least 1e-30 and at most 1e30. A NaN counts as -inf; infinite logits share a
+ * row evenly; a row of nothing but -inf is zeros. probs: f32 [rows, n], does not
+ * overlap the inputs. rows is at most 65535. workspace: at least
+ * fh_logits_probs_workspace() bytes, 16-byte aligned, no initial contents;
+ * calls that share a workspace must not run concurrently. */
+int fh_logits_probs(fh_device *dev, const void *logits, int dtype, int64_t rows, int64_t n,
+                    const float *temperatures, void *workspace, uint64_t workspace_bytes,
+                    float *probs);
+
+/* Bytes of device workspace fh_verify_draft needs for these sizes, never less
+ * for a larger batch. */
+int fh_verify_draft_workspace(int64_t batch, int64_t width, int64_t n, uint64_t *bytes);
+
+/* Which of a tree's drafted tokens the target's distributions accept, and the
+ * token after them, so that what is emitted is distributed as the target alone
+ * would have it. probs: f32 [batch, width, n], row i the target's distribution
+ * behind node i; draft_probs: the same of the draft model, row i what node i's
+ * children were drawn from, or null where the drafted tokens were picked without
+ * chance (then q below is 1 at the child's token, 0 elsewhere). tokens, parents:
+ * u32 [batch, width], node i's token and parent (parents null: i - 1; node 0 has
+ * none, tokens[b, 0] is not read); counts: u32 [batch], nodes in use (more than
+ * width count as width; null: width); uniforms: f32 [batch, width] in [0, 1).
+ *   Start at node a = 0 with w = probs[a], Z = 1. Its children are asked in order:
+ *   child i of token x is accepted if uniforms[i] * q(x) * Z < w(x): go on from a = i.
+ *   Else w becomes max(w - Z q, 0) and Z its sum (q at x alone: w(x) becomes 0, and Z
+ *   is less by what it was).
+ *   When no child is left, the first token whose running sum of w is past uniforms[0]
+ *   times w's sum follows (w = probs[a] again where nothing was left of it).
+ * path (u32 [batch, width]) gets the accepted nodes, the root first, accepted
+ * (u32 [batch]) their number, out_tokens (u32 [batch, width]) their tokens
+ * without the root's, then the one that follows; 0xFFFFFFFF behind them, and in
+ * place of a token that follows a row without any positive entry. A sequence of
+ * no nodes accepts 0. Sums and comparisons are fp64; entries of probs that are
+ * not above 0 count as 0; no entry of either is infinite, none of draft_probs
+ * negative or NaN (a sequence with one may get any token below n, or
+ * 0xFFFFFFFF). A child whose token is >= n, or whose
+ * parent does not come before it, is passed over. With width 1 this draws
+ * a token of each row. width is 1 to 1024, batch at most 65535; no output
+ * overlaps an input or another. workspace: at least fh_verify_draft_workspace()
+ * bytes, 16-byte aligned, no initial contents; calls that share a workspace must
+ * not run concurrently. */
+int fh_verify_draft(fh_device *dev, const float *probs, const float *draft_probs, int64_t batch,
+                    int64_t width, int64_t n, const uint32_t *tokens, const uint32_t *parents,
+                    const uint32_t *counts, const float *uniforms, void *workspace,
+                    uint64_t workspace_bytes, uint32_t *path, uint32_t *out_tokens,
+                    uint32_t *accepted);
+
+/* One layer's pools of a paged cache. */
+typedef struct fh_paged_pool {
+    uint16_t *k_pages;
+    uint16_t *v_pages;
+} fh_paged_pool;
+
+/* A paged cache of all layers, for the calls below: pools is a host array of
+ * n_layers entries (at most 128), which share the page table; page_table (u32
+ * [n_seqs, max_pages]), lengths (u32 [n_seqs], tokens of each sequence) and refs
+ * (u32 [n_pages], how many table entries name each page; 0: the page is free)
+ * are device memory. No two of them overlap. Entries of a row that hold no page
+ * name none (0xFFFFFFFF). n_seqs is at most 16384. */
+typedef struct fh_paged_cache {
+    const fh_paged_pool *pools;
+    int64_t n_layers, n_kv, head_dim, n_pages, page_size;
+    uint32_t *page_table;
+    int64_t n_seqs, max_pages;
+    uint32_t *lengths;
+    uint32_t *refs;
+} fh_paged_cache;
+
+/* Pages for the next extra[s] tokens of each sequence: the table entries of
+ * places lengths[s] .. lengths[s] + extra[s] - 1 that name no page get the lowest
+ * free pages, by sequence, then by entry; their refs become 1. missing (u32
+ * [n_seqs], or null) gets how many entries of a sequence got none, since the
+ * table or the free pages ended. At most 16384 pages are handed out in a call.
+ * extra: u32 [n_seqs]. pools and n_layers are not used, and pools may be null. */
+int fh_paged_reserve(fh_device *dev, const fh_paged_cache *cache, const uint32_t *extra,
+                     uint32_t *missing);
+
+/* Makes sequence to[i] a copy of sequence from[i], for i < n: to's own pages are
+ * freed, from's whole pages shared, and the tokens of its last page, if that is
+ * not full, copied in every layer to the lowest free page (forks in order).
+ * lengths[to] = lengths[from]; pages past from's length stay its own. lost (u32
+ * [n]) gets 1 where no page was free (to is then empty) or the fork was passed
+ * over and changed nothing: from[i] or to[i] >= n_seqs, to[i] among from or
+ * among the entries of to before i, or a length past the table; else 0. from,
+ * to: u32 [n], n at most 1024. */
+int fh_paged_fork(fh_device *dev, const fh_paged_cache *cache, const uint32_t *from,
+                  const uint32_t *to, int64_t n, uint32_t *lost);
+
+/* Empties the sequences seqs[i], i < n (u32 [n]; >= n_seqs: passed over): the refs
+ * of their pages are one less, their table entries name no page, their lengths
+ * are 0. A sequence named twice is emptied once. n is at most 65535. pools and
+ * n_layers are not used, and pools may be null. */
+int fh_paged_free(fh_device *dev, const fh_paged_cache *cache, const uint32_t *seqs, int64_t n);
+
+/* Moves an accepted path's keys and values to the front of its tree, in every
+ * layer: place lengths[s] + i takes what is at lengths[s] + path[s, i], for i <
+ * accepted[s] (at most width), as fh_verify_draft gives them: path[s, i] is
+ * at least i and rises with i (of other paths a place may get another node's
+ * values). Places past the table or without a page are passed over.
+ * new_lengths[s] = lengths[s] + accepted[s]; it is lengths itself (one launch
+ * more) or overlaps nothing. path: u32 [n_seqs, width]; accepted: u32 [n_seqs].
+ * refs is not used, and may be null; a place's page is one sequence's alone, as
+ * fh_paged_fork leaves them. */
+int fh_paged_compact(fh_device *dev, const fh_paged_cache *cache, const uint32_t *path,
+                     const uint32_t *accepted, int64_t width, uint32_t *new_lengths);
+
+/* ======================================================================
  * The decoder forward issued from native code: the layer loop that a
  * caller would otherwise drive op by op, so an eager prefill is not bound
  * by per-call host overhead.
