@@ -2,18 +2,65 @@
 // (fh_paged_tree_attention).
 #include <algorithm>
 #include <tuple>
+#include <type_traits>
 
 #include "paged_cache.hpp"
 
 namespace fh {
 
+// The mathematics: one pass over the keys with the running reference m, sum l and
+// weighted values o of each row (a node's query head),
+//   l' = l 2^((m - m') k) + 2^((s - m') k), o' = o 2^((m - m') k) + 2^((s - m') k) v,
+// k = scale log2 e, joined over disjoint key ranges by the same rule. m follows the
+// largest score only where that has grown by more than kSlack in the exponent, so
+// that o is seldom multiplied; the weights are then up to 2^kSlack, which fp32 sums
+// and 16-bit factors hold as well as those up to 1.
+//
+// The split: the rows of one KV head (nodes x the query heads that share it) are
+// cut into tiles of 16 NT. A block of four wavefronts takes a tile and a part of
+// the batch's keys (whole steps of kStepKeys); every wavefront has the tile's q and
+// o in registers and streams a quarter of the part's keys, 32 at a time, and the four
+// join in LDS. So K and V are read once per tile, straight into the fragments that
+// the matrix cores take. The parts are laid out from lengths and counts on the
+// device (see Layout): the same launch serves one long context and a ragged batch,
+// and may be captured.
+//
+// Per 32 keys the scores are S^T = K Q^T (v_mfma_f32_16x16x32_bf16, 16 keys x 16
+// rows): a lane ends up with its row's scores of keys 4 q .. 4 q + 3 (q = lane / 16)
+// of both 16-key groups. Those eight weights are the fragment that O^T = V^T P^T
+// needs of that lane if its keys are numbered so, so P never leaves its lane; V's rows,
+// read as they lie, become V^T fragments by byte permutes within a lane, once for all
+// NT row groups. P goes in twice, as what rounding to bf16 leaves and as what it
+// loses, for 16 bits of P: what those lose, 2^-16 of a term, is far below the half
+// step of 2^-8 that bf16 V is off by itself. m, l and o are fp32.
 constexpr uint32_t kMaxTree = 1024;
+constexpr uint32_t kTreeThreads = 256;
+constexpr uint32_t kWaves = kTreeThreads / 64;
+constexpr uint32_t kStepKeys = 128;
+constexpr float kSlack = 8.0f;
+// Tables of so few positions (times head_dim) take one block per sequence and tile,
+// and no join: one launch.
+constexpr uint32_t kWholeElements = 65536;
+// Larger batches take one part per sequence, as every block would lay them all out.
+constexpr uint32_t kPlanBatch = 1024;
+
+typedef __attribute__((ext_vector_type(8))) __bf16 ta_bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) float ta_f32x4_t;
+
+__device__ __forceinline__ ta_f32x4_t ta_mfma(uint4 a, uint4 b, ta_f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ta_bf16x8_t, a),
+                                                   __builtin_bit_cast(ta_bf16x8_t, b), c, 0, 0, 0);
+}
 
 struct TreeArgs {
     const uint16_t *q, *k_pages, *v_pages;
     const uint32_t *page_table, *lengths, *counts, *masks;
     uint32_t batch, width, n_heads, n_kv, n_pages, page_size, max_pages;
-    float scale;
+    uint32_t tiles;       // row tiles of a KV head
+    uint32_t want_parts;  // parts of one (KV head, tile); 0: a block per sequence
+    uint32_t grid_parts;  // blocks of one (KV head, tile)
+    float k, slack;       // scale log2 e; kSlack in scores
+    float *records;
     uint16_t *out;
 };
 
@@ -24,70 +71,499 @@ __device__ __forceinline__ uint32_t nodes_of(const TreeArgs &a, uint32_t b) {
     return len <= capacity && count <= capacity - len ? count : 0;
 }
 
-// One pass over the keys with the running maximum m, sum l and weighted values o:
-//   m' = max(m, s), l' = l e^(m - m') + e^(s - m'), o' = o e^(m - m') + e^(s - m') v.
-// One wavefront per row (head, node, sequence): a lane scores one of 64 keys, then
-// adds up HD / 64 of the values' dims.
-template <int HD>
-__global__ __launch_bounds__(64) void tree_row_kernel(const TreeArgs a) {
-    constexpr int DL = HD / 64;
-    __shared__ float qs[HD], ps[64];
-    __shared__ uint64_t at[64];
-    const uint32_t h = blockIdx.x, node = blockIdx.y, b = blockIdx.z, lane = threadIdx.x;
-    const uint64_t row = ((static_cast<uint64_t>(b) * a.width + node) * a.n_heads + h) * HD;
-    const uint32_t kv = h / (a.n_heads / a.n_kv), count = nodes_of(a, b);
-    float o[DL] = {}, m = -INFINITY, l = 0.0f;
-    bool any = false;
-    if (node < count) {
-        for (int d = lane; d < HD; d += 64) qs[d] = bf(a.q[row + d]);
-        __syncthreads();
-        const uint32_t len = a.lengths[b], keys = len + count, words = (a.width + 31) / 32;
-        for (uint32_t j0 = 0; j0 < keys; j0 += 64) {
-            const uint32_t j = j0 + lane;
-            bool seen = j < keys;
-            if (seen && j >= len) {
-                const uint32_t i = j - len;
-                seen = a.masks ? a.masks[(static_cast<uint64_t>(b) * a.width + node) * words + i / 32] >> (i % 32) & 1u
-                               : i <= node;
-            }
-            float s = -INFINITY;
-            if (seen) {
-                const uint32_t page = a.page_table[static_cast<uint64_t>(b) * a.max_pages + j / a.page_size];
-                seen = page < a.n_pages;
-                if (seen) {
-                    const uint64_t region = (static_cast<uint64_t>(page) * a.n_kv + kv) * a.page_size * HD;
-                    const uint16_t *k = a.k_pages + region;
-                    at[lane] = region + static_cast<uint64_t>(j % a.page_size) * HD;
-                    float dot = 0.0f;
-                    for (uint32_t d = 0; d < HD; d += 8) {
-                        float x[8];
-                        unpack8(*reinterpret_cast<const uint4 *>(k + k_offset(j % a.page_size, d, a.page_size, HD)), x);
+// The steps of sequence b for rows from row0 on.
+__device__ __forceinline__ uint32_t steps_of(const TreeArgs &a, uint32_t b, uint32_t row0) {
+    const uint32_t count = nodes_of(a, b);
+    return count * (a.n_heads / a.n_kv) > row0 ? (a.lengths[b] + count + kStepKeys - 1) / kStepKeys : 0;
+}
+
+__device__ __forceinline__ uint32_t scan_wave(uint32_t v, uint32_t lane) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) dot = fmaf(qs[d + e], x[e], dot);
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t o = __shfl_up(v, off, 64);
+        if (lane >= static_cast<uint32_t>(off)) v += o;
+    }
+    return v;
+}
+
+// The steps of all sequences that have rows in a tile, in order, are cut into equal
+// parts: part x takes steps x * size .. of them, which may be the end of one
+// sequence, whole ones, and the start of another. Of a part's pieces only the
+// first and the last can be less than a sequence: they leave records 2 x (the first)
+// and 2 x + 1. Every wavefront works the layout out for itself, 64 sequences at a time.
+struct Layout {
+    uint32_t size;   // steps of a part
+    uint32_t row0;   // the tile's first row
+    uint32_t b0;     // first sequence of the 64 at hand
+    uint32_t mine;   // lane's sequence's steps
+    uint32_t upto;   // and the batch's steps up to its end
+};
+
+__device__ __forceinline__ void layout_at(const TreeArgs &a, Layout &y, uint32_t b0, uint32_t before, uint32_t lane) {
+    y.b0 = b0;
+    y.mine = b0 + lane < a.batch ? steps_of(a, b0 + lane, y.row0) : 0;
+    y.upto = before + scan_wave(y.mine, lane);
+}
+
+__device__ __forceinline__ Layout layout_of(const TreeArgs &a, uint32_t row0, uint32_t lane) {
+    Layout y;
+    y.row0 = row0;
+    uint32_t total = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+        layout_at(a, y, b0, total, lane);
+        total = __builtin_amdgcn_readlane(y.upto, 63);
+    }
+    y.size = max(1u, (total + a.want_parts - 1) / a.want_parts);
+    if (a.batch > 64) layout_at(a, y, 0, 0, lane);
+    return y;
+}
+
+// Moves to the sequence that holds step `at` of the batch and returns it, its
+// steps in n and the steps before it in `start`; ~0 behind the last one.
+__device__ __forceinline__ uint32_t sequence_of(const TreeArgs &a, Layout &y, uint32_t at, uint32_t lane, uint32_t &n,
+                                                uint32_t &start) {
+    for (;;) {
+        const uint64_t hit = __ballot(at < y.upto);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            n = __builtin_amdgcn_readlane(y.mine, l);
+            start = __builtin_amdgcn_readlane(y.upto, l) - n;
+            return y.b0 + l;
+        }
+        if (y.b0 + 64 >= a.batch) return ~0u;
+        layout_at(a, y, y.b0 + 64, __builtin_amdgcn_readlane(y.upto, 63), lane);
+    }
+}
+
+// A record: what a piece leaves to be joined, [16 NT rows][HD] weighted values,
+// then m, l and whether any key was there, of each row.
+template <int HD, int NT>
+constexpr uint32_t record_floats() { return 16 * NT * (HD + 3); }
+
+// Which of the 32 keys from key0 on the row of `node` sees, as far as lengths and masks go.
+__device__ __forceinline__ uint32_t window(const TreeArgs &a, uint32_t seq, uint32_t node, uint32_t key0, uint32_t len,
+                                           uint32_t count) {
+    if (key0 + 32 <= len) return ~0u;
+    const uint32_t before = key0 < len ? len - key0 : 0;  // tokens among them, less than 32
+    const uint32_t j0 = key0 < len ? 0 : key0 - len;      // the first node among them
+    if (j0 >= count) return 0;  // no token either: nodes follow the tokens, and there are some
+    const uint32_t left = count - j0;
+    uint32_t bits;
+    if (a.masks) {
+        const uint32_t words = (a.width + 31) / 32, w = j0 / 32;
+        const uint32_t *mask = a.masks + (static_cast<uint64_t>(seq) * a.width + node) * words;
+        const uint64_t two = mask[w] | (w + 1 < words ? static_cast<uint64_t>(mask[w + 1]) << 32 : 0);
+        bits = static_cast<uint32_t>(two >> (j0 % 32));
+    } else {
+        bits = node < j0 ? 0 : node - j0 >= 31 ? ~0u : (2u << (node - j0)) - 1;
+    }
+    if (left < 32) bits &= (1u << left) - 1;
+    return before ? bits << before | ((1u << before) - 1) : bits;
+}
+
+__device__ __forceinline__ bool is_special(float v) { return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u; }
+
+template <int HD, int NT>
+__global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ? 1 : 2) void tree_part_kernel(
+    const TreeArgs a) {
+    constexpr int KC = HD / 32;                  // score products per 16 keys
+    constexpr int VP = HD == 64 ? 1 : HD / 128;  // pieces of a lane's V row
+    constexpr int PD = HD == 64 ? 4 : 8;         // dims of a piece
+    constexpr int VT = VP * PD;                  // products per 32 keys
+    __shared__ float part_o[kWaves][16][HD + 4];
+    __shared__ float part_ml[kWaves][3][16];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
+    const uint32_t group = a.n_heads / a.n_kv;
+    const uint32_t tile = blockIdx.y % a.tiles, kv = blockIdx.y / a.tiles, row0 = tile * (16 * NT);
+    const uint32_t groups_pp = a.page_size / 16;
+    Layout y;
+    uint32_t at = 0, end = 1;
+    if (a.want_parts) {
+        y = layout_of(a, row0, lane);
+        at = blockIdx.x * y.size;
+        end = at + y.size;
+    }
+    uint32_t slot = 0;  // of the piece's record
+    while (at < end) {
+        // the next piece: `steps` from `first` of sequence seq
+        uint32_t seq = blockIdx.x, first = 0, steps, whole = 1;
+        if (a.want_parts) {
+            uint32_t n, start;
+            seq = sequence_of(a, y, at, lane, n, start);
+            if (seq == ~0u) break;
+            first = at - start;
+            steps = min(n - first, end - at);
+            whole = steps == n;
+            at += steps;
+        } else {
+            steps = steps_of(a, seq, row0);
+            at = end;
+            if (steps == 0) break;
+        }
+        const uint32_t count = nodes_of(a, seq), len = a.lengths[seq], keys = len + count, rows = count * group;
+        // this wavefront's keys: from .. to, in tiles of 32
+        const uint32_t share = (steps * (kStepKeys / 32) + kWaves - 1) / kWaves * 32;
+        const uint32_t from = first * kStepKeys + wave * share;
+        const uint32_t to = min(from + share, min(keys, (first + steps) * kStepKeys));
+        const uint32_t n_tiles = from < to ? (to - from + 31) / 32 : 0;
+
+        // the lane's rows (behind the last one: that again, left out at the end)
+        uint4 qf[NT][KC];
+        uint32_t node[NT];
+#pragma unroll
+        for (int r = 0; r < NT; ++r) {
+            const uint32_t row = min(row0 + r * 16 + c, rows - 1);
+            node[r] = row / group;
+            const uint64_t place = static_cast<uint64_t>(seq) * a.width + node[r];
+            const uint16_t *qrow = a.q + (place * a.n_heads + kv * group + row % group) * HD + q * 8;
+#pragma unroll
+            for (int s = 0; s < KC; ++s) qf[r][s] = *reinterpret_cast<const uint4 *>(qrow + s * 32);
+        }
+        ta_f32x4_t acc[NT][VT];
+        float m[NT], l[NT];
+        bool any[NT];
+        // Once as above. Where that leaves a sum that is not finite, again with care: keys that have an
+        // inf or NaN among their values stay out of the products, where weights of 0 (a row that does not
+        // see the key, a P that lost nothing) would make NaN of them, and are added row by row.
+        auto stream = [&](auto care) {
+            constexpr bool careful = decltype(care)::value;
+#pragma unroll
+            for (int r = 0; r < NT; ++r) {
+#pragma unroll
+                for (int t = 0; t < VT; ++t) acc[r][t] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                m[r] = -INFINITY, l[r] = 0.0f, any[r] = false;
+            }
+            for (uint32_t t0 = 0; t0 < n_tiles; t0 += 32) {
+                // lane i: where the i-th 16-key group of the next 32 tiles lies, in
+                // groups from the pools' start; ~0 for none (past the keys, no page)
+                const uint32_t g = from / 16 + t0 * 2 + lane;
+                uint32_t where = ~0u;
+                if (g * 16 < to) {
+                    const uint32_t pi = g / groups_pp;
+                    const uint32_t page = a.page_table[static_cast<uint64_t>(seq) * a.max_pages + pi];
+                    if (page < a.n_pages) where = (page * a.n_kv + kv) * groups_pp + (g - pi * groups_pp);
+                }
+                const uint32_t batch_tiles = min(32u, n_tiles - t0);
+                uint4 kf[2][KC];
+                uint4 vf[8][VP];
+                // a missing group reads the pool's first group, whose scores are left out
+                auto group_at = [&](uint32_t t, int half) {
+                    const uint32_t w = __builtin_amdgcn_readlane(where, t * 2 + half);
+                    return static_cast<uint64_t>(w == ~0u ? 0u : w) * (16 * HD);
+                };
+                auto load_k = [&](uint32_t t) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint16_t *src = a.k_pages + group_at(t, h) + c * 32 + q * 8;
+#pragma unroll
+                        for (int s = 0; s < KC; ++s) kf[h][s] = *reinterpret_cast<const uint4 *>(src + s * 512);
                     }
-                    s = dot * a.scale;
+                };
+                auto load_v = [&](uint32_t t) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint16_t *src = a.v_pages + group_at(t, i / 4) + (q * 4 + i % 4) * HD + c * PD;
+#pragma unroll
+                        for (int u = 0; u < VP; ++u) {
+                            if constexpr (HD == 64) {
+                                const uint2 v = *reinterpret_cast<const uint2 *>(src);
+                                vf[i][u] = make_uint4(v.x, v.y, 0, 0);
+                            } else {
+                                vf[i][u] = *reinterpret_cast<const uint4 *>(src + u * 128);
+                            }
+                        }
+                    }
+                };
+                ta_f32x4_t s0[NT], s1[NT];
+                auto scores = [&] {
+#pragma unroll
+                    for (int r = 0; r < NT; ++r) s0[r] = s1[r] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int s = 0; s < KC; ++s)
+#pragma unroll
+                        for (int r = 0; r < NT; ++r) {
+                            s0[r] = ta_mfma(kf[0][s], qf[r][s], s0[r]);
+                            s1[r] = ta_mfma(kf[1][s], qf[r][s], s1[r]);
+                        }
+                };
+                uint4 hi[NT], lo[NT];
+                auto weigh = [&](uint32_t t) {
+                    const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2);
+                    const uint32_t w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
+                    const uint32_t key0 = from + (t0 + t) * 32;
+                    const bool plain = key0 + 32 <= len && w0 != ~0u && w1 != ~0u;
+                    const uint32_t there = (w0 != ~0u ? 0xFFFFu : 0u) | (w1 != ~0u ? 0xFFFF0000u : 0u);
+                    if (!plain) {
+                        // keys behind the last or of no page: no value, whatever lies there
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t at = (i / 4) * 16 + q * 4 + i % 4;
+                            if (key0 + at >= keys || !(there >> at & 1u))
+#pragma unroll
+                                for (int u = 0; u < VP; ++u) vf[i][u] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < NT; ++r) {
+                        float s[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[i] = s0[r][i], s[4 + i] = s1[r][i];
+                        if (!plain) {
+                            const uint32_t seen = window(a, seq, node[r], key0, len, count) & there;
+                            any[r] = any[r] || seen;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (!(seen >> ((i / 4) * 16 + q * 4 + i % 4) & 1u)) s[i] = -INFINITY;
+                        } else {
+                            any[r] = true;
+                        }
+                        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                                          fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+                        top = fmaxf(top, __shfl_xor(top, 16, 64));
+                        top = fmaxf(top, __shfl_xor(top, 32, 64));
+                        const bool grown = m[r] == -INFINITY ? top > m[r] : top > m[r] + a.slack;
+                        if (__any(grown)) {
+                            const float next = grown ? top : m[r];
+                            const float keep =
+                                __builtin_amdgcn_exp2f(m[r] == -INFINITY ? -INFINITY : (m[r] - next) * a.k);
+                            l[r] *= keep;
+#pragma unroll
+                            for (int t = 0; t < VT; ++t) acc[r][t] *= keep;
+                            m[r] = next;
+                        }
+                        const float ref = m[r] == -INFINITY ? 0.0f : m[r];
+                        uint32_t wh[4], wl[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float p0 = __builtin_amdgcn_exp2f((s[2 * i] - ref) * a.k);
+                            const float p1 = __builtin_amdgcn_exp2f((s[2 * i + 1] - ref) * a.k);
+                            l[r] += p0 + p1;
+                            wh[i] = f32x2_to_bf16x2_rne(p0, p1);
+                            wl[i] = f32x2_to_bf16x2_rne(p0 - bf(wh[i] & 0xFFFFu),
+                                                        p1 - __uint_as_float(wh[i] & 0xFFFF0000u));
+                        }
+                        hi[r] = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+                        lo[r] = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+                    }
+                };
+                // keys with an inf or NaN among their values: added to the rows that see them, and taken out of vf
+                auto special = [&](uint32_t t) {
+                    const uint32_t key0 = from + (t0 + t) * 32;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t found = 0;
+#pragma unroll
+                        for (int u = 0; u < VP; ++u)
+                            found |= bf16_specials(vf[i][u].x) | bf16_specials(vf[i][u].y) |
+                                     bf16_specials(vf[i][u].z) | bf16_specials(vf[i][u].w);
+                        const uint64_t lanes = __ballot(found != 0);
+                        if (lanes == 0) continue;
+                        for (uint32_t of = 0; of < 4; ++of) {
+                            if (!(lanes >> (of * 16) & 0xFFFFu)) continue;
+                            const uint32_t at = (i / 4) * 16 + of * 4 + i % 4;
+                            if (q == of)
+#pragma unroll
+                                for (int u = 0; u < VP; ++u) vf[i][u] = make_uint4(0, 0, 0, 0);
+                            const uint16_t *v = a.v_pages + group_at(t, i / 4) + (of * 4 + i % 4) * HD;
+#pragma unroll
+                            for (int r = 0; r < NT; ++r) {
+                                // the row's weight of this key, from the lane that has it
+                                auto half = [&](const uint4 p) {
+                                    const uint32_t two = i / 4 ? (i % 4 / 2 ? p.w : p.z) : (i % 4 / 2 ? p.y : p.x);
+                                    return bf(i % 2 ? two >> 16 : two & 0xFFFFu);
+                                };
+                                const float w = __shfl(half(hi[r]) + half(lo[r]), of * 16 + c, 64);
+                                if (window(a, seq, node[r], key0, len, count) >> at & 1u)
+#pragma unroll
+                                    for (int t = 0; t < VT; ++t)
+#pragma unroll
+                                        for (int x = 0; x < 4; ++x)
+                                            acc[r][t][x] = fmaf(w, bf(v[(t / PD) * 128 + (q * 4 + x) * PD + t % PD]),
+                                                                acc[r][t][x]);
+                            }
+                        }
+                    }
+                };
+                auto values = [&] {
+#pragma unroll
+                    for (int t = 0; t < VT; ++t) {
+                        const int u = t / PD, d = t % PD;
+                        auto word = [&](int i) {
+                            const uint4 v = vf[i][u];
+                            return d / 2 == 0 ? v.x : d / 2 == 1 ? v.y : d / 2 == 2 ? v.z : v.w;
+                        };
+                        const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
+                        auto pair = [&](int i) { return __builtin_amdgcn_perm(word(i + 1), word(i), sel); };
+                        const uint4 f = make_uint4(pair(0), pair(2), pair(4), pair(6));
+#pragma unroll
+                        for (int r = 0; r < NT; ++r) acc[r][t] = ta_mfma(f, hi[r], acc[r][t]);
+#pragma unroll
+                        for (int r = 0; r < NT; ++r) acc[r][t] = ta_mfma(f, lo[r], acc[r][t]);
+                    }
+                };
+                // each tile's keys are in flight behind the values before them
+                load_k(0);
+                load_v(0);
+                for (uint32_t t = 0; t < batch_tiles; ++t) {
+                    scores();
+                    if (t + 1 < batch_tiles) load_k(t + 1);
+                    weigh(t);
+                    if constexpr (careful) special(t);
+                    values();
+                    if (t + 1 < batch_tiles) load_v(t + 1);
                 }
             }
-            const float next = fmaxf(m, wave_max(s)), ref = next == -INFINITY ? 0.0f : next;
-            const float keep = __expf(m - ref), p = seen ? __expf(s - ref) : 0.0f;
-            m = next;
-            l = l * keep + wave_sum(p);
-            ps[lane] = p;
-            __syncthreads();
+        };
+        stream(std::false_type{});
+        bool bad = false;
 #pragma unroll
-            for (int d = 0; d < DL; ++d) o[d] *= keep;
-            uint64_t left = __ballot(seen);
-            any = any || left != 0;
-            while (left) {
-                const int i = __builtin_ctzll(left);
-                left &= left - 1;
+        for (int r = 0; r < NT; ++r)
 #pragma unroll
-                for (int d = 0; d < DL; ++d) o[d] = fmaf(ps[i], bf(a.v_pages[at[i] + lane * DL + d]), o[d]);
+            for (int t = 0; t < VT; ++t)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) bad = bad || is_special(acc[r][t][x]);
+        if (__any(bad)) stream(std::true_type{});
+
+        // the four wavefronts joined, 16 rows at a time: thread (row, dims)
+        constexpr int DT = 16 * HD / kTreeThreads;  // dims of a thread
+        const uint32_t h = threadIdx.x / (HD / DT), d0 = threadIdx.x % (HD / DT) * DT;
+        float *rec = a.records + (static_cast<uint64_t>(blockIdx.x * 2 + slot) * gridDim.y + blockIdx.y) *
+                                     record_floats<HD, NT>();
+#pragma unroll
+        for (int r = 0; r < NT; ++r) {
+            if (row0 + r * 16 >= rows) break;
+            float sum_l = l[r];
+            sum_l += __shfl_xor(sum_l, 16, 64);
+            sum_l += __shfl_xor(sum_l, 32, 64);
+#pragma unroll
+            for (int t = 0; t < VT; ++t)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    part_o[wave][c][(t / PD) * 128 + (q * 4 + x) * PD + t % PD] = acc[r][t][x];
+            if (lane < 16) {
+                part_ml[wave][0][c] = m[r];
+                part_ml[wave][1][c] = sum_l;
+                part_ml[wave][2][c] = any[r] ? 1.0f : 0.0f;
             }
             __syncthreads();
+            float top = -INFINITY;
+            bool some = false;
+#pragma unroll
+            for (uint32_t w = 0; w < kWaves; ++w) {
+                top = fmaxf(top, part_ml[w][0][h]);
+                some = some || part_ml[w][2][h] != 0.0f;
+            }
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f, o[DT];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f((part_ml[w][0][h] - ref) * a.k);
+                sum = fmaf(f, part_ml[w][1][h], sum);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part_o[w][h][d0 + d], o[d]);
+            }
+            const uint32_t row = row0 + r * 16 + h;
+            if (whole) {
+                if (row < rows) {
+                    uint16_t *to = a.out +
+                                   ((static_cast<uint64_t>(seq) * a.width + row / group) * a.n_heads + kv * group +
+                                    row % group) * HD + d0;
+#pragma unroll
+                    for (int d = 0; d < DT; d += 2)
+                        *reinterpret_cast<uint32_t *>(to + d) =
+                            some ? f32x2_to_bf16x2_rne(o[d] / sum, o[d + 1] / sum) : 0u;
+                }
+            } else {
+                const uint32_t i = r * 16 + h;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) rec[i * HD + d0 + d] = o[d];
+                if (d0 == 0) {
+                    rec[16 * NT * HD + i] = top;
+                    rec[16 * NT * (HD + 1) + i] = sum;
+                    rec[16 * NT * (HD + 2) + i] = some ? 1.0f : 0.0f;
+                }
+            }
+            __syncthreads();  // the LDS is read: the next rows may write it
+        }
+        slot = 1;
+    }
+    // rows of the tile past their sequence's nodes
+    for (uint32_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        const uint32_t lo = max(row0, nodes_of(a, b) * group), hi = min(row0 + 16 * NT, a.width * group);
+        for (uint32_t i = threadIdx.x; lo < hi && i < (hi - lo) * (HD / 8); i += kTreeThreads) {
+            const uint32_t row = lo + i / (HD / 8);
+            uint16_t *to = a.out +
+                           ((static_cast<uint64_t>(b) * a.width + row / group) * a.n_heads + kv * group + row % group) *
+                               HD + i % (HD / 8) * 8;
+            *reinterpret_cast<uint4 *>(to) = make_uint4(0, 0, 0, 0);
         }
     }
-    for (int d = 0; d < DL; ++d) a.out[row + lane * DL + d] = any ? rne(o[d] / l) : 0;
+}
+
+// Joins the pieces of rows of one sequence: block (sequence, KV head and rows), a
+// row by HD / 4 threads, kJoinLoads pieces requested together.
+constexpr int kJoinLoads = 8;
+
+template <int HD, int NT>
+__global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs a) {
+    constexpr uint32_t kRow = HD / 4, kRows = kTreeThreads / kRow, kBlocks = (16 * NT + kRows - 1) / kRows;
+    const uint32_t seq = blockIdx.x, lane = threadIdx.x & 63u, d = threadIdx.x % kRow * 4;
+    const uint32_t unit = blockIdx.y / kBlocks, tile = unit % a.tiles, kv = unit / a.tiles;
+    const uint32_t i = blockIdx.y % kBlocks * kRows + threadIdx.x / kRow;  // the row in its tile
+    const uint32_t group = a.n_heads / a.n_kv, row0 = tile * (16 * NT), row = row0 + i;
+    const uint32_t rows = nodes_of(a, seq) * group;
+    if (row0 >= rows) return;
+    Layout y = layout_of(a, row0, lane);
+    while (y.b0 + 64 <= seq) layout_at(a, y, y.b0 + 64, __builtin_amdgcn_readlane(y.upto, 63), lane);
+    const uint32_t n = __builtin_amdgcn_readlane(y.mine, seq - y.b0);
+    const uint32_t start = __builtin_amdgcn_readlane(y.upto, seq - y.b0) - n;
+    const uint32_t first = start / y.size, pieces = (start + n - 1) / y.size - first + 1;
+    if (pieces == 1 || row >= rows || i >= 16 * NT) return;  // written by its block, or no row
+    // the first piece is the last of its part, unless it is that part's first too
+    const uint64_t stride = static_cast<uint64_t>(a.n_kv) * a.tiles * record_floats<HD, NT>();
+    const float *rec = a.records + static_cast<uint64_t>(unit) * record_floats<HD, NT>();
+    auto piece = [&](uint32_t p) {
+        return rec + (static_cast<uint64_t>(first + p) * 2 + (p == 0 && start % y.size != 0)) * stride;
+    };
+    float m = -INFINITY, l = 0.0f, some = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (uint32_t p0 = 0; p0 < pieces; p0 += kJoinLoads) {
+        float pm[kJoinLoads], pl[kJoinLoads], ps[kJoinLoads];
+        float4 v[kJoinLoads];
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u) {
+            const float *x = piece(min(p0 + u, pieces - 1));
+            pm[u] = x[16 * NT * HD + i];
+            pl[u] = x[16 * NT * (HD + 1) + i];
+            ps[u] = x[16 * NT * (HD + 2) + i];
+            v[u] = *reinterpret_cast<const float4 *>(x + i * HD + d);
+        }
+        float next = m;
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u) {
+            if (p0 + u >= pieces) pm[u] = -INFINITY;
+            next = fmaxf(next, pm[u]);
+        }
+        const float ref = next == -INFINITY ? 0.0f : next, f = __builtin_amdgcn_exp2f((m - ref) * a.k);
+        m = next;
+        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u)
+            if (p0 + u < pieces) {
+                const float g = __builtin_amdgcn_exp2f((pm[u] - ref) * a.k);
+                some = fmaxf(some, ps[u]);
+                l = fmaf(pl[u], g, l);
+                o.x = fmaf(v[u].x, g, o.x), o.y = fmaf(v[u].y, g, o.y);
+                o.z = fmaf(v[u].z, g, o.z), o.w = fmaf(v[u].w, g, o.w);
+            }
+    }
+    uint16_t *to = a.out +
+                   ((static_cast<uint64_t>(seq) * a.width + row / group) * a.n_heads + kv * group + row % group) * HD + d;
+    *reinterpret_cast<uint2 *>(to) = some != 0.0f ? make_uint2(f32x2_to_bf16x2_rne(o.x / l, o.y / l),
+                                                              f32x2_to_bf16x2_rne(o.z / l, o.w / l))
+                                                  : make_uint2(0, 0);
 }
 
 }  // namespace fh
@@ -108,10 +584,55 @@ int check_shape(const char *fn, int64_t batch, int64_t width, int64_t n_heads, i
     if (width < 1 || width > kMaxTree)
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: width %lld must be 1 to %u", fn, (long long)width, kMaxTree);
     if (batch > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: batch %lld exceeds 65535", fn, (long long)batch);
-    if (batch * width * n_heads > 0x3FFFFFF)
-        return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld sequences of %lld nodes and %lld heads", fn, (long long)batch,
-                    (long long)width, (long long)n_heads);
+    // the joining launch's rows of blocks (16 NT * head_dim / 1024 to a tile, NT at most 4) fit its grid
+    if ((width * n_heads + 64 * n_kv) * head_dim / 1024 > 65535)
+        return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld nodes of %lld heads", fn, (long long)width, (long long)n_heads);
+    // the steps of all sequences are counted in 32 bits (pages may be shared, so their number bounds nothing)
+    if (batch * (max_pages * page_size / kStepKeys + 1) > 0x7FFFFFFFll)
+        return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld sequences of %lld positions", fn, (long long)batch,
+                    (long long)(max_pages * page_size));
     return FH_OK;
+}
+
+// The launch for these sizes: 16-row groups per block, tiles of a KV head, parts per
+// (KV head, tile), or 0 for a block per sequence, and the bytes of the pieces' records.
+struct Plan {
+    uint32_t groups, tiles, want_parts, grid_parts;
+    uint64_t bytes;
+};
+
+Plan plan(int64_t batch, int64_t width, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t page_size,
+          int64_t max_pages) {
+    const uint64_t rows = width * (n_heads / n_kv), capacity = static_cast<uint64_t>(max_pages) * page_size;
+    const uint32_t groups = rows <= 16 ? 1 : rows <= 32 || head_dim == 256 ? 2 : 4;
+    const uint64_t tiles = (rows + 16 * groups - 1) / (16 * groups), units = tiles * n_kv;
+    Plan w{groups, static_cast<uint32_t>(tiles), 0, static_cast<uint32_t>(batch), 16};
+    if (capacity * head_dim <= kWholeElements) return w;
+    // what serves the largest batch serves smaller ones: the bytes of those that are split
+    const uint64_t split = std::min<uint64_t>(batch, kPlanBatch);
+    // a block's registers leave room for two on a CU, or for one
+    const uint64_t blocks = head_dim == 256 || (head_dim == 128 && groups == 4) ? 256 : 512;
+    // a table of few steps has no use for more parts than steps
+    const uint64_t steps = (capacity + kStepKeys - 1) / kStepKeys;
+    const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>(blocks / units, split * steps));
+    w.bytes = parts * 2 * units * (16 * groups * (head_dim + 3) * 4) + 16;
+    if (batch <= kPlanBatch) w.want_parts = w.grid_parts = static_cast<uint32_t>(parts);
+    return w;
+}
+
+template <int HD, int NT>
+int launch(fh_device *dev, const char *fn, const TreeArgs &a) {
+    const dim3 grid(a.grid_parts, a.n_kv * a.tiles), threads(kTreeThreads);
+    if (int rc = dispatch(dev, fn, [&] {
+            hipLaunchKernelGGL((tree_part_kernel<HD, NT>), grid, threads, 0, dev->stream, a);
+        }))
+        return rc;
+    if (a.want_parts <= 1) return FH_OK;
+    constexpr uint32_t kRows = kTreeThreads / (HD / 4), kBlocks = (16 * NT + kRows - 1) / kRows;
+    const dim3 join(a.batch, a.n_kv * a.tiles * kBlocks);
+    return dispatch(dev, fn, [&] {
+        hipLaunchKernelGGL((tree_join_kernel<HD, NT>), join, threads, 0, dev->stream, a);
+    });
 }
 
 }  // namespace
@@ -122,7 +643,7 @@ extern "C" int fh_paged_tree_attention_workspace(int64_t batch, int64_t width, i
     const char *fn = "fh_paged_tree_attention_workspace";
     if (bytes == nullptr) return fail(FH_ERR_INVALID_ARGUMENT, "%s: bytes is null", fn);
     if (int rc = check_shape(fn, batch, width, n_heads, n_kv, head_dim, page_size, max_pages)) return rc;
-    *bytes = 16;
+    *bytes = plan(batch, width, n_heads, n_kv, head_dim, page_size, max_pages).bytes;
     return FH_OK;
 }
 
@@ -177,6 +698,8 @@ extern "C" int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_
                 if (int rc = refuse_overlap(fn, what, ptr, size, with, p, n)) return rc;
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "out", out, rows)) return rc;
     if (int rc = set_current(dev, fn)) return rc;
+    const Plan w = plan(batch, width, n_heads, n_kv, head_dim, page_size, max_pages);
+    const float k = scale * 1.4426950408889634f;
     const TreeArgs a{q,
                      k_pages,
                      v_pages,
@@ -191,15 +714,18 @@ extern "C" int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_
                      static_cast<uint32_t>(n_pages),
                      static_cast<uint32_t>(page_size),
                      static_cast<uint32_t>(max_pages),
-                     scale,
+                     w.tiles,
+                     w.want_parts,
+                     w.grid_parts,
+                     k,
+                     kSlack / k,
+                     static_cast<float *>(workspace),
                      out};
-    const dim3 grid(static_cast<uint32_t>(n_heads), static_cast<uint32_t>(width), static_cast<uint32_t>(batch));
-    return dispatch(dev, fn, [&] {
-        if (head_dim == 64)
-            hipLaunchKernelGGL(tree_row_kernel<64>, grid, dim3(64), 0, dev->stream, a);
-        else if (head_dim == 128)
-            hipLaunchKernelGGL(tree_row_kernel<128>, grid, dim3(64), 0, dev->stream, a);
-        else
-            hipLaunchKernelGGL(tree_row_kernel<256>, grid, dim3(64), 0, dev->stream, a);
-    });
+    if (head_dim == 64)
+        return w.groups == 1 ? launch<64, 1>(dev, fn, a)
+                             : w.groups == 2 ? launch<64, 2>(dev, fn, a) : launch<64, 4>(dev, fn, a);
+    if (head_dim == 128)
+        return w.groups == 1 ? launch<128, 1>(dev, fn, a)
+                             : w.groups == 2 ? launch<128, 2>(dev, fn, a) : launch<128, 4>(dev, fn, a);
+    return w.groups == 1 ? launch<256, 1>(dev, fn, a) : launch<256, 2>(dev, fn, a);
 }

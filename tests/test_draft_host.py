@@ -30,7 +30,7 @@ def test_tree_attention_workspace():
     refused(_lib.ERR_UNSUPPORTED, name, 1, 4, 4, 2, 96, 16, 4)
     refused(_lib.ERR_INDEX_TOO_LARGE, name, 65536, 4, 4, 2, 64, 16, 4)
     refused(_lib.ERR_INDEX_TOO_LARGE, name, 1, 4, 4, 2, 64, 16, 1 << 27)
-    refused(_lib.ERR_INDEX_TOO_LARGE, name, 65535, 1024, 64, 2, 64, 16, 4)
+    refused(_lib.ERR_INDEX_TOO_LARGE, name, 1, 1024, 65534, 2, 64, 16, 4)
     assert _lib.load().fh_paged_tree_attention_workspace(1, 4, 4, 2, 64, 16, 4, None) == bad
 
 
