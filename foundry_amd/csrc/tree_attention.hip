@@ -46,8 +46,10 @@ constexpr uint32_t kPlanBatch = 1024;
 
 typedef __attribute__((ext_vector_type(8))) __bf16 ta_bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float ta_f32x4_t;
+// whole registers of a fragment: a struct of words would be carried around loops word by word
+typedef __attribute__((ext_vector_type(4))) uint32_t ta_u32x4_t;
 
-__device__ __forceinline__ ta_f32x4_t ta_mfma(uint4 a, uint4 b, ta_f32x4_t c) {
+__device__ __forceinline__ ta_f32x4_t ta_mfma(ta_u32x4_t a, ta_u32x4_t b, ta_f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ta_bf16x8_t, a),
                                                    __builtin_bit_cast(ta_bf16x8_t, b), c, 0, 0, 0);
 }
@@ -140,42 +142,56 @@ __device__ __forceinline__ uint32_t sequence_of(const TreeArgs &a, Layout &y, ui
 template <int HD, int NT>
 constexpr uint32_t record_floats() { return 16 * NT * (HD + 3); }
 
-// Which of the 32 keys from key0 on the row of `node` sees, as far as lengths and masks go.
-__device__ __forceinline__ uint32_t window(const TreeArgs &a, uint32_t seq, uint32_t node, uint32_t key0, uint32_t len,
+// Which of the 32 keys from key0 on a node of these mask words sees, as far as
+// lengths and masks go.
+__device__ __forceinline__ uint32_t window(const uint32_t *mask, uint32_t words, uint32_t key0, uint32_t len,
                                            uint32_t count) {
-    if (key0 + 32 <= len) return ~0u;
-    const uint32_t before = key0 < len ? len - key0 : 0;  // tokens among them, less than 32
-    const uint32_t j0 = key0 < len ? 0 : key0 - len;      // the first node among them
-    if (j0 >= count) return 0;  // no token either: nodes follow the tokens, and there are some
-    const uint32_t left = count - j0;
-    uint32_t bits;
-    if (a.masks) {
-        const uint32_t words = (a.width + 31) / 32, w = j0 / 32;
-        const uint32_t *mask = a.masks + (static_cast<uint64_t>(seq) * a.width + node) * words;
-        const uint64_t two = mask[w] | (w + 1 < words ? static_cast<uint64_t>(mask[w + 1]) << 32 : 0);
-        bits = static_cast<uint32_t>(two >> (j0 % 32));
-    } else {
-        bits = node < j0 ? 0 : node - j0 >= 31 ? ~0u : (2u << (node - j0)) - 1;
-    }
-    if (left < 32) bits &= (1u << left) - 1;
-    return before ? bits << before | ((1u << before) - 1) : bits;
+    const int32_t past = static_cast<int32_t>(key0 - len);           // places below 2^31
+    const uint32_t before = min(max(-past, 0), 32);                  // tokens among them
+    const uint32_t j0 = min(max(past, 0), static_cast<int>(count));  // the first node among them
+    const uint32_t left = min(count - j0, 32u), w = min(j0 / 32, words - 1);
+    const uint64_t two = mask[w] | static_cast<uint64_t>(mask[min(w + 1, words - 1)]) << 32;
+    const uint64_t nodes = (two >> (j0 % 32)) & ((1ull << left) - 1);
+    return static_cast<uint32_t>(nodes << before | ((1ull << before) - 1));
 }
 
 __device__ __forceinline__ bool is_special(float v) { return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u; }
 
+// The maximum over the lanes that share lane % 16.
+__device__ __forceinline__ float max_over_quarters(float v) {
+    typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+    const u32x2_t a = __builtin_bit_cast(
+        u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const u32x2_t b = __builtin_bit_cast(
+        u32x2_t, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 template <int HD, int NT>
-__global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ? 1 : 2) void tree_part_kernel(
-    const TreeArgs a) {
+__global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) void tree_part_kernel(const TreeArgs a) {
     constexpr int KC = HD / 32;                  // score products per 16 keys
     constexpr int VP = HD == 64 ? 1 : HD / 128;  // pieces of a lane's V row
     constexpr int PD = HD == 64 ? 4 : 8;         // dims of a piece
     constexpr int VT = VP * PD;                  // products per 32 keys
-    __shared__ float part_o[kWaves][16][HD + 4];
-    __shared__ float part_ml[kWaves][3][16];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
+    // The tile's q as fragments [KC][NT][64 lanes], read for every 32 keys (in registers they would
+    // leave no room for a second block on the CU), and after them the wavefronts' results.
+    struct Results {
+        float o[kWaves][16][HD + 4];
+        float ml[kWaves][3][16];
+    };
+    union Shared {
+        ta_u32x4_t q[KC * NT * 64];
+        Results results;
+    };
+    __shared__ Shared shared;
+    __shared__ uint32_t bits[(16 * NT + 1) * (kMaxTree / 32)];  // the mask words of the tile's nodes
+    // (the wavefront's number as a scalar: its loops then count in scalars too)
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t c = lane & 15u, q = lane >> 4;
     const uint32_t group = a.n_heads / a.n_kv;
     const uint32_t tile = blockIdx.y % a.tiles, kv = blockIdx.y / a.tiles, row0 = tile * (16 * NT);
-    const uint32_t groups_pp = a.page_size / 16;
+    const uint32_t groups_pp = a.page_size / 16, words = (a.width + 31) / 32, node0 = row0 / group;
     Layout y;
     uint32_t at = 0, end = 1;
     if (a.want_parts) {
@@ -206,22 +222,46 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
         const uint32_t from = first * kStepKeys + wave * share;
         const uint32_t to = min(from + share, min(keys, (first + steps) * kStepKeys));
         const uint32_t n_tiles = from < to ? (to - from + 31) / 32 : 0;
-
-        // the lane's rows (behind the last one: that again, left out at the end)
-        uint4 qf[NT][KC];
+        // lane i: where the i-th 16-key group from tile t0 on lies, in groups from the
+        // pools' start; ~0 for none (past the keys, no page)
+        auto places = [&](uint32_t t0) {
+            const uint32_t g = from / 16 + t0 * 2 + lane;
+            uint32_t w = ~0u;
+            if (t0 < n_tiles && g * 16 < to) {
+                const uint32_t pi = g / groups_pp;
+                const uint32_t page = a.page_table[static_cast<uint64_t>(seq) * a.max_pages + pi];
+                if (page < a.n_pages) w = (page * a.n_kv + kv) * groups_pp + (g - pi * groups_pp);
+            }
+            return w;
+        };
+        uint32_t first_where = places(0);
+        // the tile's rows (behind the last one: that again, left out at the end)
+        for (uint32_t i = threadIdx.x; i < KC * NT * 64; i += kTreeThreads) {
+            const uint32_t row = min(row0 + i / 64 % NT * 16 + i % 16, rows - 1);
+            const uint16_t *from_q =
+                a.q + ((static_cast<uint64_t>(seq) * a.width + row / group) * a.n_heads + kv * group + row % group) * HD +
+                i / (64 * NT) * 32 + i % 64 / 16 * 8;
+            shared.q[i] = *reinterpret_cast<const ta_u32x4_t *>(from_q);
+        }
+        if ((first + steps) * kStepKeys > len) {
+            const uint32_t nodes = (min(row0 + 16 * NT, rows) - 1) / group - node0 + 1;
+            const uint32_t *mask = a.masks + (static_cast<uint64_t>(seq) * a.width + node0) * words;
+            for (uint32_t i = threadIdx.x; i < nodes * words; i += kTreeThreads) {
+                const uint32_t upto = node0 + i / words + 1, from_node = i % words * 32;  // of a chain
+                bits[i] = a.masks ? mask[i]
+                                  : upto <= from_node ? 0u : upto - from_node >= 32 ? ~0u : (1u << (upto - from_node)) - 1;
+            }
+        }
         uint32_t node[NT];
 #pragma unroll
-        for (int r = 0; r < NT; ++r) {
-            const uint32_t row = min(row0 + r * 16 + c, rows - 1);
-            node[r] = row / group;
-            const uint64_t place = static_cast<uint64_t>(seq) * a.width + node[r];
-            const uint16_t *qrow = a.q + (place * a.n_heads + kv * group + row % group) * HD + q * 8;
-#pragma unroll
-            for (int s = 0; s < KC; ++s) qf[r][s] = *reinterpret_cast<const uint4 *>(qrow + s * 32);
-        }
+        for (int r = 0; r < NT; ++r) node[r] = min(row0 + r * 16 + c, rows - 1) / group;
+        auto seen_by = [&](int r, uint32_t key0) {
+            return window(bits + (node[r] - node0) * words, words, key0, len, count);
+        };
+        __syncthreads();
         ta_f32x4_t acc[NT][VT];
         float m[NT], l[NT];
-        bool any[NT];
+        uint32_t any[NT];
         // Once as above. Where that leaves a sum that is not finite, again with care: keys that have an
         // inf or NaN among their values stay out of the products, where weights of 0 (a row that does not
         // see the key, a P that lost nothing) would make NaN of them, and are added row by row.
@@ -231,21 +271,16 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
             for (int r = 0; r < NT; ++r) {
 #pragma unroll
                 for (int t = 0; t < VT; ++t) acc[r][t] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-                m[r] = -INFINITY, l[r] = 0.0f, any[r] = false;
+                m[r] = -INFINITY, l[r] = 0.0f, any[r] = 0;
             }
+            uint32_t where, next_where = first_where;
+#pragma unroll 1
             for (uint32_t t0 = 0; t0 < n_tiles; t0 += 32) {
-                // lane i: where the i-th 16-key group of the next 32 tiles lies, in
-                // groups from the pools' start; ~0 for none (past the keys, no page)
-                const uint32_t g = from / 16 + t0 * 2 + lane;
-                uint32_t where = ~0u;
-                if (g * 16 < to) {
-                    const uint32_t pi = g / groups_pp;
-                    const uint32_t page = a.page_table[static_cast<uint64_t>(seq) * a.max_pages + pi];
-                    if (page < a.n_pages) where = (page * a.n_kv + kv) * groups_pp + (g - pi * groups_pp);
-                }
+                where = next_where;
+                next_where = places(t0 + 32);
                 const uint32_t batch_tiles = min(32u, n_tiles - t0);
-                uint4 kf[2][KC];
-                uint4 vf[8][VP];
+                ta_u32x4_t kf[2][KC];
+                ta_u32x4_t vf[8][VP];
                 // a missing group reads the pool's first group, whose scores are left out
                 auto group_at = [&](uint32_t t, int half) {
                     const uint32_t w = __builtin_amdgcn_readlane(where, t * 2 + half);
@@ -256,7 +291,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
                     for (int h = 0; h < 2; ++h) {
                         const uint16_t *src = a.k_pages + group_at(t, h) + c * 32 + q * 8;
 #pragma unroll
-                        for (int s = 0; s < KC; ++s) kf[h][s] = *reinterpret_cast<const uint4 *>(src + s * 512);
+                        for (int s = 0; s < KC; ++s) kf[h][s] = *reinterpret_cast<const ta_u32x4_t *>(src + s * 512);
                     }
                 };
                 auto load_v = [&](uint32_t t) {
@@ -267,83 +302,96 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
                         for (int u = 0; u < VP; ++u) {
                             if constexpr (HD == 64) {
                                 const uint2 v = *reinterpret_cast<const uint2 *>(src);
-                                vf[i][u] = make_uint4(v.x, v.y, 0, 0);
+                                vf[i][u] = ta_u32x4_t{v.x, v.y, 0, 0};
                             } else {
-                                vf[i][u] = *reinterpret_cast<const uint4 *>(src + u * 128);
+                                vf[i][u] = *reinterpret_cast<const ta_u32x4_t *>(src + u * 128);
                             }
                         }
                     }
                 };
                 ta_f32x4_t s0[NT], s1[NT];
                 auto scores = [&] {
+                    asm volatile("" ::: "memory");  // q stays in LDS
 #pragma unroll
                     for (int r = 0; r < NT; ++r) s0[r] = s1[r] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int s = 0; s < KC; ++s)
 #pragma unroll
                         for (int r = 0; r < NT; ++r) {
-                            s0[r] = ta_mfma(kf[0][s], qf[r][s], s0[r]);
-                            s1[r] = ta_mfma(kf[1][s], qf[r][s], s1[r]);
+                            const ta_u32x4_t qf = shared.q[(s * NT + r) * 64 + lane];
+                            s0[r] = ta_mfma(kf[0][s], qf, s0[r]);
+                            s1[r] = ta_mfma(kf[1][s], qf, s1[r]);
                         }
                 };
-                uint4 hi[NT], lo[NT];
+                ta_u32x4_t hi[NT], lo[NT];
                 auto weigh = [&](uint32_t t) {
                     const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2);
                     const uint32_t w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
                     const uint32_t key0 = from + (t0 + t) * 32;
-                    const bool plain = key0 + 32 <= len && w0 != ~0u && w1 != ~0u;
-                    const uint32_t there = (w0 != ~0u ? 0xFFFFu : 0u) | (w1 != ~0u ? 0xFFFF0000u : 0u);
-                    if (!plain) {
+                    if (key0 + 32 > len || w0 == ~0u || w1 == ~0u) {
+                        const uint32_t there = (w0 != ~0u ? 0xFFFFu : 0u) | (w1 != ~0u ? 0xFFFF0000u : 0u);
                         // keys behind the last or of no page: no value, whatever lies there
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const uint32_t at = (i / 4) * 16 + q * 4 + i % 4;
                             if (key0 + at >= keys || !(there >> at & 1u))
 #pragma unroll
-                                for (int u = 0; u < VP; ++u) vf[i][u] = make_uint4(0, 0, 0, 0);
+                                for (int u = 0; u < VP; ++u) vf[i][u] = ta_u32x4_t{0, 0, 0, 0};
+                        }
+#pragma unroll
+                        for (int r = 0; r < NT; ++r) {
+                            const uint32_t seen = seen_by(r, key0) & there;
+                            any[r] |= seen;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (!(seen >> (q * 4 + i) & 1u)) s0[r][i] = -INFINITY;
+                                if (!(seen >> (16 + q * 4 + i) & 1u)) s1[r][i] = -INFINITY;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < NT; ++r) any[r] = 1;
+                    }
+                    float top[NT];
+                    bool grown = false;
+#pragma unroll
+                    for (int r = 0; r < NT; ++r) {
+                        const ta_f32x4_t x = s0[r], z = s1[r];
+                        top[r] = max_over_quarters(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                                         fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]))));
+                        // m = -inf: any score at all
+                        top[r] = top[r] > (m[r] == -INFINITY ? m[r] : m[r] + a.slack) ? top[r] : m[r];
+                        grown = grown || top[r] != m[r];
+                    }
+                    if (__any(grown)) {
+#pragma unroll
+                        for (int r = 0; r < NT; ++r) {
+                            const float keep = top[r] == m[r] ? 1.0f : __builtin_amdgcn_exp2f((m[r] - top[r]) * a.k);
+                            l[r] *= keep;
+#pragma unroll
+                            for (int t = 0; t < VT; ++t) acc[r][t] *= keep;
+                            m[r] = top[r];
                         }
                     }
 #pragma unroll
                     for (int r = 0; r < NT; ++r) {
-                        float s[8];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[i] = s0[r][i], s[4 + i] = s1[r][i];
-                        if (!plain) {
-                            const uint32_t seen = window(a, seq, node[r], key0, len, count) & there;
-                            any[r] = any[r] || seen;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (!(seen >> ((i / 4) * 16 + q * 4 + i % 4) & 1u)) s[i] = -INFINITY;
-                        } else {
-                            any[r] = true;
-                        }
-                        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
-                                          fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-                        top = fmaxf(top, __shfl_xor(top, 16, 64));
-                        top = fmaxf(top, __shfl_xor(top, 32, 64));
-                        const bool grown = m[r] == -INFINITY ? top > m[r] : top > m[r] + a.slack;
-                        if (__any(grown)) {
-                            const float next = grown ? top : m[r];
-                            const float keep =
-                                __builtin_amdgcn_exp2f(m[r] == -INFINITY ? -INFINITY : (m[r] - next) * a.k);
-                            l[r] *= keep;
-#pragma unroll
-                            for (int t = 0; t < VT; ++t) acc[r][t] *= keep;
-                            m[r] = next;
-                        }
                         const float ref = m[r] == -INFINITY ? 0.0f : m[r];
+                        float p[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = __builtin_amdgcn_exp2f((s0[r][i] - ref) * a.k);
+                            p[4 + i] = __builtin_amdgcn_exp2f((s1[r][i] - ref) * a.k);
+                        }
+                        l[r] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
                         uint32_t wh[4], wl[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float p0 = __builtin_amdgcn_exp2f((s[2 * i] - ref) * a.k);
-                            const float p1 = __builtin_amdgcn_exp2f((s[2 * i + 1] - ref) * a.k);
-                            l[r] += p0 + p1;
-                            wh[i] = f32x2_to_bf16x2_rne(p0, p1);
-                            wl[i] = f32x2_to_bf16x2_rne(p0 - bf(wh[i] & 0xFFFFu),
-                                                        p1 - __uint_as_float(wh[i] & 0xFFFF0000u));
+                            wh[i] = f32x2_to_bf16x2_rne(p[2 * i], p[2 * i + 1]);
+                            wl[i] = f32x2_to_bf16x2_rne(p[2 * i] - bf(wh[i] & 0xFFFFu),
+                                                        p[2 * i + 1] - __uint_as_float(wh[i] & 0xFFFF0000u));
                         }
-                        hi[r] = make_uint4(wh[0], wh[1], wh[2], wh[3]);
-                        lo[r] = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+                        hi[r] = ta_u32x4_t{wh[0], wh[1], wh[2], wh[3]};
+                        lo[r] = ta_u32x4_t{wl[0], wl[1], wl[2], wl[3]};
                     }
                 };
                 // keys with an inf or NaN among their values: added to the rows that see them, and taken out of vf
@@ -363,17 +411,17 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
                             const uint32_t at = (i / 4) * 16 + of * 4 + i % 4;
                             if (q == of)
 #pragma unroll
-                                for (int u = 0; u < VP; ++u) vf[i][u] = make_uint4(0, 0, 0, 0);
+                                for (int u = 0; u < VP; ++u) vf[i][u] = ta_u32x4_t{0, 0, 0, 0};
                             const uint16_t *v = a.v_pages + group_at(t, i / 4) + (of * 4 + i % 4) * HD;
 #pragma unroll
                             for (int r = 0; r < NT; ++r) {
                                 // the row's weight of this key, from the lane that has it
-                                auto half = [&](const uint4 p) {
+                                auto half = [&](const ta_u32x4_t p) {
                                     const uint32_t two = i / 4 ? (i % 4 / 2 ? p.w : p.z) : (i % 4 / 2 ? p.y : p.x);
                                     return bf(i % 2 ? two >> 16 : two & 0xFFFFu);
                                 };
                                 const float w = __shfl(half(hi[r]) + half(lo[r]), of * 16 + c, 64);
-                                if (window(a, seq, node[r], key0, len, count) >> at & 1u)
+                                if (seen_by(r, key0) >> at & 1u)
 #pragma unroll
                                     for (int t = 0; t < VT; ++t)
 #pragma unroll
@@ -388,29 +436,27 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
 #pragma unroll
                     for (int t = 0; t < VT; ++t) {
                         const int u = t / PD, d = t % PD;
-                        auto word = [&](int i) {
-                            const uint4 v = vf[i][u];
-                            return d / 2 == 0 ? v.x : d / 2 == 1 ? v.y : d / 2 == 2 ? v.z : v.w;
-                        };
+                        auto word = [&](int i) { return vf[i][u][d / 2]; };
                         const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
                         auto pair = [&](int i) { return __builtin_amdgcn_perm(word(i + 1), word(i), sel); };
-                        const uint4 f = make_uint4(pair(0), pair(2), pair(4), pair(6));
+                        const ta_u32x4_t f = {pair(0), pair(2), pair(4), pair(6)};
 #pragma unroll
                         for (int r = 0; r < NT; ++r) acc[r][t] = ta_mfma(f, hi[r], acc[r][t]);
 #pragma unroll
                         for (int r = 0; r < NT; ++r) acc[r][t] = ta_mfma(f, lo[r], acc[r][t]);
                     }
                 };
-                // each tile's keys are in flight behind the values before them
+                // each tile's keys are in flight behind the values before them (behind the last: that tile again)
                 load_k(0);
                 load_v(0);
+#pragma unroll 1
                 for (uint32_t t = 0; t < batch_tiles; ++t) {
                     scores();
-                    if (t + 1 < batch_tiles) load_k(t + 1);
+                    load_k(min(t + 1, batch_tiles - 1));
                     weigh(t);
                     if constexpr (careful) special(t);
                     values();
-                    if (t + 1 < batch_tiles) load_v(t + 1);
+                    load_v(min(t + 1, batch_tiles - 1));
                 }
             }
         };
@@ -429,9 +475,11 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
         const uint32_t h = threadIdx.x / (HD / DT), d0 = threadIdx.x % (HD / DT) * DT;
         float *rec = a.records + (static_cast<uint64_t>(blockIdx.x * 2 + slot) * gridDim.y + blockIdx.y) *
                                      record_floats<HD, NT>();
+        Results &part = shared.results;
 #pragma unroll
         for (int r = 0; r < NT; ++r) {
             if (row0 + r * 16 >= rows) break;
+            __syncthreads();  // q, or the rows before, are read
             float sum_l = l[r];
             sum_l += __shfl_xor(sum_l, 16, 64);
             sum_l += __shfl_xor(sum_l, 32, 64);
@@ -439,19 +487,19 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
             for (int t = 0; t < VT; ++t)
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    part_o[wave][c][(t / PD) * 128 + (q * 4 + x) * PD + t % PD] = acc[r][t][x];
+                    part.o[wave][c][(t / PD) * 128 + (q * 4 + x) * PD + t % PD] = acc[r][t][x];
             if (lane < 16) {
-                part_ml[wave][0][c] = m[r];
-                part_ml[wave][1][c] = sum_l;
-                part_ml[wave][2][c] = any[r] ? 1.0f : 0.0f;
+                part.ml[wave][0][c] = m[r];
+                part.ml[wave][1][c] = sum_l;
+                part.ml[wave][2][c] = any[r] ? 1.0f : 0.0f;
             }
             __syncthreads();
             float top = -INFINITY;
             bool some = false;
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
-                top = fmaxf(top, part_ml[w][0][h]);
-                some = some || part_ml[w][2][h] != 0.0f;
+                top = fmaxf(top, part.ml[w][0][h]);
+                some = some || part.ml[w][2][h] != 0.0f;
             }
             const float ref = top == -INFINITY ? 0.0f : top;
             float sum = 0.0f, o[DT];
@@ -459,10 +507,10 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
             for (int d = 0; d < DT; ++d) o[d] = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f((part_ml[w][0][h] - ref) * a.k);
-                sum = fmaf(f, part_ml[w][1][h], sum);
+                const float f = __builtin_amdgcn_exp2f((part.ml[w][0][h] - ref) * a.k);
+                sum = fmaf(f, part.ml[w][1][h], sum);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part_o[w][h][d0 + d], o[d]);
+                for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part.o[w][h][d0 + d], o[d]);
             }
             const uint32_t row = row0 + r * 16 + h;
             if (whole) {
@@ -485,8 +533,8 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || (HD == 128 && NT == 4) ?
                     rec[16 * NT * (HD + 2) + i] = some ? 1.0f : 0.0f;
                 }
             }
-            __syncthreads();  // the LDS is read: the next rows may write it
         }
+        __syncthreads();  // the LDS is read: the next piece may write it
         slot = 1;
     }
     // rows of the tile past their sequence's nodes
@@ -611,7 +659,7 @@ Plan plan(int64_t batch, int64_t width, int64_t n_heads, int64_t n_kv, int64_t h
     // what serves the largest batch serves smaller ones: the bytes of those that are split
     const uint64_t split = std::min<uint64_t>(batch, kPlanBatch);
     // a block's registers leave room for two on a CU, or for one
-    const uint64_t blocks = head_dim == 256 || (head_dim == 128 && groups == 4) ? 256 : 512;
+    const uint64_t blocks = head_dim == 256 || head_dim * groups > 384 ? 256 : 512;
     // a table of few steps has no use for more parts than steps
     const uint64_t steps = (capacity + kStepKeys - 1) / kStepKeys;
     const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>(blocks / units, split * steps));
@@ -725,7 +773,9 @@ extern "C" int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_
         return w.groups == 1 ? launch<64, 1>(dev, fn, a)
                              : w.groups == 2 ? launch<64, 2>(dev, fn, a) : launch<64, 4>(dev, fn, a);
     if (head_dim == 128)
-        return w.groups == 1 ? launch<128, 1>(dev, fn, a)
-                             : w.groups == 2 ? launch<128, 2>(dev, fn, a) : launch<128, 4>(dev, fn, a);
+        return w.groups == 1   ? launch<128, 1>(dev, fn, a)
+               : w.groups == 2 ? launch<128, 2>(dev, fn, a)
+               : w.groups == 3 ? launch<128, 3>(dev, fn, a)
+                               : launch<128, 4>(dev, fn, a);
     return w.groups == 1 ? launch<256, 1>(dev, fn, a) : launch<256, 2>(dev, fn, a);
 }
