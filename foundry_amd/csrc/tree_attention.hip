@@ -2,7 +2,6 @@
 // (fh_paged_tree_attention).
 #include <algorithm>
 #include <tuple>
-#include <type_traits>
 
 #include "paged_cache.hpp"
 
@@ -54,13 +53,27 @@ __device__ __forceinline__ ta_f32x4_t ta_mfma(ta_u32x4_t a, ta_u32x4_t b, ta_f32
                                                    __builtin_bit_cast(ta_bf16x8_t, b), c, 0, 0, 0);
 }
 
+// n / by for n below 2^27, by up to 2^27, as one product: with m = ceil(2^k / by), k = 27
+// + ceil(log2 by), the quotient is off by n (m by - 2^k) / (by 2^k) < 1 / by.
+struct Divider {
+    uint32_t by, m, k;
+    explicit Divider(uint32_t d) : by(d), k(27) {
+        while ((1u << (k - 27)) < d) ++k;
+        m = static_cast<uint32_t>(((1ull << k) + d - 1) / d);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        return static_cast<uint32_t>(static_cast<uint64_t>(n) * m >> k);
+    }
+};
+
 struct TreeArgs {
     const uint16_t *q, *k_pages, *v_pages;
     const uint32_t *page_table, *lengths, *counts, *masks;
-    uint32_t batch, width, n_heads, n_kv, n_pages, page_size, max_pages;
+    uint32_t batch, width, n_heads, n_kv, n_pages, max_pages, capacity;
+    Divider group;        // query heads of a KV head
+    Divider page_groups;  // 16-key groups of a page
     uint32_t tiles;       // row tiles of a KV head
     uint32_t want_parts;  // parts of one (KV head, tile); 0: a block per sequence
-    uint32_t grid_parts;  // blocks of one (KV head, tile)
     float k, slack;       // scale log2 e; kSlack in scores
     float *records;
     uint16_t *out;
@@ -69,14 +82,13 @@ struct TreeArgs {
 // The nodes of sequence b, 0 where they do not fit its table.
 __device__ __forceinline__ uint32_t nodes_of(const TreeArgs &a, uint32_t b) {
     const uint32_t count = a.counts ? min(a.counts[b], a.width) : a.width;
-    const uint32_t capacity = a.max_pages * a.page_size, len = a.lengths[b];
-    return len <= capacity && count <= capacity - len ? count : 0;
+    const uint32_t len = a.lengths[b];
+    return len <= a.capacity && count <= a.capacity - len ? count : 0;
 }
 
-// The steps of sequence b for rows from row0 on.
-__device__ __forceinline__ uint32_t steps_of(const TreeArgs &a, uint32_t b, uint32_t row0) {
-    const uint32_t count = nodes_of(a, b);
-    return count * (a.n_heads / a.n_kv) > row0 ? (a.lengths[b] + count + kStepKeys - 1) / kStepKeys : 0;
+// The steps of a sequence of `len` tokens and `count` nodes for rows from row0 on.
+__device__ __forceinline__ uint32_t steps_of(const TreeArgs &a, uint32_t len, uint32_t count, uint32_t row0) {
+    return count * a.group.by > row0 ? (len + count + kStepKeys - 1) / kStepKeys : 0;
 }
 
 __device__ __forceinline__ uint32_t scan_wave(uint32_t v, uint32_t lane) {
@@ -97,13 +109,16 @@ struct Layout {
     uint32_t size;   // steps of a part
     uint32_t row0;   // the tile's first row
     uint32_t b0;     // first sequence of the 64 at hand
-    uint32_t mine;   // lane's sequence's steps
+    uint32_t len, count;  // lane's sequence's tokens and nodes
+    uint32_t mine;   // its steps
     uint32_t upto;   // and the batch's steps up to its end
 };
 
 __device__ __forceinline__ void layout_at(const TreeArgs &a, Layout &y, uint32_t b0, uint32_t before, uint32_t lane) {
     y.b0 = b0;
-    y.mine = b0 + lane < a.batch ? steps_of(a, b0 + lane, y.row0) : 0;
+    y.count = b0 + lane < a.batch ? nodes_of(a, b0 + lane) : 0;
+    y.len = y.count ? a.lengths[b0 + lane] : 0;
+    y.mine = steps_of(a, y.len, y.count, y.row0);
     y.upto = before + scan_wave(y.mine, lane);
 }
 
@@ -123,11 +138,13 @@ __device__ __forceinline__ Layout layout_of(const TreeArgs &a, uint32_t row0, ui
 // Moves to the sequence that holds step `at` of the batch and returns it, its
 // steps in n and the steps before it in `start`; ~0 behind the last one.
 __device__ __forceinline__ uint32_t sequence_of(const TreeArgs &a, Layout &y, uint32_t at, uint32_t lane, uint32_t &n,
-                                                uint32_t &start) {
+                                                uint32_t &start, uint32_t &len, uint32_t &count) {
     for (;;) {
         const uint64_t hit = __ballot(at < y.upto);
         if (hit) {
             const int l = __builtin_ctzll(hit);
+            len = __builtin_amdgcn_readlane(y.len, l);
+            count = __builtin_amdgcn_readlane(y.count, l);
             n = __builtin_amdgcn_readlane(y.mine, l);
             start = __builtin_amdgcn_readlane(y.upto, l) - n;
             return y.b0 + l;
@@ -155,7 +172,12 @@ __device__ __forceinline__ uint32_t window(const uint32_t *mask, uint32_t words,
     return static_cast<uint32_t>(nodes << before | ((1ull << before) - 1));
 }
 
-__device__ __forceinline__ bool is_special(float v) { return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u; }
+// v, worked out again from here on: what depends on it alone is not kept in registers
+// over the loop around.
+__device__ __forceinline__ uint32_t anew(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 // The maximum over the lanes that share lane % 16.
 __device__ __forceinline__ float max_over_quarters(float v) {
@@ -169,54 +191,65 @@ __device__ __forceinline__ float max_over_quarters(float v) {
 }
 
 template <int HD, int NT>
-__global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) void tree_part_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_kernel(const TreeArgs a) {
     constexpr int KC = HD / 32;                  // score products per 16 keys
     constexpr int VP = HD == 64 ? 1 : HD / 128;  // pieces of a lane's V row
     constexpr int PD = HD == 64 ? 4 : 8;         // dims of a piece
     constexpr int VT = VP * PD;                  // products per 32 keys
-    // The tile's q as fragments [KC][NT][64 lanes], read for every 32 keys (in registers they would
-    // leave no room for a second block on the CU), and after them the wavefronts' results.
-    struct Results {
-        float o[kWaves][16][HD + 4];
-        float ml[kWaves][3][16];
+    struct Results {  // of the wavefronts
+        float o[kWaves][16 * NT][HD + 4];
+        float ml[kWaves][3][16 * NT];
     };
-    union Shared {
-        ta_u32x4_t q[KC * NT * 64];
-        Results results;
-    };
-    __shared__ Shared shared;
-    __shared__ uint32_t bits[(16 * NT + 1) * (kMaxTree / 32)];  // the mask words of the tile's nodes
+    __shared__ __attribute__((aligned(16))) Results part;
+    constexpr uint32_t kWords = kMaxTree / 32;
+    __shared__ uint32_t bits[(16 * NT + 1) * kWords];  // the mask words of the tile's nodes
     // (the wavefront's number as a scalar: its loops then count in scalars too)
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 15u, q = lane >> 4;
-    const uint32_t group = a.n_heads / a.n_kv;
-    const uint32_t tile = blockIdx.y % a.tiles, kv = blockIdx.y / a.tiles, row0 = tile * (16 * NT);
-    const uint32_t groups_pp = a.page_size / 16, words = (a.width + 31) / 32, node0 = row0 / group;
+    const uint32_t group = a.group.by, kv = blockIdx.z, row0 = blockIdx.y * (16 * NT);
+    const uint32_t unit = kv * a.tiles + blockIdx.y;  // of the records
+    const uint32_t words = (a.width + 31) / 32, node0 = a.group(row0);
+    // where row `row` of sequence seq lies in q and out
+    auto place = [&](uint32_t seq, uint32_t row) {
+        const uint32_t node = a.group(row);
+        return ((static_cast<uint64_t>(seq) * a.width + node) * a.n_heads + kv * group + (row - node * group)) * HD;
+    };
+    // zeros to the tile's rows past the nodes of sequence b
+    auto clear = [&](uint32_t b, uint32_t count) {
+        const uint32_t lo = max(row0, count * group), hi = min(row0 + 16 * NT, a.width * group);
+        for (uint32_t i = anew(threadIdx.x); lo < hi && i < (hi - lo) * (HD / 8); i += kTreeThreads)
+            *reinterpret_cast<uint4 *>(a.out + place(b, lo + i / (HD / 8)) + i % (HD / 8) * 8) = make_uint4(0, 0, 0, 0);
+    };
     Layout y;
     uint32_t at = 0, end = 1;
     if (a.want_parts) {
         y = layout_of(a, row0, lane);
         at = blockIdx.x * y.size;
         end = at + y.size;
+        for (uint32_t b = blockIdx.x; b < a.batch; b += gridDim.x)
+            clear(b, b < 64 ? __builtin_amdgcn_readlane(y.count, b) : nodes_of(a, b));
     }
     uint32_t slot = 0;  // of the piece's record
     while (at < end) {
         // the next piece: `steps` from `first` of sequence seq
-        uint32_t seq = blockIdx.x, first = 0, steps, whole = 1;
+        uint32_t seq = blockIdx.x, first = 0, steps, whole = 1, len, count;
         if (a.want_parts) {
             uint32_t n, start;
-            seq = sequence_of(a, y, at, lane, n, start);
+            seq = sequence_of(a, y, at, lane, n, start, len, count);
             if (seq == ~0u) break;
             first = at - start;
             steps = min(n - first, end - at);
             whole = steps == n;
             at += steps;
         } else {
-            steps = steps_of(a, seq, row0);
+            count = nodes_of(a, seq);
+            len = a.lengths[seq];
+            steps = steps_of(a, len, count, row0);
             at = end;
+            clear(seq, count);
             if (steps == 0) break;
         }
-        const uint32_t count = nodes_of(a, seq), len = a.lengths[seq], keys = len + count, rows = count * group;
+        const uint32_t keys = len + count, rows = count * group;
         // this wavefront's keys: from .. to, in tiles of 32
         const uint32_t share = (steps * (kStepKeys / 32) + kWaves - 1) / kWaves * 32;
         const uint32_t from = first * kStepKeys + wave * share;
@@ -228,35 +261,38 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) v
             const uint32_t g = from / 16 + t0 * 2 + lane;
             uint32_t w = ~0u;
             if (t0 < n_tiles && g * 16 < to) {
-                const uint32_t pi = g / groups_pp;
+                const uint32_t pi = a.page_groups(g);
                 const uint32_t page = a.page_table[static_cast<uint64_t>(seq) * a.max_pages + pi];
-                if (page < a.n_pages) w = (page * a.n_kv + kv) * groups_pp + (g - pi * groups_pp);
+                if (page < a.n_pages) w = (page * a.n_kv + kv) * a.page_groups.by + (g - pi * a.page_groups.by);
             }
             return w;
         };
         uint32_t first_where = places(0);
-        // the tile's rows (behind the last one: that again, left out at the end)
-        for (uint32_t i = threadIdx.x; i < KC * NT * 64; i += kTreeThreads) {
-            const uint32_t row = min(row0 + i / 64 % NT * 16 + i % 16, rows - 1);
-            const uint16_t *from_q =
-                a.q + ((static_cast<uint64_t>(seq) * a.width + row / group) * a.n_heads + kv * group + row % group) * HD +
-                i / (64 * NT) * 32 + i % 64 / 16 * 8;
-            shared.q[i] = *reinterpret_cast<const ta_u32x4_t *>(from_q);
-        }
-        if ((first + steps) * kStepKeys > len) {
-            const uint32_t nodes = (min(row0 + 16 * NT, rows) - 1) / group - node0 + 1;
-            const uint32_t *mask = a.masks + (static_cast<uint64_t>(seq) * a.width + node0) * words;
-            for (uint32_t i = threadIdx.x; i < nodes * words; i += kTreeThreads) {
-                const uint32_t upto = node0 + i / words + 1, from_node = i % words * 32;  // of a chain
-                bits[i] = a.masks ? mask[i]
-                                  : upto <= from_node ? 0u : upto - from_node >= 32 ? ~0u : (1u << (upto - from_node)) - 1;
-            }
-        }
+        // the lane's rows (behind the last one: that again, left out at the end)
+        ta_u32x4_t qf[NT][KC];
         uint32_t node[NT];
 #pragma unroll
-        for (int r = 0; r < NT; ++r) node[r] = min(row0 + r * 16 + c, rows - 1) / group;
+        for (int r = 0; r < NT; ++r) {
+            const uint32_t row = min(row0 + r * 16 + c, rows - 1);
+            node[r] = a.group(row) - node0;
+            const uint16_t *qrow = a.q + place(seq, row) + q * 8;
+#pragma unroll
+            for (int s = 0; s < KC; ++s) qf[r][s] = *reinterpret_cast<const ta_u32x4_t *>(qrow + s * 32);
+        }
+        if ((first + steps) * kStepKeys > len) {
+            const uint32_t tid = anew(threadIdx.x), w = tid % kWords;
+            const uint32_t nodes = a.group(min(row0 + 16 * NT, rows) - 1) - node0 + 1;
+            const uint32_t *mask = a.masks + (static_cast<uint64_t>(seq) * a.width + node0) * words + w;
+            for (uint32_t i = tid / kWords; i < nodes && w < words; i += kTreeThreads / kWords) {
+                const uint32_t upto = node0 + i + 1;  // of a chain
+                bits[i * kWords + w] = a.masks           ? mask[i * words]
+                                       : upto <= w * 32       ? 0u
+                                       : upto - w * 32 >= 32 ? ~0u
+                                                             : (1u << (upto - w * 32)) - 1;
+            }
+        }
         auto seen_by = [&](int r, uint32_t key0) {
-            return window(bits + (node[r] - node0) * words, words, key0, len, count);
+            return window(bits + node[r] * kWords, words, key0, len, count);
         };
         __syncthreads();
         ta_f32x4_t acc[NT][VT];
@@ -265,71 +301,65 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) v
         // Once as above. Where that leaves a sum that is not finite, again with care: keys that have an
         // inf or NaN among their values stay out of the products, where weights of 0 (a row that does not
         // see the key, a P that lost nothing) would make NaN of them, and are added row by row.
-        auto stream = [&](auto care) {
-            constexpr bool careful = decltype(care)::value;
+#pragma unroll 1
+        for (bool careful = false;; careful = true) {
 #pragma unroll
             for (int r = 0; r < NT; ++r) {
 #pragma unroll
                 for (int t = 0; t < VT; ++t) acc[r][t] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
                 m[r] = -INFINITY, l[r] = 0.0f, any[r] = 0;
             }
-            uint32_t where, next_where = first_where;
-#pragma unroll 1
-            for (uint32_t t0 = 0; t0 < n_tiles; t0 += 32) {
-                where = next_where;
-                next_where = places(t0 + 32);
-                const uint32_t batch_tiles = min(32u, n_tiles - t0);
+            if (n_tiles) {
+                uint32_t where = first_where, next_where = places(32);
+                // a tile's two groups; a missing one reads the pool's first group, whose scores are left out
+                uint32_t g0 = __builtin_amdgcn_readlane(where, 0), g1 = __builtin_amdgcn_readlane(where, 1);
                 ta_u32x4_t kf[2][KC];
                 ta_u32x4_t vf[8][VP];
-                // a missing group reads the pool's first group, whose scores are left out
-                auto group_at = [&](uint32_t t, int half) {
-                    const uint32_t w = __builtin_amdgcn_readlane(where, t * 2 + half);
-                    return static_cast<uint64_t>(w == ~0u ? 0u : w) * (16 * HD);
-                };
-                auto load_k = [&](uint32_t t) {
+                auto start_of = [&](uint32_t g) { return static_cast<uint64_t>(g == ~0u ? 0u : g) * (16 * HD); };
+                // (a scalar address and the lane's bytes from there)
+                auto load_k = [&](uint32_t g0, uint32_t g1) {
+                    const uint32_t mine = anew(c * 64 + q * 16);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint16_t *src = a.k_pages + group_at(t, h) + c * 32 + q * 8;
+                        const char *src = reinterpret_cast<const char *>(a.k_pages + start_of(h ? g1 : g0));
 #pragma unroll
-                        for (int s = 0; s < KC; ++s) kf[h][s] = *reinterpret_cast<const ta_u32x4_t *>(src + s * 512);
+                        for (int s = 0; s < KC; ++s)
+                            kf[h][s] = *reinterpret_cast<const ta_u32x4_t *>(src + mine + s * 1024);
                     }
                 };
-                auto load_v = [&](uint32_t t) {
+                auto load_v = [&](uint32_t g0, uint32_t g1) {
+                    const uint32_t mine = anew(q * (8 * HD) + c * (2 * PD));
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const uint16_t *src = a.v_pages + group_at(t, i / 4) + (q * 4 + i % 4) * HD + c * PD;
+                        const char *src = reinterpret_cast<const char *>(a.v_pages + start_of(i / 4 ? g1 : g0));
 #pragma unroll
                         for (int u = 0; u < VP; ++u) {
                             if constexpr (HD == 64) {
-                                const uint2 v = *reinterpret_cast<const uint2 *>(src);
+                                const uint2 v = *reinterpret_cast<const uint2 *>(src + mine + i % 4 * (2 * HD));
                                 vf[i][u] = ta_u32x4_t{v.x, v.y, 0, 0};
                             } else {
-                                vf[i][u] = *reinterpret_cast<const ta_u32x4_t *>(src + u * 128);
+                                vf[i][u] =
+                                    *reinterpret_cast<const ta_u32x4_t *>(src + mine + i % 4 * (2 * HD) + u * 256);
                             }
                         }
                     }
                 };
                 ta_f32x4_t s0[NT], s1[NT];
                 auto scores = [&] {
-                    asm volatile("" ::: "memory");  // q stays in LDS
 #pragma unroll
                     for (int r = 0; r < NT; ++r) s0[r] = s1[r] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int s = 0; s < KC; ++s)
 #pragma unroll
                         for (int r = 0; r < NT; ++r) {
-                            const ta_u32x4_t qf = shared.q[(s * NT + r) * 64 + lane];
-                            s0[r] = ta_mfma(kf[0][s], qf, s0[r]);
-                            s1[r] = ta_mfma(kf[1][s], qf, s1[r]);
+                            s0[r] = ta_mfma(kf[0][s], qf[r][s], s0[r]);
+                            s1[r] = ta_mfma(kf[1][s], qf[r][s], s1[r]);
                         }
                 };
                 ta_u32x4_t hi[NT], lo[NT];
-                auto weigh = [&](uint32_t t) {
-                    const uint32_t w0 = __builtin_amdgcn_readlane(where, t * 2);
-                    const uint32_t w1 = __builtin_amdgcn_readlane(where, t * 2 + 1);
-                    const uint32_t key0 = from + (t0 + t) * 32;
-                    if (key0 + 32 > len || w0 == ~0u || w1 == ~0u) {
-                        const uint32_t there = (w0 != ~0u ? 0xFFFFu : 0u) | (w1 != ~0u ? 0xFFFF0000u : 0u);
+                auto weigh = [&](uint32_t key0) {
+                    if (key0 + 32 > len || g0 == ~0u || g1 == ~0u) {
+                        const uint32_t there = (g0 != ~0u ? 0xFFFFu : 0u) | (g1 != ~0u ? 0xFFFF0000u : 0u), q = anew(lane) >> 4;
                         // keys behind the last or of no page: no value, whatever lies there
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
@@ -387,7 +417,8 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) v
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             wh[i] = f32x2_to_bf16x2_rne(p[2 * i], p[2 * i + 1]);
-                            wl[i] = f32x2_to_bf16x2_rne(p[2 * i] - bf(wh[i] & 0xFFFFu),
+                            asm("" : "+v"(wh[i]));  // both halves from this one conversion
+                            wl[i] = f32x2_to_bf16x2_rne(p[2 * i] - __uint_as_float(wh[i] << 16),
                                                         p[2 * i + 1] - __uint_as_float(wh[i] & 0xFFFF0000u));
                         }
                         hi[r] = ta_u32x4_t{wh[0], wh[1], wh[2], wh[3]};
@@ -395,8 +426,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) v
                     }
                 };
                 // keys with an inf or NaN among their values: added to the rows that see them, and taken out of vf
-                auto special = [&](uint32_t t) {
-                    const uint32_t key0 = from + (t0 + t) * 32;
+                auto special = [&](uint32_t key0) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         uint32_t found = 0;
@@ -412,7 +442,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) v
                             if (q == of)
 #pragma unroll
                                 for (int u = 0; u < VP; ++u) vf[i][u] = ta_u32x4_t{0, 0, 0, 0};
-                            const uint16_t *v = a.v_pages + group_at(t, i / 4) + (of * 4 + i % 4) * HD;
+                            const uint16_t *v = a.v_pages + start_of(i / 4 ? g1 : g0) + (of * 4 + i % 4) * HD;
 #pragma unroll
                             for (int r = 0; r < NT; ++r) {
                                 // the row's weight of this key, from the lane that has it
@@ -421,13 +451,16 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) v
                                     return bf(i % 2 ? two >> 16 : two & 0xFFFFu);
                                 };
                                 const float w = __shfl(half(hi[r]) + half(lo[r]), of * 16 + c, 64);
+                                const uint16_t *mine = v + anew(q * (4 * PD));
                                 if (seen_by(r, key0) >> at & 1u)
 #pragma unroll
-                                    for (int t = 0; t < VT; ++t)
+                                    for (int t = 0; t < VT; ++t) {
+                                        asm volatile("" ::: "memory");  // four loads at a time
 #pragma unroll
                                         for (int x = 0; x < 4; ++x)
-                                            acc[r][t][x] = fmaf(w, bf(v[(t / PD) * 128 + (q * 4 + x) * PD + t % PD]),
-                                                                acc[r][t][x]);
+                                            acc[r][t][x] =
+                                                fmaf(w, bf(mine[(t / PD) * 128 + x * PD + t % PD]), acc[r][t][x]);
+                                    }
                             }
                         }
                     }
@@ -446,107 +479,100 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 || HD * NT > 384 ? 1 : 2) v
                         for (int r = 0; r < NT; ++r) acc[r][t] = ta_mfma(f, lo[r], acc[r][t]);
                     }
                 };
-                // each tile's keys are in flight behind the values before them (behind the last: that tile again)
-                load_k(0);
-                load_v(0);
+                // each tile's keys are in flight behind the values before them (behind the last: that tile
+                // again; a load that may not be there would have the values wait for all of them)
+                load_k(g0, g1);
+                load_v(g0, g1);
 #pragma unroll 1
-                for (uint32_t t = 0; t < batch_tiles; ++t) {
+                for (uint32_t t = 0; t < n_tiles; ++t) {
                     scores();
-                    load_k(min(t + 1, batch_tiles - 1));
-                    weigh(t);
-                    if constexpr (careful) special(t);
+                    const uint32_t next = min(t + 1, n_tiles - 1);
+                    if (next / 32 != t / 32) {
+                        where = next_where;
+                        next_where = places(next + 32);
+                    }
+                    const uint32_t n0 = __builtin_amdgcn_readlane(where, next % 32 * 2);
+                    const uint32_t n1 = __builtin_amdgcn_readlane(where, next % 32 * 2 + 1);
+                    load_k(n0, n1);
+                    weigh(from + t * 32);
+                    if (careful) special(from + t * 32);
                     values();
-                    load_v(min(t + 1, batch_tiles - 1));
+                    load_v(n0, n1);
+                    g0 = n0, g1 = n1;
                 }
             }
-        };
-        stream(std::false_type{});
-        bool bad = false;
+            float zero = 0.0f;  // NaN if a sum is not finite
 #pragma unroll
-        for (int r = 0; r < NT; ++r)
+            for (int r = 0; r < NT; ++r)
 #pragma unroll
-            for (int t = 0; t < VT; ++t)
+                for (int t = 0; t < VT; ++t)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) bad = bad || is_special(acc[r][t][x]);
-        if (__any(bad)) stream(std::true_type{});
+                    for (int x = 0; x < 4; ++x) zero = fmaf(acc[r][t][x], 0.0f, zero);
+            if (careful || !__any(zero != 0.0f)) break;
+        }
 
-        // the four wavefronts joined, 16 rows at a time: thread (row, dims)
-        constexpr int DT = 16 * HD / kTreeThreads;  // dims of a thread
-        const uint32_t h = threadIdx.x / (HD / DT), d0 = threadIdx.x % (HD / DT) * DT;
-        float *rec = a.records + (static_cast<uint64_t>(blockIdx.x * 2 + slot) * gridDim.y + blockIdx.y) *
-                                     record_floats<HD, NT>();
-        Results &part = shared.results;
+        // the four wavefronts joined: thread (row, dims), 16 rows at a time
 #pragma unroll
         for (int r = 0; r < NT; ++r) {
-            if (row0 + r * 16 >= rows) break;
-            __syncthreads();  // q, or the rows before, are read
-            float sum_l = l[r];
-            sum_l += __shfl_xor(sum_l, 16, 64);
-            sum_l += __shfl_xor(sum_l, 32, 64);
+            l[r] += __shfl_xor(l[r], 16, 64);
+            l[r] += __shfl_xor(l[r], 32, 64);
+            const uint32_t at = anew(lane), i = r * 16 + at % 16, q = at >> 4;
 #pragma unroll
-            for (int t = 0; t < VT; ++t)
+            for (int t = 0; t < VT; t += 4)
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    part.o[wave][c][(t / PD) * 128 + (q * 4 + x) * PD + t % PD] = acc[r][t][x];
+                    *reinterpret_cast<float4 *>(&part.o[wave][i][(t / PD) * 128 + (q * 4 + x) * PD + t % PD]) =
+                        make_float4(acc[r][t][x], acc[r][t + 1][x], acc[r][t + 2][x], acc[r][t + 3][x]);
             if (lane < 16) {
-                part.ml[wave][0][c] = m[r];
-                part.ml[wave][1][c] = sum_l;
-                part.ml[wave][2][c] = any[r] ? 1.0f : 0.0f;
+                part.ml[wave][0][i] = m[r];
+                part.ml[wave][1][i] = l[r];
+                part.ml[wave][2][i] = any[r] ? 1.0f : 0.0f;
             }
-            __syncthreads();
-            float top = -INFINITY;
-            bool some = false;
+        }
+        __syncthreads();
+        constexpr uint32_t DT = 16 * HD / kTreeThreads;  // dims of a thread
+        const uint32_t tid = anew(threadIdx.x), d0 = tid % (HD / DT) * DT;
+        float *rec = a.records + (static_cast<uint64_t>(blockIdx.x * 2 + slot) * (a.n_kv * a.tiles) + unit) *
+                                     record_floats<HD, NT>();
+#pragma unroll 1
+        for (uint32_t i = tid / (HD / DT); i < 16 * NT && row0 + i < rows; i += 16) {
+            float top = -INFINITY, some = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
-                top = fmaxf(top, part.ml[w][0][h]);
-                some = some || part.ml[w][2][h] != 0.0f;
+                top = fmaxf(top, part.ml[w][0][i]);
+                some = fmaxf(some, part.ml[w][2][i]);
             }
             const float ref = top == -INFINITY ? 0.0f : top;
             float sum = 0.0f, o[DT];
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] = 0.0f;
+            for (uint32_t d = 0; d < DT; ++d) o[d] = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f((part.ml[w][0][h] - ref) * a.k);
-                sum = fmaf(f, part.ml[w][1][h], sum);
+                const float f = __builtin_amdgcn_exp2f((part.ml[w][0][i] - ref) * a.k);
+                sum = fmaf(f, part.ml[w][1][i], sum);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] = fmaf(f, part.o[w][h][d0 + d], o[d]);
+                for (uint32_t d = 0; d < DT; ++d) o[d] = fmaf(f, part.o[w][i][d0 + d], o[d]);
             }
-            const uint32_t row = row0 + r * 16 + h;
             if (whole) {
-                if (row < rows) {
-                    uint16_t *to = a.out +
-                                   ((static_cast<uint64_t>(seq) * a.width + row / group) * a.n_heads + kv * group +
-                                    row % group) * HD + d0;
+                uint16_t *to = a.out + place(seq, row0 + i) + d0;
+                const float inv = 1.0f / sum;
 #pragma unroll
-                    for (int d = 0; d < DT; d += 2)
-                        *reinterpret_cast<uint32_t *>(to + d) =
-                            some ? f32x2_to_bf16x2_rne(o[d] / sum, o[d + 1] / sum) : 0u;
-                }
+                for (uint32_t d = 0; d < DT; d += 2)
+                    *reinterpret_cast<uint32_t *>(to + d) =
+                        some != 0.0f ? f32x2_to_bf16x2_rne(o[d] * inv, o[d + 1] * inv) : 0u;
             } else {
-                const uint32_t i = r * 16 + h;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) rec[i * HD + d0 + d] = o[d];
+                for (uint32_t d = 0; d < DT; d += 4)
+                    *reinterpret_cast<float4 *>(rec + i * HD + d0 + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
                 if (d0 == 0) {
                     rec[16 * NT * HD + i] = top;
                     rec[16 * NT * (HD + 1) + i] = sum;
-                    rec[16 * NT * (HD + 2) + i] = some ? 1.0f : 0.0f;
+                    rec[16 * NT * (HD + 2) + i] = some;
                 }
             }
         }
         __syncthreads();  // the LDS is read: the next piece may write it
         slot = 1;
-    }
-    // rows of the tile past their sequence's nodes
-    for (uint32_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
-        const uint32_t lo = max(row0, nodes_of(a, b) * group), hi = min(row0 + 16 * NT, a.width * group);
-        for (uint32_t i = threadIdx.x; lo < hi && i < (hi - lo) * (HD / 8); i += kTreeThreads) {
-            const uint32_t row = lo + i / (HD / 8);
-            uint16_t *to = a.out +
-                           ((static_cast<uint64_t>(b) * a.width + row / group) * a.n_heads + kv * group + row % group) *
-                               HD + i % (HD / 8) * 8;
-            *reinterpret_cast<uint4 *>(to) = make_uint4(0, 0, 0, 0);
-        }
     }
 }
 
@@ -558,14 +584,14 @@ template <int HD, int NT>
 __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs a) {
     constexpr uint32_t kRow = HD / 4, kRows = kTreeThreads / kRow, kBlocks = (16 * NT + kRows - 1) / kRows;
     const uint32_t seq = blockIdx.x, lane = threadIdx.x & 63u, d = threadIdx.x % kRow * 4;
-    const uint32_t unit = blockIdx.y / kBlocks, tile = unit % a.tiles, kv = unit / a.tiles;
+    const uint32_t tile = blockIdx.y / kBlocks, kv = blockIdx.z, unit = kv * a.tiles + tile;
     const uint32_t i = blockIdx.y % kBlocks * kRows + threadIdx.x / kRow;  // the row in its tile
-    const uint32_t group = a.n_heads / a.n_kv, row0 = tile * (16 * NT), row = row0 + i;
-    const uint32_t rows = nodes_of(a, seq) * group;
-    if (row0 >= rows) return;
+    const uint32_t row0 = tile * (16 * NT), row = row0 + i;
     Layout y = layout_of(a, row0, lane);
     while (y.b0 + 64 <= seq) layout_at(a, y, y.b0 + 64, __builtin_amdgcn_readlane(y.upto, 63), lane);
     const uint32_t n = __builtin_amdgcn_readlane(y.mine, seq - y.b0);
+    if (n == 0) return;  // no row here
+    const uint32_t rows = __builtin_amdgcn_readlane(y.count, seq - y.b0) * a.group.by;
     const uint32_t start = __builtin_amdgcn_readlane(y.upto, seq - y.b0) - n;
     const uint32_t first = start / y.size, pieces = (start + n - 1) / y.size - first + 1;
     if (pieces == 1 || row >= rows || i >= 16 * NT) return;  // written by its block, or no row
@@ -607,10 +633,13 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs 
                 o.z = fmaf(v[u].z, g, o.z), o.w = fmaf(v[u].w, g, o.w);
             }
     }
+    const uint32_t node = a.group(row);
     uint16_t *to = a.out +
-                   ((static_cast<uint64_t>(seq) * a.width + row / group) * a.n_heads + kv * group + row % group) * HD + d;
-    *reinterpret_cast<uint2 *>(to) = some != 0.0f ? make_uint2(f32x2_to_bf16x2_rne(o.x / l, o.y / l),
-                                                              f32x2_to_bf16x2_rne(o.z / l, o.w / l))
+                   ((static_cast<uint64_t>(seq) * a.width + node) * a.n_heads + kv * a.group.by +
+                    (row - node * a.group.by)) * HD + d;
+    const float inv = 1.0f / l;
+    *reinterpret_cast<uint2 *>(to) = some != 0.0f ? make_uint2(f32x2_to_bf16x2_rne(o.x * inv, o.y * inv),
+                                                              f32x2_to_bf16x2_rne(o.z * inv, o.w * inv))
                                                   : make_uint2(0, 0);
 }
 
@@ -632,8 +661,8 @@ int check_shape(const char *fn, int64_t batch, int64_t width, int64_t n_heads, i
     if (width < 1 || width > kMaxTree)
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: width %lld must be 1 to %u", fn, (long long)width, kMaxTree);
     if (batch > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: batch %lld exceeds 65535", fn, (long long)batch);
-    // the joining launch's rows of blocks (16 NT * head_dim / 1024 to a tile, NT at most 4) fit its grid
-    if ((width * n_heads + 64 * n_kv) * head_dim / 1024 > 65535)
+    // rows of a KV head (below 2^27, and the joining launch's blocks of at least 4), and KV heads
+    if (width * (n_heads / n_kv) > 4 * 65535 - 64 || n_kv > 65535)
         return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld nodes of %lld heads", fn, (long long)width, (long long)n_heads);
     // the steps of all sequences are counted in 32 bits (pages may be shared, so their number bounds nothing)
     if (batch * (max_pages * page_size / kStepKeys + 1) > 0x7FFFFFFFll)
@@ -645,39 +674,39 @@ int check_shape(const char *fn, int64_t batch, int64_t width, int64_t n_heads, i
 // The launch for these sizes: 16-row groups per block, tiles of a KV head, parts per
 // (KV head, tile), or 0 for a block per sequence, and the bytes of the pieces' records.
 struct Plan {
-    uint32_t groups, tiles, want_parts, grid_parts;
+    uint32_t groups, tiles, want_parts;
     uint64_t bytes;
 };
 
 Plan plan(int64_t batch, int64_t width, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t page_size,
           int64_t max_pages) {
     const uint64_t rows = width * (n_heads / n_kv), capacity = static_cast<uint64_t>(max_pages) * page_size;
-    const uint32_t groups = rows <= 16 ? 1 : rows <= 32 || head_dim == 256 ? 2 : 4;
+    const uint32_t groups = rows <= 16 ? 1 : 2;
     const uint64_t tiles = (rows + 16 * groups - 1) / (16 * groups), units = tiles * n_kv;
-    Plan w{groups, static_cast<uint32_t>(tiles), 0, static_cast<uint32_t>(batch), 16};
+    Plan w{groups, static_cast<uint32_t>(tiles), 0, 16};
     if (capacity * head_dim <= kWholeElements) return w;
     // what serves the largest batch serves smaller ones: the bytes of those that are split
     const uint64_t split = std::min<uint64_t>(batch, kPlanBatch);
     // a block's registers leave room for two on a CU, or for one
-    const uint64_t blocks = head_dim == 256 || head_dim * groups > 384 ? 256 : 512;
+    const uint64_t blocks = head_dim == 256 ? 256 : 512;
     // a table of few steps has no use for more parts than steps
     const uint64_t steps = (capacity + kStepKeys - 1) / kStepKeys;
     const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>(blocks / units, split * steps));
     w.bytes = parts * 2 * units * (16 * groups * (head_dim + 3) * 4) + 16;
-    if (batch <= kPlanBatch) w.want_parts = w.grid_parts = static_cast<uint32_t>(parts);
+    if (batch <= kPlanBatch) w.want_parts = static_cast<uint32_t>(parts);
     return w;
 }
 
 template <int HD, int NT>
 int launch(fh_device *dev, const char *fn, const TreeArgs &a) {
-    const dim3 grid(a.grid_parts, a.n_kv * a.tiles), threads(kTreeThreads);
+    const dim3 grid(a.want_parts ? a.want_parts : a.batch, a.tiles, a.n_kv), threads(kTreeThreads);
     if (int rc = dispatch(dev, fn, [&] {
             hipLaunchKernelGGL((tree_part_kernel<HD, NT>), grid, threads, 0, dev->stream, a);
         }))
         return rc;
     if (a.want_parts <= 1) return FH_OK;
     constexpr uint32_t kRows = kTreeThreads / (HD / 4), kBlocks = (16 * NT + kRows - 1) / kRows;
-    const dim3 join(a.batch, a.n_kv * a.tiles * kBlocks);
+    const dim3 join(a.batch, a.tiles * kBlocks, a.n_kv);
     return dispatch(dev, fn, [&] {
         hipLaunchKernelGGL((tree_join_kernel<HD, NT>), join, threads, 0, dev->stream, a);
     });
@@ -760,22 +789,19 @@ extern "C" int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_
                      static_cast<uint32_t>(n_heads),
                      static_cast<uint32_t>(n_kv),
                      static_cast<uint32_t>(n_pages),
-                     static_cast<uint32_t>(page_size),
                      static_cast<uint32_t>(max_pages),
+                     static_cast<uint32_t>(max_pages * page_size),
+                     Divider(static_cast<uint32_t>(n_heads / n_kv)),
+                     Divider(static_cast<uint32_t>(page_size / 16)),
                      w.tiles,
                      w.want_parts,
-                     w.grid_parts,
                      k,
                      kSlack / k,
                      static_cast<float *>(workspace),
                      out};
     if (head_dim == 64)
-        return w.groups == 1 ? launch<64, 1>(dev, fn, a)
-                             : w.groups == 2 ? launch<64, 2>(dev, fn, a) : launch<64, 4>(dev, fn, a);
+        return w.groups == 1 ? launch<64, 1>(dev, fn, a) : launch<64, 2>(dev, fn, a);
     if (head_dim == 128)
-        return w.groups == 1   ? launch<128, 1>(dev, fn, a)
-               : w.groups == 2 ? launch<128, 2>(dev, fn, a)
-               : w.groups == 3 ? launch<128, 3>(dev, fn, a)
-                               : launch<128, 4>(dev, fn, a);
+        return w.groups == 1 ? launch<128, 1>(dev, fn, a) : launch<128, 2>(dev, fn, a);
     return w.groups == 1 ? launch<256, 1>(dev, fn, a) : launch<256, 2>(dev, fn, a);
 }
