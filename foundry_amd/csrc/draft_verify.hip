@@ -1,4 +1,6 @@
 // Which drafted tokens the target's distributions accept (fh_verify_draft).
+#include <algorithm>
+
 #include "serving_checks.hpp"
 
 namespace fh {
@@ -10,18 +12,34 @@ namespace fh {
 // max(max(p - c q, 0) - Z q, 0) = max(p - (c + Z) q, 0) for q >= 0. So a refusal costs
 // one sum over the two rows, and nothing is stored. Without the draft's
 // distribution w is p without the refused tokens, and Z one subtraction.
-constexpr uint32_t kVerifyThreads = 1024;
+//
+// The walk down the tree needs single entries of the rows, which are loaded for all
+// nodes at once, up to the first refusal that has to be summed up: at the only
+// child of its parent (a chain), that sum is of what the next token is drawn
+// from. So every block of a first launch walks that far for itself and adds up one
+// piece of the rows that count then, and only those rows are read; a second
+// launch's block per sequence goes on from there, finds the piece that the
+// token lies in and reads that. Further refusals (trees with the draft's
+// distributions) are summed by that block alone.
+constexpr uint32_t kVerifyThreads = 256;
 constexpr uint32_t kMaxWidth = 1024;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
-// Tokens that a block goes over at a time.
+// Tokens that a block goes over at a time (16 of a thread), and the shortest piece
+// of a row and the blocks that the first launch aims for before pieces get longer.
 constexpr uint32_t kVerifyTokens = 4096;
+constexpr uint32_t kLeastPiece = 1024;
+constexpr uint32_t kVerifyBlocks = 2048;
+// Pieces of a row at most.
+constexpr uint32_t kMaxPieces = 1024;
 
 struct VerifyArgs {
     const float *probs, *draft_probs;
     const uint32_t *tokens, *parents, *counts;
     const float *uniforms;
-    uint32_t batch, width, n;
+    uint32_t batch, width, n, piece, pieces;
     uint32_t *path, *out_tokens, *accepted;
+    double *sums;        // [batch][pieces] of the rows that the first launch stopped at
+    struct Walk *walks;  // [batch]
 };
 
 // The drafted nodes of one sequence, in LDS: parent (kNone for what is passed
@@ -34,6 +52,7 @@ struct Nodes {
 // Where a walk stands: at node `at`, its children up to `last` asked.
 struct Walk {
     uint32_t at, last, took;
+    uint32_t open;  // a child is left to ask, once the sum is known
     double cut, mass;
 };
 
@@ -54,22 +73,23 @@ __device__ __forceinline__ uint32_t load_nodes(const VerifyArgs &a, uint32_t b, 
     return count;
 }
 
+// The next child of w.at to ask, kNone for none.
+__device__ __forceinline__ uint32_t next_child(const Nodes &nodes, uint32_t count, const Walk &w) {
+    for (uint32_t base = (w.last + 1) & ~63u; base < count; base += 64) {
+        const uint32_t k = base + (threadIdx.x & 63u);
+        const uint64_t hit = __ballot(k > w.last && k < count && nodes.parent[min(k, count - 1)] == w.at);
+        if (hit) return base + __builtin_ctzll(hit);
+    }
+    return kNone;
+}
+
 // Goes on until a refusal needs the sum of what it leaves (true), or no child is
 // left to ask. Every wavefront of a block does the same.
 __device__ __forceinline__ bool walk(const VerifyArgs &a, Nodes &nodes, uint32_t count, Walk &w) {
 #pragma clang fp contract(off)
     const uint32_t lane = threadIdx.x & 63u;
     for (;;) {
-        // the next child of w.at
-        uint32_t i = kNone;
-        for (uint32_t base = (w.last + 1) & ~63u; base < count; base += 64) {
-            const uint32_t k = base + lane;
-            const uint64_t hit = __ballot(k > w.last && k < count && nodes.parent[min(k, count - 1)] == w.at);
-            if (hit) {
-                i = base + __builtin_ctzll(hit);
-                break;
-            }
-        }
+        const uint32_t i = next_child(nodes, count, w);
         if (i == kNone) return false;
         w.last = i;
         const double q = nodes.q[i], p = nodes.p[i];
@@ -99,20 +119,57 @@ __device__ __forceinline__ bool walk(const VerifyArgs &a, Nodes &nodes, uint32_t
     }
 }
 
-// What is left of token j: w's weight, or p's own (plain).
+// What is left of the tokens behind a node.
 struct Weights {
     const float *p, *q;  // the node's rows; q null without the draft's distribution
     double cut;
     const uint32_t *gone;  // bits of the refused tokens from `base` on, null for none
-    uint32_t base;
-    __device__ __forceinline__ double operator()(uint32_t j) const {
+    uint32_t n, base;
+    bool wide;  // rows begin at 16-byte boundaries less `before` tokens, p's and q's the same
+    uint32_t before;
+
+    __device__ __forceinline__ double of(float pj, float qj, uint32_t j) const {
 #pragma clang fp contract(off)
-        double v = p[j];
-        if (q) v = v - cut * static_cast<double>(q[j]);
+        double v = pj;
+        if (q) v = v - cut * static_cast<double>(qj);
         if (gone && gone[(j - base) / 32] >> ((j - base) % 32) & 1u) v = 0;
         return v > 0 ? v : 0;
     }
+    // The weights of tokens j0 .. j0 + 3 (0 outside the row); j0 + before is a multiple of 4.
+    __device__ __forceinline__ void four(int32_t j0, double (&w)[4]) const {
+        float x[4], y[4] = {0, 0, 0, 0};
+        if (wide && j0 >= 0 && j0 + 4 <= static_cast<int32_t>(n)) {
+            const float4 a = *reinterpret_cast<const float4 *>(p + j0);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+            if (q) {
+                const float4 b = *reinterpret_cast<const float4 *>(q + j0);
+                y[0] = b.x, y[1] = b.y, y[2] = b.z, y[3] = b.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = j0 + e >= 0 && j0 + e < static_cast<int32_t>(n);
+                x[e] = in ? p[j0 + e] : 0.0f;
+                if (q) y[e] = in ? q[j0 + e] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = j0 + e >= 0 && j0 + e < static_cast<int32_t>(n) ? of(x[e], y[e], j0 + e) : 0;
+    }
 };
+
+// The rows behind w.at.
+__device__ __forceinline__ Weights weights_of(const VerifyArgs &a, uint32_t b, const Walk &w) {
+    const uint64_t row = (static_cast<uint64_t>(b) * a.width + w.at) * a.n;
+    Weights x{};
+    x.p = a.probs + row;
+    x.q = a.draft_probs ? a.draft_probs + row : nullptr;
+    x.cut = w.cut;
+    x.n = a.n;
+    x.before = (reinterpret_cast<uintptr_t>(x.p) & 15u) / 4;
+    x.wide = !x.q || (reinterpret_cast<uintptr_t>(x.q) & 15u) / 4 == x.before;
+    return x;
+}
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
@@ -120,115 +177,230 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return v;
 }
 
-// One block per sequence: the walk, and each sum over the rows by the whole block.
-__global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const VerifyArgs a) {
+struct Scratch {
+    double part[kVerifyThreads / 64];
+    uint32_t gone[kVerifyTokens / 32];
+    uint32_t best, last;
+};
+
+// The block's sum, the same in every thread.
+__device__ __forceinline__ double block_sum(double v, Scratch &s) {
+    v = wave_sum_f64(v);
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0) s.part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+    for (uint32_t i = 0; i < kVerifyThreads / 64; ++i) v += s.part[i];
+    return v;
+}
+
+// Marks the refused children's tokens among kVerifyTokens from lo - x.before on.
+__device__ __forceinline__ void mark(Weights &x, uint32_t lo, const Nodes &nodes, uint32_t count, uint32_t at,
+                                     Scratch &s) {
+    if (!x.gone) return;
+    x.base = lo - x.before;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kVerifyTokens / 32; i += kVerifyThreads) s.gone[i] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count; i += kVerifyThreads) {
+        const uint32_t bit = nodes.token[i] - x.base;
+        if (nodes.parent[i] == at && bit < kVerifyTokens) atomicOr(&s.gone[bit / 32], 1u << (bit % 32));
+    }
+    __syncthreads();
+}
+
+// The sum of the weights of tokens lo - x.before .. hi - x.before - 1 of a row, by the block.
+__device__ __forceinline__ double sum_of(Weights &x, uint64_t lo, uint64_t hi, const Nodes &nodes, uint32_t count,
+                                         uint32_t at, Scratch &s) {
+    double sum = 0;
+    for (uint64_t base = lo; base < hi; base += kVerifyTokens) {
+        mark(x, static_cast<uint32_t>(base), nodes, count, at, s);
+        double w[4][4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint64_t j = base + (k * kVerifyThreads + threadIdx.x) * 4;
+            if (j < hi)
+                x.four(static_cast<int32_t>(j) - static_cast<int32_t>(x.before), w[k]);
+            else
+                w[k][0] = w[k][1] = w[k][2] = w[k][3] = 0;
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) sum += (w[k][0] + w[k][1]) + (w[k][2] + w[k][3]);
+    }
+    return block_sum(sum, s);
+}
+
+// Block (piece, sequence): the walk to the first sum, and this piece of it.
+__global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(const VerifyArgs a) {
     __shared__ Nodes nodes;
-    __shared__ uint32_t gone[kVerifyTokens / 32];
-    __shared__ double part[kVerifyThreads / 64];
-    __shared__ uint32_t best, lastpos;
-    const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    __shared__ Scratch scratch;
+    const uint32_t b = blockIdx.y, tid = threadIdx.x;
     const uint32_t count = load_nodes(a, b, nodes);
     const uint64_t first = static_cast<uint64_t>(b) * a.width;
     if (count == 0) {
+        if (blockIdx.x) return;
         for (uint32_t i = tid; i < a.width; i += kVerifyThreads) a.path[first + i] = a.out_tokens[first + i] = kNone;
         if (tid == 0) a.accepted[b] = 0;
         return;
     }
     if (tid == 0) nodes.path[0] = 0;
-    Walk w{0, 0, 1, 0.0, 1.0};
-    Weights weight{};
-    // marks the refused tokens among the next ones
-    auto mark = [&](uint32_t base) {
-        weight.base = base;
-        if (!weight.gone) return;
-        __syncthreads();
-        for (uint32_t i = tid; i < kVerifyTokens / 32; i += kVerifyThreads) gone[i] = 0;
-        __syncthreads();
-        for (uint32_t i = tid; i < count; i += kVerifyThreads)
-            if (nodes.parent[i] == w.at && nodes.token[i] - base < kVerifyTokens)
-                atomicOr(&gone[(nodes.token[i] - base) / 32], 1u << ((nodes.token[i] - base) % 32));
-        __syncthreads();
-    };
-    auto rows = [&] {
-        weight.p = a.probs + (first + w.at) * a.n;
-        weight.q = a.draft_probs ? a.draft_probs + (first + w.at) * a.n : nullptr;
-        weight.cut = w.cut;
-    };
+    Walk w{0, 0, 1, 0, 0.0, 1.0};
+    w.open = walk(a, nodes, count, w) && next_child(nodes, count, w) != kNone;
+    Weights x = weights_of(a, b, w);
+    if (!a.draft_probs) x.gone = scratch.gone;
+    const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * a.piece;
+    const double sum = sum_of(x, lo, min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before), nodes, count, w.at, scratch);
+    if (tid == 0) a.sums[static_cast<uint64_t>(b) * a.pieces + blockIdx.x] = sum;
+    if (blockIdx.x) return;
+    __syncthreads();
+    if (tid == 0) a.walks[b] = w, a.accepted[b] = w.took;
+    for (uint32_t i = tid; i < a.width; i += kVerifyThreads) {
+        a.path[first + i] = i < w.took ? nodes.path[i] : kNone;
+        a.out_tokens[first + i] = i + 1 < w.took ? nodes.token[nodes.path[i + 1]] : kNone;
+    }
+}
+
+// Block (sequence): what is left of the walk, and the token behind it.
+__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const VerifyArgs a) {
+    __shared__ Nodes nodes;
+    __shared__ Scratch scratch;
+    __shared__ double sums[kMaxPieces];
+    const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    const uint64_t first = static_cast<uint64_t>(b) * a.width;
+    uint32_t count = a.counts ? min(a.counts[b], a.width) : a.width;
+    if (count == 0) return;
+    Walk w = a.walks[b];
+    for (uint32_t i = tid; i < a.pieces; i += kVerifyThreads) sums[i] = a.sums[static_cast<uint64_t>(b) * a.pieces + i];
+    const double u = a.uniforms[first];
+    const uint32_t before_took = w.took;
+    // nodes: where children are left to ask, or refused tokens to leave out
+    if (w.open || !a.draft_probs) load_nodes(a, b, nodes);
+    Weights x = weights_of(a, b, w);
     auto total = [&] {
         double sum = 0;
-        for (uint32_t base = 0; base < a.n; base += kVerifyTokens) {
-            mark(base);
-            for (uint32_t j = base + tid; j < min(base + kVerifyTokens, a.n); j += kVerifyThreads) sum += weight(j);
-        }
-        sum = wave_sum_f64(sum);
         __syncthreads();
-        if (lane == 0) part[wave] = sum;
-        __syncthreads();
-        sum = 0;
-        for (uint32_t i = 0; i < kVerifyThreads / 64; ++i) sum += part[i];
-        return sum;
+        for (uint32_t i = tid; i < a.pieces; i += kVerifyThreads) sum += sums[i];
+        return block_sum(sum, scratch);
     };
-    while (walk(a, nodes, count, w)) {
-        rows();
-        w.mass = total();
-    }
-    rows();
-    if (!a.draft_probs) weight.gone = gone;
+    // the pieces' sums anew
+    auto pieces = [&] {
+        for (uint32_t i = 0; i < a.pieces; ++i) {
+            const uint64_t lo = static_cast<uint64_t>(i) * a.piece;
+            const uint64_t hi = min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before);
+            const double sum = lo < hi ? sum_of(x, lo, hi, nodes, count, w.at, scratch) : 0;
+            if (tid == 0) sums[i] = sum;
+        }
+        __syncthreads();
+    };
+    if (!a.draft_probs) x.gone = scratch.gone;
     double sum = total();
-    if (!(sum > 0)) {
-        weight.q = nullptr, weight.gone = nullptr, weight.cut = 0;
+    if (w.open) {
+        do {
+            w.mass = sum;
+            // a refusal (or no child left) has the rows at hand summed up again
+            const bool more = walk(a, nodes, count, w);
+            x = weights_of(a, b, w);
+            pieces();
+            sum = total();
+            w.open = more;
+        } while (w.open);
+        for (uint32_t i = before_took + tid; i < w.took; i += kVerifyThreads) {
+            a.path[first + i] = nodes.path[i];
+            a.out_tokens[first + i - 1] = nodes.token[nodes.path[i]];
+        }
+        if (tid == 0) a.accepted[b] = w.took;
+    }
+    if (!(sum > 0)) {  // nothing is left: p itself
+        x.q = nullptr, x.gone = nullptr, x.cut = 0;
+        pieces();
         sum = total();
     }
-    const double target = static_cast<double>(nodes.u[0]) * sum;
-    if (tid == 0) best = kNone, lastpos = 0;
-    double before = 0;
-    for (uint32_t base = 0; base < a.n; base += kVerifyTokens) {
-        mark(base);
-        constexpr uint32_t E = kVerifyTokens / kVerifyThreads;
-        double v[E], own = 0;
+    // the piece whose running sum passes the target, then the token in it
+    const double target = u * sum;
+    if (tid == 0) scratch.best = kNone, scratch.last = 0;
+    __syncthreads();
+    // finds the first of the block's values (thread by thread, E of each) whose running sum from
+    // `from` passes the target, and the last that is positive; `from` moves on
+    auto find = [&](auto &v, uint32_t base, double &from) {
+        constexpr uint32_t E = sizeof(v) / sizeof(double);
+        double own = 0;
         uint32_t any = 0;
+#pragma unroll
         for (uint32_t e = 0; e < E; ++e) {
-            const uint32_t j = base + tid * E + e;
-            v[e] = j < a.n ? weight(j) : 0;
             own += v[e];
-            if (v[e] > 0) any = j + 1;
+            if (v[e] > 0) any = base + tid * E + e + 1;
         }
         double upto = own;
+#pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const double o = __shfl_up(upto, off, 64);
             if (lane >= static_cast<uint32_t>(off)) upto += o;
         }
         __syncthreads();
-        if (lane == 63) part[wave] = upto;
-        if (any) atomicMax(&lastpos, any);
+        if (lane == 63) scratch.part[wave] = upto;
+        if (any) atomicMax(&scratch.last, any);
         __syncthreads();
-        double at = before + (upto - own);
+        double at = from + (upto - own);
         for (uint32_t i = 0; i < kVerifyThreads / 64; ++i) {
-            if (i < wave) at += part[i];
-            before += part[i];
+            if (i < wave) at += scratch.part[i];
+            from += scratch.part[i];
         }
+#pragma unroll
         for (uint32_t e = 0; e < E; ++e) {
             at += v[e];
             if (v[e] > 0 && at > target) {
-                atomicMin(&best, base + tid * E + e);
+                atomicMin(&scratch.best, base + tid * E + e);
                 break;
             }
         }
         __syncthreads();
-        if (best != kNone) break;
+    };
+    double from = 0;
+    for (uint32_t base = 0; base < a.pieces && scratch.best == kNone; base += kVerifyThreads) {
+        double v[1] = {base + tid < a.pieces ? sums[base + tid] : 0.0};
+        find(v, base, from);
     }
-    // rounding may leave the last running sum at the target
-    const uint32_t next = best != kNone ? best : lastpos - 1;
-    for (uint32_t i = tid; i < a.width; i += kVerifyThreads) {
-        a.path[first + i] = i < w.took ? nodes.path[i] : kNone;
-        a.out_tokens[first + i] = i + 1 < w.took ? nodes.token[nodes.path[i + 1]] : i + 1 == w.took ? next : kNone;
+    // (rounding may leave the last running sum at the target: the last piece and token with a weight)
+    const uint32_t piece = scratch.best != kNone ? scratch.best : scratch.last - 1;
+    uint32_t next = kNone;
+    if (piece != kNone) {
+        from = 0;
+        for (uint32_t i = 0; i < piece; ++i) from += sums[i];
+        __syncthreads();
+        if (tid == 0) scratch.best = kNone, scratch.last = 0;
+        __syncthreads();
+        const uint64_t lo = static_cast<uint64_t>(piece) * a.piece;
+        const uint64_t hi = min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before);
+        for (uint64_t base = lo; base < hi && scratch.best == kNone; base += kVerifyThreads * 4) {
+            // (a piece of 4 tokens to a thread; marked tokens reach as far)
+            mark(x, static_cast<uint32_t>(base), nodes, count, w.at, scratch);
+            double v[4] = {0, 0, 0, 0};
+            if (base + tid * 4 < hi) x.four(static_cast<int32_t>(base + tid * 4) - static_cast<int32_t>(x.before), v);
+            find(v, static_cast<uint32_t>(base), from);
+        }
+        next = (scratch.best != kNone ? scratch.best : scratch.last - 1) - x.before;
+        if (scratch.best == kNone && scratch.last == 0) next = kNone;
     }
-    if (tid == 0) a.accepted[b] = w.took;
+    if (tid == 0) a.out_tokens[first + w.took - 1] = next;
 }
 
 }  // namespace fh
 
 using namespace fh;
+
+namespace {
+
+// Tokens of a row's piece for these sizes, and pieces of a row (which may begin up to three tokens before it).
+uint32_t piece_of(int64_t batch, int64_t n) {
+    uint64_t piece = kLeastPiece;
+    while (piece < kVerifyTokens && batch * ((n + piece - 1) / piece) > kVerifyBlocks) piece *= 2;
+    while ((n + 3 + piece - 1) / piece > kMaxPieces) piece *= 2;
+    return static_cast<uint32_t>(piece);
+}
+
+uint64_t pieces_of(int64_t n, uint32_t piece) { return (static_cast<uint64_t>(n) + 3 + piece - 1) / piece; }
+
+}  // namespace
 
 extern "C" int fh_verify_draft_workspace(int64_t batch, int64_t width, int64_t n, uint64_t *bytes) {
     const char *fn = "fh_verify_draft_workspace";
@@ -239,7 +411,9 @@ extern "C" int fh_verify_draft_workspace(int64_t batch, int64_t width, int64_t n
     if (batch > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: batch %lld exceeds 65535", fn, (long long)batch);
     if (n < 1 || n > 0x7FFFFFFFll - kVerifyTokens)
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: n %lld", fn, (long long)n);
-    *bytes = 16;
+    // pieces get longer where there are more than kVerifyBlocks of them, not counting a row's last four tokens
+    *bytes = static_cast<uint64_t>(batch) * sizeof(Walk) + 16 +
+             std::max<uint64_t>(kVerifyBlocks + kMaxPieces + batch, batch * pieces_of(n, piece_of(65535, n))) * 8;
     return FH_OK;
 }
 
@@ -291,6 +465,7 @@ extern "C" int fh_verify_draft(fh_device *dev, const float *probs, const float *
                 if (int rc = refuse_overlap(fn, o.what, o.ptr, o.bytes, i.what, i.ptr, i.bytes)) return rc;
     }
     if (int rc = set_current(dev, fn)) return rc;
+    const uint32_t piece = piece_of(batch, n);
     const VerifyArgs a{probs,
                        draft_probs,
                        tokens,
@@ -300,10 +475,19 @@ extern "C" int fh_verify_draft(fh_device *dev, const float *probs, const float *
                        static_cast<uint32_t>(batch),
                        static_cast<uint32_t>(width),
                        static_cast<uint32_t>(n),
+                       piece,
+                       static_cast<uint32_t>(pieces_of(n, piece)),
                        path,
                        out_tokens,
-                       accepted};
+                       accepted,
+                       reinterpret_cast<double *>(static_cast<char *>(workspace) + batch * sizeof(Walk)),
+                       static_cast<Walk *>(workspace)};
+    const dim3 grid(a.pieces, a.batch), threads(kVerifyThreads);
+    if (int rc = dispatch(dev, fn, [&] {
+            hipLaunchKernelGGL(verify_walk_kernel, grid, threads, 0, dev->stream, a);
+        }))
+        return rc;
     return dispatch(dev, fn, [&] {
-        hipLaunchKernelGGL(verify_kernel, dim3(static_cast<uint32_t>(batch)), dim3(kVerifyThreads), 0, dev->stream, a);
+        hipLaunchKernelGGL(verify_draw_kernel, dim3(a.batch), threads, 0, dev->stream, a);
     });
 }

@@ -1,82 +1,257 @@
 // Distributions of logits at a temperature (fh_logits_probs).
+#include <algorithm>
 #include <tuple>
-#include <type_traits>
 
 #include "serving_checks.hpp"
 
 namespace fh {
 
-// p_j = 2^((z_j - max z) log2 e / t) / sum. One block per row, which it reads three
-// times: for the maximum (and, for a greedy row, its first place), the sum, and p.
-constexpr uint32_t kProbThreads = 1024;
+// p_j = 2^((z_j - max z) k) / sum, k = log2 e / t. Bound by memory: the logits are
+// read, the probabilities written. A row is cut into runs of tokens: one launch
+// takes each run's maximum and its sum relative to that (and a greedy row's first
+// largest token), the next joins a row's runs, reads the logits again, from the
+// caches where they hold them, and writes. Runs are as long as a filled GPU allows.
+constexpr uint32_t kProbTokens = 8192;
+constexpr uint32_t kProbThreads = 256;
+// The shortest run, and the blocks that a launch aims for before runs get longer.
+constexpr uint32_t kProbLeast = 1024;
+constexpr uint32_t kProbBlocks = 2048;
+
+struct RunStats {
+    float m, sum;
+    uint32_t first;  // the first token of logit m
+};
 
 template <typename T>
-__device__ __forceinline__ float logit(const T *z, uint32_t j) {
-    float v;
-    if constexpr (sizeof(T) == 2)
-        v = bf(z[j]);
-    else
-        v = z[j];
-    return fmaxf(v, -INFINITY);  // a NaN counts as -inf
+struct ProbArgs {
+    const T *z;
+    uint32_t n, run;
+    const float *temperatures;
+    RunStats *stats;  // [rows][runs]
+    float *probs;
+};
+
+// A piece's logits, NaN as -inf.
+template <typename T, uint32_t E>
+__device__ __forceinline__ void logits_of(const uint4 raw, float (&v)[E]) {
+    if constexpr (sizeof(T) == 2) {
+        unpack8(raw, v);
+    } else {
+        v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y);
+        v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) v[e] = fmaxf(v[e], -INFINITY);
 }
 
 template <typename T>
-__global__ __launch_bounds__(kProbThreads) void probs_kernel(const T *__restrict__ z, uint32_t n,
-                                                             const float *__restrict__ temperatures,
-                                                             float *__restrict__ probs) {
+__device__ __forceinline__ float logit_of(T z) {
+    if constexpr (sizeof(T) == 2)
+        return fmaxf(bf(z), -INFINITY);
+    else
+        return fmaxf(z, -INFINITY);
+}
+
+__device__ __forceinline__ float factor_of(float t) { return 1.4426950408889634f / fminf(fmaxf(t, 1e-30f), 1e30f); }
+
+// The weight of v beside a largest logit m > -inf; infinite logits all weigh 1.
+__device__ __forceinline__ float weight_of(float v, float m, float k) {
+    return v == m ? 1.0f : __builtin_amdgcn_exp2f((v - m) * k);
+}
+
+// What a block has of its run: whole pieces of 16 bytes (a row's first may begin before it), the
+// row's ends left to single tokens.
+template <typename T>
+struct Run {
+    static constexpr uint32_t E = 16 / sizeof(T), kPieces = kProbTokens / (kProbThreads * E);
+    const T *from;
+    int32_t lo;  // the run's first token (below 0 where the first piece begins before the row)
+    uint32_t n, run;
+    __device__ __forceinline__ Run(const ProbArgs<T> &a, uint32_t x, uint32_t row) : n(a.n), run(a.run) {
+        from = a.z + static_cast<uint64_t>(row) * n;
+        lo = static_cast<int32_t>(x * run) - static_cast<int32_t>((reinterpret_cast<uintptr_t>(from) & 15u) / sizeof(T));
+    }
+    // token of the thread's piece p, and whether it is whole
+    __device__ __forceinline__ int32_t token(uint32_t p) const {
+        return lo + static_cast<int32_t>((p * kProbThreads + threadIdx.x) * E);
+    }
+    __device__ __forceinline__ bool inside(uint32_t p) const {
+        return (p * kProbThreads + threadIdx.x) * E < run && token(p) < static_cast<int32_t>(n);
+    }
+    __device__ __forceinline__ bool whole(uint32_t p) const {
+        return inside(p) && token(p) >= 0 && token(p) + E <= n;
+    }
+    // the logits of piece p, -inf outside the row
+    __device__ __forceinline__ void get(uint32_t p, const uint4 raw, float (&v)[E]) const {
+        if (whole(p)) {
+            logits_of<T, E>(raw, v);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < E; ++e) {
+                const int32_t j = token(p) + static_cast<int32_t>(e);
+                v[e] = inside(p) && j >= 0 && j < static_cast<int32_t>(n) ? logit_of<T>(from[j]) : -INFINITY;
+            }
+        }
+    }
+};
+
+// Block (run, row).
+template <typename T>
+__global__ __launch_bounds__(kProbThreads) void prob_stats_kernel(const ProbArgs<T> a) {
+    using R = Run<T>;
     __shared__ float part[kProbThreads / 64];
     __shared__ uint32_t first;
-    const T *row = z + static_cast<uint64_t>(blockIdx.x) * n;
-    float *to = probs + static_cast<uint64_t>(blockIdx.x) * n;
+    const R r(a, blockIdx.x, blockIdx.y);
+    uint4 raw[R::kPieces];
+#pragma unroll
+    for (uint32_t p = 0; p < R::kPieces; ++p)
+        if (r.whole(p)) raw[p] = *reinterpret_cast<const uint4 *>(r.from + r.token(p));
+    const float t = a.temperatures ? a.temperatures[blockIdx.y] : 1.0f;
     const uint32_t wave = threadIdx.x / 64;
     float m = -INFINITY;
-    for (uint32_t j = threadIdx.x; j < n; j += kProbThreads) m = fmaxf(m, logit(row, j));
+    float v[R::kPieces][R::E];
+#pragma unroll
+    for (uint32_t p = 0; p < R::kPieces; ++p) {
+        r.get(p, raw[p], v[p]);
+#pragma unroll
+        for (uint32_t e = 0; e < R::E; ++e) m = fmaxf(m, v[p][e]);
+    }
     m = wave_max(m);
     if (threadIdx.x % 64 == 0) part[wave] = m;
-    if (threadIdx.x == 0) first = n;
+    if (threadIdx.x == 0) first = a.n;
     __syncthreads();
+#pragma unroll
     for (uint32_t w = 0; w < kProbThreads / 64; ++w) m = fmaxf(m, part[w]);
     __syncthreads();
-    const float t = temperatures ? temperatures[blockIdx.x] : 1.0f;
-    if (m == -INFINITY) {
-        for (uint32_t j = threadIdx.x; j < n; j += kProbThreads) to[j] = 0.0f;
-        return;
-    }
-    if (!(t > 0.0f)) {
-        for (uint32_t j = threadIdx.x; j < n; j += kProbThreads)
-            if (logit(row, j) == m) {
-                atomicMin(&first, j);
-                break;
-            }
-        __syncthreads();
-        for (uint32_t j = threadIdx.x; j < n; j += kProbThreads) to[j] = j == first ? 1.0f : 0.0f;
-        return;
-    }
-    const float k = 1.4426950408889634f / fminf(fmaxf(t, 1e-30f), 1e30f);
-    auto weight = [&](uint32_t j) {
-        const float v = logit(row, j);
-        return v == m ? 1.0f : __builtin_amdgcn_exp2f((v - m) * k);
-    };
     float sum = 0.0f;
-    for (uint32_t j = threadIdx.x; j < n; j += kProbThreads) sum += weight(j);
-    sum = wave_sum(sum);
-    if (threadIdx.x % 64 == 0) part[wave] = sum;
+    if (!(t > 0.0f)) {  // greedy
+#pragma unroll
+        for (uint32_t p = 0; p < R::kPieces; ++p)
+#pragma unroll
+            for (uint32_t e = 0; e < R::E; ++e) {
+                const int32_t j = r.token(p) + static_cast<int32_t>(e);
+                if (v[p][e] == m && r.inside(p) && j >= 0 && j < static_cast<int32_t>(a.n))
+                    atomicMin(&first, static_cast<uint32_t>(j));
+            }
+    } else if (m > -INFINITY) {
+        const float k = factor_of(t);
+#pragma unroll
+        for (uint32_t p = 0; p < R::kPieces; ++p) {
+            float s = 0.0f;
+#pragma unroll
+            for (uint32_t e = 0; e < R::E; ++e) s += weight_of(v[p][e], m, k);
+            sum += s;
+        }
+        sum = wave_sum(sum);
+        if (threadIdx.x % 64 == 0) part[wave] = sum;
+    }
     __syncthreads();
-    sum = 0.0f;
-    for (uint32_t w = 0; w < kProbThreads / 64; ++w) sum += part[w];
-    for (uint32_t j = threadIdx.x; j < n; j += kProbThreads) to[j] = weight(j) / sum;
+    if (threadIdx.x == 0) {
+        sum = 0.0f;
+        if (t > 0.0f && m > -INFINITY)
+            for (uint32_t w = 0; w < kProbThreads / 64; ++w) sum += part[w];
+        a.stats[static_cast<uint64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = {m, sum, first};
+    }
+}
+
+// Block (run, row): every wavefront joins the row's runs, 64 at a time.
+template <typename T>
+__global__ __launch_bounds__(kProbThreads) void prob_write_kernel(const ProbArgs<T> a) {
+    using R = Run<T>;
+    const R r(a, blockIdx.x, blockIdx.y);
+    if (r.lo >= static_cast<int32_t>(a.n)) return;
+    uint4 raw[R::kPieces];
+#pragma unroll
+    for (uint32_t p = 0; p < R::kPieces; ++p)
+        if (r.whole(p)) raw[p] = *reinterpret_cast<const uint4 *>(r.from + r.token(p));
+    const float t = a.temperatures ? a.temperatures[blockIdx.y] : 1.0f;
+    const float k = factor_of(t);
+    const RunStats *stats = a.stats + static_cast<uint64_t>(blockIdx.y) * gridDim.x;
+    const uint32_t lane = threadIdx.x % 64;
+    float m = -INFINITY, sum = 0.0f;
+    uint32_t first = a.n;
+    for (uint32_t i = lane; i < gridDim.x; i += 64) {
+        const RunStats x = stats[i];
+        if (x.m > m) {  // the first run of the largest maximum
+            sum = x.sum + sum * weight_of(m, x.m, k);
+            m = x.m, first = x.first;
+        } else if (x.m > -INFINITY) {
+            sum += x.sum * weight_of(x.m, m, k);
+        }
+    }
+    const float top = wave_max(m);
+    sum = wave_sum(m > -INFINITY ? sum * weight_of(m, top, k) : 0.0f);
+    if (m != top) first = a.n;
+#pragma unroll
+    for (int off = 32; off; off >>= 1) first = min(first, static_cast<uint32_t>(__shfl_xor(first, off, 64)));
+    const bool greedy = !(t > 0.0f), none = top == -INFINITY;
+    const float inv = 1.0f / sum;
+    float *to = a.probs + static_cast<uint64_t>(blockIdx.y) * a.n;
+    const bool aligned = (reinterpret_cast<uintptr_t>(to + r.lo) & 15u) == 0;
+#pragma unroll
+    for (uint32_t p = 0; p < R::kPieces; ++p) {
+        if (!r.inside(p)) break;
+        const int32_t j0 = r.token(p);
+        float v[R::E];
+        r.get(p, raw[p], v);
+#pragma unroll
+        for (uint32_t e = 0; e < R::E; ++e) {
+            const float w = greedy ? (j0 + static_cast<int32_t>(e) == static_cast<int32_t>(first) ? 1.0f : 0.0f)
+                                   : weight_of(v[e], top, k) * inv;
+            v[e] = none ? 0.0f : w;
+        }
+        if (aligned && r.whole(p)) {
+#pragma unroll
+            for (uint32_t e = 0; e < R::E; e += 4)
+                __builtin_nontemporal_store(
+                    __builtin_bit_cast(stream_u32x4_t, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3])),
+                    reinterpret_cast<stream_u32x4_t *>(to + j0 + e));
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < R::E; ++e) {
+                const int32_t j = j0 + static_cast<int32_t>(e);
+                if (j >= 0 && j < static_cast<int32_t>(a.n)) to[j] = v[e];
+            }
+        }
+    }
 }
 
 }  // namespace fh
 
 using namespace fh;
 
+namespace {
+
+// Tokens of a run for these sizes, and runs of a row (one may begin up to a piece before it).
+uint32_t run_of(int64_t rows, int64_t n) {
+    uint32_t run = kProbLeast;
+    while (run < kProbTokens && rows * ((n + run - 1) / run) > kProbBlocks) run *= 2;
+    return run;
+}
+
+uint64_t runs_of(int64_t n, uint32_t run) { return (static_cast<uint64_t>(n) + 7 + run - 1) / run; }
+
+template <typename T>
+int launch(fh_device *dev, const char *fn, const dim3 grid, const ProbArgs<T> &a) {
+    if (int rc = dispatch(dev, fn, [&] {
+            hipLaunchKernelGGL(prob_stats_kernel<T>, grid, dim3(kProbThreads), 0, dev->stream, a);
+        }))
+        return rc;
+    return dispatch(dev, fn, [&] {
+        hipLaunchKernelGGL(prob_write_kernel<T>, grid, dim3(kProbThreads), 0, dev->stream, a);
+    });
+}
+
+}  // namespace
+
 extern "C" int fh_logits_probs_workspace(int64_t rows, int64_t n, uint64_t *bytes) {
     const char *fn = "fh_logits_probs_workspace";
     if (bytes == nullptr) return fail(FH_ERR_INVALID_ARGUMENT, "%s: bytes is null", fn);
     if (int rc = fh_check_dims(fn, {rows, n})) return rc;
     if (rows > 65535) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld rows exceed 65535", fn, (long long)rows);
-    *bytes = 16;
+    if (n > 0x7FFFFFFFll - 2 * kProbTokens) return fail(FH_ERR_INDEX_TOO_LARGE, "%s: n %lld", fn, (long long)n);
+    // runs get longer where there are more than kProbBlocks of them, not counting a row's last piece
+    *bytes = std::max<uint64_t>(kProbBlocks + rows, rows * runs_of(n, kProbTokens)) * sizeof(RunStats) + 16;
     return FH_OK;
 }
 
@@ -111,13 +286,14 @@ extern "C" int fh_logits_probs(fh_device *dev, const void *logits, int dtype, in
     }
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "probs", probs, count * 4)) return rc;
     if (int rc = set_current(dev, fn)) return rc;
-    const dim3 grid(static_cast<uint32_t>(rows)), threads(kProbThreads);
-    return dispatch(dev, fn, [&] {
-        if (dtype == FH_F32)
-            hipLaunchKernelGGL(probs_kernel<float>, grid, threads, 0, dev->stream, static_cast<const float *>(logits),
-                               static_cast<uint32_t>(n), temperatures, probs);
-        else
-            hipLaunchKernelGGL(probs_kernel<uint16_t>, grid, threads, 0, dev->stream,
-                               static_cast<const uint16_t *>(logits), static_cast<uint32_t>(n), temperatures, probs);
-    });
+    const uint32_t run = run_of(rows, n);
+    const dim3 grid(static_cast<uint32_t>(runs_of(n, run)), static_cast<uint32_t>(rows));
+    RunStats *stats = static_cast<RunStats *>(workspace);
+    if (dtype == FH_F32)
+        return launch(dev, fn, grid,
+                      ProbArgs<float>{static_cast<const float *>(logits), static_cast<uint32_t>(n), run, temperatures,
+                                      stats, probs});
+    return launch(dev, fn, grid,
+                  ProbArgs<uint16_t>{static_cast<const uint16_t *>(logits), static_cast<uint32_t>(n), run, temperatures,
+                                     stats, probs});
 }

@@ -200,7 +200,13 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
         float o[kWaves][16 * NT][HD + 4];
         float ml[kWaves][3][16 * NT];
     };
-    __shared__ __attribute__((aligned(16))) Results part;
+    // The tile's q as fragments [KC][NT][64 lanes], read for every 32 keys (registers are short), and
+    // after them the wavefronts' results.
+    __shared__ union {
+        ta_u32x4_t q[KC * NT * 64];
+        Results results;
+    } shared;
+    Results &part = shared.results;
     constexpr uint32_t kWords = kMaxTree / 32;
     __shared__ uint32_t bits[(16 * NT + 1) * kWords];  // the mask words of the tile's nodes
     // (the wavefront's number as a scalar: its loops then count in scalars too)
@@ -268,17 +274,14 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
             return w;
         };
         uint32_t first_where = places(0);
-        // the lane's rows (behind the last one: that again, left out at the end)
-        ta_u32x4_t qf[NT][KC];
+        // the tile's rows (behind the last one: that again, left out at the end)
+        for (uint32_t i = anew(threadIdx.x); i < KC * NT * 64; i += kTreeThreads) {
+            const uint32_t row = min(row0 + i / 64 % NT * 16 + i % 16, rows - 1);
+            shared.q[i] = *reinterpret_cast<const ta_u32x4_t *>(a.q + place(seq, row) + i / (64 * NT) * 32 + i / 16 % 4 * 8);
+        }
         uint32_t node[NT];
 #pragma unroll
-        for (int r = 0; r < NT; ++r) {
-            const uint32_t row = min(row0 + r * 16 + c, rows - 1);
-            node[r] = a.group(row) - node0;
-            const uint16_t *qrow = a.q + place(seq, row) + q * 8;
-#pragma unroll
-            for (int s = 0; s < KC; ++s) qf[r][s] = *reinterpret_cast<const ta_u32x4_t *>(qrow + s * 32);
-        }
+        for (int r = 0; r < NT; ++r) node[r] = a.group(min(row0 + r * 16 + c, rows - 1)) - node0;
         if ((first + steps) * kStepKeys > len) {
             const uint32_t tid = anew(threadIdx.x), w = tid % kWords;
             const uint32_t nodes = a.group(min(row0 + 16 * NT, rows) - 1) - node0 + 1;
@@ -310,9 +313,9 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                 m[r] = -INFINITY, l[r] = 0.0f, any[r] = 0;
             }
             if (n_tiles) {
-                uint32_t where = first_where, next_where = places(32);
+                uint32_t even = first_where, odd = 0;  // the places of 32 tiles each, in turn
                 // a tile's two groups; a missing one reads the pool's first group, whose scores are left out
-                uint32_t g0 = __builtin_amdgcn_readlane(where, 0), g1 = __builtin_amdgcn_readlane(where, 1);
+                uint32_t g0 = __builtin_amdgcn_readlane(even, 0), g1 = __builtin_amdgcn_readlane(even, 1);
                 ta_u32x4_t kf[2][KC];
                 ta_u32x4_t vf[8][VP];
                 auto start_of = [&](uint32_t g) { return static_cast<uint64_t>(g == ~0u ? 0u : g) * (16 * HD); };
@@ -345,19 +348,22 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                     }
                 };
                 ta_f32x4_t s0[NT], s1[NT];
-                auto scores = [&] {
+                auto scores = [&](ta_f32x4_t(&x0)[NT], ta_f32x4_t(&x1)[NT]) {
+                    const ta_u32x4_t *qf = shared.q + anew(lane);
 #pragma unroll
-                    for (int r = 0; r < NT; ++r) s0[r] = s1[r] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int r = 0; r < NT; ++r) x0[r] = x1[r] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int s = 0; s < KC; ++s)
 #pragma unroll
                         for (int r = 0; r < NT; ++r) {
-                            s0[r] = ta_mfma(kf[0][s], qf[r][s], s0[r]);
-                            s1[r] = ta_mfma(kf[1][s], qf[r][s], s1[r]);
+                            const ta_u32x4_t f = qf[(s * NT + r) * 64];
+                            x0[r] = ta_mfma(kf[0][s], f, x0[r]);
+                            x1[r] = ta_mfma(kf[1][s], f, x1[r]);
                         }
                 };
                 ta_u32x4_t hi[NT], lo[NT];
-                auto weigh = [&](uint32_t key0) {
+                // the scores at hand: what no row sees goes, and the references follow
+                auto limit = [&](uint32_t key0) {
                     if (key0 + 32 > len || g0 == ~0u || g1 == ~0u) {
                         const uint32_t there = (g0 != ~0u ? 0xFFFFu : 0u) | (g1 != ~0u ? 0xFFFF0000u : 0u), q = anew(lane) >> 4;
                         // keys behind the last or of no page: no value, whatever lies there
@@ -403,6 +409,8 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                             m[r] = top[r];
                         }
                     }
+                };
+                auto weigh = [&] {
 #pragma unroll
                     for (int r = 0; r < NT; ++r) {
                         const float ref = m[r] == -INFINITY ? 0.0f : m[r];
@@ -479,26 +487,42 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                         for (int r = 0; r < NT; ++r) acc[r][t] = ta_mfma(f, lo[r], acc[r][t]);
                     }
                 };
-                // each tile's keys are in flight behind the values before them (behind the last: that tile
-                // again; a load that may not be there would have the values wait for all of them)
+                // The next tile's scores are formed on the matrix cores while this one's weights are; its
+                // keys are two tiles ahead, its values one. (Behind the last: that tile again; a load that
+                // may not be there would have the values wait for all of them.)
+                auto groups = [&](uint32_t t, uint32_t &x0, uint32_t &x1) {
+                    t = min(t, n_tiles - 1);
+                    x0 = __builtin_amdgcn_readlane(t / 32 % 2 ? odd : even, t % 32 * 2);
+                    x1 = __builtin_amdgcn_readlane(t / 32 % 2 ? odd : even, t % 32 * 2 + 1);
+                };
+                uint32_t n0, n1;
+                groups(1, n0, n1);
                 load_k(g0, g1);
+                scores(s0, s1);
+                load_k(n0, n1);
                 load_v(g0, g1);
 #pragma unroll 1
                 for (uint32_t t = 0; t < n_tiles; ++t) {
-                    scores();
-                    const uint32_t next = min(t + 1, n_tiles - 1);
-                    if (next / 32 != t / 32) {
-                        where = next_where;
-                        next_where = places(next + 32);
+                    limit(from + t * 32);
+                    if (t % 32 == 8) (t / 32 % 2 ? even : odd) = places((t / 32 + 1) * 32);
+                    weigh();
+                    ta_f32x4_t x0[NT], x1[NT];
+                    scores(x0, x1);
+#pragma unroll
+                    for (int i = 0; i < KC * NT; ++i) {  // a fragment, its two products, and weights meanwhile
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 16, 0);
                     }
-                    const uint32_t n0 = __builtin_amdgcn_readlane(where, next % 32 * 2);
-                    const uint32_t n1 = __builtin_amdgcn_readlane(where, next % 32 * 2 + 1);
-                    load_k(n0, n1);
-                    weigh(from + t * 32);
+                    uint32_t f0, f1;
+                    groups(t + 2, f0, f1);
+                    load_k(f0, f1);
                     if (careful) special(from + t * 32);
                     values();
                     load_v(n0, n1);
-                    g0 = n0, g1 = n1;
+#pragma unroll
+                    for (int r = 0; r < NT; ++r) s0[r] = x0[r], s1[r] = x1[r];
+                    g0 = n0, g1 = n1, n0 = f0, n1 = f1;
                 }
             }
             float zero = 0.0f;  // NaN if a sum is not finite
@@ -512,6 +536,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
         }
 
         // the four wavefronts joined: thread (row, dims), 16 rows at a time
+        __syncthreads();  // q is read
 #pragma unroll
         for (int r = 0; r < NT; ++r) {
             l[r] += __shfl_xor(l[r], 16, 64);
