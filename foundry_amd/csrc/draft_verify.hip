@@ -181,6 +181,7 @@ struct Scratch {
     double part[kVerifyThreads / 64];
     uint32_t gone[kVerifyTokens / 32];
     uint32_t best, last;
+    double from;  // the running sum before the best one's thread
 };
 
 // The block's sum, the same in every thread.
@@ -240,7 +241,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(const Verif
     if (count == 0) {
         if (blockIdx.x) return;
         for (uint32_t i = tid; i < a.width; i += kVerifyThreads) a.path[first + i] = a.out_tokens[first + i] = kNone;
-        if (tid == 0) a.accepted[b] = 0;
+        if (tid == 0) a.accepted[b] = 0, a.walks[b] = Walk{0, 0, 0, 0, 0.0, 0.0};
         return;
     }
     if (tid == 0) nodes.path[0] = 0;
@@ -267,14 +268,14 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
     __shared__ double sums[kMaxPieces];
     const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint64_t first = static_cast<uint64_t>(b) * a.width;
-    uint32_t count = a.counts ? min(a.counts[b], a.width) : a.width;
-    if (count == 0) return;
     Walk w = a.walks[b];
-    for (uint32_t i = tid; i < a.pieces; i += kVerifyThreads) sums[i] = a.sums[static_cast<uint64_t>(b) * a.pieces + i];
     const double u = a.uniforms[first];
+    if (w.took == 0) return;  // no node
+    for (uint32_t i = tid; i < a.pieces; i += kVerifyThreads) sums[i] = a.sums[static_cast<uint64_t>(b) * a.pieces + i];
     const uint32_t before_took = w.took;
     // nodes: where children are left to ask, or refused tokens to leave out
-    if (w.open || !a.draft_probs) load_nodes(a, b, nodes);
+    uint32_t count = 0;
+    if (w.open || !a.draft_probs) count = load_nodes(a, b, nodes);
     Weights x = weights_of(a, b, w);
     auto total = [&] {
         double sum = 0;
@@ -345,15 +346,16 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
             if (i < wave) at += scratch.part[i];
             from += scratch.part[i];
         }
+        const double start = at;
+        uint32_t mine = kNone;
 #pragma unroll
         for (uint32_t e = 0; e < E; ++e) {
             at += v[e];
-            if (v[e] > 0 && at > target) {
-                atomicMin(&scratch.best, base + tid * E + e);
-                break;
-            }
+            if (v[e] > 0 && at > target && mine == kNone) mine = base + tid * E + e;
         }
+        if (mine != kNone) atomicMin(&scratch.best, mine);
         __syncthreads();
+        if (mine != kNone && mine == scratch.best) scratch.from = start;
     };
     double from = 0;
     for (uint32_t base = 0; base < a.pieces && scratch.best == kNone; base += kVerifyThreads) {
@@ -361,21 +363,26 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
         find(v, base, from);
     }
     // (rounding may leave the last running sum at the target: the last piece and token with a weight)
+    __syncthreads();
     const uint32_t piece = scratch.best != kNone ? scratch.best : scratch.last - 1;
     uint32_t next = kNone;
     if (piece != kNone) {
-        from = 0;
-        for (uint32_t i = 0; i < piece; ++i) from += sums[i];
+        from = scratch.best != kNone ? scratch.from : from - sums[piece];
         __syncthreads();
         if (tid == 0) scratch.best = kNone, scratch.last = 0;
         __syncthreads();
         const uint64_t lo = static_cast<uint64_t>(piece) * a.piece;
         const uint64_t hi = min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before);
-        for (uint64_t base = lo; base < hi && scratch.best == kNone; base += kVerifyThreads * 4) {
-            // (a piece of 4 tokens to a thread; marked tokens reach as far)
+        for (uint64_t base = lo; base < hi && scratch.best == kNone; base += kVerifyTokens) {
             mark(x, static_cast<uint32_t>(base), nodes, count, w.at, scratch);
-            double v[4] = {0, 0, 0, 0};
-            if (base + tid * 4 < hi) x.four(static_cast<int32_t>(base + tid * 4) - static_cast<int32_t>(x.before), v);
+            double v[16];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {  // 16 tokens in a row
+                double w4[4] = {0, 0, 0, 0};
+                const uint64_t j = base + tid * 16 + k * 4;
+                if (j < hi) x.four(static_cast<int32_t>(j) - static_cast<int32_t>(x.before), w4);
+                v[k * 4] = w4[0], v[k * 4 + 1] = w4[1], v[k * 4 + 2] = w4[2], v[k * 4 + 3] = w4[3];
+            }
             find(v, static_cast<uint32_t>(base), from);
         }
         next = (scratch.best != kNone ? scratch.best : scratch.last - 1) - x.before;

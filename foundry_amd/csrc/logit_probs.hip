@@ -1,6 +1,7 @@
 // Distributions of logits at a temperature (fh_logits_probs).
 #include <algorithm>
 #include <tuple>
+#include <type_traits>
 
 #include "serving_checks.hpp"
 
@@ -31,17 +32,20 @@ struct ProbArgs {
     float *probs;
 };
 
+__device__ __forceinline__ uint32_t word_of(const uint4 raw, uint32_t i) {
+    return i == 0 ? raw.x : i == 1 ? raw.y : i == 2 ? raw.z : raw.w;
+}
+__device__ __forceinline__ uint32_t word_of(const uint2 raw, uint32_t i) { return i == 0 ? raw.x : raw.y; }
+
 // A piece's logits, NaN as -inf.
-template <typename T, uint32_t E>
-__device__ __forceinline__ void logits_of(const uint4 raw, float (&v)[E]) {
-    if constexpr (sizeof(T) == 2) {
-        unpack8(raw, v);
-    } else {
-        v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y);
-        v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
-    }
+template <typename T, uint32_t E, typename Raw>
+__device__ __forceinline__ void logits_of(const Raw raw, float (&v)[E]) {
 #pragma unroll
-    for (uint32_t e = 0; e < E; ++e) v[e] = fmaxf(v[e], -INFINITY);
+    for (uint32_t e = 0; e < E; ++e) {
+        const uint32_t word = word_of(raw, e * sizeof(T) / 4);
+        v[e] = __uint_as_float(sizeof(T) == 4 ? word : e % 2 ? word & 0xFFFF0000u : word << 16);
+        v[e] = fmaxf(v[e], -INFINITY);
+    }
 }
 
 template <typename T>
@@ -59,11 +63,13 @@ __device__ __forceinline__ float weight_of(float v, float m, float k) {
     return v == m ? 1.0f : __builtin_amdgcn_exp2f((v - m) * k);
 }
 
-// What a block has of its run: whole pieces of 16 bytes (a row's first may begin before it), the
+// What a block has of its run: whole pieces of E tokens (a row's first may begin before it), the
 // row's ends left to single tokens.
-template <typename T>
+template <typename T, uint32_t Tokens>
 struct Run {
-    static constexpr uint32_t E = 16 / sizeof(T), kPieces = kProbTokens / (kProbThreads * E);
+    static constexpr uint32_t E = Tokens, kPieces = kProbTokens / (kProbThreads * E);
+    typedef std::conditional_t<E * sizeof(T) == 16, uint4, uint2> Raw;
+    __device__ __forceinline__ Raw load(uint32_t p) const { return *reinterpret_cast<const Raw *>(from + token(p)); }
     const T *from;
     int32_t lo;  // the run's first token (below 0 where the first piece begins before the row)
     uint32_t n, run;
@@ -82,7 +88,7 @@ struct Run {
         return inside(p) && token(p) >= 0 && token(p) + E <= n;
     }
     // the logits of piece p, -inf outside the row
-    __device__ __forceinline__ void get(uint32_t p, const uint4 raw, float (&v)[E]) const {
+    __device__ __forceinline__ void get(uint32_t p, const Raw raw, float (&v)[E]) const {
         if (whole(p)) {
             logits_of<T, E>(raw, v);
         } else {
@@ -98,14 +104,14 @@ struct Run {
 // Block (run, row).
 template <typename T>
 __global__ __launch_bounds__(kProbThreads) void prob_stats_kernel(const ProbArgs<T> a) {
-    using R = Run<T>;
+    using R = Run<T, 16 / sizeof(T)>;  // loads of 16 bytes
     __shared__ float part[kProbThreads / 64];
     __shared__ uint32_t first;
     const R r(a, blockIdx.x, blockIdx.y);
-    uint4 raw[R::kPieces];
+    typename R::Raw raw[R::kPieces];
 #pragma unroll
     for (uint32_t p = 0; p < R::kPieces; ++p)
-        if (r.whole(p)) raw[p] = *reinterpret_cast<const uint4 *>(r.from + r.token(p));
+        if (r.whole(p)) raw[p] = r.load(p);
     const float t = a.temperatures ? a.temperatures[blockIdx.y] : 1.0f;
     const uint32_t wave = threadIdx.x / 64;
     float m = -INFINITY;
@@ -157,13 +163,13 @@ __global__ __launch_bounds__(kProbThreads) void prob_stats_kernel(const ProbArgs
 // Block (run, row): every wavefront joins the row's runs, 64 at a time.
 template <typename T>
 __global__ __launch_bounds__(kProbThreads) void prob_write_kernel(const ProbArgs<T> a) {
-    using R = Run<T>;
+    using R = Run<T, 4>;  // stores of 16 bytes, next to each other
     const R r(a, blockIdx.x, blockIdx.y);
     if (r.lo >= static_cast<int32_t>(a.n)) return;
-    uint4 raw[R::kPieces];
+    typename R::Raw raw[R::kPieces];
 #pragma unroll
     for (uint32_t p = 0; p < R::kPieces; ++p)
-        if (r.whole(p)) raw[p] = *reinterpret_cast<const uint4 *>(r.from + r.token(p));
+        if (r.whole(p)) raw[p] = r.load(p);
     const float t = a.temperatures ? a.temperatures[blockIdx.y] : 1.0f;
     const float k = factor_of(t);
     const RunStats *stats = a.stats + static_cast<uint64_t>(blockIdx.y) * gridDim.x;
@@ -201,11 +207,8 @@ __global__ __launch_bounds__(kProbThreads) void prob_write_kernel(const ProbArgs
             v[e] = none ? 0.0f : w;
         }
         if (aligned && r.whole(p)) {
-#pragma unroll
-            for (uint32_t e = 0; e < R::E; e += 4)
-                __builtin_nontemporal_store(
-                    __builtin_bit_cast(stream_u32x4_t, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3])),
-                    reinterpret_cast<stream_u32x4_t *>(to + j0 + e));
+            __builtin_nontemporal_store(__builtin_bit_cast(stream_u32x4_t, make_float4(v[0], v[1], v[2], v[3])),
+                                        reinterpret_cast<stream_u32x4_t *>(to + j0));
         } else {
 #pragma unroll
             for (uint32_t e = 0; e < R::E; ++e) {

@@ -217,52 +217,52 @@ struct CompactArgs {
 
 constexpr uint32_t kMoves = 8;
 
-// Block (sequence, layer, K or V). A thread moves its pieces of a head for one
-// path entry after the other, kMoves of them loaded before any is stored: no entry's
+// Block (sequence, layer, K or V). A thread moves its pieces of heads for one path
+// entry after the other, kMoves of them loaded before any is stored: no entry's
 // source is a place that an earlier entry's goes to, since path[i] >= i rises.
 __global__ __launch_bounds__(256) void compact_kernel(const PageArgs a, const CompactArgs c, const PoolArgs p) {
-    __shared__ uint64_t from[kMoves], to[kMoves];  // places of the pool's rows, ~0 for none
+    __shared__ uint64_t rows[2][kMoves];  // where a source and its place begin in the pool, ~0 for none
     const uint32_t s = blockIdx.x, tid = threadIdx.x;
-    const uint32_t len = a.lengths[s], count = min(c.accepted[s], c.width);
     const bool keys = blockIdx.z == 0;
-    if (c.new_lengths && blockIdx.y == 0 && keys && tid == 0) c.new_lengths[s] = len + count;
     uint16_t *pool = keys ? p.pools[blockIdx.y].k_pages : p.pools[blockIdx.y].v_pages;
     const uint64_t capacity = static_cast<uint64_t>(a.max_pages) * a.page_size;
     const uint64_t region = static_cast<uint64_t>(a.page_size) * p.head_dim;
     const uint32_t pieces = p.head_dim / 8;
-    auto place = [&](uint64_t j) {
-        if (j >= capacity) return ~0ull;
-        const uint32_t page = a.table[static_cast<uint64_t>(s) * a.max_pages + j / a.page_size];
-        if (page >= a.n_pages) return ~0ull;
-        const uint32_t slot = j % a.page_size;
-        return static_cast<unsigned long long>(static_cast<uint64_t>(page) * p.n_kv * region +
-                                               (keys ? k_offset(slot, 0, a.page_size, p.head_dim)
-                                                     : static_cast<uint64_t>(slot) * p.head_dim));
-    };
     const uint32_t *path = c.path + static_cast<uint64_t>(s) * c.width;
+    // threads 2 u and 2 u + 1 look up move u; its node is read before the count is known
+    const uint32_t u = tid / 2, to = tid % 2;
+    uint32_t node = u < min(kMoves, c.width) ? path[u] : 0;
+    const uint32_t len = a.lengths[s], count = min(c.accepted[s], c.width);
+    if (c.new_lengths && blockIdx.y == 0 && keys && tid == 0) c.new_lengths[s] = len + count;
     for (uint32_t i0 = 0; i0 < count; i0 += kMoves) {
-        __syncthreads();
-        if (tid < kMoves) {
-            const uint32_t i = i0 + tid;
-            const bool moves = i < count && path[i] != i;
-            const uint64_t f = moves ? place(static_cast<uint64_t>(len) + path[i]) : ~0ull;
-            const uint64_t t = moves ? place(static_cast<uint64_t>(len) + i) : ~0ull;
-            from[tid] = t == ~0ull ? t : f;
-            to[tid] = f == ~0ull ? f : t;
+        if (u < kMoves) {
+            const uint32_t i = i0 + u;
+            if (i0) node = i < count ? path[i] : i;
+            const uint64_t j = static_cast<uint64_t>(len) + (to ? i : node);
+            uint32_t page = kNoPage;
+            if (i < count && node != i && j < capacity)
+                page = a.table[static_cast<uint64_t>(s) * a.max_pages + j / a.page_size];
+            const uint32_t other = __shfl_xor(page, 1, 64);
+            const bool there = page < a.n_pages && other < a.n_pages;
+            const uint32_t slot = j % a.page_size;
+            rows[to][u] = there ? page * p.n_kv * region + (keys ? k_offset(slot, 0, a.page_size, p.head_dim)
+                                                                 : static_cast<uint64_t>(slot) * p.head_dim)
+                                : ~0ull;
         }
         __syncthreads();
         for (uint32_t x = tid; x < p.n_kv * pieces; x += blockDim.x) {
             const uint32_t d = x % pieces * 8;
             // a group's keys lie 32 dims apart: dim d of a K row is (d / 32) * 512 + d % 32 further on
-            const uint64_t at = x / pieces * region + (keys ? (d / 32) * 512 + d % 32 : d);
-            uint4 v[kMoves];
+            uint16_t *mine = pool + x / pieces * region + (keys ? (d / 32) * 512 + d % 32 : d);
+            stream_u32x4_t v[kMoves];
 #pragma unroll
-            for (uint32_t u = 0; u < kMoves; ++u)
-                if (from[u] != ~0ull) v[u] = *reinterpret_cast<const uint4 *>(pool + from[u] + at);
+            for (uint32_t m = 0; m < kMoves; ++m)
+                if (rows[0][m] != ~0ull) v[m] = *reinterpret_cast<const stream_u32x4_t *>(mine + rows[0][m]);
 #pragma unroll
-            for (uint32_t u = 0; u < kMoves; ++u)
-                if (to[u] != ~0ull) *reinterpret_cast<uint4 *>(pool + to[u] + at) = v[u];
+            for (uint32_t m = 0; m < kMoves; ++m)
+                if (rows[1][m] != ~0ull) *reinterpret_cast<stream_u32x4_t *>(mine + rows[1][m]) = v[m];
         }
+        __syncthreads();
     }
 }
 
@@ -436,8 +436,10 @@ extern "C" int fh_paged_compact(fh_device *dev, const fh_paged_cache *cache, con
                              &a, &p))
         return rc;
     const CompactArgs c{path, accepted, static_cast<uint32_t>(width), in_place ? nullptr : new_lengths};
+    // a thread for each piece of a token's heads
+    const uint32_t threads = std::min(256u, (p.n_kv * (p.head_dim / 8) + 63) / 64 * 64);
     if (int rc = dispatch(dev, fn, [&] {
-            hipLaunchKernelGGL(compact_kernel, dim3(a.n_seqs, static_cast<uint32_t>(cache->n_layers), 2), dim3(256), 0,
+            hipLaunchKernelGGL(compact_kernel, dim3(a.n_seqs, static_cast<uint32_t>(cache->n_layers), 2), dim3(threads), 0,
                                dev->stream, a, c, p);
         }))
         return rc;
