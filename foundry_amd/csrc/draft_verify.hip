@@ -180,8 +180,10 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 struct Scratch {
     double part[kVerifyThreads / 64];
     uint32_t gone[kVerifyTokens / 32];
-    uint32_t best, last;
-    double from;  // the running sum before the best one's thread
+    // of each wavefront: its first value past the target, the running sum before that
+    // value's thread, and its last positive value
+    uint32_t first[kVerifyThreads / 64], last[kVerifyThreads / 64];
+    double from[kVerifyThreads / 64];
 };
 
 // The block's sum, the same in every thread.
@@ -318,11 +320,13 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
     }
     // the piece whose running sum passes the target, then the token in it
     const double target = u * sum;
-    if (tid == 0) scratch.best = kNone, scratch.last = 0;
-    __syncthreads();
-    // finds the first of the block's values (thread by thread, E of each) whose running sum from
-    // `from` passes the target, and the last that is positive; `from` moves on
-    auto find = [&](auto &v, uint32_t base, double &from) {
+    // best: the first of the block's values (thread by thread, E of each) whose running sum from
+    // `from` passes the target, kNone if none does; last: one more than the last that is positive.
+    // `from` moves on, to the running sum before best's thread once there is one. The wavefronts'
+    // results are picked by ballots: atomics of 256 threads on one place took 4 us.
+    uint32_t best = kNone, last = 0;
+    double from = 0;
+    auto find = [&](auto &v, uint32_t base) {
         constexpr uint32_t E = sizeof(v) / sizeof(double);
         double own = 0;
         uint32_t any = 0;
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
         }
         __syncthreads();
         if (lane == 63) scratch.part[wave] = upto;
-        if (any) atomicMax(&scratch.last, any);
+        if (lane == 0) scratch.first[wave] = kNone, scratch.last[wave] = 0;
         __syncthreads();
         double at = from + (upto - own);
         for (uint32_t i = 0; i < kVerifyThreads / 64; ++i) {
@@ -353,27 +357,28 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
             at += v[e];
             if (v[e] > 0 && at > target && mine == kNone) mine = base + tid * E + e;
         }
-        if (mine != kNone) atomicMin(&scratch.best, mine);
+        const uint64_t past = __ballot(mine != kNone), some = __ballot(any != 0);
+        if (past && lane == __builtin_ctzll(past)) scratch.first[wave] = mine, scratch.from[wave] = start;
+        if (some && lane == 63u - __builtin_clzll(some)) scratch.last[wave] = any;
         __syncthreads();
-        if (mine != kNone && mine == scratch.best) scratch.from = start;
+        for (uint32_t i = kVerifyThreads / 64; i-- > 0;) {
+            if (scratch.first[i] != kNone) best = scratch.first[i], from = scratch.from[i];
+            last = max(last, scratch.last[i]);
+        }
     };
-    double from = 0;
-    for (uint32_t base = 0; base < a.pieces && scratch.best == kNone; base += kVerifyThreads) {
+    for (uint32_t base = 0; base < a.pieces && best == kNone; base += kVerifyThreads) {
         double v[1] = {base + tid < a.pieces ? sums[base + tid] : 0.0};
-        find(v, base, from);
+        find(v, base);
     }
     // (rounding may leave the last running sum at the target: the last piece and token with a weight)
-    __syncthreads();
-    const uint32_t piece = scratch.best != kNone ? scratch.best : scratch.last - 1;
+    const uint32_t piece = best != kNone ? best : last - 1;
     uint32_t next = kNone;
     if (piece != kNone) {
-        from = scratch.best != kNone ? scratch.from : from - sums[piece];
-        __syncthreads();
-        if (tid == 0) scratch.best = kNone, scratch.last = 0;
-        __syncthreads();
+        if (best == kNone) from -= sums[piece];
+        best = kNone, last = 0;
         const uint64_t lo = static_cast<uint64_t>(piece) * a.piece;
         const uint64_t hi = min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before);
-        for (uint64_t base = lo; base < hi && scratch.best == kNone; base += kVerifyTokens) {
+        for (uint64_t base = lo; base < hi && best == kNone; base += kVerifyTokens) {
             mark(x, static_cast<uint32_t>(base), nodes, count, w.at, scratch);
             double v[16];
 #pragma unroll
@@ -383,10 +388,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
                 if (j < hi) x.four(static_cast<int32_t>(j) - static_cast<int32_t>(x.before), w4);
                 v[k * 4] = w4[0], v[k * 4 + 1] = w4[1], v[k * 4 + 2] = w4[2], v[k * 4 + 3] = w4[3];
             }
-            find(v, static_cast<uint32_t>(base), from);
+            find(v, static_cast<uint32_t>(base));
         }
-        next = (scratch.best != kNone ? scratch.best : scratch.last - 1) - x.before;
-        if (scratch.best == kNone && scratch.last == 0) next = kNone;
+        if (best != kNone || last) next = (best != kNone ? best : last - 1) - x.before;
     }
     if (tid == 0) a.out_tokens[first + w.took - 1] = next;
 }
