@@ -44,9 +44,17 @@ struct VerifyArgs {
 
 // The drafted nodes of one sequence, in LDS: parent (kNone for what is passed
 // over), token, and the token's p and q at the parent.
+// The launch gives it room for `width` of them: 64 take 1.5 KB, the most 24 KB, which
+// let only six blocks onto a CU.
 struct Nodes {
-    uint32_t parent[kMaxWidth], token[kMaxWidth], path[kMaxWidth];
-    float p[kMaxWidth], q[kMaxWidth], u[kMaxWidth];
+    uint32_t *parent, *token, *path;
+    float *p, *q, *u;
+    __device__ __forceinline__ explicit Nodes(uint32_t width) {
+        extern __shared__ uint32_t room[];
+        parent = room, token = room + width, path = room + 2 * width;
+        p = reinterpret_cast<float *>(room + 3 * width), q = p + width, u = q + width;
+    }
+    static uint32_t bytes(uint32_t width) { return 24 * width; }
 };
 
 // Where a walk stands: at node `at`, its children up to `last` asked.
@@ -235,7 +243,7 @@ __device__ __forceinline__ double sum_of(Weights &x, uint64_t lo, uint64_t hi, c
 
 // Block (piece, sequence): the walk to the first sum, and this piece of it.
 __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(const VerifyArgs a) {
-    __shared__ Nodes nodes;
+    Nodes nodes(a.width);
     __shared__ Scratch scratch;
     const uint32_t b = blockIdx.y, tid = threadIdx.x;
     const uint32_t count = load_nodes(a, b, nodes);
@@ -265,7 +273,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(const Verif
 
 // Block (sequence): what is left of the walk, and the token behind it.
 __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const VerifyArgs a) {
-    __shared__ Nodes nodes;
+    Nodes nodes(a.width);
     __shared__ Scratch scratch;
     __shared__ double sums[kMaxPieces];
     const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
@@ -495,10 +503,10 @@ extern "C" int fh_verify_draft(fh_device *dev, const float *probs, const float *
                        static_cast<Walk *>(workspace)};
     const dim3 grid(a.pieces, a.batch), threads(kVerifyThreads);
     if (int rc = dispatch(dev, fn, [&] {
-            hipLaunchKernelGGL(verify_walk_kernel, grid, threads, 0, dev->stream, a);
+            hipLaunchKernelGGL(verify_walk_kernel, grid, threads, Nodes::bytes(a.width), dev->stream, a);
         }))
         return rc;
     return dispatch(dev, fn, [&] {
-        hipLaunchKernelGGL(verify_draw_kernel, dim3(a.batch), threads, 0, dev->stream, a);
+        hipLaunchKernelGGL(verify_draw_kernel, dim3(a.batch), threads, Nodes::bytes(a.width), dev->stream, a);
     });
 }
