@@ -9,9 +9,10 @@ namespace fh {
 
 // The mathematics: one pass over the keys with the running reference m, sum l and
 // weighted values o of each row (a node's query head),
-//   l' = l 2^((m - m') k) + 2^((s - m') k), o' = o 2^((m - m') k) + 2^((s - m') k) v,
-// k = scale log2 e, joined over disjoint key ranges by the same rule. m follows the
-// largest score only where that has grown by more than kSlack in the exponent, so
+//   l' = l 2^(m k - m' k) + 2^(s k - m' k), o' = o 2^(m k - m' k) + 2^(s k - m' k) v,
+// k = scale log2 e, joined over disjoint key ranges by the same rule. m k is rounded
+// once, the same way wherever it stands, so that its rounding is no weight's. m follows
+// the largest score only where that has grown by more than kSlack in the exponent, so
 // that o is seldom multiplied; the weights are then up to 2^kSlack, which fp32 sums
 // and 16-bit factors hold as well as those up to 1.
 //
@@ -159,6 +160,13 @@ __device__ __forceinline__ uint32_t sequence_of(const TreeArgs &a, Layout &y, ui
 template <int HD, int NT>
 constexpr uint32_t record_floats() { return 16 * NT * (HD + 3); }
 
+// The exponent of reference a's weights beside reference b > -inf, for products too large for fp32 too.
+__device__ __forceinline__ float apart(float a, float b, float k) {
+#pragma clang fp contract(off)
+    const float x = a * k, y = b * k;
+    return fabsf(y) < INFINITY && x < INFINITY ? x - y : (a - b) * k;
+}
+
 // Which of the 32 keys from key0 on a node of these mask words sees, as far as
 // lengths and masks go.
 __device__ __forceinline__ uint32_t window(const uint32_t *mask, uint32_t words, uint32_t key0, uint32_t len,
@@ -301,7 +309,8 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
         ta_f32x4_t acc[NT][VT];
         float m[NT], l[NT];
         uint32_t any[NT];
-        // Once as above. Where that leaves a sum that is not finite, again with care: keys that have an
+        // Once as above. Where that leaves a sum that is not finite, or m k is not, again with care: scores
+        // whose products with k are too large are taken relative to m first, and keys that have an
         // inf or NaN among their values stay out of the products, where weights of 0 (a row that does not
         // see the key, a P that lost nothing) would make NaN of them, and are added row by row.
 #pragma unroll 1
@@ -348,20 +357,35 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                     }
                 };
                 ta_f32x4_t s0[NT], s1[NT];
+                // half of the tile's q: requested before the weights are formed, and the other half while
+                // the products of the first are
+                ta_u32x4_t qf[KC / 2 * NT];
+                auto load_q = [&](int s) {
+                    const ta_u32x4_t *src = shared.q + anew(lane);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) qf[s % (KC / 2) * NT + i] = src[(s * NT + i) * 64];
+                };
+                auto load_first_q = [&] {
+#pragma unroll
+                    for (int s = 0; s < KC / 2; ++s) load_q(s);
+                    __builtin_amdgcn_sched_barrier(0);
+                };
                 auto scores = [&](ta_f32x4_t(&x0)[NT], ta_f32x4_t(&x1)[NT]) {
-                    const ta_u32x4_t *qf = shared.q + anew(lane);
 #pragma unroll
                     for (int r = 0; r < NT; ++r) x0[r] = x1[r] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int s = 0; s < KC; ++s)
+                    for (int s = 0; s < KC; ++s) {
 #pragma unroll
                         for (int r = 0; r < NT; ++r) {
-                            const ta_u32x4_t f = qf[(s * NT + r) * 64];
+                            const ta_u32x4_t f = qf[s % (KC / 2) * NT + r];
                             x0[r] = ta_mfma(kf[0][s], f, x0[r]);
                             x1[r] = ta_mfma(kf[1][s], f, x1[r]);
                         }
+                        if (s < KC / 2) load_q(s + KC / 2);
+                    }
                 };
                 ta_u32x4_t hi[NT], lo[NT];
+                float ref[NT];  // m k, as far as there is one
                 // the scores at hand: what no row sees goes, and the references follow
                 auto limit = [&](uint32_t key0) {
                     if (key0 + 32 > len || g0 == ~0u || g1 == ~0u) {
@@ -402,23 +426,32 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                     if (__any(grown)) {
 #pragma unroll
                         for (int r = 0; r < NT; ++r) {
-                            const float keep = top[r] == m[r] ? 1.0f : __builtin_amdgcn_exp2f((m[r] - top[r]) * a.k);
+                            const float keep = top[r] == m[r] ? 1.0f : __builtin_amdgcn_exp2f(apart(m[r], top[r], a.k));
                             l[r] *= keep;
 #pragma unroll
                             for (int t = 0; t < VT; ++t) acc[r][t] *= keep;
                             m[r] = top[r];
                         }
                     }
+#pragma unroll
+                    for (int r = 0; r < NT; ++r) {
+                        ref[r] = m[r] == -INFINITY ? 0.0f : m[r] * a.k;
+                        if (careful) {
+                            const bool big = !(fabsf(ref[r]) < INFINITY);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s0[r][i] -= big ? m[r] : 0.0f, s1[r][i] -= big ? m[r] : 0.0f;
+                            ref[r] = big ? 0.0f : ref[r];
+                        }
+                    }
                 };
                 auto weigh = [&] {
 #pragma unroll
                     for (int r = 0; r < NT; ++r) {
-                        const float ref = m[r] == -INFINITY ? 0.0f : m[r];
                         float p[8];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            p[i] = __builtin_amdgcn_exp2f((s0[r][i] - ref) * a.k);
-                            p[4 + i] = __builtin_amdgcn_exp2f((s1[r][i] - ref) * a.k);
+                            p[i] = __builtin_amdgcn_exp2f(fmaf(s0[r][i], a.k, -ref[r]));
+                            p[4 + i] = __builtin_amdgcn_exp2f(fmaf(s1[r][i], a.k, -ref[r]));
                         }
                         l[r] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
                         uint32_t wh[4], wl[4];
@@ -498,6 +531,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                 uint32_t n0, n1;
                 groups(1, n0, n1);
                 load_k(g0, g1);
+                load_first_q();
                 scores(s0, s1);
                 load_k(n0, n1);
                 load_v(g0, g1);
@@ -505,15 +539,10 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                 for (uint32_t t = 0; t < n_tiles; ++t) {
                     limit(from + t * 32);
                     if (t % 32 == 8) (t / 32 % 2 ? even : odd) = places((t / 32 + 1) * 32);
+                    load_first_q();
                     weigh();
                     ta_f32x4_t x0[NT], x1[NT];
                     scores(x0, x1);
-#pragma unroll
-                    for (int i = 0; i < KC * NT; ++i) {  // a fragment, its two products, and weights meanwhile
-                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 16, 0);
-                    }
                     uint32_t f0, f1;
                     groups(t + 2, f0, f1);
                     load_k(f0, f1);
@@ -527,11 +556,13 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
             }
             float zero = 0.0f;  // NaN if a sum is not finite
 #pragma unroll
-            for (int r = 0; r < NT; ++r)
+            for (int r = 0; r < NT; ++r) {
+                zero = fmaf(m[r] == -INFINITY ? 0.0f : m[r] * a.k, 0.0f, zero);
 #pragma unroll
                 for (int t = 0; t < VT; ++t)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) zero = fmaf(acc[r][t][x], 0.0f, zero);
+            }
             if (careful || !__any(zero != 0.0f)) break;
         }
 
@@ -573,7 +604,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
             for (uint32_t d = 0; d < DT; ++d) o[d] = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f((part.ml[w][0][i] - ref) * a.k);
+                const float f = __builtin_amdgcn_exp2f(apart(part.ml[w][0][i], ref, a.k));
                 sum = fmaf(f, part.ml[w][1][i], sum);
 #pragma unroll
                 for (uint32_t d = 0; d < DT; ++d) o[d] = fmaf(f, part.o[w][i][d0 + d], o[d]);
@@ -645,13 +676,13 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs 
             if (p0 + u >= pieces) pm[u] = -INFINITY;
             next = fmaxf(next, pm[u]);
         }
-        const float ref = next == -INFINITY ? 0.0f : next, f = __builtin_amdgcn_exp2f((m - ref) * a.k);
+        const float ref = next == -INFINITY ? 0.0f : next, f = __builtin_amdgcn_exp2f(apart(m, ref, a.k));
         m = next;
         l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
 #pragma unroll
         for (int u = 0; u < kJoinLoads; ++u)
             if (p0 + u < pieces) {
-                const float g = __builtin_amdgcn_exp2f((pm[u] - ref) * a.k);
+                const float g = __builtin_amdgcn_exp2f(apart(pm[u], ref, a.k));
                 some = fmaxf(some, ps[u]);
                 l = fmaf(pl[u], g, l);
                 o.x = fmaf(v[u].x, g, o.x), o.y = fmaf(v[u].y, g, o.y);
