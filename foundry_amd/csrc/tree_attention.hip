@@ -160,6 +160,17 @@ __device__ __forceinline__ uint32_t sequence_of(const TreeArgs &a, Layout &y, ui
 template <int HD, int NT>
 constexpr uint32_t record_floats() { return 16 * NT * (HD + 3); }
 
+// p less one half of a word of two bf16, as a product of the word with (-1, 0) or (0, -1). Exact where
+// the half is p's rounding.
+template <int H>
+__device__ __forceinline__ float less_half(float p, uint32_t two) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+    uint32_t unit = H ? 0xBF800000u : 0x0000BF80u;
+    asm("" : "+s"(unit));  // in a register: written as the constant -1.0 it would stand in the upper half
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), __builtin_bit_cast(bf16x2_t, unit), p,
+                                           false);
+}
+
 // The exponent of reference a's weights beside reference b > -inf, for products too large for fp32 too.
 __device__ __forceinline__ float apart(float a, float b, float k) {
 #pragma clang fp contract(off)
@@ -307,7 +318,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
         };
         __syncthreads();
         ta_f32x4_t acc[NT][VT];
-        float m[NT], l[NT];
+        float m[NT], ref[NT], l[NT];  // ref: m k, as far as there is one
         uint32_t any[NT];
         // Once as above. Where that leaves a sum that is not finite, or m k is not, again with care: scores
         // whose products with k are too large are taken relative to m first, and keys that have an
@@ -319,7 +330,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
             for (int r = 0; r < NT; ++r) {
 #pragma unroll
                 for (int t = 0; t < VT; ++t) acc[r][t] = ta_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-                m[r] = -INFINITY, l[r] = 0.0f, any[r] = 0;
+                m[r] = -INFINITY, ref[r] = 0.0f, l[r] = 0.0f, any[r] = 0;
             }
             if (n_tiles) {
                 uint32_t even = first_where, odd = 0;  // the places of 32 tiles each, in turn
@@ -385,7 +396,6 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                     }
                 };
                 ta_u32x4_t hi[NT], lo[NT];
-                float ref[NT];  // m k, as far as there is one
                 // the scores at hand: what no row sees goes, and the references follow
                 auto limit = [&](uint32_t key0) {
                     if (key0 + 32 > len || g0 == ~0u || g1 == ~0u) {
@@ -417,30 +427,30 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
 #pragma unroll
                     for (int r = 0; r < NT; ++r) {
                         const ta_f32x4_t x = s0[r], z = s1[r];
-                        top[r] = max_over_quarters(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                                         fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]))));
-                        // m = -inf: any score at all
-                        top[r] = top[r] > (m[r] == -INFINITY ? m[r] : m[r] + a.slack) ? top[r] : m[r];
-                        grown = grown || top[r] != m[r];
+                        top[r] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                       fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
+                        grown = grown || top[r] > m[r] + a.slack;  // m = -inf: any score at all
                     }
                     if (__any(grown)) {
 #pragma unroll
                         for (int r = 0; r < NT; ++r) {
+                            top[r] = max_over_quarters(top[r]);
+                            top[r] = top[r] > m[r] + a.slack ? top[r] : m[r];
                             const float keep = top[r] == m[r] ? 1.0f : __builtin_amdgcn_exp2f(apart(m[r], top[r], a.k));
                             l[r] *= keep;
 #pragma unroll
                             for (int t = 0; t < VT; ++t) acc[r][t] *= keep;
                             m[r] = top[r];
+                            ref[r] = m[r] == -INFINITY ? 0.0f : m[r] * a.k;
                         }
                     }
+                    if (careful) {
 #pragma unroll
-                    for (int r = 0; r < NT; ++r) {
-                        ref[r] = m[r] == -INFINITY ? 0.0f : m[r] * a.k;
-                        if (careful) {
-                            const bool big = !(fabsf(ref[r]) < INFINITY);
+                        for (int r = 0; r < NT; ++r) {
+                            const bool big = m[r] > -INFINITY && !(fabsf(m[r] * a.k) < INFINITY);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) s0[r][i] -= big ? m[r] : 0.0f, s1[r][i] -= big ? m[r] : 0.0f;
-                            ref[r] = big ? 0.0f : ref[r];
+                            if (big) ref[r] = 0.0f;
                         }
                     }
                 };
@@ -459,8 +469,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                         for (int i = 0; i < 4; ++i) {
                             wh[i] = f32x2_to_bf16x2_rne(p[2 * i], p[2 * i + 1]);
                             asm("" : "+v"(wh[i]));  // both halves from this one conversion
-                            wl[i] = f32x2_to_bf16x2_rne(p[2 * i] - __uint_as_float(wh[i] << 16),
-                                                        p[2 * i + 1] - __uint_as_float(wh[i] & 0xFFFF0000u));
+                            wl[i] = f32x2_to_bf16x2_rne(less_half<0>(p[2 * i], wh[i]), less_half<1>(p[2 * i + 1], wh[i]));
                         }
                         hi[r] = ta_u32x4_t{wh[0], wh[1], wh[2], wh[3]};
                         lo[r] = ta_u32x4_t{wl[0], wl[1], wl[2], wl[3]};
