@@ -22,9 +22,10 @@ namespace fh {
 // token lies in and reads that. Further refusals (trees with the draft's
 // distributions) are summed by that block alone.
 constexpr uint32_t kVerifyThreads = 256;
+constexpr uint32_t kWavesMost = 16;  // of a block that goes on with a walk
 constexpr uint32_t kMaxWidth = 1024;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
-// Tokens that a block goes over at a time (16 of a thread), and the shortest piece
+// Tokens that a block goes over at a time, and the shortest piece
 // of a row and the blocks that the first launch aims for before pieces get longer.
 constexpr uint32_t kVerifyTokens = 4096;
 constexpr uint32_t kLeastPiece = 1024;
@@ -164,6 +165,34 @@ struct Weights {
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = j0 + e >= 0 && j0 + e < static_cast<int32_t>(n) ? of(x[e], y[e], j0 + e) : 0;
     }
+    // The sum of K times four tokens' weights, j0 + 256 k on, up to token hi. Where the
+    // wavefront's are all whole, with every load on its way before the first is used.
+    template <uint32_t K>
+    __device__ __forceinline__ double sum(int32_t j0, int32_t hi, bool all_whole) const {
+        double all = 0;
+        if (wide && all_whole) {
+            float4 x[K], y[K];
+#pragma unroll
+            for (uint32_t k = 0; k < K; ++k) {
+                x[k] = *reinterpret_cast<const float4 *>(p + j0 + k * 256);
+                y[k] = q ? *reinterpret_cast<const float4 *>(q + j0 + k * 256) : make_float4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < K; ++k) {
+                const uint32_t j = j0 + k * 256;
+                all += (of(x[k].x, y[k].x, j) + of(x[k].y, y[k].y, j + 1)) +
+                       (of(x[k].z, y[k].z, j + 2) + of(x[k].w, y[k].w, j + 3));
+            }
+        } else {
+            for (uint32_t k = 0; k < K; ++k) {
+                const int32_t j = j0 + static_cast<int32_t>(k) * 256;
+                double w[4] = {0, 0, 0, 0};
+                if (j < hi) four(j, w);
+                all += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+        }
+        return all;
+    }
 };
 
 // The rows behind w.at.
@@ -186,22 +215,23 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 }
 
 struct Scratch {
-    double part[kVerifyThreads / 64];
+    static constexpr uint32_t kWaves = kVerifyThreads / 64;
+    double part[kWavesMost];
     uint32_t gone[kVerifyTokens / 32];
     // of each wavefront: its first value past the target, the running sum before that
     // value's thread, and its last positive value
-    uint32_t first[kVerifyThreads / 64], last[kVerifyThreads / 64];
-    double from[kVerifyThreads / 64];
+    uint32_t first[kWaves], last[kWaves];
+    double from[kWaves];
 };
 
 // The block's sum, the same in every thread.
-__device__ __forceinline__ double block_sum(double v, Scratch &s) {
+__device__ __forceinline__ double block_sum(double v, Scratch &s, uint32_t waves) {
     v = wave_sum_f64(v);
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) s.part[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
-    for (uint32_t i = 0; i < kVerifyThreads / 64; ++i) v += s.part[i];
+    for (uint32_t i = 0; i < waves; ++i) v += s.part[i];
     return v;
 }
 
@@ -220,25 +250,17 @@ __device__ __forceinline__ void mark(Weights &x, uint32_t lo, const Nodes &nodes
     __syncthreads();
 }
 
-// The sum of the weights of tokens lo - x.before .. hi - x.before - 1 of a row, by the block.
-__device__ __forceinline__ double sum_of(Weights &x, uint64_t lo, uint64_t hi, const Nodes &nodes, uint32_t count,
-                                         uint32_t at, Scratch &s) {
+// The sum of the weights of tokens lo - x.before .. hi - x.before - 1 of a row by a wavefront, where
+// none is marked. hi is at most n + x.before.
+__device__ __forceinline__ double wave_sum_of(const Weights &x, uint64_t lo, uint64_t hi) {
+    constexpr uint32_t K = 4;
     double sum = 0;
-    for (uint64_t base = lo; base < hi; base += kVerifyTokens) {
-        mark(x, static_cast<uint32_t>(base), nodes, count, at, s);
-        double w[4][4];
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            const uint64_t j = base + (k * kVerifyThreads + threadIdx.x) * 4;
-            if (j < hi)
-                x.four(static_cast<int32_t>(j) - static_cast<int32_t>(x.before), w[k]);
-            else
-                w[k][0] = w[k][1] = w[k][2] = w[k][3] = 0;
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) sum += (w[k][0] + w[k][1]) + (w[k][2] + w[k][3]);
+    for (uint64_t base = lo; base < hi; base += K * 256) {
+        const int32_t j0 = static_cast<int32_t>(base) - static_cast<int32_t>(x.before);
+        sum += x.sum<K>(j0 + static_cast<int32_t>(threadIdx.x & 63u) * 4,
+                        static_cast<int32_t>(hi) - static_cast<int32_t>(x.before), j0 >= 0 && base + K * 256 <= hi);
     }
-    return block_sum(sum, s);
+    return wave_sum_f64(sum);
 }
 
 // Block (piece, sequence): the walk to the first sum, and this piece of it.
@@ -260,7 +282,22 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(const Verif
     Weights x = weights_of(a, b, w);
     if (!a.draft_probs) x.gone = scratch.gone;
     const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * a.piece;
-    const double sum = sum_of(x, lo, min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before), nodes, count, w.at, scratch);
+    const uint64_t hi = min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before);
+    double sum = 0;
+    for (uint64_t base = lo; base < hi; base += kVerifyTokens) {
+        mark(x, static_cast<uint32_t>(base), nodes, count, w.at, scratch);
+        constexpr uint32_t K = kVerifyTokens / (4 * kVerifyThreads);
+        double v[K][4];
+#pragma unroll
+        for (uint32_t k = 0; k < K; ++k) {
+            const uint64_t j = base + (k * kVerifyThreads + tid) * 4;
+            v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0;
+            if (j < hi) x.four(static_cast<int32_t>(j) - static_cast<int32_t>(x.before), v[k]);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < K; ++k) sum += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
+    }
+    sum = block_sum(sum, scratch, Scratch::kWaves);
     if (tid == 0) a.sums[static_cast<uint64_t>(b) * a.pieces + blockIdx.x] = sum;
     if (blockIdx.x) return;
     __syncthreads();
@@ -271,17 +308,21 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(const Verif
     }
 }
 
-// Block (sequence): what is left of the walk, and the token behind it.
-__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const VerifyArgs a) {
+// Block (sequence): what is left of the walk, by all its wavefronts, and the token behind
+// it, by four of them (more only wait for each other there: 5.4 us with four, 9.0 with
+// sixteen; 8 sequences' trees of 32 nodes took 476 us with four, 81 with sixteen).
+__global__ __launch_bounds__(64 * kWavesMost) void verify_draw_kernel(const VerifyArgs a) {
     Nodes nodes(a.width);
     __shared__ Scratch scratch;
     __shared__ double sums[kMaxPieces];
-    const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint64_t first = static_cast<uint64_t>(b) * a.width;
     Walk w = a.walks[b];
     const double u = a.uniforms[first];
-    if (w.took == 0) return;  // no node
-    for (uint32_t i = tid; i < a.pieces; i += kVerifyThreads) sums[i] = a.sums[static_cast<uint64_t>(b) * a.pieces + i];
+    uint32_t waves = w.open ? blockDim.x / 64 : Scratch::kWaves;
+    if (w.took == 0 || wave >= waves) return;  // no node, or nothing for this wavefront
+    for (uint32_t i = tid; i < a.pieces; i += 64 * waves) sums[i] = a.sums[static_cast<uint64_t>(b) * a.pieces + i];
     const uint32_t before_took = w.took;
     // nodes: where children are left to ask, or refused tokens to leave out
     uint32_t count = 0;
@@ -290,16 +331,17 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
     auto total = [&] {
         double sum = 0;
         __syncthreads();
-        for (uint32_t i = tid; i < a.pieces; i += kVerifyThreads) sum += sums[i];
-        return block_sum(sum, scratch);
+        for (uint32_t i = tid; i < a.pieces; i += 64 * waves) sum += sums[i];
+        return block_sum(sum, scratch, waves);
     };
-    // the pieces' sums anew
+    // the pieces' sums anew, a wavefront's after one another
     auto pieces = [&] {
-        for (uint32_t i = 0; i < a.pieces; ++i) {
+        __syncthreads();
+        for (uint32_t i = wave; i < a.pieces; i += waves) {
             const uint64_t lo = static_cast<uint64_t>(i) * a.piece;
             const uint64_t hi = min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before);
-            const double sum = lo < hi ? sum_of(x, lo, hi, nodes, count, w.at, scratch) : 0;
-            if (tid == 0) sums[i] = sum;
+            const double sum = lo < hi ? wave_sum_of(x, lo, hi) : 0;
+            if (lane == 0) sums[i] = sum;
         }
         __syncthreads();
     };
@@ -315,11 +357,14 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
             sum = total();
             w.open = more;
         } while (w.open);
-        for (uint32_t i = before_took + tid; i < w.took; i += kVerifyThreads) {
+        for (uint32_t i = before_took + tid; i < w.took; i += 64 * waves) {
             a.path[first + i] = nodes.path[i];
             a.out_tokens[first + i - 1] = nodes.token[nodes.path[i]];
         }
         if (tid == 0) a.accepted[b] = w.took;
+        waves = Scratch::kWaves;
+        __syncthreads();  // the sum is read
+        if (wave >= waves) return;
     }
     if (!(sum > 0)) {  // nothing is left: p itself
         x.q = nullptr, x.gone = nullptr, x.cut = 0;
@@ -331,7 +376,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
     // best: the first of the block's values (thread by thread, E of each) whose running sum from
     // `from` passes the target, kNone if none does; last: one more than the last that is positive.
     // `from` moves on, to the running sum before best's thread once there is one. The wavefronts'
-    // results are picked by ballots: atomics of 256 threads on one place took 4 us.
+    // results are picked by ballots: atomics of all threads on one place took 4 us.
     uint32_t best = kNone, last = 0;
     double from = 0;
     auto find = [&](auto &v, uint32_t base) {
@@ -388,6 +433,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
         const uint64_t hi = min(lo + a.piece, static_cast<uint64_t>(a.n) + x.before);
         for (uint64_t base = lo; base < hi && best == kNone; base += kVerifyTokens) {
             mark(x, static_cast<uint32_t>(base), nodes, count, w.at, scratch);
+            static_assert(kVerifyTokens == 16 * kVerifyThreads);
             double v[16];
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {  // 16 tokens in a row
@@ -501,12 +547,12 @@ extern "C" int fh_verify_draft(fh_device *dev, const float *probs, const float *
                        accepted,
                        reinterpret_cast<double *>(static_cast<char *>(workspace) + batch * sizeof(Walk)),
                        static_cast<Walk *>(workspace)};
-    const dim3 grid(a.pieces, a.batch), threads(kVerifyThreads);
+    const dim3 grid(a.pieces, a.batch);
     if (int rc = dispatch(dev, fn, [&] {
-            hipLaunchKernelGGL(verify_walk_kernel, grid, threads, Nodes::bytes(a.width), dev->stream, a);
+            hipLaunchKernelGGL(verify_walk_kernel, grid, dim3(kVerifyThreads), Nodes::bytes(a.width), dev->stream, a);
         }))
         return rc;
     return dispatch(dev, fn, [&] {
-        hipLaunchKernelGGL(verify_draw_kernel, dim3(a.batch), threads, Nodes::bytes(a.width), dev->stream, a);
+        hipLaunchKernelGGL(verify_draw_kernel, dim3(a.batch), dim3(a.draft_probs ? 64 * kWavesMost : kVerifyThreads), Nodes::bytes(a.width), dev->stream, a);
     });
 }
