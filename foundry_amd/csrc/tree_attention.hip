@@ -1,6 +1,7 @@
 // Attention of a tree of drafted tokens over a paged cache
 // (fh_paged_tree_attention).
 #include <algorithm>
+#include <limits>
 #include <tuple>
 
 #include "paged_cache.hpp"
@@ -800,8 +801,10 @@ extern "C" int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_
     if (int rc = check_shape(fn, batch, width, n_heads, n_kv, head_dim, page_size, max_pages)) return rc;
     if (int rc = fh_check_dims(fn, {n_pages})) return rc;
     if (int rc = check_pages(fn, n_pages, page_size, max_pages)) return rc;
-    if (!(scale > 0.0f && scale < INFINITY))
-        return fail(FH_ERR_INVALID_ARGUMENT, "%s: scale %g must be finite and above 0", fn, static_cast<double>(scale));
+    const float k = scale * 1.4426950408889634f;
+    if (!(scale > 0.0f && k < INFINITY))
+        return fail(FH_ERR_INVALID_ARGUMENT, "%s: scale %g must be above 0 and at most 2e38", fn,
+                    static_cast<double>(scale));
     if (batch == 0) return FH_OK;
     uint64_t need = 0;
     if (int rc = fh_paged_tree_attention_workspace(batch, width, n_heads, n_kv, head_dim, page_size, max_pages, &need))
@@ -841,7 +844,6 @@ extern "C" int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_
     if (int rc = refuse_overlap(fn, "workspace", workspace, need, "out", out, rows)) return rc;
     if (int rc = set_current(dev, fn)) return rc;
     const Plan w = plan(batch, width, n_heads, n_kv, head_dim, page_size, max_pages);
-    const float k = scale * 1.4426950408889634f;
     const TreeArgs a{q,
                      k_pages,
                      v_pages,
@@ -861,7 +863,7 @@ extern "C" int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_
                      w.tiles,
                      w.want_parts,
                      k,
-                     kSlack / k,
+                     std::min(kSlack / k, std::numeric_limits<float>::max()),
                      static_cast<float *>(workspace),
                      out};
     if (head_dim == 64)

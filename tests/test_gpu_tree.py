@@ -359,6 +359,18 @@ def test_attention_extreme_scores(device, heads, kv, hd, pages):
     assert np.isnan(got[4]).all()
 
 
+@pytest.mark.parametrize("scale,size", [(2.0 ** -126, 63), (1e-30, 49), (2e38, -60), (2e36, -60)])
+@pytest.mark.parametrize("pages", [18, 600])
+def test_attention_extreme_scales(device, scale, size, pages):
+    """Factors at fp32's ends, with scores that they bring to a few units (hundreds for the largest)."""
+    lens, counts = [250, 3], [5, 5]
+    q, k, v, table, lens, counts, masks = cache(pages, lens, counts, 5, 4, 2, 64, 16, pages=pages)
+    big = lambda a: synth.bf16_rne((synth.bf16_to_f32(a) * 2.0 ** size).astype(np.float32))
+    q[..., 0], k[..., 0] = big(q[..., 0] * 0 + 0x3F80), big(k[..., 0])
+    q[..., 1:] = 0
+    check_attention(device, q, k, v, table, lens, counts, masks, scale)
+
+
 def test_attention_leaves_out_entries_that_name_no_page(device):
     q, k, v, table, lens, counts, masks = cache(13, [100, 300, 40, 20], [6] * 4, 6, 4, 2, 64, 16)
     table[0, 2] = k.shape[0]          # a page in the middle
@@ -476,7 +488,7 @@ def test_attention_refusals(device):
               dict(pages=0), dict(n_pages=0), dict(nbytes=nbytes - 1), dict(ws=p(st["ws"], 8)), dict(q=p(st["q"], 2)),
               dict(out=p(st["q"])), dict(out=p(st["v"])), dict(out=p(st["ws"])), dict(ws=p(st["k"])),
               dict(scale=ctypes.c_float(0)), dict(scale=ctypes.c_float(-1)), dict(scale=ctypes.c_float(np.nan)),
-              dict(scale=ctypes.c_float(np.inf))):
+              dict(scale=ctypes.c_float(np.inf)), dict(scale=ctypes.c_float(3e38))):
         refused(bad, name, *args(**o))
     refused(_lib.ERR_UNSUPPORTED, name, *args(hd=32))
     refused(_lib.ERR_INDEX_TOO_LARGE, name, *args(batch=70000))
