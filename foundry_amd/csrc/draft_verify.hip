@@ -29,7 +29,8 @@ constexpr uint32_t kNone = 0xFFFFFFFFu;
 // of a row and the blocks that the first launch aims for before pieces get longer.
 constexpr uint32_t kVerifyTokens = 4096;
 constexpr uint32_t kLeastPiece = 1024;
-constexpr uint32_t kVerifyBlocks = 2048;
+// (16 chains with 2048 blocks 14.0 us, 12.8 with these; 1 or 64 the same.)
+constexpr uint32_t kVerifyBlocks = 1024;
 // Pieces of a row at most.
 constexpr uint32_t kMaxPieces = 1024;
 

@@ -14,9 +14,11 @@ namespace fh {
 // caches where they hold them, and writes. Runs are as long as a filled GPU allows.
 constexpr uint32_t kProbTokens = 8192;
 constexpr uint32_t kProbThreads = 256;
-// The shortest run, and the blocks that a launch aims for before runs get longer.
-constexpr uint32_t kProbLeast = 1024;
-constexpr uint32_t kProbBlocks = 2048;
+// The shortest run, and the blocks that a launch aims for before runs get longer: each block of the
+// second launch joins all runs of its row, so fewer are better (rows of 128256, with runs of 1024 and
+// 2048 blocks beside these: 16 rows 14.1 and 9.1 us, 64 rows 16.3 and 14.0, 1 row 8.0 and 7.4).
+constexpr uint32_t kProbLeast = 2048;
+constexpr uint32_t kProbBlocks = 512;
 
 struct RunStats {
     float m, sum;

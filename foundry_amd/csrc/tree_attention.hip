@@ -40,8 +40,11 @@ constexpr uint32_t kWaves = kTreeThreads / 64;
 constexpr uint32_t kStepKeys = 128;
 constexpr float kSlack = 8.0f;
 // Tables of so few positions (times head_dim) take one block per sequence and tile,
-// and no join: one launch.
+// and no join: one launch (512 positions of head_dim 128, 24 rows: 10.7 us, 12.5 in parts; 850:
+// 12.2 and 12.4; 1500: 18.9 and 14.1).
 constexpr uint32_t kWholeElements = 65536;
+// Batches of more steps take at least two to a part.
+constexpr uint32_t kFewSteps = 16;
 // Larger batches take one part per sequence, as every block would lay them all out.
 constexpr uint32_t kPlanBatch = 1024;
 
@@ -132,7 +135,9 @@ __device__ __forceinline__ Layout layout_of(const TreeArgs &a, uint32_t row0, ui
         layout_at(a, y, b0, total, lane);
         total = __builtin_amdgcn_readlane(y.upto, 63);
     }
-    y.size = max(1u, (total + a.want_parts - 1) / a.want_parts);
+    // (a part of one step is mostly its start and join: 32 steps of 32 rows took 18.3 us by one
+    // and 15.1 by two; for a dozen steps single ones are as good or better, 12.4 against 13.0)
+    y.size = max(total > kFewSteps ? 2u : 1u, (total + a.want_parts - 1) / a.want_parts);
     if (a.batch > 64) layout_at(a, y, 0, 0, lane);
     return y;
 }
@@ -747,14 +752,20 @@ struct Plan {
 Plan plan(int64_t batch, int64_t width, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t page_size,
           int64_t max_pages) {
     const uint64_t rows = width * (n_heads / n_kv), capacity = static_cast<uint64_t>(max_pages) * page_size;
+    // 4 nodes of 4 heads over 30000 tokens: 36.4 us as one group, 38.8 as two; four groups (64 rows,
+    // registers for one block to a CU) took 80 where two took 63, 64 nodes over 8 x 3000
     const uint32_t groups = rows <= 16 ? 1 : 2;
     const uint64_t tiles = (rows + 16 * groups - 1) / (16 * groups), units = tiles * n_kv;
     Plan w{groups, static_cast<uint32_t>(tiles), 0, 16};
     if (capacity * head_dim <= kWholeElements) return w;
     // what serves the largest batch serves smaller ones: the bytes of those that are split
     const uint64_t split = std::min<uint64_t>(batch, kPlanBatch);
-    // a block's registers leave room for two on a CU, or for one
-    const uint64_t blocks = head_dim == 256 ? 256 : 512;
+    // A block's registers leave room for two on a CU, or for one with head_dim 256 (8 x 3000 tokens, 32
+    // nodes of 8 heads: 29 us, 43 with 512 blocks). Where a KV head has one tile, memory is the bound, which
+    // one block per CU draws on as well, and there are half as many pieces to join (8 nodes over 131000
+    // tokens 105 us, 115 with 512; over 30000 33.9 and 39.5; 64 x 600, 37.1 and 33.6, pays for it);
+    // with more tiles two keep the matrix cores busier (64 nodes over 30000: 68 us, 79 with 256).
+    const uint64_t blocks = head_dim == 256 || tiles == 1 ? 256 : 512;
     // a table of few steps has no use for more parts than steps
     const uint64_t steps = (capacity + kStepKeys - 1) / kStepKeys;
     const uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>(blocks / units, split * steps));
