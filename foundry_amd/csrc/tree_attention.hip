@@ -37,9 +37,10 @@ namespace fh {
 //
 // Measured, 32 heads of 128 over 8 KV heads: 64 nodes of 8 sequences of 1900 to 4111 tokens 73 us
 // (295 TFLOP/s), 32 nodes behind 131077 tokens 167 us (3.2 TB/s, 411 TFLOP/s), 8 nodes 106 us
-// (5.1 TB/s), 6 nodes behind 700 tokens 12.2 us. Many nodes are bound by the vector
-// instructions around the products (about 190 of 4 cycles for 48 products of 16, per 32 keys and rows), few
-// by memory, short contexts by two launches of dependent loads.
+// (5.1 TB/s), 6 nodes behind 700 tokens 12.2 us. Many nodes are bound by K and V on
+// their way through the L1, once per 32 rows (45 of its 64 bytes a cycle), and by the vector instructions around
+// the products (about 190 of 4 cycles for 48 products of 16, per 32 keys and rows), few nodes by memory,
+// short contexts by two launches of dependent loads.
 constexpr uint32_t kMaxTree = 1024;
 constexpr uint32_t kTreeThreads = 256;
 constexpr uint32_t kWaves = kTreeThreads / 64;

@@ -183,6 +183,24 @@ def test_verify_a_full_vocabulary(device, drafts):
     check_verify(device, *drafted(5, 3, 4, 128256, drafts, drafts, spread=2.5))
 
 
+@pytest.mark.parametrize("n", [50, 9001, 30004])
+@pytest.mark.parametrize("at,q_at", [(0, 1), (3, 0), (2, 2), (1, 3)])
+def test_verify_rows_of_any_alignment(device, n, at, q_at):
+    """probs and draft_probs that begin `at` and `q_at` elements behind their storages' starts."""
+    b, width = 3, 10
+    pr, q, tokens, parents, counts, u = drafted(n + at, b, width, n, True, True, noise=1.5)
+    behind = lambda a, skip: up(device, np.concatenate([np.full(skip, np.nan, np.float32), a.ravel()]))
+    st = [behind(pr, at), behind(q, q_at)] + [up(device, a) for a in (tokens, parents, counts, u)]
+    out = [up(device, np.full(b * width, 7, np.uint32)) for _ in range(2)] + [up(device, np.full(b, 7, np.uint32))]
+    nbytes = _lib.verify_draft_workspace_bytes(b, width, n)
+    ws = up(device, np.full(nbytes, 0xFF, np.uint8))
+    _lib.call("fh_verify_draft", device.handle, p(st[0], 4 * at), p(st[1], 4 * q_at), b, width, n, *[p(s) for s in st[2:]],
+              p(ws), nbytes, *[p(s) for s in out])
+    want = D.verify(pr, q, tokens, parents, counts, u)
+    for s, w in zip(out, want):
+        assert np.array_equal(down(device, s, np.uint32, w.shape), w)
+
+
 @pytest.mark.parametrize("drafts", [False, True])
 def test_verify_refuses_every_child_of_wide_trees(device, drafts):
     """Many children of the root, of unlike and of the same tokens, none accepted: u is as large as it gets."""
