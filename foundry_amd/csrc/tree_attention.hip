@@ -36,8 +36,8 @@ namespace fh {
 // step of 2^-8 that bf16 V is off by itself. m, l and o are fp32.
 //
 // Measured, 32 heads of 128 over 8 KV heads: 64 nodes of 8 sequences of 1900 to 4111 tokens 73 us
-// (295 TFLOP/s), 32 nodes behind 131077 tokens 167 us (3.2 TB/s, 411 TFLOP/s), 8 nodes 106 us
-// (5.1 TB/s), 6 nodes behind 700 tokens 12.2 us. Many nodes are bound by K and V on
+// (295 TFLOP/s), 32 nodes behind 131077 tokens 166 us (3.2 TB/s, 414 TFLOP/s), 8 nodes 106 us
+// (5.1 TB/s), 6 nodes behind 700 tokens 12.4 us. Many nodes are bound by K and V on
 // their way through the L1, once per 32 rows (45 of its 64 bytes a cycle), and by the vector instructions around
 // the products (about 190 of 4 cycles for 48 products of 16, per 32 keys and rows), few nodes by memory,
 // short contexts by two launches of dependent loads.
@@ -52,6 +52,10 @@ constexpr float kSlack = 8.0f;
 constexpr uint32_t kWholeElements = 65536;
 // Batches of more steps take at least two to a part.
 constexpr uint32_t kFewSteps = 16;
+// What a sequence's start and join count beside its steps where parts of several sequences are
+// cut (with 0, 2, 4, 6, 9: 12 nodes of 64 sequences of 17 to 16384 tokens 107, 95, 97, 101, 106 us,
+// 64 nodes of 8 of 1900 to 4111 71, 68, 65, 64, 65, 8 nodes of 32 over one KV head of 256 49, 43, 36, 36, 36).
+constexpr uint32_t kStart = 4;
 // Larger batches take one part per sequence, as every block would lay them all out.
 constexpr uint32_t kPlanBatch = 1024;
 
@@ -112,18 +116,19 @@ __device__ __forceinline__ uint32_t scan_wave(uint32_t v, uint32_t lane) {
     return v;
 }
 
-// The steps of all sequences that have rows in a tile, in order, are cut into equal
-// parts: part x takes steps x * size .. of them, which may be the end of one
-// sequence, whole ones, and the start of another. Of a part's pieces only the
-// first and the last can be less than a sequence: they leave records 2 x (the first)
-// and 2 x + 1. Every wavefront works the layout out for itself, 64 sequences at a time.
+// The steps of all sequences that have rows in a tile, in order and (of more than one)
+// kStart blank ones before each sequence's, are cut into equal parts: part x takes steps x * size .. of
+// them, which may be the end of one sequence, whole ones, and the start of another. Of
+// a part's pieces only two can be less than a sequence: what began before it leaves record
+// 2 x, and what goes on behind it, from its sequence's first step, 2 x + 1. Every
+// wavefront works the layout out for itself, 64 sequences at a time.
 struct Layout {
-    uint32_t size;   // steps of a part
+    uint32_t size;   // steps of a part, blank ones among them
     uint32_t row0;   // the tile's first row
     uint32_t b0;     // first sequence of the 64 at hand
     uint32_t len, count;  // lane's sequence's tokens and nodes
-    uint32_t mine;   // its steps
-    uint32_t upto;   // and the batch's steps up to its end
+    uint32_t mine;   // its steps, without the blank ones
+    uint32_t upto;   // and all steps up to its end
 };
 
 __device__ __forceinline__ void layout_at(const TreeArgs &a, Layout &y, uint32_t b0, uint32_t before, uint32_t lane) {
@@ -131,7 +136,7 @@ __device__ __forceinline__ void layout_at(const TreeArgs &a, Layout &y, uint32_t
     y.count = b0 + lane < a.batch ? nodes_of(a, b0 + lane) : 0;
     y.len = y.count ? a.lengths[b0 + lane] : 0;
     y.mine = steps_of(a, y.len, y.count, y.row0);
-    y.upto = before + scan_wave(y.mine, lane);
+    y.upto = before + scan_wave(y.mine && a.batch > 1 ? y.mine + kStart : y.mine, lane);
 }
 
 __device__ __forceinline__ Layout layout_of(const TreeArgs &a, uint32_t row0, uint32_t lane) {
@@ -150,7 +155,7 @@ __device__ __forceinline__ Layout layout_of(const TreeArgs &a, uint32_t row0, ui
 }
 
 // Moves to the sequence that holds step `at` of the batch and returns it, its
-// steps in n and the steps before it in `start`; ~0 behind the last one.
+// steps in n and all before its first in `start`; ~0 behind the last one.
 __device__ __forceinline__ uint32_t sequence_of(const TreeArgs &a, Layout &y, uint32_t at, uint32_t lane, uint32_t &n,
                                                 uint32_t &start, uint32_t &len, uint32_t &count) {
     for (;;) {
@@ -160,7 +165,7 @@ __device__ __forceinline__ uint32_t sequence_of(const TreeArgs &a, Layout &y, ui
             len = __builtin_amdgcn_readlane(y.len, l);
             count = __builtin_amdgcn_readlane(y.count, l);
             n = __builtin_amdgcn_readlane(y.mine, l);
-            start = __builtin_amdgcn_readlane(y.upto, l) - n;
+            start = __builtin_amdgcn_readlane(y.upto, l) - n;  // behind the blank ones
             return y.b0 + l;
         }
         if (y.b0 + 64 >= a.batch) return ~0u;
@@ -267,7 +272,6 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
         for (uint32_t b = blockIdx.x; b < a.batch; b += gridDim.x)
             clear(b, b < 64 ? __builtin_amdgcn_readlane(y.count, b) : nodes_of(a, b));
     }
-    uint32_t slot = 0;  // of the piece's record
     while (at < end) {
         // the next piece: `steps` from `first` of sequence seq
         uint32_t seq = blockIdx.x, first = 0, steps, whole = 1, len, count;
@@ -275,10 +279,11 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
             uint32_t n, start;
             seq = sequence_of(a, y, at, lane, n, start, len, count);
             if (seq == ~0u) break;
-            first = at - start;
-            steps = min(n - first, end - at);
+            first = max(at, start) - start;
+            at = min(end, start + n);
+            if (at <= start + first) continue;  // blank steps alone
+            steps = at - start - first;
             whole = steps == n;
-            at += steps;
         } else {
             count = nodes_of(a, seq);
             len = a.lengths[seq];
@@ -610,7 +615,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
         __syncthreads();
         constexpr uint32_t DT = 16 * HD / kTreeThreads;  // dims of a thread
         const uint32_t tid = anew(threadIdx.x), d0 = tid % (HD / DT) * DT;
-        float *rec = a.records + (static_cast<uint64_t>(blockIdx.x * 2 + slot) * (a.n_kv * a.tiles) + unit) *
+        float *rec = a.records + (static_cast<uint64_t>(blockIdx.x * 2 + (first == 0)) * (a.n_kv * a.tiles) + unit) *
                                      record_floats<HD, NT>();
 #pragma unroll 1
         for (uint32_t i = tid / (HD / DT); i < 16 * NT && row0 + i < rows; i += 16) {
@@ -650,7 +655,6 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
             }
         }
         __syncthreads();  // the LDS is read: the next piece may write it
-        slot = 1;
     }
 }
 
@@ -673,11 +677,10 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs 
     const uint32_t start = __builtin_amdgcn_readlane(y.upto, seq - y.b0) - n;
     const uint32_t first = start / y.size, pieces = (start + n - 1) / y.size - first + 1;
     if (pieces == 1 || row >= rows || i >= 16 * NT) return;  // written by its block, or no row
-    // the first piece is the last of its part, unless it is that part's first too
     const uint64_t stride = static_cast<uint64_t>(a.n_kv) * a.tiles * record_floats<HD, NT>();
     const float *rec = a.records + static_cast<uint64_t>(unit) * record_floats<HD, NT>();
     auto piece = [&](uint32_t p) {
-        return rec + (static_cast<uint64_t>(first + p) * 2 + (p == 0 && start % y.size != 0)) * stride;
+        return rec + (static_cast<uint64_t>(first + p) * 2 + (p == 0)) * stride;
     };
     float m = -INFINITY, l = 0.0f, some = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
@@ -743,7 +746,7 @@ int check_shape(const char *fn, int64_t batch, int64_t width, int64_t n_heads, i
     if (width * (n_heads / n_kv) > 4 * 65535 - 64 || n_kv > 65535)
         return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld nodes of %lld heads", fn, (long long)width, (long long)n_heads);
     // the steps of all sequences are counted in 32 bits (pages may be shared, so their number bounds nothing)
-    if (batch * (max_pages * page_size / kStepKeys + 1) > 0x7FFFFFFFll)
+    if (batch * (max_pages * page_size / kStepKeys + 1 + kStart) > 0x7FFFFFFFll)
         return fail(FH_ERR_INDEX_TOO_LARGE, "%s: %lld sequences of %lld positions", fn, (long long)batch,
                     (long long)(max_pages * page_size));
     return FH_OK;
