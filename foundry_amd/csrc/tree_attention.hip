@@ -58,6 +58,10 @@ constexpr uint32_t kFewSteps = 16;
 constexpr uint32_t kStart = 4;
 // Larger batches take one part per sequence, as every block would lay them all out.
 constexpr uint32_t kPlanBatch = 1024;
+// Where a sum of values passes 2^64 (or is not finite) the values are taken 2^-48 times as large: 2^31 keys of
+// weights up to 2^16 and values up to the type's largest then stay below fp32's. What is multiplied so is exact down
+// to 2^-78. Sums that are not stay so far below fp32's largest that joining them cannot pass it.
+constexpr float kShrink = 0x1p-48f, kGrow = 0x1p48f;
 
 typedef __attribute__((ext_vector_type(8))) __bf16 ta_bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float ta_f32x4_t;
@@ -174,7 +178,8 @@ __device__ __forceinline__ uint32_t sequence_of(const TreeArgs &a, Layout &y, ui
 }
 
 // A record: what a piece leaves to be joined, [16 NT rows][HD] weighted values,
-// then m, l and whether any key was there, of each row.
+// then m, l and whether any key was there (0: none, 1: yes, 2: yes, and the values are kShrink times as large), of
+// each row.
 template <int HD, int NT>
 constexpr uint32_t record_floats() { return 16 * NT * (HD + 3); }
 
@@ -338,12 +343,13 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
         ta_f32x4_t acc[NT][VT];
         float m[NT], ref[NT], l[NT];  // ref: m k, as far as there is one
         uint32_t any[NT];
-        // Once as above. Where that leaves a sum that is not finite, or m k is not, again with care: scores
-        // whose products with k are too large are taken relative to m first, and keys that have an
-        // inf or NaN among their values stay out of the products, where weights of 0 (a row that does not
-        // see the key, a P that lost nothing) would make NaN of them, and are added row by row.
+        // Once as above. Where that leaves a sum whose square is not finite, or m k is not, again with care: scores
+        // whose products with k are too large are taken relative to m first, values are kShrink times as large,
+        // and keys that have an inf or NaN among their values stay out of the products, where weights of 0 (a row
+        // that does not see the key, a P that lost nothing) would make NaN of them, and are added row by row.
+        bool careful = false;
 #pragma unroll 1
-        for (bool careful = false;; careful = true) {
+        for (;; careful = true) {
 #pragma unroll
             for (int r = 0; r < NT; ++r) {
 #pragma unroll
@@ -493,7 +499,8 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                         lo[r] = ta_u32x4_t{wl[0], wl[1], wl[2], wl[3]};
                     }
                 };
-                // keys with an inf or NaN among their values: added to the rows that see them, and taken out of vf
+                // keys with an inf or NaN among their values: added to the rows that see them, and taken out of vf;
+                // the others' values are made smaller
                 auto special = [&](uint32_t key0) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -526,12 +533,20 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                                         asm volatile("" ::: "memory");  // four loads at a time
 #pragma unroll
                                         for (int x = 0; x < 4; ++x)
-                                            acc[r][t][x] =
-                                                fmaf(w, bf(mine[(t / PD) * 128 + x * PD + t % PD]), acc[r][t][x]);
+                                            acc[r][t][x] = fmaf(w, bf(mine[(t / PD) * 128 + x * PD + t % PD]) * kShrink,
+                                                                acc[r][t][x]);
                                     }
                             }
                         }
                     }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int u = 0; u < VP; ++u)
+#pragma unroll
+                            for (int x = 0; x < PD / 2; ++x)
+                                vf[i][u][x] = f32x2_to_bf16x2_rne(bf(vf[i][u][x] & 0xFFFFu) * kShrink,
+                                                                  bf(vf[i][u][x] >> 16) * kShrink);
                 };
                 auto values = [&] {
 #pragma unroll
@@ -573,7 +588,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                     uint32_t f0, f1;
                     groups(t + 2, f0, f1);
                     load_k(f0, f1);
-                    if (careful) special(from + t * 32);
+                    if (__builtin_expect(careful, false)) special(from + t * 32);
                     values();
                     load_v(n0, n1);
 #pragma unroll
@@ -581,16 +596,16 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                     g0 = n0, g1 = n1, n0 = f0, n1 = f1;
                 }
             }
-            float zero = 0.0f;  // NaN if a sum is not finite
+            ta_f32x4_t size = {0.0f, 0.0f, 0.0f, 0.0f};  // not finite if a sum's square is not
 #pragma unroll
             for (int r = 0; r < NT; ++r) {
-                zero = fmaf(m[r] == -INFINITY ? 0.0f : m[r] * a.k, 0.0f, zero);
+                size[0] = fmaf(m[r] == -INFINITY ? 0.0f : m[r] * a.k, 0.0f, size[0]);
 #pragma unroll
                 for (int t = 0; t < VT; ++t)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) zero = fmaf(acc[r][t][x], 0.0f, zero);
+                    for (int x = 0; x < 4; ++x) size[x] = fmaf(acc[r][t][x], acc[r][t][x], size[x]);
             }
-            if (careful || !__any(zero != 0.0f)) break;
+            if (careful || !__any(!((size[0] + size[1]) + (size[2] + size[3]) < INFINITY))) break;
         }
 
         // the four wavefronts joined: thread (row, dims), 16 rows at a time
@@ -609,7 +624,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
             if (lane < 16) {
                 part.ml[wave][0][i] = m[r];
                 part.ml[wave][1][i] = l[r];
-                part.ml[wave][2][i] = any[r] ? 1.0f : 0.0f;
+                part.ml[wave][2][i] = !any[r] ? 0.0f : careful ? 2.0f : 1.0f;
             }
         }
         __syncthreads();
@@ -626,23 +641,25 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                 some = fmaxf(some, part.ml[w][2][i]);
             }
             const float ref = top == -INFINITY ? 0.0f : top;
+            const bool shrunk = some > 1.0f;
             float sum = 0.0f, o[DT];
 #pragma unroll
             for (uint32_t d = 0; d < DT; ++d) o[d] = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
                 const float f = __builtin_amdgcn_exp2f(apart(part.ml[w][0][i], ref, a.k));
+                const float g = shrunk && part.ml[w][2][i] <= 1.0f ? f * kShrink : f;
                 sum = fmaf(f, part.ml[w][1][i], sum);
 #pragma unroll
-                for (uint32_t d = 0; d < DT; ++d) o[d] = fmaf(f, part.o[w][i][d0 + d], o[d]);
+                for (uint32_t d = 0; d < DT; ++d) o[d] = fmaf(g, part.o[w][i][d0 + d], o[d]);
             }
             if (whole) {
                 uint16_t *to = a.out + place(seq, row0 + i) + d0;
-                const float inv = 1.0f / sum;
+                const float inv = 1.0f / sum, grow = shrunk ? kGrow : 1.0f;
 #pragma unroll
                 for (uint32_t d = 0; d < DT; d += 2)
                     *reinterpret_cast<uint32_t *>(to + d) =
-                        some != 0.0f ? f32x2_to_bf16x2_rne(o[d] * inv, o[d + 1] * inv) : 0u;
+                        some != 0.0f ? f32x2_to_bf16x2_rne(o[d] * inv * grow, o[d + 1] * inv * grow) : 0u;
             } else {
 #pragma unroll
                 for (uint32_t d = 0; d < DT; d += 4)
@@ -703,24 +720,30 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs 
         }
         const float ref = next == -INFINITY ? 0.0f : next, f = __builtin_amdgcn_exp2f(apart(m, ref, a.k));
         m = next;
-        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+        const bool before = some > 1.0f;
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u)
+            if (p0 + u < pieces) some = fmaxf(some, ps[u]);
+        const bool shrunk = some > 1.0f;
+        const float h = shrunk && !before ? f * kShrink : f;
+        l *= f, o.x *= h, o.y *= h, o.z *= h, o.w *= h;
 #pragma unroll
         for (int u = 0; u < kJoinLoads; ++u)
             if (p0 + u < pieces) {
                 const float g = __builtin_amdgcn_exp2f(apart(pm[u], ref, a.k));
-                some = fmaxf(some, ps[u]);
+                const float e = shrunk && ps[u] <= 1.0f ? g * kShrink : g;
                 l = fmaf(pl[u], g, l);
-                o.x = fmaf(v[u].x, g, o.x), o.y = fmaf(v[u].y, g, o.y);
-                o.z = fmaf(v[u].z, g, o.z), o.w = fmaf(v[u].w, g, o.w);
+                o.x = fmaf(v[u].x, e, o.x), o.y = fmaf(v[u].y, e, o.y);
+                o.z = fmaf(v[u].z, e, o.z), o.w = fmaf(v[u].w, e, o.w);
             }
     }
     const uint32_t node = a.group(row);
     uint16_t *to = a.out +
                    ((static_cast<uint64_t>(seq) * a.width + node) * a.n_heads + kv * a.group.by +
                     (row - node * a.group.by)) * HD + d;
-    const float inv = 1.0f / l;
-    *reinterpret_cast<uint2 *>(to) = some != 0.0f ? make_uint2(f32x2_to_bf16x2_rne(o.x * inv, o.y * inv),
-                                                              f32x2_to_bf16x2_rne(o.z * inv, o.w * inv))
+    const float inv = 1.0f / l, grow = some > 1.0f ? kGrow : 1.0f;
+    *reinterpret_cast<uint2 *>(to) = some != 0.0f ? make_uint2(f32x2_to_bf16x2_rne(o.x * inv * grow, o.y * inv * grow),
+                                                              f32x2_to_bf16x2_rne(o.z * inv * grow, o.w * inv * grow))
                                                   : make_uint2(0, 0);
 }
 

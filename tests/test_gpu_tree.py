@@ -337,6 +337,45 @@ def test_attention_infinite_values_of_nodes_and_tokens(device):
     assert np.isfinite(got[0][:, :, rest]).all() and np.isfinite(got[1]).all()
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(4, 1, 64), (8, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("n,width,pages", [(250, 5, 16), (250, 5, 700), (3000, 5, None), (700, 40, 300)])
+def test_attention_finite_values_of_any_size(device, heads, kv, hd, n, width, pages):
+    """Values up to the type's largest: their sums pass fp32 (weights of equal keys, of keys far below a
+    later one, of keys above the first ones) where what they come to does not. One sequence of each kind,
+    one of ordinary values, and one with an infinity that some nodes see."""
+    lens, counts = [n] * 7, [width] * 7
+    q, k, v, table, lens, counts, masks = cache(hd + n, lens, counts, width, heads, kv, hd, 16, pages=pages)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 0x3F80  # 1.0: the score is the key's dim 0
+    top = synth.bf16_to_f32(np.array([0x7F7F], np.uint16))[0]
+    sign = np.where(np.random.default_rng(n).random((n + width, hd)) < 0.5, -1.0, 1.0)
+    ordinary = np.random.default_rng(n + 1).standard_normal((n + width, hd))
+    j = np.arange(n + width)
+    one = np.ones((n + width, hd))
+    # (scores in powers of two, values)
+    rows = [(0 * j, top * one), (0 * j, top * sign), (np.where(j % 97 == 60, 7, 0), top * sign),
+            (np.where(j == n // 2, 0, -60), np.where(j == n // 2, 1.0, top)[:, None] * one),
+            (0 * j, np.where(j < 30, top, 1.0)[:, None] * one), (0 * j, ordinary), (j % 5, top * one)]
+    for s, (score, value) in enumerate(rows):
+        score, value = synth.bf16_rne(score.astype(np.float32)), synth.bf16_rne(value.astype(np.float32))
+        for i in j:
+            k[table[s, i // 16], :, i % 16, 0], v[table[s, i // 16], :, i % 16] = score[i], value[i]
+    at = table[6, (n + 1) // 16], slice(None), (n + 1) % 16, 5
+    v[at] = 0x7F80
+    got = S.f64(attention(device, q, k, v, table, lens, counts, masks, np.log(2.0)))
+    ref, weight, reach = D.tree_attend(S.f64(q), S.f64(k), S.f64(v), table, lens, counts, masks, float(np.float32(np.log(2.0))))
+    finite = np.isfinite(ref)
+    seen = D.visible(width, width, masks[6])[:, 1]
+    assert np.array_equal(~finite[6, :, :, 5], np.broadcast_to(seen[:, None], (width, heads))) and finite[:6].all()
+    assert np.array_equal(got[~finite], ref[~finite])
+    ok = bound(hd, n + width, ref, weight, reach)
+    with np.errstate(invalid="ignore"):
+        assert (np.abs(got - ref) <= ok)[finite].all()
+    # the ordinary sequence is what it is without the others, bit for bit
+    alone = attention(device, q[5:6], k, v, table[5:6], lens[5:6], counts[5:6], masks[5:6], np.log(2.0)) if pages == 16 else None
+    assert alone is None or np.array_equal(S.f64(alone)[0], got[5])
+
+
 @pytest.mark.parametrize("heads,kv,hd", [(2, 1, 64), (8, 1, 128), (4, 1, 256)])
 @pytest.mark.parametrize("pages", [18, 600])
 def test_attention_extreme_scores(device, heads, kv, hd, pages):
