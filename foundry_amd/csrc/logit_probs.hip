@@ -278,6 +278,7 @@ extern "C" int fh_logits_probs(fh_device *dev, const void *logits, int dtype, in
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: logits and probs must be aligned to their types", fn);
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", fn);
+    if (int rc = check_words(fn, {{"temperatures", temperatures}})) return rc;
     const uint64_t each = static_cast<uint64_t>(rows) * 4;
     if (int rc = check_range(dev, logits, count * elem, fn, "logits")) return rc;
     if (int rc = check_range(dev, probs, count * 4, fn, "probs")) return rc;

@@ -214,6 +214,11 @@ int check_append(fh_device *dev, const char *fn, const uint16_t *qkv, int64_t to
                           static_cast<const void *>(norm.q_norm), static_cast<const void *>(norm.k_norm)})
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
             return fail(FH_ERR_INVALID_ARGUMENT, "%s: operands must be 16-byte aligned", fn);
+    if (int rc = check_words(fn, {{"sequences", sequences},
+                                  {"positions", positions},
+                                  {"slots", norm.slots},
+                                  {"page_table", page_table}}))
+        return rc;
     const uint64_t width = static_cast<uint64_t>(n_heads + 2 * n_kv) * head_dim, t = static_cast<uint64_t>(tokens);
     const uint64_t table = static_cast<uint64_t>(table_len) * head_dim * 2;
     uint64_t pool;

@@ -25,4 +25,17 @@ inline int refuse_overlap(const char *fn, const char *what, const void *p, uint6
     return FH_OK;
 }
 
+// Refuses lists of 4-byte entries that do not begin at a multiple of 4 bytes: scalar
+// loads pass over an address's lowest two bits, and would read other entries.
+struct Words {
+    const char *what;
+    const void *ptr;
+};
+inline int check_words(const char *fn, std::initializer_list<Words> lists) {
+    for (const Words &w : lists)
+        if (reinterpret_cast<uintptr_t>(w.ptr) % 4 != 0)
+            return fail(FH_ERR_INVALID_ARGUMENT, "%s: %s must be 4-byte aligned", fn, w.what);
+    return FH_OK;
+}
+
 }  // namespace fh

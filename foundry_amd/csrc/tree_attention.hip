@@ -859,6 +859,9 @@ extern "C" int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) &
         15u)
         return fail(FH_ERR_INVALID_ARGUMENT, "%s: q, out and workspace must be 16-byte aligned", fn);
+    if (int rc = check_words(
+            fn, {{"page_table", page_table}, {"lengths", lengths}, {"counts", counts}, {"masks", masks}}))
+        return rc;
     const uint64_t nodes = static_cast<uint64_t>(batch) * width, each = static_cast<uint64_t>(batch) * 4;
     const uint64_t rows = nodes * n_heads * head_dim * 2, bits = nodes * ((width + 31) / 32) * 4;
     uint64_t pool;

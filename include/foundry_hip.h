@@ -511,7 +511,7 @@ int fh_append_token_advance(fh_device *dev, const uint32_t *token, int64_t rows,
  * device data that the host cannot check: an entry that names no page
  * (>= n_pages) is left alone, as described for each call. max_pages *
  * page_size is at most 2^31 - 1; pools may pass 4 GiB. Pools and 2-byte
- * operands are 16-byte aligned.
+ * operands are 16-byte aligned, lists of 4-byte entries 4-byte aligned.
  * ====================================================================== */
 
 /* apply_rotary_pos_emb on q and k of each token, then k and v written to the

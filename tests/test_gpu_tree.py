@@ -535,3 +535,30 @@ def test_attention_refusals(device):
     refused(_lib.ERR_OUT_OF_BOUNDS, name, *args(mask=p(st["mask"], 4)), match="masks")
     with pytest.raises(_lib.HipError):
         _lib.call(name, *args(len=None))
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_lists_that_are_not_aligned_are_refused(device, off):
+    """4-byte entries at other addresses than multiples of 4, all within their storages."""
+    heads, kv, hd, page, n_pages, t = 4, 2, 64, 16, 4, 2
+    big = lambda: device.zeros(n_pages * kv * page * hd * 2)
+    qkv, k, v, q, cos, sin, ws = (big() for _ in range(7))
+    even, odd = device.zeros(4096), device.zeros(4096)
+    bad, good, at = _lib.ERR_INVALID_ARGUMENT, p(even), p(odd, off)
+    for i, what in enumerate(("sequences", "positions", "slots", "page_table")):
+        seq, pos, slot, table = (at if i == x else good for x in range(4))
+        refused(bad, "fh_paged_norm_rope_kv", device.handle, p(qkv), t, heads, kv, hd, None, None, ctypes.c_float(0), p(cos),
+                p(sin), 16, seq, pos, slot, table, 2, 2, p(k), p(v), n_pages, page, p(q), match=f"{what} must be 4-byte")
+        if what != "slots":
+            refused(bad, "fh_paged_rope_kv", device.handle, p(qkv), t, heads, kv, hd, p(cos), p(sin), 16, seq, pos, table, 2,
+                    2, p(k), p(v), n_pages, page, p(q), match=f"{what} must be 4-byte")
+    nbytes = _lib.paged_tree_attention_workspace_bytes(2, 3, heads, kv, hd, page, 2)
+    assert nbytes <= n_pages * kv * page * hd * 2
+    for i, what in enumerate(("page_table", "lengths", "counts", "masks")):
+        table, lens, counts, masks = (at if i == x else good for x in range(4))
+        refused(bad, "fh_paged_tree_attention", device.handle, p(qkv), 2, 3, heads, kv, hd, p(k), p(v), n_pages, page, table, 2,
+                lens, counts, masks, ctypes.c_float(1), p(ws), nbytes, p(q), match=f"{what} must be 4-byte")
+    nbytes = _lib.logits_probs_workspace_bytes(2, 30)
+    assert nbytes <= n_pages * kv * page * hd * 2
+    refused(bad, "fh_logits_probs", device.handle, p(qkv), _lib.F32, 2, 30, at, p(ws), nbytes, p(q),
+            match="temperatures must be 4-byte")
