@@ -52,6 +52,37 @@ def tree_attend(q, keys, values, table, lengths, counts, masks, scale):
     return out, weight, reach
 
 
+def tree_attend_whole(q, keys, values, table, lengths, counts, masks, scale):
+    """tree_attend, all nodes of a head at once, for long contexts."""
+    b, width, heads, hd = q.shape
+    n_pages, kv, page, _ = keys.shape
+    out, weight, reach = np.zeros(q.shape), np.zeros(q.shape), np.zeros((b, width, heads, 1))
+    for s in range(b):
+        n, count = int(lengths[s]), min(int(counts[s]), width) if counts is not None else width
+        if count == 0 or n + count > table.shape[1] * page:
+            continue
+        j = np.arange(n + count)
+        pages, slots = table[s, j // page].astype(np.int64), j % page
+        there = pages < n_pages
+        pages = np.where(there, pages, 0)
+        seen = visible(width, count, masks[s] if masks is not None else None)[:count, :count]
+        seen = np.concatenate([np.ones((count, n), bool), seen], 1) & there
+        some = seen.any(1, keepdims=True)
+        for h in range(heads):
+            k, v = keys[pages, h * kv // heads, slots], values[pages, h * kv // heads, slots]
+            sc = np.where(seen, q[s, :count, h] @ k.T * scale, -np.inf)
+            e = np.where(seen, np.exp(sc - np.where(some, sc.max(1, keepdims=True), 0)), 0)
+            p = e / np.where(some, e.sum(1, keepdims=True), 1)
+            bad = ~np.isfinite(v).all(1)  # keys that are added to the rows that see them alone
+            out[s, :count, h], weight[s, :count, h] = p[:, ~bad] @ v[~bad], p[:, ~bad] @ np.abs(v[~bad])
+            for i in np.nonzero(bad)[0]:
+                with np.errstate(invalid="ignore"):
+                    out[s, :count, h] += np.where(seen[:, i:i + 1], p[:, i:i + 1] * v[i], 0)
+                    weight[s, :count, h] += np.where(seen[:, i:i + 1], p[:, i:i + 1] * np.abs(v[i]), 0)
+            reach[s, :count, h, 0] = np.where(seen, np.abs(q[s, :count, h]) @ np.abs(k).T, 0).max(1) * scale
+    return out, weight, reach
+
+
 def probs(z, temperatures=None):
     """softmax(z / t) of each row in float64; z float64 (NaN counts as -inf)."""
     z = np.where(np.isnan(z), -np.inf, z)

@@ -137,3 +137,16 @@ def test_reference_pages_by_hand():
     g.k[0, 3, 0, 4:9] = np.arange(5).reshape(5, 1)
     assert g.compact(np.array([[0, 2, 3], [0] * 3, [0] * 3], np.uint32), np.array([3, 0, 0])).tolist() == [23, 0, 20]
     assert g.k[0, 3, 0, 4:9, 0].tolist() == [0, 2, 3, 3, 4]
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_reference_tree_attention_whole_is_the_other(masked):
+    rng = np.random.default_rng(3)
+    q, k, v = (rng.standard_normal(s) for s in ((3, 5, 4, 8), (9, 2, 16, 8), (9, 2, 16, 8)))
+    table = np.array([[1, 4, 9, 0], [7, 8, D.NONE, D.NONE], [2, 3, 5, 6]], np.uint32)
+    masks = rng.integers(0, 32, (3, 5, 1)).astype(np.uint32) if masked else None
+    v[4, :, 3], v[8, 1, 1, 2], v[3, 0, 15, 1] = np.inf, np.nan, -np.inf
+    for lengths, counts in (([40, 20, 59], [5, 3, 5]), ([0, 12, 60], None), ([0, 0, 0], [1, 0, 4])):
+        a, b = (f(q, k, v, table, lengths, counts, masks, 0.7) for f in (D.tree_attend, D.tree_attend_whole))
+        for x, y in zip(a, b):
+            assert np.allclose(x, y, rtol=1e-12, atol=1e-14, equal_nan=True)

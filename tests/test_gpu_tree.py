@@ -562,3 +562,53 @@ def test_lists_that_are_not_aligned_are_refused(device, off):
     assert nbytes <= n_pages * kv * page * hd * 2
     refused(bad, "fh_logits_probs", device.handle, p(qkv), _lib.F32, 2, 30, at, p(ws), nbytes, p(q),
             match="temperatures must be 4-byte")
+
+
+# ------------------------------------------------------------ long contexts
+
+def marked(seed, lens, counts, width, heads, kv, hd, page, pages):
+    """A cache whose keys weigh much alike, and whose values name their key's 128: a run of keys that is
+    left out or taken twice moves the dims of that run by as much as they have."""
+    q, k, v, table, lens, counts, masks = cache(seed, lens, counts, width, heads, kv, hd, page, pages=pages, sharp=0.5)
+    v = synth.bf16_rne((synth.bf16_to_f32(v) * 0.1).astype(np.float32))
+    for s, n in enumerate(lens.astype(np.int64) + counts):
+        j = np.arange(n)
+        for h in range(kv):
+            v[table[s, j // page], h, j % page, j // 128 % hd] = 0x4080
+    return q, k, v, table, lens, counts, masks
+
+
+def check_long(dev, q, k, v, table, lens, counts, masks, scale):
+    got = S.f64(attention(dev, q, k, v, table, lens, counts, masks, scale))
+    ref, weight, reach = D.tree_attend_whole(S.f64(q), S.f64(k), S.f64(v), table, lens, counts, masks, scale)
+    keys = (lens.astype(np.int64) + q.shape[1]).reshape(-1, 1, 1, 1)
+    finite = np.isfinite(ref)
+    assert np.array_equal(got[~finite], ref[~finite])
+    with np.errstate(invalid="ignore"):
+        assert (np.abs(got - ref) <= bound(k.shape[3], keys, ref, weight, reach))[finite].all()
+    return got, finite
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_attention_of_one_long_sequence_in_an_unsplit_batch(device, hd, infinite):
+    """Past 1024 sequences a block takes a whole one: 137 tiles for each of its wavefronts, so that the pages'
+    places are read again four times; with infinities in tile 101 of a wavefront and in a node, in the second pass too."""
+    lens, counts = [i % 4 for i in range(1026)], [1 + i % 2 for i in range(1026)]
+    lens[700], counts[700] = 17500, 2
+    q, k, v, table, lens, counts, masks = marked(hd, lens, counts, 2, 2, 1, hd, 16, 1200)
+    if infinite:
+        for j, d in ((12000, 5), (17501, 7)):
+            v[table[700, j // 16], 0, j % 16, d] = 0x7F80
+    got, finite = check_long(device, q, k, v, table, lens, counts, masks, hd ** -0.5)
+    assert finite.all() != infinite and got[700].any(-1).all()
+
+
+@pytest.mark.parametrize("hd,width,lens,page,pages", [
+    (64, 600, [9000, 333, 70], 16, 700),  # 304 tiles in all: one part, every block goes over the whole batch
+    (256, 600, [2500, 0, 40], 48, 70),
+    (64, 256, [17500], 16, 1200),         # 128 tiles in all: four parts, 35 tiles for a wavefront
+])
+def test_attention_of_many_tiles(device, hd, width, lens, page, pages):
+    counts = [width, width - 50, 3][:len(lens)]
+    check_long(device, *marked(sum(lens) + hd, lens, counts, width, 16, 16, hd, page, pages), hd ** -0.5)
