@@ -350,3 +350,49 @@ def test_verify_refusals(device):
     refused(_lib.ERR_INDEX_TOO_LARGE, name, *args(b=65536))
     refused(_lib.ERR_OUT_OF_BOUNDS, name, *args(n=31))
     refused(_lib.ERR_OUT_OF_BOUNDS, name, *args(par=p(st["par"], 4)), match="parents")
+
+
+# ------------------------------------------------ bounds of the sums as they are
+
+@pytest.mark.parametrize("n", [1, 7, 64, 1000, 2049, 4097, 8192, 32003, 128256, 131073, 600001])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_probs_and_their_sums_are_as_near_as_the_additions_allow(device, n, f32, rows):
+    """A thread adds at most 12 partial sums one after another (8 tokens of 4 pieces, or 4 of 8), a wavefront's
+    lanes 6, a block's wavefronts 4; a lane joins J = ceil(runs / 64) runs (a product and a sum each), then one
+    product and 6 sums more; a division and a product make the probability. A term of the sum has its own
+    exponential and those of at most J + 1 joins, 2^-22 each, whose exponents add up to the term's own, e; the
+    difference, log2 e, its division by t and the product are four roundings of that, 4 ln 2 < 3 times 2^-24 e."""
+    rng = np.random.default_rng(n + rows)
+    z = (3 * rng.standard_normal((rows, n))).astype(np.float32)
+    z = z if f32 else synth.bf16_rne(z)
+    t = np.resize(np.array([1.0, 0.3, 7.0, 0.05, 0.8], np.float32), rows)
+    got = run_probs(device, z, t).astype(np.float64)
+    z64 = z.astype(np.float64) if f32 else S.f64(z)
+    ref = D.probs(z64, t)
+    e = (z64.max(-1, keepdims=True) - z64) / t.astype(np.float64).reshape(-1, 1) * 1.4427
+    runs = (n + 7) // 2048 + 1
+    joins = -(-runs // 64)
+    rel = 3 * 2.0 ** -24 * (e + (ref * e).sum(-1, keepdims=True)) + (joins + 3) * 2.0 ** -22 \
+        + (12 + 6 + 4 + 2 * joins + 1 + 6 + 2) * 2.0 ** -24
+    ok = rel * ref + 2.0 ** -126 * ref.max(-1, keepdims=True)
+    assert (np.abs(got - ref) <= ok).all()
+    assert (np.abs(got.sum(-1) - 1) <= ok.sum(-1)).all()
+
+
+@pytest.mark.parametrize("drafts", [False, True])
+@pytest.mark.parametrize("n", [300001, 4300003])
+@pytest.mark.parametrize("u", [0.0, 0.5, 0.97, 0.99999])
+def test_verify_rows_of_many_or_long_pieces(device, n, drafts, u):
+    """More pieces than a block has threads, and pieces longer than a block takes at a time; the first sequence's
+    drafted token is accepted, the second's refused, the third's row has its whole weight at the end."""
+    rng = np.random.default_rng(n)
+    pr, q = (softmax(rng.standard_normal((3, 2, n)).astype(np.float32)) for _ in range(2))
+    pr[2, 0], pr[2, 0, n - 3:] = 0, (0.25, 0.5, 0.25)
+    tokens = np.array([[0, n // 2], [0, 5], [0, 9]], np.uint32)
+    draws = np.array([[u, 0], [u, 1 - 2.0 ** -24], [u, 0.5]], np.float32)
+    pr[1, 0, 5] = 0
+    for b in range(3):  # one sequence, whose pieces are the shortest, and all of them
+        check_verify(device, pr[b:b + 1], q[b:b + 1] if drafts else None, tokens[b:b + 1], None, None, draws[b:b + 1])
+    got = check_verify(device, pr, q if drafts else None, tokens, None, None, draws)
+    assert got[2].tolist() == [2, 1, 1] and got[1][2, 0] >= n - 3
