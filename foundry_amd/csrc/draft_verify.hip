@@ -20,8 +20,10 @@ namespace fh {
 // piece of the rows that count then, and only those rows are read; a second
 // launch's block per sequence goes on from there, finds the piece that the
 // token lies in and reads that. Further refusals (trees with the draft's
-// distributions) are summed by that block alone. Bound by memory: 64 chains of 6 over 128256
-// tokens take 21.7 us (14.7, at 4.5 TB/s, and 6.6 of the launches), one 10.3 us.
+// distributions) are summed by that block alone, those behind the last one twice. Bound by memory: 64 chains of 6
+// over 128256 tokens take 21.8 us (15.0, at 4.4 TB/s, and 6.8 of the launches; 20.0 without the draft's
+// distributions), one 10.5 us. Trees with the draft's distributions are bound by that one block's reads: 8 of 32
+// nodes 62 us, one of 64 33, by the refusals; without them 8 of 32 13.5 us.
 constexpr uint32_t kVerifyThreads = 256;
 constexpr uint32_t kWavesMost = 16;  // of a block that goes on with a walk
 constexpr uint32_t kMaxWidth = 1024;
@@ -312,7 +314,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(const Verif
 
 // Block (sequence): what is left of the walk, by all its wavefronts, and the token behind
 // it, by four of them (more only wait for each other there: 5.4 us with four, 9.0 with
-// sixteen; 8 sequences' trees of 32 nodes took 476 us with four, 81 with sixteen).
+// sixteen; 8 sequences' trees of 32 nodes, the same ones, took 476 us with four, 81 with sixteen).
 __global__ __launch_bounds__(64 * kWavesMost) void verify_draw_kernel(const VerifyArgs a) {
     Nodes nodes(a.width);
     __shared__ Scratch scratch;

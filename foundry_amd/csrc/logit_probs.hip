@@ -12,12 +12,13 @@ namespace fh {
 // takes each run's maximum and its sum relative to that (and a greedy row's first
 // largest token), the next joins a row's runs, reads the logits again, from the
 // caches where they hold them, and writes. Runs are as long as a filled GPU allows.
-// 512 bf16 rows of 128256 take 83 us (4.75 TB/s; 23 and 58 of the launches), one row 7.1 us.
+// 512 bf16 rows of 128256 take 83 us (4.75 TB/s; 23 and 59 of the launches), 384 f32 rows 102 (3.9 TB/s), one
+// bf16 row 7.1 us.
 constexpr uint32_t kProbTokens = 8192;
 constexpr uint32_t kProbThreads = 256;
 // The shortest run, and the blocks that a launch aims for before runs get longer: each block of the
-// second launch joins all runs of its row, so fewer are better (rows of 128256, with runs of 1024 and
-// 2048 blocks beside these: 16 rows 14.1 and 9.1 us, 64 rows 16.3 and 14.0, 1 row 8.0 and 7.4).
+// second launch joins all runs of its row, so fewer are better (rows of 128256, one call over and over, with runs
+// of 1024 and 2048 blocks beside these: 16 rows 14.1 and 9.1 us, 64 rows 16.3 and 14.0, 1 row 8.0 and 7.4).
 constexpr uint32_t kProbLeast = 2048;
 constexpr uint32_t kProbBlocks = 512;
 

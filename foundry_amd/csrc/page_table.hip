@@ -3,8 +3,12 @@
 // fh_paged_compact). Page counts stay on the device, so that none of these waits
 // for the host; the lowest free page goes to the first that asks, so that results
 // do not depend on the order in which threads run. The tables' kernels are bound by
-// dependent loads, 4 to 5 us each; the copies by memory: 16 forks of 28 layers' pages take 21.5 us
-// (4.75 TB/s), 24 sequences' paths over 28 layers 8.4 us (2.6 TB/s behind five dependent loads).
+// dependent loads: 4 to 5 us each for tens of sequences, a few entries of each and pools of hundreds of pages.
+// fh_paged_reserve fills a sequence's entries one after another in one thread and looks for free pages from page 0
+// on, so that it grows with both: 2048 entries of one sequence (32768 tokens) take 0.57 ms, 8192 2.2 ms, one of
+// each of 64 sequences 51 us where the first 90000 of 100000 pages are in use. The copies are bound by memory: 16
+// forks of 28 layers' pages take 21.2 us (4.8 TB/s), 24 sequences' paths over 28 layers 8 to 9 us (2.4 to 2.8
+// TB/s behind five dependent loads).
 #include <algorithm>
 #include <vector>
 

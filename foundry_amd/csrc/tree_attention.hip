@@ -35,26 +35,27 @@ namespace fh {
 // loses, for 16 bits of P: what those lose, 2^-16 of a term, is far below the half
 // step of 2^-8 that bf16 V is off by itself. m, l and o are fp32.
 //
-// Measured, 32 heads of 128 over 8 KV heads: 64 nodes of 8 sequences of 1900 to 4111 tokens 73 us
-// (295 TFLOP/s), 32 nodes behind 131077 tokens 166 us (3.2 TB/s, 414 TFLOP/s), 8 nodes 106 us
-// (5.1 TB/s), 6 nodes behind 700 tokens 12.4 us. Many nodes are bound by K and V on
+// Measured among calls on other data, 32 heads of 128 over 8 KV heads: 64 nodes of 8 sequences of 1900 to 4111
+// tokens 74 us (291 TFLOP/s), 32 nodes behind 131077 tokens 167 us (3.2 TB/s, 412 TFLOP/s), 8 nodes 107 us
+// (5.0 TB/s), 6 nodes behind 700 tokens 12.8 us. Many nodes are bound by K and V on
 // their way through the L1, once per 32 rows (45 of its 64 bytes a cycle), and by the vector instructions around
 // the products (about 190 of 4 cycles for 48 products of 16, per 32 keys and rows), few nodes by memory,
-// short contexts by two launches of dependent loads.
+// short contexts by two launches of dependent loads. Figures of settings side by side below are of one call over
+// and over, which finds its keys in the caches as far as they hold them (64 nodes of the 8 sequences 66 us).
 constexpr uint32_t kMaxTree = 1024;
 constexpr uint32_t kTreeThreads = 256;
 constexpr uint32_t kWaves = kTreeThreads / 64;
 constexpr uint32_t kStepKeys = 128;
 constexpr float kSlack = 8.0f;
 // Tables of so few positions (times head_dim) take one block per sequence and tile,
-// and no join: one launch (512 positions of head_dim 128, 24 rows: 10.7 us, 12.5 in parts; 850:
-// 12.2 and 12.4; 1500: 18.9 and 14.1).
+// and no join: one launch (512 positions of head_dim 128, 24 rows: 10.9 us, 12.7 in parts; 850:
+// 13.2 and 12.9; 1506: 18.8 and 14.8).
 constexpr uint32_t kWholeElements = 65536;
 // Batches of more steps take at least two to a part.
 constexpr uint32_t kFewSteps = 16;
 // What a sequence's start and join count beside its steps where parts of several sequences are
-// cut (with 0, 2, 4, 6, 9: 12 nodes of 64 sequences of 17 to 16384 tokens 107, 95, 97, 101, 106 us,
-// 64 nodes of 8 of 1900 to 4111 71, 68, 65, 64, 65, 8 nodes of 32 over one KV head of 256 49, 43, 36, 36, 36).
+// cut (with 0, 2, 4, 6, 9: 12 nodes of 64 sequences of 17 to 16384 tokens 107, 95, 97, 100, 105 us,
+// 64 nodes of 8 of 1900 to 4111 72, 69, 66, 66, 67, 8 nodes of 32 over one KV head of 256 50, 43, 36, 37, 36).
 constexpr uint32_t kStart = 4;
 // Larger batches take one part per sequence, as every block would lay them all out.
 constexpr uint32_t kPlanBatch = 1024;
@@ -151,8 +152,8 @@ __device__ __forceinline__ Layout layout_of(const TreeArgs &a, uint32_t row0, ui
         layout_at(a, y, b0, total, lane);
         total = __builtin_amdgcn_readlane(y.upto, 63);
     }
-    // (a part of one step is mostly its start and join: 32 steps of 32 rows took 18.3 us by one
-    // and 15.1 by two; for a dozen steps single ones are as good or better, 12.4 against 13.0)
+    // (a part of one step is mostly its start and join: 32 steps of 32 rows take 19.2 us by one
+    // and 15.6 by two; 12 steps 14.7 and 14.4, 7 steps 12.9 and 13.1)
     y.size = max(total > kFewSteps ? 2u : 1u, (total + a.want_parts - 1) / a.want_parts);
     if (a.batch > 64) layout_at(a, y, 0, 0, lane);
     return y;
@@ -785,8 +786,8 @@ struct Plan {
 Plan plan(int64_t batch, int64_t width, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t page_size,
           int64_t max_pages) {
     const uint64_t rows = width * (n_heads / n_kv), capacity = static_cast<uint64_t>(max_pages) * page_size;
-    // 4 nodes of 4 heads over 30000 tokens: 36.4 us as one group, 38.8 as two; four groups (64 rows,
-    // registers for one block to a CU) took 80 where two took 63, 64 nodes over 8 x 3000
+    // 4 nodes of 4 heads over 30000 tokens: 32.4 us as one group, 33.8 as two; four groups (64 rows,
+    // registers for one block to a CU) took 80 where two then took 63, 64 nodes over 8 x 3000
     const uint32_t groups = rows <= 16 ? 1 : 2;
     const uint64_t tiles = (rows + 16 * groups - 1) / (16 * groups), units = tiles * n_kv;
     Plan w{groups, static_cast<uint32_t>(tiles), 0, 16};
@@ -794,10 +795,12 @@ Plan plan(int64_t batch, int64_t width, int64_t n_heads, int64_t n_kv, int64_t h
     // what serves the largest batch serves smaller ones: the bytes of those that are split
     const uint64_t split = std::min<uint64_t>(batch, kPlanBatch);
     // A block's registers leave room for two on a CU, or for one with head_dim 256 (8 x 3000 tokens, 32
-    // nodes of 8 heads: 29 us, 43 with 512 blocks). Where a KV head has one tile, memory is the bound, which
+    // nodes of 8 heads: 32 us, 44 with 512 blocks). Where a KV head has one tile, memory is the bound, which
     // one block per CU draws on as well, and there are half as many pieces to join (8 nodes over 131000
-    // tokens 105 us, 115 with 512; over 30000 33.9 and 39.5; 64 x 600, 37.1 and 33.6, pays for it);
-    // with more tiles two keep the matrix cores busier (64 nodes over 30000: 68 us, 79 with 256).
+    // tokens 106 us, 116 with 512; over 30000 34.8 and 41.1; 64 x 600, 37.4 and 33.5, pays for it);
+    // with more tiles two keep the matrix cores busier (64 nodes over 30000: 68 us, 74 with 256).
+    // Parts are whole for each (KV head, tile), so that up to half of the blocks may be missing where these do not
+    // divide their number: 8 x 3000 tokens, 256 nodes 222 us (512 blocks), 260 373 us (264).
     const uint64_t blocks = head_dim == 256 || tiles == 1 ? 256 : 512;
     // a table of few steps has no use for more parts than steps
     const uint64_t steps = (capacity + kStepKeys - 1) / kStepKeys;

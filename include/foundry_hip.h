@@ -645,8 +645,9 @@ int fh_logits_process(fh_device *dev, const void *logits, int dtype, int64_t row
  * places apart from the positions:
  *   q' = RNE(n * cos + rot(n) * sin), n = q * w / sqrt(sum(q^2) / head_dim + eps),
  * w = q_norm for q's heads, k_norm for k's (bf16 [head_dim]; null: n = q, n =
- * k); v as it is. The sum of squares, n and the rotation are fp32 (squares past
- * fp32's largest make n zero). positions (u32 [tokens]) give the rotation,
+ * k); v as it is. The sum of squares, n and the rotation are fp32: squares past
+ * fp32's largest make n zero, those below its smallest count as 0 (with eps 0 a
+ * head of nothing else has no finite n). positions (u32 [tokens]) give the rotation,
  * slots (u32 [tokens], null: the positions) the place in the sequence: the nodes
  * of a tree share positions. A token whose position is >= table_len, whose slot
  * is >= max_pages * page_size, whose sequence is >= n_seqs or whose page is >=
