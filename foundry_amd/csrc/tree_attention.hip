@@ -59,10 +59,12 @@ constexpr uint32_t kFewSteps = 16;
 constexpr uint32_t kStart = 4;
 // Larger batches take one part per sequence, as every block would lay them all out.
 constexpr uint32_t kPlanBatch = 1024;
-// Where a sum of values passes 2^64 (or is not finite) the values are taken 2^-48 times as large: 2^31 keys of
-// weights up to 2^16 and values up to the type's largest then stay below fp32's. What is multiplied so is exact down
-// to 2^-78. Sums that are not stay so far below fp32's largest that joining them cannot pass it.
+// Where a sum of values passes 2^64 (or is not finite) and finite ones from 2^40 on are among them, they are taken
+// 2^-48 times as large: 2^31 keys of weights up to 2^16 and values up to the type's largest then stay below
+// fp32's. What is multiplied so is exact down to 2^-78. Sums that are not stay so far below fp32's largest (2^64, or
+// 2^31 keys of 2^16 times 2^40) that joining them cannot pass it.
 constexpr float kShrink = 0x1p-48f, kGrow = 0x1p48f;
+constexpr uint16_t kLarge = (127 + 40) << 7, kInfinite = 0x7F80;  // bf16 2^40 and infinity
 
 typedef __attribute__((ext_vector_type(8))) __bf16 ta_bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float ta_f32x4_t;
@@ -345,12 +347,13 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
         float m[NT], ref[NT], l[NT];  // ref: m k, as far as there is one
         uint32_t any[NT];
         // Once as above. Where that leaves a sum whose square is not finite, or m k is not, again with care: scores
-        // whose products with k are too large are taken relative to m first, values are kShrink times as large,
-        // and keys that have an inf or NaN among their values stay out of the products, where weights of 0 (a row
-        // that does not see the key, a P that lost nothing) would make NaN of them, and are added row by row.
-        bool careful = false;
+        // whose products with k are too large are taken relative to m first, and keys that have an inf or NaN
+        // among their values stay out of the products, where weights of 0 (a row that does not see the key, a P
+        // that lost nothing) would make NaN of them, and are added row by row. Where large finite values were
+        // among the keys, once more with all values kShrink times as large.
+        bool careful = false, large = false, shrunk = false;
 #pragma unroll 1
-        for (;; careful = true) {
+        for (;;) {
 #pragma unroll
             for (int r = 0; r < NT; ++r) {
 #pragma unroll
@@ -501,8 +504,20 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                     }
                 };
                 // keys with an inf or NaN among their values: added to the rows that see them, and taken out of vf;
-                // the others' values are made smaller
+                // large finite values are noted, or all made smaller
                 auto special = [&](uint32_t key0) {
+                    typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
+                    const float unit = shrunk ? kShrink : 1.0f;
+                    u16x2_t least = {0xFFFF, 0xFFFF};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int u = 0; u < VP; ++u)
+#pragma unroll
+                            for (int x = 0; x < PD / 2; ++x)
+                                least = __builtin_elementwise_min(
+                                    least, __builtin_bit_cast(u16x2_t, vf[i][u][x] & 0x7FFF7FFFu) - u16x2_t{kLarge, kLarge});
+                    large = large || __any(min(least[0], least[1]) < kInfinite - kLarge);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         uint32_t found = 0;
@@ -534,12 +549,13 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                                         asm volatile("" ::: "memory");  // four loads at a time
 #pragma unroll
                                         for (int x = 0; x < 4; ++x)
-                                            acc[r][t][x] = fmaf(w, bf(mine[(t / PD) * 128 + x * PD + t % PD]) * kShrink,
+                                            acc[r][t][x] = fmaf(w, bf(mine[(t / PD) * 128 + x * PD + t % PD]) * unit,
                                                                 acc[r][t][x]);
                                     }
                             }
                         }
                     }
+                    if (!shrunk) return;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -606,7 +622,9 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
 #pragma unroll
                     for (int x = 0; x < 4; ++x) size[x] = fmaf(acc[r][t][x], acc[r][t][x], size[x]);
             }
-            if (careful || !__any(!((size[0] + size[1]) + (size[2] + size[3]) < INFINITY))) break;
+            if (careful ? shrunk || !large : !__any(!((size[0] + size[1]) + (size[2] + size[3]) < INFINITY))) break;
+            shrunk = careful;
+            careful = true;
         }
 
         // the four wavefronts joined: thread (row, dims), 16 rows at a time
@@ -625,7 +643,7 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
             if (lane < 16) {
                 part.ml[wave][0][i] = m[r];
                 part.ml[wave][1][i] = l[r];
-                part.ml[wave][2][i] = !any[r] ? 0.0f : careful ? 2.0f : 1.0f;
+                part.ml[wave][2][i] = !any[r] ? 0.0f : shrunk ? 2.0f : 1.0f;
             }
         }
         __syncthreads();
@@ -642,25 +660,24 @@ __global__ __launch_bounds__(kTreeThreads, HD == 256 ? 1 : 2) void tree_part_ker
                 some = fmaxf(some, part.ml[w][2][i]);
             }
             const float ref = top == -INFINITY ? 0.0f : top;
-            const bool shrunk = some > 1.0f;
             float sum = 0.0f, o[DT];
 #pragma unroll
             for (uint32_t d = 0; d < DT; ++d) o[d] = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
                 const float f = __builtin_amdgcn_exp2f(apart(part.ml[w][0][i], ref, a.k));
-                const float g = shrunk && part.ml[w][2][i] <= 1.0f ? f * kShrink : f;
+                const float g = f * (part.ml[w][2][i] < some ? kShrink : 1.0f);  // (0 for none: its sums are 0)
                 sum = fmaf(f, part.ml[w][1][i], sum);
 #pragma unroll
                 for (uint32_t d = 0; d < DT; ++d) o[d] = fmaf(g, part.o[w][i][d0 + d], o[d]);
             }
             if (whole) {
                 uint16_t *to = a.out + place(seq, row0 + i) + d0;
-                const float inv = 1.0f / sum, grow = shrunk ? kGrow : 1.0f;
+                const float inv = (some > 1.0f ? kGrow : 1.0f) / sum;
 #pragma unroll
                 for (uint32_t d = 0; d < DT; d += 2)
                     *reinterpret_cast<uint32_t *>(to + d) =
-                        some != 0.0f ? f32x2_to_bf16x2_rne(o[d] * inv * grow, o[d + 1] * inv * grow) : 0u;
+                        some != 0.0f ? f32x2_to_bf16x2_rne(o[d] * inv, o[d + 1] * inv) : 0u;
             } else {
 #pragma unroll
                 for (uint32_t d = 0; d < DT; d += 4)
@@ -721,18 +738,17 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs 
         }
         const float ref = next == -INFINITY ? 0.0f : next, f = __builtin_amdgcn_exp2f(apart(m, ref, a.k));
         m = next;
-        const bool before = some > 1.0f;
+        const float before = some;
 #pragma unroll
         for (int u = 0; u < kJoinLoads; ++u)
             if (p0 + u < pieces) some = fmaxf(some, ps[u]);
-        const bool shrunk = some > 1.0f;
-        const float h = shrunk && !before ? f * kShrink : f;
+        const float h = f * (before < some ? kShrink : 1.0f);
         l *= f, o.x *= h, o.y *= h, o.z *= h, o.w *= h;
 #pragma unroll
         for (int u = 0; u < kJoinLoads; ++u)
             if (p0 + u < pieces) {
                 const float g = __builtin_amdgcn_exp2f(apart(pm[u], ref, a.k));
-                const float e = shrunk && ps[u] <= 1.0f ? g * kShrink : g;
+                const float e = g * (ps[u] < some ? kShrink : 1.0f);
                 l = fmaf(pl[u], g, l);
                 o.x = fmaf(v[u].x, e, o.x), o.y = fmaf(v[u].y, e, o.y);
                 o.z = fmaf(v[u].z, e, o.z), o.w = fmaf(v[u].w, e, o.w);
@@ -742,9 +758,9 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(const TreeArgs 
     uint16_t *to = a.out +
                    ((static_cast<uint64_t>(seq) * a.width + node) * a.n_heads + kv * a.group.by +
                     (row - node * a.group.by)) * HD + d;
-    const float inv = 1.0f / l, grow = some > 1.0f ? kGrow : 1.0f;
-    *reinterpret_cast<uint2 *>(to) = some != 0.0f ? make_uint2(f32x2_to_bf16x2_rne(o.x * inv * grow, o.y * inv * grow),
-                                                              f32x2_to_bf16x2_rne(o.z * inv * grow, o.w * inv * grow))
+    const float inv = (some > 1.0f ? kGrow : 1.0f) / l;
+    *reinterpret_cast<uint2 *>(to) = some != 0.0f ? make_uint2(f32x2_to_bf16x2_rne(o.x * inv, o.y * inv),
+                                                              f32x2_to_bf16x2_rne(o.z * inv, o.w * inv))
                                                   : make_uint2(0, 0);
 }
 

@@ -680,11 +680,12 @@ int fh_paged_tree_attention_workspace(int64_t batch, int64_t width, int64_t n_he
  * * page_size: idle) are zeros. Keys of a table entry that names no page are
  * left out. What lies at places that a row does not see is not used for it,
  * whatever its bits. A row whose every score is -inf is NaN; one of finite scores
- * and values is finite, however large they are. exp(..) as v's factor has 16 bits
- * (off by 2^-16 of a term at most). head_dim is 64, 128 or 256, any n_heads /
- * n_kv; width is 1 to 1024, batch at most 65535, scale above 0
- * and at most 2e38; out does not overlap the inputs. workspace: as for
- * fh_paged_attention, at least fh_paged_tree_attention_workspace() bytes. */
+ * and values is finite, however large they are (beside sums past 2^64, values below
+ * 2^-78 may count as 0). exp(..) as v's factor has 16 bits (off by 2^-16 of a term
+ * at most). head_dim is 64, 128 or 256, any n_heads / n_kv; width is 1 to 1024,
+ * batch at most 65535, scale above 0 and at most 2e38; out does not overlap the
+ * inputs. workspace: as for fh_paged_attention, at least
+ * fh_paged_tree_attention_workspace() bytes. */
 int fh_paged_tree_attention(fh_device *dev, const uint16_t *q, int64_t batch, int64_t width,
                             int64_t n_heads, int64_t n_kv, int64_t head_dim,
                             const uint16_t *k_pages, const uint16_t *v_pages, int64_t n_pages,

@@ -376,6 +376,35 @@ def test_attention_finite_values_of_any_size(device, heads, kv, hd, n, width, pa
     assert alone is None or np.array_equal(S.f64(alone)[0], got[5])
 
 
+@pytest.mark.parametrize("hd,pages", [(64, 16), (128, None), (256, 700)])
+@pytest.mark.parametrize("width", [5, 40])
+def test_attention_small_values_beside_infinite_ones(device, hd, pages, width):
+    """Values of 2^-90 stay what they are in rows that do not see an infinite or NaN node, and in those that do
+    in the other dims; a large finite value beside the infinite one is used as well."""
+    n = 190
+    q, k, v, table, lens, counts, masks = cache(hd, [n, n], [width, width], width, 4, 2, hd, 16, pages=pages)
+    v = synth.bf16_rne((synth.bf16_to_f32(v) * 2.0 ** -90).astype(np.float32))
+    clean = attention(device, q, k, v, table, lens, counts, masks, hd ** -0.5)
+    at = [(table[s, (n + 2) // 16], slice(None), (n + 2) % 16) for s in range(2)]
+    v[at[0]][:, 5], v[at[0]][:, 9] = 0x7F80, 0x7FC0
+    v[at[1]][:, 5], v[at[1]][:, 9] = 0x7F80, 0x7F7F  # infinite, the type's largest
+    got = attention(device, q, k, v, table, lens, counts, masks, hd ** -0.5)
+    ref, weight, reach = D.tree_attend(S.f64(q), S.f64(k), S.f64(v), table, lens, counts, masks, hd ** -0.5)
+    ok = bound(hd, n + width, ref, weight, reach)
+    rest = np.setdiff1d(np.arange(hd), [5, 9])
+    for s in range(2):
+        seen = D.visible(width, width, masks[s])[:, 2]
+        assert seen.any() and not seen.all()
+        assert (S.f64(got[s][seen])[..., 5] == np.inf).all()
+        if s == 0:
+            assert np.array_equal(got[s][~seen], clean[s][~seen])
+            # (there the node is added to the sum apart from the others: other roundings, as many)
+            assert (np.abs(S.f64(got[s, seen][..., rest]) - ref[s, seen][..., rest]) <= ok[s, seen][..., rest]).all()
+            assert np.isnan(S.f64(got[s][seen])[..., 9]).all()
+        else:
+            assert (np.abs(S.f64(got[s, seen, :, 9]) - ref[s, seen, :, 9]) <= ok[s, seen, :, 9]).all()
+
+
 @pytest.mark.parametrize("heads,kv,hd", [(2, 1, 64), (8, 1, 128), (4, 1, 256)])
 @pytest.mark.parametrize("pages", [18, 600])
 def test_attention_extreme_scores(device, heads, kv, hd, pages):
